@@ -1,0 +1,64 @@
+// kv8.h — the 8-bit paged KV cache: launchers (arguments validated by
+// kv8_capi.cpp) and what its kernels share.  Layout: include/ie_kv8.h.
+#pragma once
+
+#include "ie_internal.h"
+#include "ie_kv8.h"
+
+namespace ie {
+
+struct Kv8Cache {
+    int8_t* k;
+    int8_t* v;
+    float* ks;
+    float* vs;
+    const int* table;  // [B, nbps]
+    int nbps;
+    int H;             // key/value heads
+    int d;
+    int bs_log2;       // pages of 1 << bs_log2 tokens
+};
+
+// Rows of B sequences into the cache (kv8_cache.hip): P each from start on, or
+// with positions one each at positions[b].
+struct Kv8Write {
+    int B, P;
+    const float* K;
+    const float* V;
+    int ld;
+    Kv8Cache c;
+    int start;
+    const int* positions;
+    int* ctx_lens;  // with positions: ctx_lens[b] = positions[b] + 1 (may be null)
+};
+void launch_kv8_write(const Kv8Write& a, hipStream_t s);
+
+struct Kv8Read {
+    int B, n;
+    const int* starts;
+    const int* lens;
+    Kv8Cache c;
+    float* K;
+    float* V;
+};
+void launch_kv8_read(const Kv8Read& a, hipStream_t s);
+
+// Attention of B x P query tokens over the cache; token t of sequence b sees
+// its first min(lens[b], max_ctx) positions (decode, P = 1), or with lens null
+// the first start + t + 1 (prompt).  Q row (b, t) at (b * P + t) * q_ld.
+struct Kv8Attn {
+    int B, P, H_q;
+    const float* Q;
+    int q_ld;
+    Kv8Cache c;
+    const int* lens;
+    int max_ctx;
+    int start;
+    float* O;  // [B, P, H_q, d]
+    float* ws;
+    int splits;
+};
+void launch_decode_attn_kv8(const Kv8Attn& a, hipStream_t s);   // kv8_decode.hip
+void launch_prefill_attn_kv8(const Kv8Attn& a, hipStream_t s);  // kv8_prefill.hip
+
+}  // namespace ie

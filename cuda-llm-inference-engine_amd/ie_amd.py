@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes
 import numbers
 import os
+from typing import NamedTuple
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libie_amd.so")
@@ -17,6 +18,7 @@ IE_OK, IE_ERR_INVALID, IE_ERR_UNSUPPORTED, IE_ERR_WORKSPACE, IE_ERR_HIP = range(
 EPI_PLAIN, EPI_BIAS, EPI_BIAS_GELU, EPI_BIAS_RESIDUAL, EPI_I32 = range(5)
 PATH_AUTO, PATH_GEMV, PATH_MFMA = range(3)
 KV_F32, KV_BF16 = 0, 1
+KV_I8 = 2  # Engine's kv_dtype only (include/ie_kv8.h)
 BACKEND_INT8, BACKEND_FP32 = 0, 1
 DA_REF_MAX_SPLITS = 16
 DA_MAX_SPLITS = 256
@@ -53,6 +55,24 @@ SIGNATURES = {
     "ie_decode_attn_noalloc": (_I, [_I, _I, _I, _I, _P, _P, _P, _I, _P, _P, _I, _I, _I, _P, _I, _P]),
 }
 DECODE_SCRATCH_BYTES = 32 << 20
+
+# include/ie_kv8.h
+KV8_SIGNATURES = {
+    "ie_kv8_cache_write": (_I, [_I, _I, _P, _P, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P]),
+    "ie_kv8_cache_append_batch": (_I, [_I, _P, _P, _I, _P, _P, _P, _P, _P, _I, _P, _I, _I, _I, _P]),
+    "ie_kv8_cache_read": (_I, [_I, _I, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P]),
+    "ie_decode_kv8_num_splits": (_I, [_I, _I, _I, _I, _I, _I]),
+    "ie_decode_attn_kv8": (_I, [_I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P, _Z, _I, _P]),
+    "ie_prefill_attn_kv8": (_I, [_I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P]),
+}
+KV8_MAX_SPLITS = 64
+
+# include/ie_logprobs.h
+LOGPROBS_SIGNATURES = {
+    "ie_token_logprobs_workspace_bytes": (_Z, [_I, _I, _I]),
+    "ie_token_logprobs": (_I, [_I, _P, _I, _I, _P, _I, _P, _P, _P, _P, _P, _P, _Z, _P]),
+}
+LOGPROBS_TOP_MAX = 128
 
 # include/ie_engine.h
 ENGINE_SIGNATURES = {
@@ -123,7 +143,8 @@ def load() -> ctypes.CDLL:
                 "(make -C cuda-llm-inference-engine_amd)")
         lib = ctypes.CDLL(LIB_PATH)
         for name, (res, args) in (list(SIGNATURES.items()) + list(ENGINE_SIGNATURES.items())
-                                  + list(TOKENIZER_SIGNATURES.items())):
+                                  + list(TOKENIZER_SIGNATURES.items()) + list(KV8_SIGNATURES.items())
+                                  + list(LOGPROBS_SIGNATURES.items())):
             fn = getattr(lib, name)
             fn.restype = res
             fn.argtypes = args
@@ -369,6 +390,244 @@ def top_k_draw(vals, idx, temperature, seed):
     check("ie_top_k_draw", v.ctypes.data, i.ctypes.data, len(v), ctypes.c_float(temperature),
           ctypes.c_uint(seed), ctypes.addressof(tok))
     return tok.value
+
+
+# ------------------------------------------- 8-bit KV cache, log probabilities
+def _check(what, dtype, tensors):
+    """Contiguous tensors of one type on the current device, or a ValueError."""
+    at = _device_index()
+    for t in tensors:
+        if t.get_device() != at or t.dtype is not dtype or not t.is_contiguous():
+            raise ValueError(f"{what}: needs contiguous {dtype} tensors on cuda:{at}, got {t.dtype} of strides "
+                             f"{tuple(t.stride())} on {t.device}")
+
+
+_device_index = None  # () -> index of the current device
+_f32 = _i32 = _i8 = _empty = None
+
+
+def _bind_torch():
+    global _device_index, _f32, _i32, _i8, _empty
+    import torch
+
+    torch.cuda.current_stream()
+    _f32, _i32, _i8, _empty = torch.float32, torch.int32, torch.int8, torch.empty
+    _device_index = torch._C._cuda_getDevice
+
+
+def _made(stream, *tensors):
+    """Tensors allocated here for a call on another stream than the current one
+    are kept from reuse until that stream has passed."""
+    if stream is not None:
+        for t in tensors:
+            t.record_stream(stream)
+
+
+class Kv8Cache(NamedTuple):
+    """The paged KV cache in 8 bits (include/ie_kv8.h has the layout): K codes
+    [pages, heads, block, d] and V codes [pages, heads, block / 16, d, 16] int8,
+    scales [pages, heads] fp32."""
+    k: "torch.Tensor"  # noqa: F821
+    v: "torch.Tensor"  # noqa: F821
+    k_scale: "torch.Tensor"  # noqa: F821
+    v_scale: "torch.Tensor"  # noqa: F821
+
+    @classmethod
+    def empty(cls, pages, heads, d, block_size=16, device="cuda"):
+        import torch
+
+        return cls(torch.empty((pages, heads, block_size, d), dtype=torch.int8, device=device),
+                   torch.empty((pages, heads, block_size // 16, d, 16), dtype=torch.int8, device=device),
+                   torch.empty((pages, heads), dtype=torch.float32, device=device),
+                   torch.empty((pages, heads), dtype=torch.float32, device=device))
+
+    def nbytes(self):
+        return sum(t.numel() * t.element_size() for t in self)
+
+
+def _kv8(what, cache, table):
+    """(heads, block size, d) of a cache whose tensors fit each other."""
+    if _device_index is None:
+        _bind_torch()
+    k, v, ks, vs = cache
+    _check(what, _i8, (k, v))
+    _check(what, _f32, (ks, vs))
+    _check(what, _i32, (table,))
+    pages, H, bs, d = k.shape
+    if v.shape != (pages, H, bs // 16, d, 16) or ks.shape != (pages, H) or vs.shape != ks.shape or table.dim() != 2:
+        raise ValueError(f"{what}: cache tensors or block table of wrong shape: {[tuple(t.shape) for t in cache]}, "
+                         f"{tuple(table.shape)}")
+    return H, bs, d
+
+
+def _kv8_rows(what, K, V, lead, H, d):
+    """Distance between rows [*lead, H, d] fp32 that may lie apart (the columns
+    of a QKV projection) but evenly so."""
+    st = K.stride()
+    if lead[-1] > 1:
+        ld = st[len(lead) - 1]
+    else:
+        ld = st[0] if lead[0] > 1 else H * d
+    at, want = _device_index(), (*lead, H, d)
+    if (K.shape != want or V.shape != want or K.dtype is not _f32 or V.dtype is not _f32 or K.get_device() != at
+            or V.get_device() != at or V.stride() != st or st[-1] != 1 or (H > 1 and st[-2] != d)
+            or (len(lead) == 2 and lead[0] > 1 and lead[1] > 1 and st[0] != lead[1] * ld)):
+        raise ValueError(f"{what}: K and V need to be fp32 {want} on cuda:{at} with equal strides, rows whole and evenly "
+                         f"spaced; got {tuple(K.shape)} strides {st}, {tuple(V.shape)} strides {V.stride()}")
+    return ld
+
+
+def kv8_cache_write(K, V, cache, block_table, start_pos, stream=None):
+    """Rows K, V [B, P, heads, d] fp32 (views into a QKV projection serve as they
+    lie) to positions start_pos .. of the sequences of block_table [B, nbps]."""
+    H, bs, d = _kv8("kv8_cache_write", cache, block_table)
+    B, P = K.shape[:2]
+    if block_table.shape[0] != B:
+        raise ValueError("kv8_cache_write: block_table has other sequences than K")
+    ld = _kv8_rows("kv8_cache_write", K, V, (B, P), H, d) if B * P else H * d
+    k, v, ks, vs = cache
+    check("ie_kv8_cache_write", B, P, K.data_ptr(), V.data_ptr(), ld, k.data_ptr(), v.data_ptr(), ks.data_ptr(),
+          vs.data_ptr(), block_table.data_ptr(), block_table.shape[1], start_pos, H, d, bs, _stream(stream))
+
+
+def kv8_cache_append_batch(K, V, cache, block_table, positions, stream=None):
+    """One row of each sequence, K, V [B, heads, d], to positions[b] (int32)."""
+    H, bs, d = _kv8("kv8_cache_append_batch", cache, block_table)
+    B = K.shape[0]
+    _check("kv8_cache_append_batch", _i32, (positions,))
+    if block_table.shape[0] != B or positions.shape != (B,):
+        raise ValueError("kv8_cache_append_batch: block_table or positions has other sequences than K")
+    ld = _kv8_rows("kv8_cache_append_batch", K, V, (B,), H, d) if B else H * d
+    k, v, ks, vs = cache
+    check("ie_kv8_cache_append_batch", B, K.data_ptr(), V.data_ptr(), ld, k.data_ptr(), v.data_ptr(), ks.data_ptr(),
+          vs.data_ptr(), block_table.data_ptr(), block_table.shape[1], positions.data_ptr(), H, d, bs, _stream(stream))
+
+
+def kv8_cache_read(cache, block_table, starts, context_lens, n, out=None, stream=None):
+    """(K, V) [B, n, heads, d] fp32: positions starts[b] .. starts[b] + n - 1 of each
+    sequence, zeros from context_lens[b] on (None: no limit)."""
+    H, bs, d = _kv8("kv8_cache_read", cache, block_table)
+    B = block_table.shape[0]
+    ints = (starts,) if context_lens is None else (starts, context_lens)
+    _check("kv8_cache_read", _i32, ints)
+    if any(t.shape != (B,) for t in ints):
+        raise ValueError("kv8_cache_read: starts or context_lens has other sequences than block_table")
+    if out is None:
+        out = tuple(_empty((B, n, H, d), dtype=_f32, device=cache.k.device) for _ in range(2))
+        _made(stream, *out)
+    K, V = out
+    _check("kv8_cache_read", _f32, out)
+    if K.shape != (B, n, H, d) or V.shape != K.shape:
+        raise ValueError(f"kv8_cache_read: out needs two tensors of shape {(B, n, H, d)}")
+    k, v, ks, vs = cache
+    check("ie_kv8_cache_read", B, n, starts.data_ptr(), _ptr(context_lens), k.data_ptr(), v.data_ptr(), ks.data_ptr(),
+          vs.data_ptr(), block_table.data_ptr(), block_table.shape[1], H, d, bs, K.data_ptr(), V.data_ptr(),
+          _stream(stream))
+    return K, V
+
+
+def decode_kv8_num_splits(B, H_q, H_kv, d, max_ctx, splits=0):
+    return call("ie_decode_kv8_num_splits", B, H_q, H_kv, d, max_ctx, splits)
+
+
+def decode_attn_kv8(Q, cache, block_table, context_lens, max_ctx, splits=0, out=None, workspace=None, stream=None):
+    """Q [B, H_q, d] fp32, one token a sequence, over the first context_lens[b]
+    <= max_ctx cached positions; returns O [B, H_q, d]."""
+    H, bs, d = _kv8("decode_attn_kv8", cache, block_table)
+    B, H_q, dq = Q.shape
+    if dq != d or block_table.shape[0] != B or context_lens.shape != (B,):
+        raise ValueError(f"decode_attn_kv8: Q {tuple(Q.shape)}, block_table {tuple(block_table.shape)}, context_lens "
+                         f"{tuple(context_lens.shape)} and heads of {d} do not fit")
+    if out is None:
+        out = _empty((B, H_q, d), dtype=_f32, device=Q.device)
+        _made(stream, out)
+    elif out.shape != Q.shape:
+        raise ValueError("decode_attn_kv8: out needs Q's shape")
+    _check("decode_attn_kv8", _f32, (Q, out))
+    _check("decode_attn_kv8", _i32, (context_lens,))
+    if workspace is None:
+        S = decode_kv8_num_splits(B, H_q, H, d, max_ctx, splits)
+        if S > 1:
+            workspace = _empty(B * H_q * S * (d + 2), dtype=_f32, device=Q.device)
+            _made(stream, workspace)
+    if workspace is not None:
+        _check("decode_attn_kv8", _f32, (workspace,))
+    k, v, ks, vs = cache
+    check("ie_decode_attn_kv8", B, H_q, H, d, Q.data_ptr(), k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(),
+          block_table.data_ptr(), context_lens.data_ptr(), max_ctx, bs, block_table.shape[1], out.data_ptr(),
+          _ptr(workspace), 0 if workspace is None else 4 * workspace.numel(), splits, _stream(stream))
+    return out
+
+
+def prefill_attn_kv8(Q, cache, block_table, start_pos, out=None, stream=None):
+    """Q [B, P, H_q, d] fp32, token t at position start_pos + t with its rows
+    cached; returns causal O [B, P, H_q, d]."""
+    H, bs, d = _kv8("prefill_attn_kv8", cache, block_table)
+    B, P, H_q, dq = Q.shape
+    if dq != d or block_table.shape[0] != B:
+        raise ValueError(f"prefill_attn_kv8: Q {tuple(Q.shape)}, block_table {tuple(block_table.shape)} and heads of {d} "
+                         "do not fit")
+    if out is None:
+        out = _empty((B, P, H_q, d), dtype=_f32, device=Q.device)
+        _made(stream, out)
+    elif out.shape != Q.shape:
+        raise ValueError("prefill_attn_kv8: out needs Q's shape")
+    _check("prefill_attn_kv8", _f32, (Q, out))
+    k, v, ks, vs = cache
+    check("ie_prefill_attn_kv8", B, P, H_q, H, d, Q.data_ptr(), k.data_ptr(), v.data_ptr(), ks.data_ptr(),
+          vs.data_ptr(), block_table.data_ptr(), block_table.shape[1], bs, start_pos, out.data_ptr(), _stream(stream))
+    return out
+
+
+class TokenLogprobs(NamedTuple):
+    """What token_logprobs returns, one entry per row; top_* are [rows, k]."""
+    logprobs: "torch.Tensor"  # noqa: F821
+    ranks: "torch.Tensor"  # noqa: F821
+    entropy: "torch.Tensor"  # noqa: F821
+    top_logprobs: "torch.Tensor"  # noqa: F821
+    top_indices: "torch.Tensor"  # noqa: F821
+
+
+def token_logprobs(logits, targets=None, k=0, out=None, workspace=None, stream=None):
+    """Log probability and rank of targets[r] (int32, -1: none) under row r of
+    logits [rows, n] fp32 (rows may lie apart), the row's entropy, and its k
+    most likely tokens with their log probabilities (include/ie_logprobs.h)."""
+    if _device_index is None:
+        _bind_torch()
+    rows, n = logits.shape
+    at = _device_index()
+    ld, step = logits.stride()
+    if logits.get_device() != at or logits.dtype is not _f32 or (n > 1 and step != 1) or (rows > 1 and ld < n):
+        raise ValueError(f"token_logprobs: logits need to be fp32 rows on cuda:{at}, got {logits.dtype} strides "
+                         f"{(ld, step)} on {logits.device}")
+    if targets is not None:
+        _check("token_logprobs", _i32, (targets,))
+        if targets.shape != (rows,):
+            raise ValueError("token_logprobs: targets needs one entry per row")
+    if out is None:
+        dev = logits.device
+        out = TokenLogprobs(_empty(rows, dtype=_f32, device=dev), _empty(rows, dtype=_i32, device=dev),
+                            _empty(rows, dtype=_f32, device=dev), _empty((rows, k), dtype=_f32, device=dev),
+                            _empty((rows, k), dtype=_i32, device=dev))
+        _made(stream, *out)
+    else:
+        _check("token_logprobs", _f32, (out[0], out[2], out[3]))
+        _check("token_logprobs", _i32, (out[1], out[4]))
+        if any(t.shape != (rows,) for t in out[:3]) or any(t.shape != (rows, k) for t in out[3:]):
+            raise ValueError(f"token_logprobs: out needs three tensors of {rows} and two of {(rows, k)}")
+        out = TokenLogprobs(*out)
+    if workspace is None:
+        need = call("ie_token_logprobs_workspace_bytes", rows, n, k)
+        if need:
+            workspace = _empty(need // 4, dtype=_f32, device=logits.device)
+            _made(stream, workspace)
+    if workspace is not None:
+        _check("token_logprobs", _f32, (workspace,))
+    lp, rk, en, tv, ti = out
+    check("ie_token_logprobs", rows, logits.data_ptr(), ld if rows > 1 else n, n, _ptr(targets), k, lp.data_ptr(),
+          rk.data_ptr(), en.data_ptr(), tv.data_ptr(), ti.data_ptr(), _ptr(workspace),
+          0 if workspace is None else 4 * workspace.numel(), _stream(stream))
+    return out
 
 
 # ---------------------------------------------------------------- engine
