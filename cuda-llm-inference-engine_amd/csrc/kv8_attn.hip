@@ -77,7 +77,6 @@ void launch(const Kv8Attn& a, hipStream_t s) {
 
 }  // namespace
 
-void launch_decode_attn_kv8(const Kv8Attn& a, hipStream_t s) { launch(a, s); }
 void launch_prefill_attn_kv8(const Kv8Attn& a, hipStream_t s) { launch(a, s); }
 
 }  // namespace ie

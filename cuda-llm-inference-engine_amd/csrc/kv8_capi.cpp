@@ -145,7 +145,13 @@ int ie_decode_kv8_num_splits(int B, int H_q, int H_kv, int d, int max_context_le
     if (B <= 0 || H_q <= 0 || H_kv <= 0 || max_context_len <= 0) return 1;
     const int tiles = (int)(((long long)max_context_len + 63) / 64);
     int s = num_splits;
-    if (s <= 0) s = 1;
+    if (s <= 0) {
+        // About two workgroups of four waves a CU, and a tile at least for each wave.
+        const int G = H_q / H_kv, heads = G <= 4 ? 4 : 8;
+        const long long units = (long long)B * H_kv * ((G + heads - 1) / heads);
+        s = (int)((512 + units - 1) / units);
+        if (s > (tiles + 3) / 4) s = (tiles + 3) / 4;
+    }
     if (s > IE_KV8_MAX_SPLITS) s = IE_KV8_MAX_SPLITS;
     return s < tiles ? s : tiles;
 }
