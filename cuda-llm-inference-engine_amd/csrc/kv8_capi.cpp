@@ -146,11 +146,14 @@ int ie_decode_kv8_num_splits(int B, int H_q, int H_kv, int d, int max_context_le
     const int tiles = (int)(((long long)max_context_len + 63) / 64);
     int s = num_splits;
     if (s <= 0) {
-        // About two workgroups of four waves a CU, and a tile at least for each wave.
-        const int G = H_q / H_kv, heads = G <= 4 ? 4 : 8;
+        // A workgroup a CU, and a tile at least for each of its four waves; one
+        // split where more would spare a wave fewer than three tiles.
+        const int G = H_q / H_kv, heads = G <= 4 ? 4 : G <= 8 ? 8 : 16;
         const long long units = (long long)B * H_kv * ((G + heads - 1) / heads);
-        s = (int)((512 + units - 1) / units);
-        if (s > (tiles + 3) / 4) s = (tiles + 3) / 4;
+        const int each = (tiles + 3) / 4;
+        s = (int)((256 + units - 1) / units);
+        if (s > each) s = each;
+        if (each - (each + s - 1) / s < 3) s = 1;
     }
     if (s > IE_KV8_MAX_SPLITS) s = IE_KV8_MAX_SPLITS;
     return s < tiles ? s : tiles;

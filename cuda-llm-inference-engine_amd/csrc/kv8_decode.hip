@@ -27,21 +27,35 @@
 // the second product accumulates in its int32 registers, which hold 2^17 keys.
 // Where it must, they are added to fp32 sums and m and W set anew (rebase).
 //
-// A wave walks tiles of its workgroup's range; a tile's K is requested when the
-// previous one's scores are done, its V when the previous one's output is, its
-// table entries one tile earlier.  A workgroup is one (sequence, KV head, split)
-// with up to 4 NT query heads; its waves merge in LDS in wave order, the splits
-// in a second launch in split order.
+// A wave walks tiles of its workgroup's range for 4 NT query heads; a tile's K
+// is requested when the previous one's scores are done, its V when the previous
+// one's output is, its table entries one tile earlier.  A workgroup is one
+// (sequence, KV head, split) with up to 4 NT HT query heads; its waves merge in
+// LDS in wave order, the splits in a second launch in split order.
+//
+// Bound by the bytes in flight: a wave's tile is 8 KB (d = 64) or 16 KB, and
+// the fp32 sums lie in LDS so that three waves a SIMD fit (four at d = 64, two
+// with eight heads a wave).  32 x (8 x 4) x 8192 x 128 95 us, 5.7 TB/s; with the
+// sums in registers 102.  Eight heads on one wave (NT = 2) read the tile once: 2 x
+// (8 x 8) x 40000 x 128 45.3 against 46.0 us on two waves of four heads each.
+// Eight or sixteen waves a workgroup are never ahead (8 x 12 x 1024 x 64: 9.5 us
+// with 4 waves, 10.0 with 8, 11.0 with 16).
 #include <algorithm>
 #include <cmath>
 
 #include "device_util.h"
 #include "kv8.h"
 
+// The lanes of a quad take different digits of one number, so they must come to
+// the same bits: no product is fused into the quad's sums (which would round one
+// of two addends, another one in each lane).
+#pragma clang fp contract(off)
+
 namespace ie {
 namespace {
 
 constexpr int kTile = 64;  // keys
+constexpr int NW = 4;      // waves a workgroup
 
 template <int CTRL>
 __device__ __forceinline__ float dpp_quad(float v) {
@@ -66,12 +80,13 @@ __device__ __forceinline__ uint32_t gather_bytes(uint32_t x0, uint32_t x1, uint3
 }
 
 // blockIdx.x = ((b * H + h) * groups + head group) * splits + split
-template <int D, int NT, int NW>
-__global__ __launch_bounds__(64 * NW) void kv8_decode_kernel(Kv8Attn a, int groups, float qscale) {
-    constexpr int KB = D / 64, JB = D / 16, HEADS = 4 * NT;
-    __shared__ float sh_o[NW][HEADS][D];
-    __shared__ float sh_m[NW][HEADS], sh_l[NW][HEADS];
-    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+template <int D, int NT, int HT>
+__global__ __launch_bounds__(64 * NW, D == 64 ? (NT == 1 ? 4 : 3) : (NT == 1 ? 3 : 2)) void kv8_decode_kernel(Kv8Attn a, int groups, float qscale) {
+    constexpr int KB = D / 64, JB = D / 16, HEADS = 4 * NT * HT;
+    constexpr int TW = NW / HT;  // waves that share a set of heads
+    __shared__ float sh_o[NW][4 * NT][D];
+    __shared__ float sh_m[NW][4 * NT], sh_l[NW][4 * NT];
+    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, ht = wid % HT, tw = wid / HT;
     unsigned id = blockIdx.x;
     const int split = (int)(id % (unsigned)a.splits);
     id /= (unsigned)a.splits;
@@ -109,8 +124,10 @@ __global__ __launch_bounds__(64 * NW) void kv8_decode_kernel(Kv8Attn a, int grou
 
     float m[NT], l[NT];
     int ub[NT];  // biased exponent of W * 2^-30
-    float of[NT][JB][4];
     i32x4 acc[NT][JB];
+    // The fp32 sums, digits joined: rarely touched, so in LDS.  Lane (col, q4)
+    // with digit 0 has channels 16 j + 4 q4 .. + 3 of head col / 4.
+    auto sums = [&](int c, int j) { return reinterpret_cast<float4*>(&sh_o[wid][4 * c + (col >> 2)][16 * j + 4 * q4]); };
 #pragma unroll
     for (int c = 0; c < NT; ++c) {
         m[c] = -INFINITY;
@@ -119,15 +136,43 @@ __global__ __launch_bounds__(64 * NW) void kv8_decode_kernel(Kv8Attn a, int grou
 #pragma unroll
         for (int j = 0; j < JB; ++j) {
             acc[c][j] = i32x4{0, 0, 0, 0};
-#pragma unroll
-            for (int r = 0; r < 4; ++r) of[c][j][r] = 0.0f;
+            if (digit == 0) *sums(c, j) = make_float4(0.f, 0.f, 0.f, 0.f);
         }
     }
+    // sums = (sums + acc) * f
+    auto flush = [&](int c, float f) {
+        const float f0 = pow2(ub[c]) * pow2(127 + 8 * digit);
+#pragma unroll
+        for (int j = 0; j < JB; ++j) {
+            float o[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[r] = quad_sum((float)acc[c][j][r] * f0);
+            if (digit == 0) {
+                const float4 was = *sums(c, j);
+                *sums(c, j) = make_float4((was.x + o[0]) * f, (was.y + o[1]) * f, (was.z + o[2]) * f, (was.w + o[3]) * f);
+            }
+        }
+    };
     const float digit_w = pow2(127 + 8 * digit);  // 256^digit
     const uint32_t sel = (uint32_t)digit * 0x0101u + 0x0400u;
 
-    int tile = t0 + wid;
+    int tile = t0 + tw;
     if (tile < t1) {  // uniform over the wave
+        // The queries' channels 64 kb + 16 q4 .. + 15 of head col / 4 of each
+        // column tile, requested ahead of the table entries' round trip.
+        float x[NT][KB][16];
+#pragma unroll
+        for (int c = 0; c < NT; ++c) {
+            const int g = min(g0 + 4 * (ht * NT + c) + (col >> 2), G - 1);
+            const float* qp = a.Q + (size_t)b * a.q_ld + ((size_t)h * G + g) * D + q4 * 16;
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float4 f = *reinterpret_cast<const float4*>(qp + kb * 64 + 4 * i);
+                    x[c][kb][4 * i] = f.x; x[c][kb][4 * i + 1] = f.y; x[c][kb][4 * i + 2] = f.z; x[c][kb][4 * i + 3] = f.w;
+                }
+        }
         i32x4 kw[4][KB], vw[JB];
         float ks, vs;
         Where w = place(tile, entry(tile, gk), entry(tile, gv));
@@ -146,30 +191,19 @@ __global__ __launch_bounds__(64 * NW) void kv8_decode_kernel(Kv8Attn a, int grou
         };
         load_k();
         load_v();
-        int next = min(tile + NW, t1 - 1);
+        int next = min(tile + TW, t1 - 1);
         int pk = entry(next, gk), pv = entry(next, gv);
 
-        // The queries' digits: lane (col, q4) holds digit `digit` of channels
-        // 64 kb + 16 q4 .. + 15 of head col / 4 of each column tile.
+        // Their digits: lane (col, q4) holds digit `digit`.
         i32x4 qd[NT][KB];
         float qw[NT];  // what a score's digit counts
 #pragma unroll
         for (int c = 0; c < NT; ++c) {
-            const int g = min(g0 + 4 * c + (col >> 2), G - 1);
-            const float* qp = a.Q + (size_t)b * a.q_ld + ((size_t)h * G + g) * D + q4 * 16;
-            float x[KB][16];
             uint32_t mx = 0;
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float4 f = *reinterpret_cast<const float4*>(qp + kb * 64 + 4 * i);
-                    x[kb][4 * i] = f.x; x[kb][4 * i + 1] = f.y; x[kb][4 * i + 2] = f.z; x[kb][4 * i + 3] = f.w;
-                }
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) mx = max(mx, __builtin_bit_cast(uint32_t, x[kb][i]) & 0x7fffffffu);
+                for (int i = 0; i < 16; ++i) mx = max(mx, __builtin_bit_cast(uint32_t, x[c][kb][i]) & 0x7fffffffu);
             mx = max(mx, (uint32_t)__shfl_xor((int)mx, 16, 64));
             mx = max(mx, (uint32_t)__shfl_xor((int)mx, 32, 64));
             const int e = max((int)(mx >> 23), 30);  // both factors stay normal numbers
@@ -180,7 +214,7 @@ __global__ __launch_bounds__(64 * NW) void kv8_decode_kernel(Kv8Attn a, int grou
                 for (int i = 0; i < 4; ++i) {
                     uint32_t dg[4];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) dg[k] = biased_digits((int)rintf(x[kb][4 * i + k] * up));
+                    for (int k = 0; k < 4; ++k) dg[k] = biased_digits((int)rintf(x[c][kb][4 * i + k] * up));
                     qd[c][kb][i] = (int)(gather_bytes(dg[0], dg[1], dg[2], dg[3], sel) ^ 0x80808080u);
                 }
             qw[c] = e == 255 ? __builtin_nanf("") : pow2(max(e - 29, 1)) * digit_w;
@@ -188,7 +222,7 @@ __global__ __launch_bounds__(64 * NW) void kv8_decode_kernel(Kv8Attn a, int grou
 
         int since = 0;
         for (;;) {
-            const bool more = tile + NW < t1;
+            const bool more = tile + TW < t1;
             i32x4 s[NT][4];
 #pragma unroll
             for (int c = 0; c < NT; ++c)
@@ -204,58 +238,45 @@ __global__ __launch_bounds__(64 * NW) void kv8_decode_kernel(Kv8Attn a, int grou
             const int seen = n - tile * kTile - 16 * q4;  // keys of this lane's group within the context
             w = place(next, pk, pv);
             load_k();
-            next = min(tile + 2 * NW, t1 - 1);
+            next = min(tile + 2 * TW, t1 - 1);
             pk = entry(next, gk);
             pv = entry(next, gv);
 
 #pragma unroll
             for (int c = 0; c < NT; ++c) {
                 const float sw = qw[c] * kscale;
-                float p[16];
-                auto weights = [&](float mm) {
-                    const float off = -0.25f * mm;
+                float sc[16];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        p[i] = exp2_sm(quad_sum(fmaf((float)s[c][i >> 2][i & 3], sw, off)));
-                    if (tile * kTile + kTile > n) {  // uniform: the context's last tile
+                for (int i = 0; i < 16; ++i) sc[i] = quad_sum((float)s[c][i >> 2][i & 3] * sw);
+                if (tile * kTile + kTile > n) {  // uniform: the context's last tile
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) p[i] = i < seen ? p[i] : 0.0f;
-                    }
-                };
-                weights(m[c]);
-                float pm = p[0];
+                    for (int i = 0; i < 16; ++i) sc[i] = i < seen ? sc[i] : -INFINITY;
+                }
+                float top = sc[0];
 #pragma unroll
-                for (int i = 1; i < 16; ++i) pm = fmaxf(pm, p[i]);
-                // past W, or near fp32's end although its page's scale is small
-                bool moved = fmaxf(pm * (vscale * pow2(254 - ub[c])), pm * 0x1p-70f) > 0x1p30f;
+                for (int i = 1; i < 16; ++i) top = fmaxf(top, sc[i]);
+                // log2 of the lane's largest weight, rounded up, against m
+                const float vexp = (float)(biased_exp(vscale) - 126);
+                bool moved = fmaxf(top - m[c] + vexp - (float)(ub[c] - 127), top - m[c] - 70.0f) > 30.0f;
                 if (__ballot(moved) != 0 || since == 1024) {  // uniform
-                    const float f0 = pow2(ub[c]) * digit_w;
                     moved = max_xor32(max_xor16(moved ? 1.0f : 0.0f)) > 0.0f;  // over the column
-                    float top = -INFINITY;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float sc = quad_sum((float)s[c][i >> 2][i & 3] * sw);
-                        if (i < seen) top = fmaxf(top, sc);
-                    }
-                    top = max_xor32(max_xor16(top));
-                    const float mn = moved ? fmaxf(m[c], top) : m[c];
+                    const float ctop = max_xor32(max_xor16(top));
+                    const float mn = moved ? fmaxf(m[c], ctop) : m[c];
                     const float f = moved ? exp2_sm(m[c] - mn) : 1.0f;
+                    if (since > 0) {
+                        flush(c, f);
 #pragma unroll
-                    for (int j = 0; j < JB; ++j) {
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) of[c][j][r] = fmaf((float)acc[c][j][r], f0, of[c][j][r]) * f;
-                        acc[c][j] = i32x4{0, 0, 0, 0};
+                        for (int j = 0; j < JB; ++j) acc[c][j] = i32x4{0, 0, 0, 0};
                     }
                     l[c] *= f;
                     m[c] = mn;
-                    weights(mn);
-                    pm = p[0];
-#pragma unroll
-                    for (int i = 1; i < 16; ++i) pm = fmaxf(pm, p[i]);
-                    const float wm = max_xor32(max_xor16(pm * vscale));
                     // W = 8 times the power of two above the tile's largest weight
-                    if (moved) ub[c] = min(max(biased_exp(wm) + 4 - 30, 1), 224);
+                    const float wm = max_xor32(max_xor16(top - mn + vexp));
+                    if (moved) ub[c] = (int)fminf(fmaxf(ceilf(wm) + (127.0f + 3.0f - 30.0f), 1.0f), 224.0f);
                 }
+                float p[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) p[i] = exp2_sm(sc[i] - m[c]);
                 const float wc = vscale * pow2(254 - ub[c]);
                 float sum = 0.0f;
 #pragma unroll
@@ -276,22 +297,12 @@ __global__ __launch_bounds__(64 * NW) void kv8_decode_kernel(Kv8Attn a, int grou
             load_v();
             since = since == 1024 ? 1 : since + 1;
             if (!more) break;
-            tile += NW;
+            tile += TW;
         }
     }
-    // fp32 sums, digits joined: lane (col, q4) holds channels 16 j + 4 q4 + r of head col / 4
 #pragma unroll
     for (int c = 0; c < NT; ++c) {
-        const float f0 = pow2(ub[c]) * digit_w;
-#pragma unroll
-        for (int j = 0; j < JB; ++j) {
-            float4 o;
-            o.x = quad_sum(fmaf((float)acc[c][j][0], f0, of[c][j][0]));
-            o.y = quad_sum(fmaf((float)acc[c][j][1], f0, of[c][j][1]));
-            o.z = quad_sum(fmaf((float)acc[c][j][2], f0, of[c][j][2]));
-            o.w = quad_sum(fmaf((float)acc[c][j][3], f0, of[c][j][3]));
-            if (digit == 0) *reinterpret_cast<float4*>(&sh_o[wid][4 * c + (col >> 2)][16 * j + 4 * q4]) = o;
-        }
+        flush(c, 1.0f);
         const float lt = sum_xor32(sum_xor16(l[c]));
         if (digit == 0 && q4 == 0) {
             sh_m[wid][4 * c + (col >> 2)] = m[c];
@@ -300,17 +311,17 @@ __global__ __launch_bounds__(64 * NW) void kv8_decode_kernel(Kv8Attn a, int grou
     }
     __syncthreads();
     for (int i = threadIdx.x; i < gn * D; i += 64 * NW) {
-        const int g = i / D, dim = i % D;
+        const int g = i / D, dim = i % D, gw = g % (4 * NT), w0 = g / (4 * NT);
         float mm = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) mm = fmaxf(mm, sh_m[w][g]);
+        for (int w = w0; w < NW; w += HT) mm = fmaxf(mm, sh_m[w][gw]);
         float o = 0.0f, lt = 0.0f;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) {
-            const float lw = sh_l[w][g];
-            const float f = lw == 0.0f ? 0.0f : exp2_sm(sh_m[w][g] - mm);  // a wave without keys; NaN stays
+        for (int w = w0; w < NW; w += HT) {
+            const float lw = sh_l[w][gw];
+            const float f = lw == 0.0f ? 0.0f : exp2_sm(sh_m[w][gw] - mm);  // a wave without keys; NaN stays
             lt = fmaf(lw, f, lt);
-            o = fmaf(sh_o[w][g][dim], f, o);
+            o = fmaf(sh_o[w][gw][dim], f, o);
         }
         const size_t row = (size_t)b * a.H_q + (size_t)h * G + g0 + g;
         if (a.splits == 1) {
@@ -326,50 +337,61 @@ __global__ __launch_bounds__(64 * NW) void kv8_decode_kernel(Kv8Attn a, int grou
     }
 }
 
-// Joins the splits of one (sequence, query head) with one wave, in split order.
+// Joins the splits of one (sequence, query head): a workgroup's wave w has
+// splits w, w + 4, .., all of whose rows are requested at once; then the waves'
+// sums in wave order.  D threads a wave are D / 64 channels a lane.
 template <int D>
-__global__ __launch_bounds__(256) void kv8_merge_kernel(int rows, int S, const float* __restrict__ ws,
-                                                        float* __restrict__ O) {
-    const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (row >= rows) return;
+__global__ __launch_bounds__(256) void kv8_merge_kernel(int S, const float* __restrict__ ws, float* __restrict__ O) {
+    constexpr int C = D / 64, MOST = IE_KV8_MAX_SPLITS / 4;
+    __shared__ float sh[4][D];
+    const int row = blockIdx.x, wid = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const float* w = ws + (size_t)row * S * (D + 2);
     const int sl = min(lane, S - 1);
-    const float ms = w[(size_t)sl * (D + 2) + D], ls = lane < S ? w[(size_t)sl * (D + 2) + D + 1] : 0.0f;
+    const float ms = w[(size_t)sl * (D + 2) + D];
+    float ls = w[(size_t)sl * (D + 2) + D + 1];
+    float x[MOST][C];
+#pragma unroll
+    for (int u = 0; u < MOST; ++u)
+        if (wid + 4 * u < S)  // uniform
+#pragma unroll
+            for (int i = 0; i < C; ++i) x[u][i] = w[(size_t)(wid + 4 * u) * (D + 2) + 64 * i + lane];
+    if (lane >= S) ls = 0.0f;
     const float mm = wave_max(ls == 0.0f ? -INFINITY : ms);
     const float f = ls == 0.0f ? 0.0f : exp2_sm(ms - mm);
     const float l = wave_sum(ls * f);
-    float o[D / 64];
+    float o[C];
 #pragma unroll
-    for (int i = 0; i < D / 64; ++i) o[i] = 0.0f;
-    for (int s0 = 0; s0 < S; s0 += 8) {
-        float x[8][D / 64];
+    for (int i = 0; i < C; ++i) o[i] = 0.0f;
 #pragma unroll
-        for (int u = 0; u < 8; ++u)
+    for (int u = 0; u < MOST; ++u)
+        if (wid + 4 * u < S) {
+            const float fu = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), wid + 4 * u));
 #pragma unroll
-            for (int i = 0; i < D / 64; ++i) x[u][i] = w[(size_t)min(s0 + u, S - 1) * (D + 2) + 64 * i + lane];
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            const float fu = __shfl(f, (s0 + u) & 63, 64);  // 0 past the last split
-#pragma unroll
-            for (int i = 0; i < D / 64; ++i) o[i] = fmaf(x[u][i], s0 + u < S ? fu : 0.0f, o[i]);
+            for (int i = 0; i < C; ++i) o[i] = fmaf(x[u][i], fu, o[i]);
         }
-    }
 #pragma unroll
-    for (int i = 0; i < D / 64; ++i) O[(size_t)row * D + 64 * i + lane] = l == 0.0f ? 0.0f : o[i] / l;
+    for (int i = 0; i < C; ++i) sh[wid][64 * i + lane] = o[i];
+    __syncthreads();
+    if (threadIdx.x < D) {
+        const float sum = sh[0][threadIdx.x] + sh[1][threadIdx.x] + sh[2][threadIdx.x] + sh[3][threadIdx.x];
+        O[(size_t)row * D + threadIdx.x] = l == 0.0f ? 0.0f : sum / l;
+    }
 }
 
 template <int D>
 void launch(const Kv8Attn& a, hipStream_t s) {
     const int G = a.H_q / a.c.H;
     const float qscale = (1.0f / sqrtf((float)D)) * 1.4426950408889634f;
-    const int heads = G <= 4 ? 4 : 8, groups = (G + heads - 1) / heads;
+    const int heads = G <= 4 ? 4 : G <= 8 ? 8 : 16, groups = (G + heads - 1) / heads;
     const unsigned grid = (unsigned)a.B * a.c.H * groups * a.splits;
-    if (G <= 4)
-        kv8_decode_kernel<D, 1, 4><<<grid, 256, 0, s>>>(a, groups, qscale);
+    if (heads == 4)
+        kv8_decode_kernel<D, 1, 1><<<grid, 64 * NW, 0, s>>>(a, groups, qscale);
+    else if (heads == 8)
+        kv8_decode_kernel<D, 2, 1><<<grid, 64 * NW, 0, s>>>(a, groups, qscale);
     else
-        kv8_decode_kernel<D, 2, 4><<<grid, 256, 0, s>>>(a, groups, qscale);
+        kv8_decode_kernel<D, 2, 2><<<grid, 64 * NW, 0, s>>>(a, groups, qscale);
     if (a.splits > 1)
-        kv8_merge_kernel<D><<<(a.B * a.H_q + 3) / 4, 256, 0, s>>>(a.B * a.H_q, a.splits, a.ws, a.O);
+        kv8_merge_kernel<D><<<a.B * a.H_q, 256, 0, s>>>(a.splits, a.ws, a.O);
 }
 
 }  // namespace
