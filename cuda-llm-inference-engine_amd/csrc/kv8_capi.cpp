@@ -194,9 +194,18 @@ int ie_decode_attn_kv8(int B, int H_q, int H_kv, int d, const float* Q, const vo
     return ie::check_launch(fn);
 }
 
+size_t ie_prefill_kv8_workspace_bytes(int B, int P, int H_q, int H_kv, int d, int start_pos) {
+    if (B <= 0 || P <= 0 || H_kv <= 0 || H_q <= 0 || H_q % H_kv || d <= 0 || start_pos < 0 ||
+        (long long)start_pos + P > kMaxContext || (long long)((P + 15) / 16) * H_q * B > kMaxGroups)
+        return 0;
+    const int S = ie::kv8_prefill_splits(B, P, H_q, H_kv, start_pos + P);
+    return S > 1 ? (size_t)B * P * H_q * S * (d + 2) * sizeof(float) : 0;
+}
+
 int ie_prefill_attn_kv8(int B, int P, int H_q, int H_kv, int d, const float* Q, const void* k_cache,
                         const void* v_cache, const float* k_scales, const float* v_scales, const int* block_table,
-                        int num_blocks_per_seq, int block_size, int start_pos, float* O, ie_stream_t stream) {
+                        int num_blocks_per_seq, int block_size, int start_pos, float* O, float* workspace,
+                        size_t workspace_bytes, ie_stream_t stream) {
     const char* fn = "prefill_attn_kv8";
     int st = check_layout(fn, B, H_kv, d, block_size, num_blocks_per_seq);
     if (st != IE_OK) return st;
@@ -214,7 +223,15 @@ int ie_prefill_attn_kv8(int B, int P, int H_q, int H_kv, int d, const float* Q, 
     ie::Kv8Attn a{};
     a.B = B; a.P = P; a.H_q = H_q; a.Q = Q; a.q_ld = H_q * d;
     a.c = cache(k_cache, v_cache, k_scales, v_scales, block_table, num_blocks_per_seq, H_kv, d, block_size);
-    a.start = start_pos; a.max_ctx = start_pos + P; a.O = O; a.splits = 1;
+    a.start = start_pos; a.max_ctx = start_pos + P; a.O = O;
+    a.splits = workspace ? ie::kv8_prefill_splits(B, P, H_q, H_kv, start_pos + P) : 1;
+    if (a.splits > 1) {
+        const size_t need = ie_prefill_kv8_workspace_bytes(B, P, H_q, H_kv, d, start_pos);
+        if (!aligned(workspace, 8)) return fail(IE_ERR_INVALID, "%s: workspace must be 8-byte aligned", fn);
+        if (workspace_bytes < need)
+            return fail(IE_ERR_WORKSPACE, "%s: workspace %zu bytes < %zu for %d splits", fn, workspace_bytes, need, a.splits);
+        a.ws = workspace;
+    }
     ie::launch_prefill_attn_kv8(a, (hipStream_t)stream);
     return ie::check_launch(fn);
 }

@@ -96,7 +96,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? (NT == 1 ? 4 : 3) : (NT == 1 ? 3
     const int G = a.H_q / H, g0 = hg * HEADS, gn = min(HEADS, G - g0);
     const int n = max(0, min(a.lens[b], a.max_ctx));
     const int tiles = (n + kTile - 1) / kTile;
-    const int t0 = (int)((long long)tiles * split / a.splits), t1 = (int)((long long)tiles * (split + 1) / a.splits);
+    const int t0 = (int)((unsigned)tiles * split / (unsigned)a.splits), t1 = (int)((unsigned)tiles * (split + 1) / (unsigned)a.splits);
 
     const int col = lane & 15, q4 = lane >> 4, digit = lane & 3;
     const int lgg = a.c.bs_log2 - 4;  // 16-token groups a page, log2
@@ -390,11 +390,17 @@ void launch(const Kv8Attn& a, hipStream_t s) {
         kv8_decode_kernel<D, 2, 1><<<grid, 64 * NW, 0, s>>>(a, groups, qscale);
     else
         kv8_decode_kernel<D, 2, 2><<<grid, 64 * NW, 0, s>>>(a, groups, qscale);
-    if (a.splits > 1)
-        kv8_merge_kernel<D><<<a.B * a.H_q, 256, 0, s>>>(a.splits, a.ws, a.O);
+    if (a.splits > 1) launch_kv8_merge(D, a.B * a.H_q, a.splits, a.ws, a.O, s);
 }
 
 }  // namespace
+
+void launch_kv8_merge(int d, int rows, int splits, const float* ws, float* O, hipStream_t s) {
+    if (d == 64)
+        kv8_merge_kernel<64><<<rows, 256, 0, s>>>(splits, ws, O);
+    else
+        kv8_merge_kernel<128><<<rows, 256, 0, s>>>(splits, ws, O);
+}
 
 void launch_decode_attn_kv8(const Kv8Attn& a, hipStream_t s) {
     if (a.c.d == 64)

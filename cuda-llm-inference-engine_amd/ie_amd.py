@@ -63,7 +63,8 @@ KV8_SIGNATURES = {
     "ie_kv8_cache_read": (_I, [_I, _I, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P]),
     "ie_decode_kv8_num_splits": (_I, [_I, _I, _I, _I, _I, _I]),
     "ie_decode_attn_kv8": (_I, [_I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P, _Z, _I, _P]),
-    "ie_prefill_attn_kv8": (_I, [_I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P]),
+    "ie_prefill_kv8_workspace_bytes": (_Z, [_I, _I, _I, _I, _I, _I]),
+    "ie_prefill_attn_kv8": (_I, [_I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P, _Z, _P]),
 }
 KV8_MAX_SPLITS = 64
 
@@ -559,9 +560,10 @@ def decode_attn_kv8(Q, cache, block_table, context_lens, max_ctx, splits=0, out=
     return out
 
 
-def prefill_attn_kv8(Q, cache, block_table, start_pos, out=None, stream=None):
+def prefill_attn_kv8(Q, cache, block_table, start_pos, out=None, workspace=None, stream=None):
     """Q [B, P, H_q, d] fp32, token t at position start_pos + t with its rows
-    cached; returns causal O [B, P, H_q, d]."""
+    cached; returns causal O [B, P, H_q, d].  workspace: fp32, at least
+    ie_prefill_kv8_workspace_bytes (made here where the call has use for one)."""
     H, bs, d = _kv8("prefill_attn_kv8", cache, block_table)
     B, P, H_q, dq = Q.shape
     if dq != d or block_table.shape[0] != B:
@@ -573,9 +575,17 @@ def prefill_attn_kv8(Q, cache, block_table, start_pos, out=None, stream=None):
     elif out.shape != Q.shape:
         raise ValueError("prefill_attn_kv8: out needs Q's shape")
     _check("prefill_attn_kv8", _f32, (Q, out))
+    if workspace is None:
+        need = call("ie_prefill_kv8_workspace_bytes", B, P, H_q, H, d, start_pos)
+        if need:
+            workspace = _empty(need // 4, dtype=_f32, device=Q.device)
+            _made(stream, workspace)
+    else:
+        _check("prefill_attn_kv8", _f32, (workspace,))
     k, v, ks, vs = cache
     check("ie_prefill_attn_kv8", B, P, H_q, H, d, Q.data_ptr(), k.data_ptr(), v.data_ptr(), ks.data_ptr(),
-          vs.data_ptr(), block_table.data_ptr(), block_table.shape[1], bs, start_pos, out.data_ptr(), _stream(stream))
+          vs.data_ptr(), block_table.data_ptr(), block_table.shape[1], bs, start_pos, out.data_ptr(), _ptr(workspace),
+          0 if workspace is None else 4 * workspace.numel(), _stream(stream))
     return out
 
 

@@ -92,14 +92,22 @@ int ie_decode_attn_kv8(int B, int H_q, int H_kv, int d, const float* Q, const vo
                        int block_size, int num_blocks_per_seq, float* O, float* workspace,
                        size_t workspace_bytes, int num_splits, ie_stream_t stream);
 
+/* Bytes of workspace with which ie_prefill_attn_kv8 can split the context of a
+ * call of this size (few rows behind a long one); 0 where it would not. */
+size_t ie_prefill_kv8_workspace_bytes(int B, int P, int H_q, int H_kv, int d, int start_pos);
+
 /* Causal attention of a prompt chunk over the cache, as ie_prefill_attn: Q, O
  * [B, P, H_q, d] fp32, token t of each sequence at position start_pos + t, its
  * rows cached already; it attends to positions 0 .. start_pos + t.  H_q any
- * multiple of H_kv, d in {64, 128}.  O must not overlap Q. */
+ * multiple of H_kv, d in {64, 128}.  O must not overlap Q.  With a workspace
+ * NULL the context is not split; otherwise workspace_bytes must cover
+ * ie_prefill_kv8_workspace_bytes of the call.  A repeated call repeats its
+ * bits; those of a token may depend on the chunk and batch it came in. */
 int ie_prefill_attn_kv8(int B, int P, int H_q, int H_kv, int d, const float* Q, const void* k_cache,
                         const void* v_cache, const float* k_scales, const float* v_scales,
                         const int* block_table, int num_blocks_per_seq, int block_size,
-                        int start_pos, float* O, ie_stream_t stream);
+                        int start_pos, float* O, float* workspace, size_t workspace_bytes,
+                        ie_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -43,8 +43,9 @@ def decode(ie, B=1, Hq=4, H=2, d=64, Q=P, k=P, v=P, ks=P, vs=P, table=P, lens=P,
     return ie.call("ie_decode_attn_kv8", B, Hq, H, d, Q, k, v, ks, vs, table, lens, mx, bs, nbps, O, ws, wsb, splits, None)
 
 
-def prompt(ie, B=1, n=4, Hq=4, H=2, d=64, Q=P, k=P, v=P, ks=P, vs=P, table=P, nbps=4, bs=16, start=0, O=1 << 20):
-    return ie.call("ie_prefill_attn_kv8", B, n, Hq, H, d, Q, k, v, ks, vs, table, nbps, bs, start, O, None)
+def prompt(ie, B=1, n=4, Hq=4, H=2, d=64, Q=P, k=P, v=P, ks=P, vs=P, table=P, nbps=4, bs=16, start=0, O=1 << 20,
+           ws=None, wsb=0):
+    return ie.call("ie_prefill_attn_kv8", B, n, Hq, H, d, Q, k, v, ks, vs, table, nbps, bs, start, O, ws, wsb, None)
 
 
 INVALID, UNSUPPORTED, WORKSPACE = 1, 2, 3
@@ -99,6 +100,18 @@ def test_num_splits(ie):
     for ctx in (1, 64, 1000, 8192, 1 << 20):
         for B in (1, 8, 64):
             assert 1 <= f(B, 32, 8, 128, ctx) <= min(ie.KV8_MAX_SPLITS, -(-ctx // 64))
+
+
+def test_prompt_workspace(ie):
+    """Few rows behind a long context can be split, and then the workspace has to hold it."""
+    f = ie.call
+    need = f("ie_prefill_kv8_workspace_bytes", 1, 4, 8, 2, 64, 8000)
+    assert need > 0 and need % (4 * 8 * 66 * 4) == 0
+    assert prompt(ie, n=4, Hq=8, start=8000, nbps=1000, ws=P, wsb=need - 1) == WORKSPACE
+    assert prompt(ie, n=4, Hq=8, start=8000, nbps=1000, ws=P + 4, wsb=need) == INVALID
+    assert f("ie_prefill_kv8_workspace_bytes", 4, 2048, 32, 8, 128, 0) == 0
+    for bad in ((0, 4, 8, 2, 64, 0), (1, 0, 8, 2, 64, 0), (1, 4, 7, 2, 64, 0), (1, 4, 8, 2, 64, -1), (1, 4, 8, 2, 64, 2**30)):
+        assert f("ie_prefill_kv8_workspace_bytes", *bad) == 0
 
 
 def test_oracle_rule_bounds():
