@@ -21,7 +21,13 @@
 // bit, and the least of them is the bound.  After the first tile no wave waits
 // for another before the row's end; then the lists are ranked by counting.
 //
-// Bound by HBM for many rows and by one row's chain of round trips for few.
+// Many rows are bound by HBM: 2048 x 50257, k = 20 92 us, 4.5 TB/s (a copy of 1 GiB
+// moves 4.7); k = 0 87 us.  (With the row held in registers, 25 words a thread,
+// 145 us: two rows a CU, which load and compute in step.)  Few rows are bound by
+// one wave's instructions and round trips: 8 x 50257, k = 5 12.5 us, of them 4 the
+// join's; loading a tile ahead changes nothing, 512 or 1024 threads a row gain
+// nothing (8 rows in 8 parts 13.2 and 22.5 against 13.9 us, 2048 rows 126 and 323
+// against 92).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -140,15 +146,14 @@ struct Candidates {
         bound = fmaxf(bound, key_value((uint32_t)(least >> 32)));
     }
 
-    // Adds the lanes' elements f of index i where `ok` and f reaches the bound.
-    __device__ __forceinline__ void add(float f, int i, bool ok, int k, int lane) {
-        if (__ballot(ok && f >= bound) == 0) return;
-        if (cnt + 64 > kList) cut(k, lane);
+    // Adds the lanes' elements f of index i where `ok` and f reaches the bound;
+    // there is room for 64 more.
+    __device__ __forceinline__ void add(float f, int i, bool ok, int lane) {
         const uint64_t mask = __ballot(ok && f >= bound);
+        if (mask == 0) return;  // uniform
         if (ok && f >= bound) list[cnt + __popcll(mask & ((1ull << lane) - 1))] = packed(f, i);
         cnt += __popcll(mask);
     }
-
 };
 
 // The first 20 bits of the need-th largest of the lanes' keys, need <= 64.
@@ -204,7 +209,7 @@ __global__ __launch_bounds__(T, 8) void logprobs_kernel(LogprobsArgs a, int part
     int ahead = __popcll(__ballot(xv > (xi < t ? before : xt))), above = __popcll(__ballot(lowest && xv > xt && xi < t));
 
     Candidates cand{pk + wid * kList};
-    if (k > 0) cand.add(xv, xi, xi < n, k, lane);  // (at most six, listed before there is a bound)
+    if (k > 0) cand.add(xv, xi, xi < n, lane);  // (at most six, listed before there is a bound)
 
     // Each thread's maximum m, and against it: tops elements equal to it, e = sum
     // e^d and w = sum e^d d of the others.
@@ -268,14 +273,31 @@ __global__ __launch_bounds__(T, 8) void logprobs_kernel(LogprobsArgs a, int part
             for (int i = 1; i < W; ++i) b = min(b, said[i]);
             if (b > order_key(-INFINITY)) cand.bound = fmaxf(cand.bound, key_value(b));
         }
+        int most_new = 0;
 #pragma unroll
-        for (int q = 0; q < kWords; ++q) {
-            if (__ballot(most[q] >= cand.bound) == 0) continue;  // uniform
-            const int c = c0 + q * T + tid, i = 4 * c + head;
-            cand.add(v[q].x, i, c < w1, k, lane);
-            cand.add(v[q].y, i + 1, c < w1, k, lane);
-            cand.add(v[q].z, i + 2, c < w1, k, lane);
-            cand.add(v[q].w, i + 3, c < w1, k, lane);
+        for (int q = 0; q < kWords; ++q) most_new += 4 * __popcll(__ballot(most[q] >= cand.bound));
+        if (most_new == 0) continue;
+        if (cand.cnt + most_new <= kList) {
+#pragma unroll
+            for (int q = 0; q < kWords; ++q) {
+                if (__ballot(most[q] >= cand.bound) == 0) continue;
+                const int c = c0 + q * T + tid, i = 4 * c + head;
+                cand.add(v[q].x, i, c < w1, lane);
+                cand.add(v[q].y, i + 1, c < w1, lane);
+                cand.add(v[q].z, i + 2, c < w1, lane);
+                cand.add(v[q].w, i + 3, c < w1, lane);
+            }
+        } else {  // word by word, read again, with a cut wherever one might not fit
+#pragma unroll 1
+            for (int q = 0; q < kWords; ++q) {
+                if (cand.cnt + 256 > kList) cand.cut(k, lane);
+                const int c = c0 + q * T + tid, i = 4 * c + head;
+                const float4 u = base[min(c, w1 - 1)];
+                cand.add(u.x, i, c < w1, lane);
+                cand.add(u.y, i + 1, c < w1, lane);
+                cand.add(u.z, i + 2, c < w1, lane);
+                cand.add(u.w, i + 3, c < w1, lane);
+            }
         }
     }
     if (asked && tw >= w0 && tw < w1 && wid == 0)  // the target's own word
@@ -290,7 +312,7 @@ __global__ __launch_bounds__(T, 8) void logprobs_kernel(LogprobsArgs a, int part
         if (part == parts - 1) mine += max(t - (4 * words + head), 0);
         ahead += (wid == 0 ? mine : 0) - above;
     }
-    if (k > 128 / W && cand.cnt > 128) cand.cut(k, lane);
+    if (cand.cnt > 128) cand.cut(k, lane);
 
     // the threads' sums against the row's maximum
     float rm = m;
@@ -446,13 +468,18 @@ int row_words(int n) { return std::max(n / 4, 1); }
 
 }  // namespace
 
+// A row's parts: four workgroups a CU, where at least four tiles of one workgroup
+// are shared out (the second launch costs about four tiles' time) and the join
+// ranks at most about 160 candidates.  50257 logits, k = 5: 8 rows 26.7 us in one
+// part, 13.9 in 8, 12.5 in 16; 128 rows 29.7, 20.1 in 8; 512 rows 35.7, 35.1 in 2;
+// k = 20: 16 rows 30.5, 16.5 in 8, 21.3 in 16.  64 x 8000, k = 5 (two tiles): 10.6,
+// 12.0 in 2.
 int logprobs_parts(int rows, int n, int k) {
-    int p = 256 / rows;                        // a workgroup a CU
-    p = std::min(p, row_words(n) / kWide);     // a word a thread
-    if (k > 0) p = std::min(p, 512 / k);       // candidates to join
-    const char* e = getenv("IE_P");
-    if (e) p = atoi(e);
-    return std::min(std::max(p, 1), kMostParts);
+    const int words = row_words(n);
+    if (words < 4 * kWide * kWords - kWide) return 1;
+    int p = std::min(1024 / rows, kMostParts);
+    if (k > 0) p = std::min(p, 160 / k);
+    return std::max(p, 1);
 }
 
 void launch_token_logprobs(const LogprobsArgs& a, hipStream_t s) {
