@@ -1,15 +1,19 @@
 // kv8_cache.hip — rows into and out of the 8-bit paged KV cache
 // (include/ie_kv8.h has the layout and the rule that scales follow).
 //
-// A page of one head is cut into tiles of 16 tokens x 64 channels, one wave
-// (or T tiles of one wave) each, so a tile's codes are 1 KB that the wave
-// stores as one 16-byte word a lane:
-//   K tile (rows of d bytes): lane l holds token l / 4, channels 16 (l % 4) ..
-//   V tile ([channel][16 tokens]): lane l holds channel l of all 16 tokens
-// and the fp32 rows are read as 64 contiguous bytes a lane (K) or 256 a wave
-// (V).  A workgroup holds all tiles of one (sequence, page, head) of K or of
-// V in registers, so the page's maximum, its codes and (where the scale had to
-// grow) the earlier rows' new codes come from one pass over the data.
+// A page of one head is cut into tiles of 16 tokens x 64 channels, one wave (or T
+// tiles of one wave) each.  Lane l holds tokens 4 (l / 16) .. + 3, channels 4 (l %
+// 16) .. + 3: fp32 rows move as 256 contiguous bytes for each of four rows an
+// instruction, K codes as one word (4 channels) a row, V codes as one word (4
+// tokens) a channel.  A workgroup holds all tiles of one (sequence, page, head)
+// of K or of V in registers, so the page's maximum, its codes and (where the
+// scale had to grow) the earlier rows' new codes come from one pass over the data.
+//
+// Bound by HBM: 4 x 2000 rows of 8 x 128, K and V (65.5 MB in, 16.4 out) written in
+// 18.8 us, 4.4 TB/s, and read back in 16.5, 5.0 TB/s (a copy of 1 GiB moves 4.7).
+// The maximum goes over the wave by DPP and lane swaps: by six LDS permutes, with
+// 16-byte words of codes a lane (64-byte pieces of fp32 rows an instruction), the
+// write took 25.5 us and the read 20.8.
 #include <algorithm>
 
 #include "device_util.h"
@@ -24,6 +28,18 @@ __device__ __forceinline__ uint32_t fbits(float x) { return __builtin_bit_cast(u
 __device__ __forceinline__ float bitsf(uint32_t x) { return __builtin_bit_cast(float, x); }
 // Larger of two values >= +0, where NaN is the largest.
 __device__ __forceinline__ float max_nan(float a, float b) { return bitsf(max(fbits(a), fbits(b))); }
+// Largest over the wave, in every lane.
+__device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
+    v = max(v, (uint32_t)dpp_row_ror<8>((int)v));
+    v = max(v, (uint32_t)dpp_row_ror<4>((int)v));
+    v = max(v, (uint32_t)dpp_row_ror<2>((int)v));
+    v = max(v, (uint32_t)dpp_row_ror<1>((int)v));
+    float a, b;
+    pair16(bitsf(v), a, b);
+    v = max(fbits(a), fbits(b));
+    pair32(bitsf(v), a, b);
+    return max(fbits(a), fbits(b));
+}
 // rint as an int; NaN gives 0.  |x| <= 127 * (1 + 2^-22) here: need / scale <= 1.
 __device__ __forceinline__ int code(float x) { return (int)rintf(x); }
 __device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
@@ -31,14 +47,14 @@ __device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
 }
 __device__ __forceinline__ int byte_of(uint32_t w, int i) { return (int)(int8_t)(w >> (8 * i)); }
 
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-// A lane's 16-byte word of tile t of a page.
+// Word j of a lane's four in tile t of a page: K row 4 (lane / 16) + j, V channel
+// 4 (lane % 16) + j.
 template <int D>
-__device__ __forceinline__ int word_of(int t, bool is_v, int lane) {
+__device__ __forceinline__ int word_of(int t, bool is_v, int lane, int j) {
     constexpr int HALVES = D / 64;
-    const int c0 = t % HALVES * 64;
-    return t / HALVES * D + (is_v ? c0 + lane : (lane >> 2) * (D / 16) + c0 / 16 + (lane & 3));
+    const int c = t % HALVES * 64 + 4 * (lane & 15), r = 4 * (lane >> 4);
+    return t / HALVES * (4 * D) + (is_v ? (c + j) * 4 + r / 4 : ((r + j) * D + c) / 4);
 }
 
 // blockIdx.x = ((b * npages + page) * H + h) * 2 + (K or V)
@@ -64,40 +80,34 @@ __global__ __launch_bounds__(1024) void kv8_write_kernel(Kv8Write a, int npages)
     const int lp = (start >> lg) + j, page0 = lp << lg;
     const int r0 = max(start - page0, 0), r1 = min(start + a.P - page0, bs);  // rows written here
     const size_t pair = (size_t)a.c.table[(size_t)b * a.c.nbps + lp] * a.c.H + h;
-    int8_t* codes = (is_v ? a.c.v : a.c.k) + pair * ((size_t)bs * D);
+    uint32_t* codes = reinterpret_cast<uint32_t*>((is_v ? a.c.v : a.c.k) + pair * ((size_t)bs * D));
     float* scale_at = (is_v ? a.c.vs : a.c.ks) + pair;
     const float* src = (is_v ? a.V : a.K) + (size_t)b * a.P * a.ld + (size_t)h * D;
 
-    float x[T][16];
-    u32x4 was[T];
+    float x[T][4][4];  // [row][channel]
+    uint32_t was[T][4];
     uint32_t mx = 0;
 #pragma unroll
     for (int i = 0; i < T; ++i) {
         const int t = wid * T + i, row0 = (t / HALVES) * 16, c0 = (t % HALVES) * 64;
-        if (is_v) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int row = row0 + r;
-                x[i][r] = row >= r0 && row < r1 ? src[(size_t)(page0 + row - start) * a.ld + c0 + lane] : 0.0f;
-            }
-        } else {
-            const int row = row0 + (lane >> 2);
-            const bool fresh = row >= r0 && row < r1;
-            const float4* p = reinterpret_cast<const float4*>(src + (size_t)(fresh ? page0 + row - start : 0) * a.ld +
-                                                              c0 + (lane & 3) * 16);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const float4 v = fresh ? p[q] : make_float4(0.f, 0.f, 0.f, 0.f);
-                x[i][4 * q] = v.x; x[i][4 * q + 1] = v.y; x[i][4 * q + 2] = v.z; x[i][4 * q + 3] = v.w;
-            }
+        for (int r = 0; r < 4; ++r) {
+            const int row = row0 + 4 * (lane >> 4) + r;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (row >= r0 && row < r1)
+                v = *reinterpret_cast<const float4*>(src + (size_t)(page0 + row - start) * a.ld + c0 + 4 * (lane & 15));
+            x[i][r][0] = v.x; x[i][r][1] = v.y; x[i][r][2] = v.z; x[i][r][3] = v.w;
         }
-        // the bytes that this call does not write anew
-        if (row0 < r0 || row0 + 16 > r1) was[i] = reinterpret_cast<const u32x4*>(codes)[word_of<D>(t, is_v, lane)];
+        // the bytes beside the written ones; a tile without those is read only if the scale grows
+        if ((row0 < r0 || row0 + 16 > r1) && row0 + 16 > r0 && row0 < r1)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) mx = max(mx, fbits(x[i][e]) & 0x7fffffffu);
+            for (int k = 0; k < 4; ++k) was[i][k] = codes[word_of<D>(t, is_v, lane, k)];
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) mx = max(mx, fbits(x[i][r][c]) & 0x7fffffffu);
     }
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, o, 64));
+    mx = wave_umax(mx);
     // One wave reads the old scale, so that it is read before it is replaced.
     if (wid == 0 && lane == 0) had_sh = r0 > 0 ? *scale_at : 0.0f;
     if (lane == 0) wave_mx[wid] = mx;
@@ -114,23 +124,24 @@ __global__ __launch_bounds__(1024) void kv8_write_kernel(Kv8Write a, int npages)
     for (int i = 0; i < T; ++i) {
         const int t = wid * T + i, row0 = (t / HALVES) * 16;
         if (row0 >= r1 || (row0 + 16 <= r0 && !grew)) continue;  // nothing of this tile changes (uniform)
-        u32x4 out;
         const bool whole = row0 >= r0 && row0 + 16 <= r1;
+        if (row0 + 16 <= r0)
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+            for (int k = 0; k < 4; ++k) was[i][k] = codes[word_of<D>(t, is_v, lane, k)];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
             int q[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int row = row0 + (is_v ? 4 * w + e : lane >> 2);
-                q[e] = code(x[i][4 * w + e] * inv);
+                const int r = is_v ? e : k, row = row0 + 4 * (lane >> 4) + r;
+                q[e] = code((is_v ? x[i][e][k] : x[i][k][e]) * inv);
                 if (!whole) {
-                    const int old = byte_of(was[i][w], e);
+                    const int old = byte_of(was[i][k], e);
                     q[e] = row < r0 ? (grew ? code((float)old * move) : old) : row < r1 ? q[e] : old;
                 }
             }
-            out[w] = pack4(q[0], q[1], q[2], q[3]);
+            codes[word_of<D>(t, is_v, lane, k)] = pack4(q[0], q[1], q[2], q[3]);
         }
-        reinterpret_cast<u32x4*>(codes)[word_of<D>(t, is_v, lane)] = out;
     }
 }
 
@@ -141,7 +152,7 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(Kv8Read a, int groups, un
     const int lane = threadIdx.x & 63;
     unsigned id = blockIdx.x * 4 + (threadIdx.x >> 6);
     if (id >= waves) return;
-    const int c0 = (int)(id % HALVES) * 64;
+    const int half = (int)(id % HALVES);
     id /= HALVES;
     const int h = (int)(id % (unsigned)a.c.H);
     id /= (unsigned)a.c.H;
@@ -153,36 +164,35 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(Kv8Read a, int groups, un
     if (first >= end) return;
     long long lim = (long long)a.c.nbps << lg;
     if (a.lens) lim = min(lim, (long long)a.lens[b]);
-    u32x4 kw = {0, 0, 0, 0}, vw = {0, 0, 0, 0};
+    uint32_t kw[4] = {0, 0, 0, 0}, vw[4] = {0, 0, 0, 0};
     float ks = 0.0f, vs = 0.0f;
     if (first >= 0 && first < lim) {
         const size_t pair = (size_t)a.c.table[(size_t)b * a.c.nbps + (first >> lg)] * H + h;
         const size_t at = pair * ((size_t)D << lg) + (size_t)(first & ((1 << lg) - 1)) * D;
-        kw = reinterpret_cast<const u32x4*>(a.c.k + at)[word_of<D>(c0 / 64, false, lane)];
-        vw = reinterpret_cast<const u32x4*>(a.c.v + at)[word_of<D>(c0 / 64, true, lane)];
+        const uint32_t* kc = reinterpret_cast<const uint32_t*>(a.c.k + at);
+        const uint32_t* vc = reinterpret_cast<const uint32_t*>(a.c.v + at);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            kw[k] = kc[word_of<D>(half, false, lane, k)];
+            vw[k] = vc[word_of<D>(half, true, lane, k)];
+        }
         ks = a.c.ks[pair];
         vs = a.c.vs[pair];
     }
     const size_t row_n = (size_t)H * D;
-    const size_t base = (size_t)b * a.n * row_n + (size_t)h * D + c0;
-    {
-        const long long pos = first + (lane >> 2);
-        if (pos >= start && pos < end) {
-            float4* dst = reinterpret_cast<float4*>(a.K + base + (size_t)(pos - start) * row_n + (lane & 3) * 16);
-            const float s = pos < lim ? ks : 0.0f;
+    const size_t base = (size_t)b * a.n * row_n + (size_t)h * D + half * 64 + 4 * (lane & 15);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const uint32_t w = pos < lim ? kw[q] : 0;
-                dst[q] = make_float4((float)byte_of(w, 0) * s, (float)byte_of(w, 1) * s, (float)byte_of(w, 2) * s,
-                                     (float)byte_of(w, 3) * s);
-            }
-        }
-    }
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        const long long pos = first + r;
-        if (pos >= start && pos < end)
-            a.V[base + (size_t)(pos - start) * row_n + lane] = pos < lim ? (float)byte_of(vw[r / 4], r % 4) * vs : 0.0f;
+    for (int r = 0; r < 4; ++r) {
+        const long long pos = first + 4 * (lane >> 4) + r;
+        if (pos < start || pos >= end) continue;
+        const bool in = pos < lim;
+        const size_t at = base + (size_t)(pos - start) * row_n;
+        // (a row behind the limit is zero whatever its page's scale is)
+        auto value = [&](int q, float s) { return in ? (float)q * s : 0.0f; };
+        *reinterpret_cast<float4*>(a.K + at) = make_float4(value(byte_of(kw[r], 0), ks), value(byte_of(kw[r], 1), ks),
+                                                           value(byte_of(kw[r], 2), ks), value(byte_of(kw[r], 3), ks));
+        *reinterpret_cast<float4*>(a.V + at) = make_float4(value(byte_of(vw[0], r), vs), value(byte_of(vw[1], r), vs),
+                                                           value(byte_of(vw[2], r), vs), value(byte_of(vw[3], r), vs));
     }
 }
 

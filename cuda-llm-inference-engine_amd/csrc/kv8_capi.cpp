@@ -141,19 +141,23 @@ int ie_kv8_cache_read(int B, int n, const int* starts, const int* context_lens, 
 }
 
 int ie_decode_kv8_num_splits(int B, int H_q, int H_kv, int d, int max_context_len, int num_splits) {
-    (void)d;
     if (B <= 0 || H_q <= 0 || H_kv <= 0 || max_context_len <= 0) return 1;
     const int tiles = (int)(((long long)max_context_len + 63) / 64);
     int s = num_splits;
     if (s <= 0) {
         // A workgroup a CU, and a tile at least for each of its four waves; one
-        // split where more would spare a wave fewer than three tiles.
+        // split where more would spare a wave few tiles (about 0.7 us each at
+        // d = 64, 1.3 at 128, against 2 us of the merge and, past 64 workgroups,
+        // the memory they share): 1 x 12 x 64, ctx 1024 6.9 us in one and in four,
+        // 2048 9.6 and 6.9 in eight; 8 x 12 x 64, ctx 2048 9.9 and 10.8 in two, ctx 8000
+        // 30.2, 23.5 in two, 27.4 in three; 1 x (8 x 4) x 128, ctx 1000 10.7 and 8.7 in four.
         const int G = H_q / H_kv, heads = G <= 4 ? 4 : G <= 8 ? 8 : 16;
         const long long units = (long long)B * H_kv * ((G + heads - 1) / heads);
         const int each = (tiles + 3) / 4;
-        s = (int)((256 + units - 1) / units);
-        if (s > each) s = each;
-        if (each - (each + s - 1) / s < 3) s = 1;
+        s = (int)(256 / units);
+        s = s < 1 ? 1 : s > each ? each : s;
+        const int worth = (d <= 64 ? 4 : 3) * (units > 64 ? 2 : 1);
+        if (each - (each + s - 1) / s < worth) s = 1;
     }
     if (s > IE_KV8_MAX_SPLITS) s = IE_KV8_MAX_SPLITS;
     return s < tiles ? s : tiles;

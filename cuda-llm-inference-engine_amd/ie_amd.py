@@ -394,13 +394,9 @@ def top_k_draw(vals, idx, temperature, seed):
 
 
 # ------------------------------------------- 8-bit KV cache, log probabilities
-def _check(what, dtype, tensors):
-    """Contiguous tensors of one type on the current device, or a ValueError."""
-    at = _device_index()
-    for t in tensors:
-        if t.get_device() != at or t.dtype is not dtype or not t.is_contiguous():
-            raise ValueError(f"{what}: needs contiguous {dtype} tensors on cuda:{at}, got {t.dtype} of strides "
-                             f"{tuple(t.stride())} on {t.device}")
+def _refuse(what, *tensors):
+    raise ValueError(f"{what}: needs contiguous tensors on cuda:{_device_index()} of the documented types and shapes, got "
+                     + ", ".join(f"{t.dtype} {tuple(t.shape)} strides {tuple(t.stride())} on {t.device}" for t in tensors))
 
 
 _device_index = None  # () -> index of the current device
@@ -446,22 +442,26 @@ class Kv8Cache(NamedTuple):
         return sum(t.numel() * t.element_size() for t in self)
 
 
+# The wrappers' checks are spelled out flat: an attribute of a tensor costs 50 to
+# 85 ns, a helper call or a loop over tensors as much again, and a decode step's
+# calls are about as long on the GPU as here.
 def _kv8(what, cache, table):
-    """(heads, block size, d) of a cache whose tensors fit each other."""
+    """(heads, block size, d, device) of a cache whose tensors fit each other."""
     if _device_index is None:
         _bind_torch()
     k, v, ks, vs = cache
-    _check(what, _i8, (k, v))
-    _check(what, _f32, (ks, vs))
-    _check(what, _i32, (table,))
+    at = _device_index()
     pages, H, bs, d = k.shape
-    if v.shape != (pages, H, bs // 16, d, 16) or ks.shape != (pages, H) or vs.shape != ks.shape or table.dim() != 2:
-        raise ValueError(f"{what}: cache tensors or block table of wrong shape: {[tuple(t.shape) for t in cache]}, "
-                         f"{tuple(table.shape)}")
-    return H, bs, d
+    if not (k.dtype is _i8 and v.dtype is _i8 and ks.dtype is _f32 and vs.dtype is _f32 and table.dtype is _i32
+            and k.get_device() == at and v.get_device() == at and ks.get_device() == at and vs.get_device() == at
+            and table.get_device() == at and k.is_contiguous() and v.is_contiguous() and ks.is_contiguous()
+            and vs.is_contiguous() and table.is_contiguous() and v.shape == (pages, H, bs // 16, d, 16)
+            and ks.shape == (pages, H) and vs.shape == (pages, H) and table.dim() == 2):
+        _refuse(what, k, v, ks, vs, table)
+    return H, bs, d, at
 
 
-def _kv8_rows(what, K, V, lead, H, d):
+def _kv8_rows(what, K, V, lead, H, d, at):
     """Distance between rows [*lead, H, d] fp32 that may lie apart (the columns
     of a QKV projection) but evenly so."""
     st = K.stride()
@@ -469,7 +469,7 @@ def _kv8_rows(what, K, V, lead, H, d):
         ld = st[len(lead) - 1]
     else:
         ld = st[0] if lead[0] > 1 else H * d
-    at, want = _device_index(), (*lead, H, d)
+    want = (*lead, H, d)
     if (K.shape != want or V.shape != want or K.dtype is not _f32 or V.dtype is not _f32 or K.get_device() != at
             or V.get_device() != at or V.stride() != st or st[-1] != 1 or (H > 1 and st[-2] != d)
             or (len(lead) == 2 and lead[0] > 1 and lead[1] > 1 and st[0] != lead[1] * ld)):
@@ -481,11 +481,11 @@ def _kv8_rows(what, K, V, lead, H, d):
 def kv8_cache_write(K, V, cache, block_table, start_pos, stream=None):
     """Rows K, V [B, P, heads, d] fp32 (views into a QKV projection serve as they
     lie) to positions start_pos .. of the sequences of block_table [B, nbps]."""
-    H, bs, d = _kv8("kv8_cache_write", cache, block_table)
+    H, bs, d, at = _kv8("kv8_cache_write", cache, block_table)
     B, P = K.shape[:2]
     if block_table.shape[0] != B:
         raise ValueError("kv8_cache_write: block_table has other sequences than K")
-    ld = _kv8_rows("kv8_cache_write", K, V, (B, P), H, d) if B * P else H * d
+    ld = _kv8_rows("kv8_cache_write", K, V, (B, P), H, d, at) if B * P else H * d
     k, v, ks, vs = cache
     check("ie_kv8_cache_write", B, P, K.data_ptr(), V.data_ptr(), ld, k.data_ptr(), v.data_ptr(), ks.data_ptr(),
           vs.data_ptr(), block_table.data_ptr(), block_table.shape[1], start_pos, H, d, bs, _stream(stream))
@@ -493,12 +493,12 @@ def kv8_cache_write(K, V, cache, block_table, start_pos, stream=None):
 
 def kv8_cache_append_batch(K, V, cache, block_table, positions, stream=None):
     """One row of each sequence, K, V [B, heads, d], to positions[b] (int32)."""
-    H, bs, d = _kv8("kv8_cache_append_batch", cache, block_table)
+    H, bs, d, at = _kv8("kv8_cache_append_batch", cache, block_table)
     B = K.shape[0]
-    _check("kv8_cache_append_batch", _i32, (positions,))
-    if block_table.shape[0] != B or positions.shape != (B,):
-        raise ValueError("kv8_cache_append_batch: block_table or positions has other sequences than K")
-    ld = _kv8_rows("kv8_cache_append_batch", K, V, (B,), H, d) if B else H * d
+    if (block_table.shape[0] != B or positions.shape != (B,) or positions.dtype is not _i32
+            or positions.get_device() != at or not positions.is_contiguous()):
+        _refuse("kv8_cache_append_batch", K, block_table, positions)
+    ld = _kv8_rows("kv8_cache_append_batch", K, V, (B,), H, d, at) if B else H * d
     k, v, ks, vs = cache
     check("ie_kv8_cache_append_batch", B, K.data_ptr(), V.data_ptr(), ld, k.data_ptr(), v.data_ptr(), ks.data_ptr(),
           vs.data_ptr(), block_table.data_ptr(), block_table.shape[1], positions.data_ptr(), H, d, bs, _stream(stream))
@@ -507,19 +507,19 @@ def kv8_cache_append_batch(K, V, cache, block_table, positions, stream=None):
 def kv8_cache_read(cache, block_table, starts, context_lens, n, out=None, stream=None):
     """(K, V) [B, n, heads, d] fp32: positions starts[b] .. starts[b] + n - 1 of each
     sequence, zeros from context_lens[b] on (None: no limit)."""
-    H, bs, d = _kv8("kv8_cache_read", cache, block_table)
+    H, bs, d, at = _kv8("kv8_cache_read", cache, block_table)
     B = block_table.shape[0]
-    ints = (starts,) if context_lens is None else (starts, context_lens)
-    _check("kv8_cache_read", _i32, ints)
-    if any(t.shape != (B,) for t in ints):
-        raise ValueError("kv8_cache_read: starts or context_lens has other sequences than block_table")
     if out is None:
-        out = tuple(_empty((B, n, H, d), dtype=_f32, device=cache.k.device) for _ in range(2))
+        out = tuple(_empty((B, n, H, d), dtype=_f32, device=cache[0].device) for _ in range(2))
         _made(stream, *out)
     K, V = out
-    _check("kv8_cache_read", _f32, out)
-    if K.shape != (B, n, H, d) or V.shape != K.shape:
-        raise ValueError(f"kv8_cache_read: out needs two tensors of shape {(B, n, H, d)}")
+    want = (B, n, H, d)
+    if not (starts.shape == (B,) and starts.dtype is _i32 and starts.get_device() == at and starts.is_contiguous()
+            and (context_lens is None or (context_lens.shape == (B,) and context_lens.dtype is _i32
+                                          and context_lens.get_device() == at and context_lens.is_contiguous()))
+            and K.shape == want and V.shape == want and K.dtype is _f32 and V.dtype is _f32 and K.get_device() == at
+            and V.get_device() == at and K.is_contiguous() and V.is_contiguous()):
+        _refuse("kv8_cache_read", starts, *(() if context_lens is None else (context_lens,)), K, V)
     k, v, ks, vs = cache
     check("ie_kv8_cache_read", B, n, starts.data_ptr(), _ptr(context_lens), k.data_ptr(), v.data_ptr(), ks.data_ptr(),
           vs.data_ptr(), block_table.data_ptr(), block_table.shape[1], H, d, bs, K.data_ptr(), V.data_ptr(),
@@ -534,25 +534,23 @@ def decode_kv8_num_splits(B, H_q, H_kv, d, max_ctx, splits=0):
 def decode_attn_kv8(Q, cache, block_table, context_lens, max_ctx, splits=0, out=None, workspace=None, stream=None):
     """Q [B, H_q, d] fp32, one token a sequence, over the first context_lens[b]
     <= max_ctx cached positions; returns O [B, H_q, d]."""
-    H, bs, d = _kv8("decode_attn_kv8", cache, block_table)
+    H, bs, d, at = _kv8("decode_attn_kv8", cache, block_table)
     B, H_q, dq = Q.shape
-    if dq != d or block_table.shape[0] != B or context_lens.shape != (B,):
-        raise ValueError(f"decode_attn_kv8: Q {tuple(Q.shape)}, block_table {tuple(block_table.shape)}, context_lens "
-                         f"{tuple(context_lens.shape)} and heads of {d} do not fit")
     if out is None:
         out = _empty((B, H_q, d), dtype=_f32, device=Q.device)
         _made(stream, out)
-    elif out.shape != Q.shape:
-        raise ValueError("decode_attn_kv8: out needs Q's shape")
-    _check("decode_attn_kv8", _f32, (Q, out))
-    _check("decode_attn_kv8", _i32, (context_lens,))
+    if not (dq == d and block_table.shape[0] == B and context_lens.shape == (B,) and out.shape == Q.shape
+            and Q.dtype is _f32 and out.dtype is _f32 and context_lens.dtype is _i32 and Q.get_device() == at
+            and out.get_device() == at and context_lens.get_device() == at and Q.is_contiguous() and out.is_contiguous()
+            and context_lens.is_contiguous()):
+        _refuse("decode_attn_kv8", Q, out, context_lens, block_table)
     if workspace is None:
         S = decode_kv8_num_splits(B, H_q, H, d, max_ctx, splits)
         if S > 1:
             workspace = _empty(B * H_q * S * (d + 2), dtype=_f32, device=Q.device)
             _made(stream, workspace)
-    if workspace is not None:
-        _check("decode_attn_kv8", _f32, (workspace,))
+    elif workspace.dtype is not _f32 or workspace.get_device() != at or not workspace.is_contiguous():
+        _refuse("decode_attn_kv8", workspace)
     k, v, ks, vs = cache
     check("ie_decode_attn_kv8", B, H_q, H, d, Q.data_ptr(), k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(),
           block_table.data_ptr(), context_lens.data_ptr(), max_ctx, bs, block_table.shape[1], out.data_ptr(),
@@ -564,24 +562,21 @@ def prefill_attn_kv8(Q, cache, block_table, start_pos, out=None, workspace=None,
     """Q [B, P, H_q, d] fp32, token t at position start_pos + t with its rows
     cached; returns causal O [B, P, H_q, d].  workspace: fp32, at least
     ie_prefill_kv8_workspace_bytes (made here where the call has use for one)."""
-    H, bs, d = _kv8("prefill_attn_kv8", cache, block_table)
+    H, bs, d, at = _kv8("prefill_attn_kv8", cache, block_table)
     B, P, H_q, dq = Q.shape
-    if dq != d or block_table.shape[0] != B:
-        raise ValueError(f"prefill_attn_kv8: Q {tuple(Q.shape)}, block_table {tuple(block_table.shape)} and heads of {d} "
-                         "do not fit")
     if out is None:
         out = _empty((B, P, H_q, d), dtype=_f32, device=Q.device)
         _made(stream, out)
-    elif out.shape != Q.shape:
-        raise ValueError("prefill_attn_kv8: out needs Q's shape")
-    _check("prefill_attn_kv8", _f32, (Q, out))
+    if not (dq == d and block_table.shape[0] == B and out.shape == Q.shape and Q.dtype is _f32 and out.dtype is _f32
+            and Q.get_device() == at and out.get_device() == at and Q.is_contiguous() and out.is_contiguous()):
+        _refuse("prefill_attn_kv8", Q, out, block_table)
     if workspace is None:
         need = call("ie_prefill_kv8_workspace_bytes", B, P, H_q, H, d, start_pos)
         if need:
             workspace = _empty(need // 4, dtype=_f32, device=Q.device)
             _made(stream, workspace)
-    else:
-        _check("prefill_attn_kv8", _f32, (workspace,))
+    elif workspace.dtype is not _f32 or workspace.get_device() != at or not workspace.is_contiguous():
+        _refuse("prefill_attn_kv8", workspace)
     k, v, ks, vs = cache
     check("ie_prefill_attn_kv8", B, P, H_q, H, d, Q.data_ptr(), k.data_ptr(), v.data_ptr(), ks.data_ptr(),
           vs.data_ptr(), block_table.data_ptr(), block_table.shape[1], bs, start_pos, out.data_ptr(), _ptr(workspace),
@@ -610,34 +605,35 @@ def token_logprobs(logits, targets=None, k=0, out=None, workspace=None, stream=N
     if logits.get_device() != at or logits.dtype is not _f32 or (n > 1 and step != 1) or (rows > 1 and ld < n):
         raise ValueError(f"token_logprobs: logits need to be fp32 rows on cuda:{at}, got {logits.dtype} strides "
                          f"{(ld, step)} on {logits.device}")
-    if targets is not None:
-        _check("token_logprobs", _i32, (targets,))
-        if targets.shape != (rows,):
-            raise ValueError("token_logprobs: targets needs one entry per row")
+    if targets is not None and not (targets.shape == (rows,) and targets.dtype is _i32 and targets.get_device() == at
+                                    and targets.is_contiguous()):
+        _refuse("token_logprobs", targets)
     if out is None:
         dev = logits.device
-        out = TokenLogprobs(_empty(rows, dtype=_f32, device=dev), _empty(rows, dtype=_i32, device=dev),
-                            _empty(rows, dtype=_f32, device=dev), _empty((rows, k), dtype=_f32, device=dev),
-                            _empty((rows, k), dtype=_i32, device=dev))
+        out = (_empty(rows, dtype=_f32, device=dev), _empty(rows, dtype=_i32, device=dev),
+               _empty(rows, dtype=_f32, device=dev), _empty((rows, k), dtype=_f32, device=dev),
+               _empty((rows, k), dtype=_i32, device=dev))
         _made(stream, *out)
     else:
-        _check("token_logprobs", _f32, (out[0], out[2], out[3]))
-        _check("token_logprobs", _i32, (out[1], out[4]))
-        if any(t.shape != (rows,) for t in out[:3]) or any(t.shape != (rows, k) for t in out[3:]):
-            raise ValueError(f"token_logprobs: out needs three tensors of {rows} and two of {(rows, k)}")
-        out = TokenLogprobs(*out)
+        lp, rk, en, tv, ti = out
+        if not (lp.shape == (rows,) and rk.shape == (rows,) and en.shape == (rows,) and tv.shape == (rows, k)
+                and ti.shape == (rows, k) and lp.dtype is _f32 and rk.dtype is _i32 and en.dtype is _f32
+                and tv.dtype is _f32 and ti.dtype is _i32 and lp.get_device() == at and rk.get_device() == at
+                and en.get_device() == at and tv.get_device() == at and ti.get_device() == at and lp.is_contiguous()
+                and rk.is_contiguous() and en.is_contiguous() and tv.is_contiguous() and ti.is_contiguous()):
+            _refuse("token_logprobs", lp, rk, en, tv, ti)
     if workspace is None:
         need = call("ie_token_logprobs_workspace_bytes", rows, n, k)
         if need:
             workspace = _empty(need // 4, dtype=_f32, device=logits.device)
             _made(stream, workspace)
-    if workspace is not None:
-        _check("token_logprobs", _f32, (workspace,))
+    elif workspace.dtype is not _f32 or workspace.get_device() != at or not workspace.is_contiguous():
+        _refuse("token_logprobs", workspace)
     lp, rk, en, tv, ti = out
     check("ie_token_logprobs", rows, logits.data_ptr(), ld if rows > 1 else n, n, _ptr(targets), k, lp.data_ptr(),
           rk.data_ptr(), en.data_ptr(), tv.data_ptr(), ti.data_ptr(), _ptr(workspace),
           0 if workspace is None else 4 * workspace.numel(), _stream(stream))
-    return out
+    return TokenLogprobs(*out)
 
 
 # ---------------------------------------------------------------- engine
