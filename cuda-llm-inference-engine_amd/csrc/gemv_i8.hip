@@ -1239,7 +1239,7 @@ void launch_gemv_i8(const GemmArgs& a, hipStream_t s) {
 bool gemv_fused_supported(int M, int K, int src, int epi) {
     if (M < 1 || M > kGemvMaxM) return false;
     if (src == kSrcLnQuant)
-        return K == 768 && (epi == kEpiQKV || epi == IE_EPI_BIAS_GELU || epi == IE_EPI_PLAIN);
+        return K == 768 && (epi == kEpiQKV || epi == IE_EPI_BIAS || epi == IE_EPI_BIAS_GELU || epi == IE_EPI_PLAIN);
     if (src == kSrcQuant) return (K == 768 || K == 3072) && epi == IE_EPI_BIAS_RESIDUAL;
     return false;
 }
@@ -1248,6 +1248,7 @@ void launch_gemv_fused(const GemmArgs& a, const GemvFusion& f, hipStream_t s) {
     if (a.M == 0 || a.N == 0) return;
     if (f.src == kSrcLnQuant) {
         if (a.epi == kEpiQKV) return launch_fused<kEpiQKV, 768, kSrcLnQuant>(a, f, s);
+        if (a.epi == IE_EPI_BIAS) return launch_fused<IE_EPI_BIAS, 768, kSrcLnQuant>(a, f, s);
         if (a.epi == IE_EPI_BIAS_GELU) return launch_fused<IE_EPI_BIAS_GELU, 768, kSrcLnQuant>(a, f, s);
         return launch_fused<IE_EPI_PLAIN, 768, kSrcLnQuant>(a, f, s);
     }

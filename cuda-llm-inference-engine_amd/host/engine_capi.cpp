@@ -2,6 +2,7 @@
 // Exceptions from the engine become IE_ERR_* codes with the message kept for
 // ie_last_error().
 #include "ie_engine.h"
+#include "ie_logprobs.h"
 
 #include <hip/hip_runtime.h>
 
@@ -171,6 +172,15 @@ int ie_engine_prefill(ie_engine* e, int batch, int prompt_len, const int* tokens
     return guarded("ie_engine_prefill", [&] {
         e->eng->prefill(tokens, batch, prompt_len);
         fetch_logits(e->eng, batch, logits_host, argmax_host);
+    });
+}
+
+int ie_engine_score(ie_engine* e, int batch, int prompt_len, const int* tokens, int k, float* logprobs, int* ranks,
+                    float* entropy, float* top_logprobs, int* top_idx) {
+    if (!e || !tokens || batch <= 0 || prompt_len <= 0 || k < 0)
+        return ie::fail(IE_ERR_INVALID, "ie_engine_score: bad arguments");
+    return guarded("ie_engine_score", [&] {
+        e->eng->score(tokens, batch, prompt_len, k, logprobs, ranks, entropy, top_logprobs, top_idx);
     });
 }
 

@@ -30,6 +30,8 @@
 #include <stdexcept>
 
 #include "../csrc/ie_internal.h"
+#include "../csrc/kv8.h"
+#include "ie_logprobs.h"
 #include "vendor_blas.h"
 
 namespace {
@@ -281,6 +283,7 @@ struct GPT2Engine::Impl {
     int nbps = 0, phys_blocks = 0;
     size_t layer_elems = 0;
     char *kc = nullptr, *vc = nullptr;
+    float *kv8_ks = nullptr, *kv8_vs = nullptr;  // IE_KV_I8: scales [n_layers, P, H]
     int *block_table = nullptr, *positions = nullptr, *ctx_lens = nullptr, *tokens = nullptr;
     float* ws = nullptr;
     size_t ws_bytes = 0;
@@ -352,7 +355,8 @@ struct GPT2Engine::Impl {
         cfg = m.cfg;
         opt = o;
         if (opt.max_batch < 1 || opt.max_batch > 16) throw std::runtime_error("max_batch must be 1..16");
-        if (opt.kv_dtype != IE_KV_F32 && opt.kv_dtype != IE_KV_BF16) throw std::runtime_error("kv_dtype");
+        if (opt.kv_dtype != IE_KV_F32 && opt.kv_dtype != IE_KV_BF16 && opt.kv_dtype != IE_KV_I8)
+            throw std::runtime_error("kv_dtype");
         HIPC(hipStreamCreate(&stream));
         const int d = cfg.d_model, ff = cfg.d_ff, V = cfg.vocab_size, B = opt.max_batch;
         fp32 = opt.backend == InferenceBackend::CUBLAS_FP32;
@@ -411,9 +415,12 @@ struct GPT2Engine::Impl {
         nbps = (cfg.max_seq_len + kBlock - 1) / kBlock;
         phys_blocks = B * nbps;
         layer_elems = (size_t)phys_blocks * kBlock * d;
-        const size_t esz = opt.kv_dtype == IE_KV_BF16 ? 2 : 4;
-        kc = dev<char>(layer_elems * esz * cfg.n_layers);
-        vc = dev<char>(layer_elems * esz * cfg.n_layers);
+        kc = dev<char>(layer_elems * kv_size() * cfg.n_layers);
+        vc = dev<char>(layer_elems * kv_size() * cfg.n_layers);
+        if (kv8()) {
+            kv8_ks = dev<float>((size_t)cfg.n_layers * phys_blocks * cfg.n_heads);
+            kv8_vs = dev<float>((size_t)cfg.n_layers * phys_blocks * cfg.n_heads);
+        }
         std::vector<int> table((size_t)B * nbps);
         std::iota(table.begin(), table.end(), 0);
         block_table = upload(table);
@@ -425,12 +432,12 @@ struct GPT2Engine::Impl {
         ws = dev<float>(ws_bytes / sizeof(float));
         fused = opt.fuse && (cfg.d_head == 64 || cfg.d_head == 128);
         for (int m = 1; m <= B && fused; ++m)
-            fused = ie::gemv_fused_supported(m, d, ie::kSrcLnQuant, ie::kEpiQKV) &&
+            fused = ie::gemv_fused_supported(m, d, ie::kSrcLnQuant, kv8() ? IE_EPI_BIAS : ie::kEpiQKV) &&
                     ie::gemv_fused_supported(m, d, ie::kSrcLnQuant, IE_EPI_BIAS_GELU) &&
                     ie::gemv_fused_supported(m, d, ie::kSrcQuant, IE_EPI_BIAS_RESIDUAL) &&
                     ie::gemv_fused_supported(m, ff, ie::kSrcQuant, IE_EPI_BIAS_RESIDUAL) &&
                     ie::gemv_fused_supported(m, d, ie::kSrcLnQuant, IE_EPI_PLAIN);
-        qkv_attn = fused && ie::qkv_attn_supported(d, cfg.n_heads, cfg.d_head, kBlock);
+        qkv_attn = fused && !kv8() && ie::qkv_attn_supported(d, cfg.n_heads, cfg.d_head, kBlock);
         HIPC(hipHostMalloc(&host_tokens, sizeof(int) * B));
         HIPC(hipHostMalloc(&host_ring, sizeof(int) * 2 * B, hipHostMallocCoherent));
         for (auto& e : ring_ev) HIPC(hipEventCreateWithFlags(&e, hipEventDisableTiming));
@@ -450,6 +457,7 @@ struct GPT2Engine::Impl {
             if (kv.second) (void)hipGraphExecDestroy(kv.second);
         for (void* p : allocs) (void)hipFree(p);
         for (void* p : pf_allocs) (void)hipFree(p);
+        for (void* p : sc_allocs) (void)hipFree(p);
         if (pf.host_ids) (void)hipHostFree(pf.host_ids);
         if (host_tokens) (void)hipHostFree(host_tokens);
         if (host_ring) (void)hipHostFree(host_ring);
@@ -467,8 +475,58 @@ struct GPT2Engine::Impl {
         HIPC(hipStreamSynchronize(stream));
     }
 
-    void* layer_k(int l) { return kc + layer_elems * (opt.kv_dtype == IE_KV_BF16 ? 2 : 4) * l; }
-    void* layer_v(int l) { return vc + layer_elems * (opt.kv_dtype == IE_KV_BF16 ? 2 : 4) * l; }
+    bool kv8() const { return opt.kv_dtype == IE_KV_I8; }
+    int kv_size() const { return kv8() ? 1 : opt.kv_dtype == IE_KV_BF16 ? 2 : 4; }  // bytes an element
+    void* layer_k(int l) { return kc + layer_elems * kv_size() * l; }
+    void* layer_v(int l) { return vc + layer_elems * kv_size() * l; }
+    ie::Kv8Cache layer_kv8(int l) {
+        const size_t scales = (size_t)phys_blocks * cfg.n_heads * l;
+        ie::Kv8Cache c{};
+        c.k = static_cast<int8_t*>(layer_k(l));
+        c.v = static_cast<int8_t*>(layer_v(l));
+        c.ks = kv8_ks + scales;
+        c.vs = kv8_vs + scales;
+        c.table = block_table;
+        c.nbps = nbps;
+        c.H = cfg.n_heads;
+        c.d = cfg.d_head;
+        c.bs_log2 = 4;
+        static_assert(kBlock == 16, "log2 of the page");
+        return c;
+    }
+
+    // The 8-bit cache: a decode step's K and V rows of qkv [B, 3d] appended at
+    // positions (which sets ctx_lens), then attention of its Q rows.
+    void kv8_step(int B, int l) {
+        const int d = cfg.d_model;
+        ie::Kv8Write w{};
+        w.B = B; w.P = 1; w.K = qkv + d; w.V = qkv + 2 * d; w.ld = 3 * d;
+        w.c = layer_kv8(l); w.positions = positions; w.ctx_lens = ctx_lens;
+        ie::launch_kv8_write(w, stream);
+        IEC(ie::check_launch("kv8 append"));
+        ie::Kv8Attn a{};
+        a.B = B; a.P = 1; a.H_q = cfg.n_heads; a.Q = qkv; a.q_ld = 3 * d; a.c = w.c;
+        a.lens = ctx_lens; a.max_ctx = plan.max_ctx; a.O = attn; a.ws = ws; a.splits = plan.splits;
+        ie::launch_decode_attn_kv8(a, stream);
+        IEC(ie::check_launch("decode_attn_kv8"));
+    }
+
+    // The same for a prompt chunk's rows pf.qkv [B * Pc, 3d] at positions pos ..
+    void kv8_prompt(int B, int Pc, int l) {
+        const int d = cfg.d_model, H = cfg.n_heads;
+        ie::Kv8Write w{};
+        w.B = B; w.P = Pc; w.K = pf.qkv + d; w.V = pf.qkv + 2 * d; w.ld = 3 * d;
+        w.c = layer_kv8(l); w.start = pos;
+        ie::launch_kv8_write(w, stream);
+        IEC(ie::check_launch("kv8 write"));
+        ie::Kv8Attn a{};
+        a.B = B; a.P = Pc; a.H_q = H; a.Q = pf.qkv; a.q_ld = 3 * d; a.c = w.c;
+        a.start = pos; a.max_ctx = pos + Pc; a.O = pf.attn; a.ws = ws;
+        a.splits = ie::kv8_prefill_splits(B, Pc, H, H, pos + Pc);
+        if ((size_t)B * Pc * H * a.splits * (cfg.d_head + 2) * sizeof(float) > ws_bytes) a.splits = 1;
+        ie::launch_prefill_attn_kv8(a, stream);
+        IEC(ie::check_launch("prefill_attn_kv8"));
+    }
 
     // GEMV with its activation operand built from fp32 rows in the kernel.
     void fused_gemv(int B, const QuantWeight& w, int src, const float* xin, const float* g,
@@ -490,8 +548,7 @@ struct GPT2Engine::Impl {
     // batch 16: 359.6 -> 340.6 us per step; batch 1, 28 MB, keeps plain
     // loads: 240.8 against 256.3 us with them).
     bool kv_stream_step(int B) const {
-        const double bytes = 2.0 * cfg.n_layers * (double)B * plan.max_ctx * cfg.d_model *
-                             (opt.kv_dtype == IE_KV_BF16 ? 2 : 4);
+        const double bytes = 2.0 * cfg.n_layers * (double)B * plan.max_ctx * cfg.d_model * kv_size();
         return bytes > 64.0 * (1 << 20);
     }
 
@@ -509,6 +566,14 @@ struct GPT2Engine::Impl {
         if (!emb_fused) IEC(ie_embedding_batch(B, tokens, positions, d, wte, wpe, x, (ie_stream_t)s));
         for (int l = 0; l < cfg.n_layers; ++l) {
             const Layer& L = layers[l];
+            if (kv8()) {
+                fused_gemv(B, L.qkv, ie::kSrcLnQuant, x, L.ln1_g, L.ln1_b, IE_EPI_BIAS, L.qkv_b, nullptr, qkv);
+                kv8_step(B, l);
+                fused_gemv(B, L.out, ie::kSrcQuant, attn, nullptr, nullptr, IE_EPI_BIAS_RESIDUAL, L.out_b, x, x);
+                fused_gemv(B, L.up, ie::kSrcLnQuant, x, L.ln2_g, L.ln2_b, IE_EPI_BIAS_GELU, L.up_b, nullptr, h);
+                fused_gemv(B, L.down, ie::kSrcQuant, h, nullptr, nullptr, IE_EPI_BIAS_RESIDUAL, L.down_b, x, x);
+                continue;
+            }
             ie::GemvFusion io{};
             io.q = q; io.kc = layer_k(l); io.vc = layer_v(l); io.kv_dtype = opt.kv_dtype;
             io.positions = positions; io.table = block_table; io.nbps = nbps; io.block_size = kBlock;
@@ -629,7 +694,7 @@ struct GPT2Engine::Impl {
     // the GEMM storing Q and the K/V rows itself, where prefill_qkv_write
     // would move them from pf.qkv); otherwise ln_linear into pf.qkv and
     // prefill_qkv_write.
-    bool qkv_routed() const { return !fp32 && ie::ln_quant_supported(cfg.d_model); }
+    bool qkv_routed() const { return !fp32 && !kv8() && ie::ln_quant_supported(cfg.d_model); }
 
     void prefill_qkv(int B, int Pc, int l) {
         const Layer& L = layers[l];
@@ -650,6 +715,7 @@ struct GPT2Engine::Impl {
             return;
         }
         ln_linear(M, L.ln1_g, L.ln1_b, L.qkv, L.qkv_f, IE_EPI_BIAS, L.qkv_b, pf.qkv);
+        if (kv8()) return;  // (kv8_prompt takes the rows as they lie)
         ie::launch_prefill_qkv_write(B, Pc, pos, d, pf.qkv, block_table, nbps, kBlock, pf.q, layer_k(l),
                                      layer_v(l), opt.kv_dtype, stream);
         IEC(ie::check_launch("prefill_qkv_write"));
@@ -674,12 +740,15 @@ struct GPT2Engine::Impl {
             const Layer& L = layers[l];
             IEC(ie_layernorm(B, d, x, L.ln1_g, L.ln1_b, xn, 1e-5f, st));
             linear(B, L.qkv, L.qkv_f, xn, IE_EPI_BIAS, L.qkv_b, nullptr, qkv, act_q, act_s, gemm_out);
-            ie::launch_qkv_split_append(B, d, qkv, positions, block_table, nbps, kBlock, q, layer_k(l),
-                                        layer_v(l), opt.kv_dtype, ctx_lens, s);
-            IEC(ie::check_launch("qkv_split_append"));
-            IEC(ie_decode_attn(B, H, H, cfg.d_head, q, layer_k(l), layer_v(l), opt.kv_dtype,
-                               block_table, ctx_lens, plan.max_ctx, kBlock, nbps, attn, ws, ws_bytes, plan.splits,
-                               st));
+            if (kv8()) {
+                kv8_step(B, l);
+            } else {
+                ie::launch_qkv_split_append(B, d, qkv, positions, block_table, nbps, kBlock, q, layer_k(l),
+                                            layer_v(l), opt.kv_dtype, ctx_lens, s);
+                IEC(ie::check_launch("qkv_split_append"));
+                IEC(ie_decode_attn(B, H, H, cfg.d_head, q, layer_k(l), layer_v(l), opt.kv_dtype, block_table, ctx_lens,
+                                   plan.max_ctx, kBlock, nbps, attn, ws, ws_bytes, plan.splits, st));
+            }
             linear(B, L.out, L.out_f, attn, IE_EPI_BIAS_RESIDUAL, L.out_b, x, x, act_q, act_s, gemm_out);
             IEC(ie_layernorm(B, d, x, L.ln2_g, L.ln2_b, xn, 1e-5f, st));
             linear(B, L.up, L.up_f, xn, IE_EPI_BIAS_GELU, L.up_b, nullptr, h, act_q, act_s, gemm_out);
@@ -693,9 +762,16 @@ struct GPT2Engine::Impl {
     // six 16-token chunks), at most the workspace's 16; a single split writes
     // the output directly.  Computed from the host's position mirror, so the
     // captured graph for that plan can be replayed.
+    // The 8-bit cache's attention takes contexts of up to 1024 in one split (one
+    // launch; 12 heads of 64 6.8 us, in four splits 6.9), longer ones by 512.
     static constexpr int kTokensPerSplit = 384;
     AttnPlan plan_for(int ctx) const {
         AttnPlan p;
+        if (kv8()) {
+            p.splits = ctx <= 1024 ? 1 : std::min((ctx + 511) / 512, 16);
+            p.max_ctx = p.splits == 16 ? cfg.max_seq_len : std::min(p.splits == 1 ? 1024 : p.splits * 512, cfg.max_seq_len);
+            return p;
+        }
         p.splits = std::max(1, std::min((ctx + kTokensPerSplit - 1) / kTokensPerSplit, 16));
         p.max_ctx = p.splits == 16 ? cfg.max_seq_len
                                    : std::min(p.splits * kTokensPerSplit, cfg.max_seq_len);
@@ -860,7 +936,9 @@ struct GPT2Engine::Impl {
     // logits [B, V] of each sequence's last token, their argmax in `tokens`,
     // and positions at pos + P.  The reference prefills only a fresh session
     // and feeds a continuation through decode steps; here both prefill.
-    void prefill(const int* toks, int B, int P) {
+    // With a score, the log probability of every chunk row's next token too.
+    struct Score;
+    void prefill(const int* toks, int B, int P, Score* score = nullptr) {
         if (B < 1 || B > opt.max_batch) throw std::runtime_error("batch out of range");
         if (P < 1) throw std::runtime_error("empty prompt");
         if (!prefill_applies()) throw std::runtime_error("prefill needs d_head 64 or 128");
@@ -887,14 +965,18 @@ struct GPT2Engine::Impl {
             for (int l = 0; l < cfg.n_layers; ++l) {
                 const Layer& L = layers[l];
                 prefill_qkv(B, Pc, l);
-                IEC(ie_prefill_attn(B, Pc, H, H, dh, pf.q, layer_k(l), layer_v(l), opt.kv_dtype, block_table, nbps,
-                                    kBlock, pos, pf.attn, st));
+                if (kv8())
+                    kv8_prompt(B, Pc, l);
+                else
+                    IEC(ie_prefill_attn(B, Pc, H, H, dh, pf.q, layer_k(l), layer_v(l), opt.kv_dtype, block_table, nbps,
+                                        kBlock, pos, pf.attn, st));
                 linear(M, L.out, L.out_f, pf.attn, IE_EPI_BIAS_RESIDUAL, L.out_b, pf.x, pf.x, pf.act_q, pf.act_s,
                        pf.gemm_out);
                 ln_linear(M, L.ln2_g, L.ln2_b, L.up, L.up_f, IE_EPI_BIAS_GELU, L.up_b, pf.h);
                 linear(M, L.down, L.down_f, pf.h, IE_EPI_BIAS_RESIDUAL, L.down_b, pf.x, pf.x, pf.act_q, pf.act_s,
                        pf.gemm_out);
             }
+            if (score) score_rows(*score, B, Pc, c0, P, toks);
             pos += Pc;
         }
         // hidden row of each sequence's last token -> x [B, d]
@@ -903,6 +985,110 @@ struct GPT2Engine::Impl {
         ie::launch_set_positions(B, pos, positions, ctx_lens, stream);
         IEC(ie::check_launch("set_positions"));
         enqueue_head(B, false);
+    }
+
+    // Log probabilities of a prompt's tokens into the caller's host arrays [B, P]
+    // (and [B, P, k]).
+    struct Score {
+        int k;
+        float* logprobs;
+        int* ranks;
+        float* entropy;
+        float* top_logprobs;
+        int* top_idx;
+    };
+    struct ScoreBufs {
+        int rows = 0, k = 0;
+        float *xn = nullptr, *logits = nullptr, *out = nullptr, *ws = nullptr;
+        int32_t* act_q = nullptr;
+        float* act_s = nullptr;
+        int* targets = nullptr;
+        size_t ws_bytes = 0;
+        std::vector<int> host_targets;
+        std::vector<float> host_out;
+    } sc;
+    std::vector<void*> sc_allocs;
+    // Rows of logits at a time: all that the fp32 head takes, and of the int8
+    // head's GEMM 256 (51 MB of logits for GPT-2's vocabulary, read while the
+    // Infinity Cache holds them).
+    int score_group() const { return opt.int8_lm_head ? 256 : 16; }
+
+    void ensure_score(int rows, int k) {
+        if (rows <= sc.rows && k <= sc.k) return;
+        HIPC(hipStreamSynchronize(stream));
+        rows = std::max(rows, sc.rows);
+        k = std::max(k, sc.k);
+        sc.rows = 0;
+        for (void* p : sc_allocs) (void)hipFree(p);
+        sc_allocs.clear();
+        auto get = [&](size_t bytes) {
+            void* p = nullptr;
+            HIPC(hipMalloc(&p, bytes));
+            sc_allocs.push_back(p);
+            return p;
+        };
+        const size_t d = cfg.d_model, V = cfg.vocab_size, R = rows;
+        const int G = std::min(score_group(), rows);
+        sc.xn = (float*)get(R * d * 4);
+        sc.logits = (float*)get(G * V * 4);
+        sc.out = (float*)get(R * (3 + 2 * k) * 4);
+        sc.targets = (int*)get(R * 4);
+        if (opt.int8_lm_head) {
+            sc.act_q = (int32_t*)get(R * d);
+            sc.act_s = (float*)get(R * 4);
+        }
+        sc.ws_bytes = 0;
+        for (int r = 1; r <= G; ++r)
+            for (int kk : {0, k}) sc.ws_bytes = std::max(sc.ws_bytes, ie_token_logprobs_workspace_bytes(r, (int)V, kk));
+        sc.ws = (float*)get(std::max<size_t>(sc.ws_bytes, 4));
+        sc.rows = rows;
+        sc.k = k;
+    }
+
+    // The chunk's hidden rows pf.x (row b * Pc + t is token c0 + t of sequence b,
+    // of P): final LayerNorm, LM head, and the log probability of the token that
+    // follows; the last token's row has none and gives its entropy and
+    // alternatives alone.
+    void score_rows(Score& s, int B, int Pc, int c0, int P, const int* toks) {
+        const int d = cfg.d_model, V = cfg.vocab_size, M = B * Pc, k = s.k;
+        ie_stream_t st = (ie_stream_t)stream;
+        ensure_score(M, k);
+        // device results, each array M rows: log probabilities, entropies, alternatives, then the two of integers
+        float *lp = sc.out, *en = lp + M, *tv = en + M;
+        int *rk = reinterpret_cast<int*>(tv + (size_t)M * k), *ti = rk + M;
+        sc.host_targets.resize(M);
+        sc.host_out.resize((size_t)M * (3 + 2 * k));
+        for (int r = 0; r < M; ++r) {
+            const int b = r / Pc, t = c0 + r % Pc;
+            sc.host_targets[r] = t + 1 < P ? toks[(size_t)b * P + t + 1] : -1;
+        }
+        HIPC(hipMemcpyAsync(sc.targets, sc.host_targets.data(), sizeof(int) * M, hipMemcpyHostToDevice, stream));
+        IEC(ie_layernorm(M, d, pf.x, lnf_g, lnf_b, sc.xn, 1e-5f, st));
+        if (opt.int8_lm_head) IEC(ie_quantize_fp32_to_int8(M, d, sc.xn, sc.act_q, sc.act_s, st));
+        const int G = score_group();
+        for (int r0 = 0; r0 < M; r0 += G) {
+            const int R = std::min(G, M - r0);
+            if (opt.int8_lm_head)
+                IEC(ie_int8_gemm(R, V, d, sc.act_q + (size_t)r0 * (d / 4), head.packed, sc.act_s + r0, head.scale,
+                                 IE_EPI_PLAIN, nullptr, nullptr, sc.logits, st));
+            else
+                IEC(ie_vocab_proj(R, sc.xn + (size_t)r0 * d, wte, sc.logits, d, V, st));
+            IEC(ie_token_logprobs(R, sc.logits, V, V, sc.targets + r0, k, lp + r0, rk + r0, en + r0,
+                                  tv + (size_t)r0 * k, ti + (size_t)r0 * k, sc.ws, sc.ws_bytes, st));
+        }
+        HIPC(hipMemcpyAsync(sc.host_out.data(), sc.out, sizeof(float) * sc.host_out.size(), hipMemcpyDeviceToHost,
+                            stream));
+        HIPC(hipStreamSynchronize(stream));
+        const float* h = sc.host_out.data();
+        const int* hi = reinterpret_cast<const int*>(h + (size_t)M * (2 + k));
+        for (int r = 0; r < M; ++r) {
+            const size_t at = (size_t)(r / Pc) * P + c0 + r % Pc;
+            if (s.logprobs) s.logprobs[at] = h[r];
+            if (s.entropy) s.entropy[at] = h[M + r];
+            if (s.ranks) s.ranks[at] = hi[r];
+            if (s.top_logprobs) std::memcpy(s.top_logprobs + at * k, h + 2 * M + (size_t)r * k, sizeof(float) * k);
+            if (s.top_idx) std::memcpy(s.top_idx + at * k, hi + M + (size_t)r * k, sizeof(int) * k);
+        }
     }
 
     // Prompt of B sequences x P tokens through prefill (or, if disabled, one
@@ -929,7 +1115,7 @@ struct GPT2Engine::Impl {
         w += cfg.n_layers * 4.0 * (3 * d + d + ff + d) * (fp32 ? 1 : 2);   // biases (+ scales)
         w += cfg.n_layers * 4.0 * 4 * d;                                      // LayerNorm
         w += opt.int8_lm_head ? V * d + 4 * V : 4.0 * V * d;                  // LM head
-        const double kv = 2.0 * cfg.n_layers * (double)B * ctx * d * (opt.kv_dtype == IE_KV_BF16 ? 2 : 4);
+        const double kv = 2.0 * cfg.n_layers * (double)B * ctx * (d * kv_size() + (kv8() ? 4.0 * cfg.n_heads / kBlock : 0.0));
         return w + kv;
     }
 
@@ -989,6 +1175,14 @@ double GPT2Engine::step_bytes(int batch) const { return impl_->bytes_per_step(ba
 
 void GPT2Engine::prefill(const int* tokens, int batch, int len) {
     impl_->prefill(tokens, batch, len);
+    HIPC(hipStreamSynchronize(impl_->stream));
+}
+
+void GPT2Engine::score(const int* tokens, int batch, int len, int k, float* logprobs, int* ranks, float* entropy,
+                       float* top_logprobs, int* top_idx) {
+    if (k < 0 || k > std::min(impl_->cfg.vocab_size, IE_LOGPROBS_TOP_MAX)) throw std::runtime_error("k out of range");
+    Impl::Score s{k, logprobs, ranks, entropy, top_logprobs, top_idx};
+    impl_->prefill(tokens, batch, len, &s);
     HIPC(hipStreamSynchronize(impl_->stream));
 }
 

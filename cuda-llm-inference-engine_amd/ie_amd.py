@@ -72,6 +72,7 @@ KV8_MAX_SPLITS = 64
 LOGPROBS_SIGNATURES = {
     "ie_token_logprobs_workspace_bytes": (_Z, [_I, _I, _I]),
     "ie_token_logprobs": (_I, [_I, _P, _I, _I, _P, _I, _P, _P, _P, _P, _P, _P, _Z, _P]),
+    "ie_engine_score": (_I, [_P, _I, _I, _P, _I, _P, _P, _P, _P, _P]),
 }
 LOGPROBS_TOP_MAX = 128
 
@@ -648,7 +649,8 @@ def write_random_model(path, seed=0, **cfg):
 
 class Engine:
     """GPT-2 decode engine (include/ie_engine.h).  model_dir=None builds a
-    random model of the given shape (GPT-2 Small by default)."""
+    random model of the given shape (GPT-2 Small by default).  kv_dtype: KV_F32,
+    KV_BF16 or KV_I8 (the 8-bit cache of include/ie_kv8.h)."""
 
     def __init__(self, model_dir=None, seed=0, max_batch=1, kv_dtype=KV_F32, int8_lm_head=False,
                  use_graph=True, fuse=True, prefill=True, prefill_chunk=0, backend=BACKEND_INT8, **cfg):
@@ -697,6 +699,20 @@ class Engine:
         check("ie_engine_prefill", self.h, B, P, toks.ctypes.data_as(ctypes.c_void_p),
               None if logits is None else logits.ctypes.data_as(ctypes.c_void_p), None)
         return logits
+
+    def score(self, tokens, k=0):
+        """tokens [B, P] at the current position (a prefill) -> TokenLogprobs of numpy
+        arrays [B, P] and [B, P, k]: entry [b, t] is the log probability of
+        tokens[b, t + 1] after the ones before it, its rank, and that prediction's
+        entropy and k most likely tokens; the last entry has no token to score."""
+        import numpy as np
+
+        toks = np.ascontiguousarray(tokens, dtype=np.int32)
+        B, P = toks.shape
+        out = (np.zeros((B, P), np.float32), np.zeros((B, P), np.int32), np.zeros((B, P), np.float32),
+               np.zeros((B, P, max(k, 0)), np.float32), np.zeros((B, P, max(k, 0)), np.int32))
+        check("ie_engine_score", self.h, B, P, toks.ctypes.data, k, *(a.ctypes.data for a in out))
+        return TokenLogprobs(*out)
 
     def generate(self, prompts, max_new, ignore_eos=False):
         """prompts [B, P] int -> (tokens [B, max_new] with -1 padding, metrics dict)."""

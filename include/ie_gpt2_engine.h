@@ -25,6 +25,7 @@
 #include <vector>
 
 #include "ie_amd.h"
+#include "ie_kv8.h"
 
 /* include/gpt2_types.cuh:6-14 */
 struct GPT2Config {
@@ -74,7 +75,7 @@ enum class InferenceBackend { CUSTOM_INT8, CUBLAS_FP32 };
 
 struct GPT2EngineOptions {
     int max_batch = 1;          /* sequences decoded together */
-    int kv_dtype = IE_KV_F32;   /* IE_KV_F32 (reference) or IE_KV_BF16 */
+    int kv_dtype = IE_KV_F32;   /* IE_KV_F32 (reference), IE_KV_BF16, or IE_KV_I8 (ie_kv8.h) */
     bool int8_lm_head = false;  /* reference: fp32 head over tied wte */
     bool use_graph = true;      /* replay one captured decode step per token */
     /* Fused decode step: LayerNorm and the activation quantizer run inside
@@ -126,6 +127,16 @@ public:
      * (tokens[b * len + t]) at the current position; logits of every
      * sequence's last token are left on the device. */
     void prefill(const int* tokens, int batch, int len);
+
+    /* Prefill, as above, that also gives the log probability of each token under
+     * the model: entry [b, t] of the host arrays [batch, len] is that of
+     * tokens[b * len + t + 1] after the ones before it, with its rank, the
+     * entropy of that prediction and its k most likely tokens [batch, len, k]
+     * (ie_logprobs.h); the last entry of a sequence has no token to score (0 and
+     * rank 0).  Any array may be null; 0 <= k <= min(vocabulary,
+     * IE_LOGPROBS_TOP_MAX). */
+    void score(const int* tokens, int batch, int len, int k, float* logprobs, int* ranks, float* entropy,
+               float* top_logprobs, int* top_idx);
 
     /* One decode step for the first `batch` sequences at the current position
      * (tokens on the host); logits of every sequence are left on the device. */

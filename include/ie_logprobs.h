@@ -40,6 +40,15 @@ int ie_token_logprobs(int rows, const float* logits, int row_stride, int n, cons
                       int k, float* logprobs, int* ranks, float* entropy, float* top_logprobs,
                       int* top_idx, float* workspace, size_t workspace_bytes, ie_stream_t stream);
 
+/* Scores tokens with the engine (GPT2Engine::score): prefill of tokens [batch,
+ * prompt_len] (host) at the current position; entry [b, t] of the host arrays
+ * [batch, prompt_len] is the log probability of tokens[b, t + 1] after the ones
+ * before it, its rank, and the entropy and the k most likely tokens [batch,
+ * prompt_len, k] of that prediction.  The last entry of a sequence has no token
+ * to score (0 and rank 0).  Any array may be NULL. */
+int ie_engine_score(ie_engine* e, int batch, int prompt_len, const int* tokens, int k,
+                    float* logprobs, int* ranks, float* entropy, float* top_logprobs, int* top_idx);
+
 #ifdef __cplusplus
 }
 #endif

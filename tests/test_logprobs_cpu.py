@@ -49,3 +49,8 @@ def test_workspace(ie):
 
 def test_nothing_to_do(ie):
     assert call(ie, rows=0, x=None, t=None, lp=None) == 0
+
+
+def test_score_refuses_a_null_engine(ie):
+    tokens = (ctypes.c_int * 4)()
+    assert ie.call("ie_engine_score", None, 1, 4, ctypes.addressof(tokens), 0, None, None, None, None, None) == 1
