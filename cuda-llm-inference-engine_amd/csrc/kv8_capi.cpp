@@ -11,6 +11,8 @@ bool aligned(const void* p, size_t a) { return ((uintptr_t)p % a) == 0; }
 
 // Workgroups of a launch; a grid's threads must stay below 2^32.
 constexpr long long kMaxGroups = 1ll << 21;
+// Pages x heads of a write: two workgroups of up to 1024 threads each.
+constexpr long long kMaxWritten = 1ll << 20;
 // Longest context: positions and their tiles' ends stay within an int.
 constexpr long long kMaxContext = 1ll << 30;
 
@@ -87,8 +89,8 @@ int ie_kv8_cache_write(int B, int P, const float* K_src, const float* V_src, int
     if ((st = check_source(fn, K_src, V_src, src_stride, n_heads, d_head)) != IE_OK) return st;
     if ((st = check_cache(fn, k_cache, v_cache, k_scales, v_scales, block_table)) != IE_OK) return st;
     const long long pages = ((long long)start_pos + P - 1) / block_size - start_pos / block_size + 1;
-    if (pages * n_heads > kMaxGroups || pages * n_heads * B > kMaxGroups)
-        return fail(IE_ERR_UNSUPPORTED, "%s: more than 2^21 pages x heads in one call", fn);
+    if (pages * n_heads > kMaxWritten || pages * n_heads * B > kMaxWritten)
+        return fail(IE_ERR_UNSUPPORTED, "%s: more than 2^20 pages x heads in one call", fn);
     ie::Kv8Write a{};
     a.B = B; a.P = P; a.K = K_src; a.V = V_src; a.ld = src_stride;
     a.c = cache(k_cache, v_cache, k_scales, v_scales, block_table, num_blocks_per_seq, n_heads, d_head, block_size);
@@ -108,7 +110,7 @@ int ie_kv8_cache_append_batch(int B, const float* K_src, const float* V_src, int
     if ((st = check_source(fn, K_src, V_src, src_stride, n_heads, d_head)) != IE_OK) return st;
     if ((st = check_cache(fn, k_cache, v_cache, k_scales, v_scales, block_table)) != IE_OK) return st;
     if (!positions) return fail(IE_ERR_INVALID, "%s: null pointer", fn);
-    if ((long long)B * n_heads > kMaxGroups) return fail(IE_ERR_UNSUPPORTED, "%s: B x n_heads above 2^21", fn);
+    if ((long long)B * n_heads > kMaxWritten) return fail(IE_ERR_UNSUPPORTED, "%s: B x n_heads above 2^20", fn);
     ie::Kv8Write a{};
     a.B = B; a.P = 1; a.K = K_src; a.V = V_src; a.ld = src_stride;
     a.c = cache(k_cache, v_cache, k_scales, v_scales, block_table, num_blocks_per_seq, n_heads, d_head, block_size);

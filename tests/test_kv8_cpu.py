@@ -59,8 +59,9 @@ SOURCE = [(dict(K=None), INVALID), (dict(V=None), INVALID), (dict(K=P + 4), INVA
 CASES = [(write, LAYOUT + CACHE + SOURCE + [(dict(start=-1), INVALID), (dict(n=-1), INVALID), (dict(start=61), INVALID),
                                             (dict(n=65), INVALID), (dict(start=2**31 - 1), INVALID),
                                             (dict(start=2**30, nbps=2**27, bs=256), UNSUPPORTED),
-                                            (dict(B=2**20 + 1), UNSUPPORTED)]),
-         (append, LAYOUT + CACHE + SOURCE + [(dict(pos=None), INVALID), (dict(B=2**20 + 1), UNSUPPORTED)]),
+                                            (dict(B=2**20 + 1), UNSUPPORTED), (dict(B=2**20 + 1, H=1), UNSUPPORTED)]),
+         (append, LAYOUT + CACHE + SOURCE + [(dict(pos=None), INVALID), (dict(B=2**20 + 1), UNSUPPORTED),
+                                             (dict(B=2**20 + 1, H=1), UNSUPPORTED)]),
          (read, LAYOUT + CACHE + [(dict(n=-1), INVALID), (dict(starts=None), INVALID), (dict(K=None), INVALID),
                                   (dict(V=P + 8), INVALID), (dict(n=2**31 - 1), UNSUPPORTED)]),
          (decode, LAYOUT + CACHE + [(dict(Hq=3), INVALID), (dict(Hq=0), INVALID), (dict(mx=-1), INVALID),
