@@ -175,7 +175,8 @@ __device__ __forceinline__ void weights(const f32x4 (&acc)[4], float sw, float v
         st.m = mn;
         st.ub = ub;
     }
-    const float wc = vscale * pow2(254 - st.ub), m = st.m;
+    const float m = st.m;
+    float wc = vscale * pow2(254 - st.ub);
     float p[16], sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) p[i] = exp2_sm(fmaf(acc[i >> 2][i & 3], sw, -m));
@@ -183,6 +184,7 @@ __device__ __forceinline__ void weights(const f32x4 (&acc)[4], float sw, float v
         asm volatile("");
 #pragma unroll
         for (int i = 0; i < 16; ++i) p[i] = key0 + i < lim ? p[i] : 0.0f;
+        wc = key0 < lim ? wc : 0.0f;  // (a page that the row sees nothing of may have a scale that is not finite)
     }
 #pragma unroll
     for (int i = 0; i < 16; i += 2) {

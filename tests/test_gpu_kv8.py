@@ -255,6 +255,78 @@ def test_prompt(ie, dev, H, G, d, block, start, P):
     assert np.array_equal(got, check_prompt(ie, dev, c, table, start, Q))
 
 
+# ------------------------------------------------------------------ the prompt's forms
+# By workgroups of 64 rows (row: token x query head of a KV head): below 256 the split form, the contexts behind few
+# rows cut; from 256 two teams a block, from 1024 one, with 32 rows a wave where d = 128.
+FORMS = [(2, 3, 2, 64, 16, 300, 9), (1, 2, 3, 128, 64, 4100, 5),
+         (4, 16, 1, 64, 16, 0, 250), (4, 16, 1, 128, 32, 37, 251), (2, 16, 3, 128, 64, 5, 177), (16, 16, 4, 64, 256, 0, 13),
+         (8, 32, 1, 64, 16, 0, 250), (8, 32, 1, 128, 16, 100, 249), (4, 32, 5, 128, 64, 3, 103), (16, 64, 2, 64, 128, 0, 1)]
+
+
+def prompt_in_64_bits(dev, c, table, start, Q):
+    """(outputs, tolerances a row) as ko.attend, for all rows at once."""
+    import torch
+
+    B, P, H_q, d = Q.shape
+    G, n = H_q // c.heads, start + P
+    seen = torch.arange(n, device=dev) <= start + torch.arange(P, device=dev)[:, None]
+    out, tol = torch.empty((B, P, H_q, d), dtype=torch.float64), torch.empty((B, P, H_q), dtype=torch.float64)
+    for b in range(B):
+        for h in range(c.heads):
+            k, v = on(dev, *c.rows(table[b], n, h))
+            kt, ka = k.T.contiguous(), k.abs().T.contiguous()
+            for hq in range(h * G, (h + 1) * G):
+                q = on(dev, Q[b, :, hq]).double()
+                s = (q @ kt / d**0.5).masked_fill(~seen, -float("inf"))
+                S = (q.abs() @ ka / d**0.5).masked_fill(~seen, 0).amax(1)
+                most = torch.cummax(v.abs().amax(1), 0).values[start:]
+                out[b, :, hq] = (torch.softmax(s, 1) @ v).cpu()
+                tol[b, :, hq] = ((46 * S + 24 + seen.sum(1) / 16) * ko.U * most).cpu()
+    return out.numpy(), tol.numpy()
+
+
+@pytest.mark.parametrize("B,H,G,d,block,start,P", FORMS)
+def test_prompt_forms(ie, dev, B, H, G, d, block, start, P):
+    r = rng(B + H + G + d + start + P)
+    c, table = filled(r, [start + P] * B, H, d, block)
+    Q = rows(r, B, P, H * G, d)
+    want, tol = prompt_in_64_bits(dev, c, table, start, Q)
+    cache, tab, q = c.tensors(ie, dev), on(dev, table), on(dev, Q)
+    got = ie.prefill_attn_kv8(q, cache, tab, start)
+    assert (np.abs(got.cpu().numpy() - want).max(-1) <= tol).all()
+    assert np.array_equal(got.cpu().numpy(), ie.prefill_attn_kv8(q, cache, tab, start).cpu().numpy())
+    # without a workspace: the context in one piece
+    whole = got.clone().fill_(7)
+    ie.check("ie_prefill_attn_kv8", B, P, H * G, H, d, q.data_ptr(), *(t.data_ptr() for t in cache), tab.data_ptr(),
+             tab.shape[1], block, start, whole.data_ptr(), None, 0, ie._stream())
+    assert (np.abs(whole.cpu().numpy() - want).max(-1) <= tol).all()
+    need = ie.call("ie_prefill_kv8_workspace_bytes", B, P, H * G, H, d, start)
+    if need:
+        import torch
+
+        with pytest.raises(ie.IeError):
+            ie.prefill_attn_kv8(q, cache, tab, start, workspace=torch.empty(need // 4 - 1, device=dev))
+
+
+@pytest.mark.parametrize("bad", ["k", "v"])
+@pytest.mark.parametrize("B,H,G,d,block,start,P", FORMS)
+def test_prompt_rows_before_a_bad_page(ie, dev, B, H, G, d, block, start, P, bad):
+    """A page whose scale is not finite: NaN for the rows that see a token of it, for the others the bits they had."""
+    r = rng(B + H + G + d + start + P)
+    c, table = filled(r, [start + P] * B, H, d, block)
+    q, tab = on(dev, rows(r, B, P, H * G, d)), on(dev, table)
+    good = ie.prefill_attn_kv8(q, c.tensors(ie, dev), tab, start).cpu().numpy()
+    pages = range(start // block, (start + P - 1) // block + 1)
+    at = pages[(len(pages) + 1) // 2 if len(pages) > 2 else -1]
+    scales = c.ks if bad == "k" else c.vs
+    scales[table[0, at], 0] = np.inf if bad == "k" else np.nan
+    got = ie.prefill_attn_kv8(q, c.tensors(ie, dev), tab, start).cpu().numpy()
+    hit = np.zeros(good.shape[:3], bool)
+    hit[0, max(0, at * block - start):, :G] = True
+    assert np.isnan(got[hit]).all()
+    assert np.array_equal(got[~hit], good[~hit])
+
+
 def test_nothing_behind_the_context_counts(ie, dev):
     """Pages past the end (their table entries out of range) and rows behind it, whatever they hold: the bits of the
     answer do not move."""
