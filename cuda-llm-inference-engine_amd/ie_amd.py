@@ -413,12 +413,16 @@ def _bind_torch():
     _device_index = torch._C._cuda_getDevice
 
 
-def _made(stream, *tensors):
-    """Tensors allocated here for a call on another stream than the current one
-    are kept from reuse until that stream has passed."""
-    if stream is not None:
-        for t in tensors:
-            t.record_stream(stream)
+def _new(stream, shape, dtype, device):
+    """A tensor for a call on the given stream (None: the current one), of that
+    stream's memory: what another stream still does with memory it gave back
+    cannot meet it, nor can a later call there with this tensor's once freed."""
+    if stream is None:
+        return _empty(shape, dtype=dtype, device=device)
+    import torch
+
+    with torch.cuda.stream(stream):
+        return _empty(shape, dtype=dtype, device=device)
 
 
 class Kv8Cache(NamedTuple):
@@ -511,8 +515,7 @@ def kv8_cache_read(cache, block_table, starts, context_lens, n, out=None, stream
     H, bs, d, at = _kv8("kv8_cache_read", cache, block_table)
     B = block_table.shape[0]
     if out is None:
-        out = tuple(_empty((B, n, H, d), dtype=_f32, device=cache[0].device) for _ in range(2))
-        _made(stream, *out)
+        out = tuple(_new(stream, (B, n, H, d), _f32, cache[0].device) for _ in range(2))
     K, V = out
     want = (B, n, H, d)
     if not (starts.shape == (B,) and starts.dtype is _i32 and starts.get_device() == at and starts.is_contiguous()
@@ -538,8 +541,7 @@ def decode_attn_kv8(Q, cache, block_table, context_lens, max_ctx, splits=0, out=
     H, bs, d, at = _kv8("decode_attn_kv8", cache, block_table)
     B, H_q, dq = Q.shape
     if out is None:
-        out = _empty((B, H_q, d), dtype=_f32, device=Q.device)
-        _made(stream, out)
+        out = _new(stream, (B, H_q, d), _f32, Q.device)
     if not (dq == d and block_table.shape[0] == B and context_lens.shape == (B,) and out.shape == Q.shape
             and Q.dtype is _f32 and out.dtype is _f32 and context_lens.dtype is _i32 and Q.get_device() == at
             and out.get_device() == at and context_lens.get_device() == at and Q.is_contiguous() and out.is_contiguous()
@@ -548,8 +550,7 @@ def decode_attn_kv8(Q, cache, block_table, context_lens, max_ctx, splits=0, out=
     if workspace is None:
         S = decode_kv8_num_splits(B, H_q, H, d, max_ctx, splits)
         if S > 1:
-            workspace = _empty(B * H_q * S * (d + 2), dtype=_f32, device=Q.device)
-            _made(stream, workspace)
+            workspace = _new(stream, B * H_q * S * (d + 2), _f32, Q.device)
     elif workspace.dtype is not _f32 or workspace.get_device() != at or not workspace.is_contiguous():
         _refuse("decode_attn_kv8", workspace)
     k, v, ks, vs = cache
@@ -566,16 +567,14 @@ def prefill_attn_kv8(Q, cache, block_table, start_pos, out=None, workspace=None,
     H, bs, d, at = _kv8("prefill_attn_kv8", cache, block_table)
     B, P, H_q, dq = Q.shape
     if out is None:
-        out = _empty((B, P, H_q, d), dtype=_f32, device=Q.device)
-        _made(stream, out)
+        out = _new(stream, (B, P, H_q, d), _f32, Q.device)
     if not (dq == d and block_table.shape[0] == B and out.shape == Q.shape and Q.dtype is _f32 and out.dtype is _f32
             and Q.get_device() == at and out.get_device() == at and Q.is_contiguous() and out.is_contiguous()):
         _refuse("prefill_attn_kv8", Q, out, block_table)
     if workspace is None:
         need = call("ie_prefill_kv8_workspace_bytes", B, P, H_q, H, d, start_pos)
         if need:
-            workspace = _empty(need // 4, dtype=_f32, device=Q.device)
-            _made(stream, workspace)
+            workspace = _new(stream, need // 4, _f32, Q.device)
     elif workspace.dtype is not _f32 or workspace.get_device() != at or not workspace.is_contiguous():
         _refuse("prefill_attn_kv8", workspace)
     k, v, ks, vs = cache
@@ -611,10 +610,8 @@ def token_logprobs(logits, targets=None, k=0, out=None, workspace=None, stream=N
         _refuse("token_logprobs", targets)
     if out is None:
         dev = logits.device
-        out = (_empty(rows, dtype=_f32, device=dev), _empty(rows, dtype=_i32, device=dev),
-               _empty(rows, dtype=_f32, device=dev), _empty((rows, k), dtype=_f32, device=dev),
-               _empty((rows, k), dtype=_i32, device=dev))
-        _made(stream, *out)
+        out = (_new(stream, rows, _f32, dev), _new(stream, rows, _i32, dev), _new(stream, rows, _f32, dev),
+               _new(stream, (rows, k), _f32, dev), _new(stream, (rows, k), _i32, dev))
     else:
         lp, rk, en, tv, ti = out
         if not (lp.shape == (rows,) and rk.shape == (rows,) and en.shape == (rows,) and tv.shape == (rows, k)
@@ -626,8 +623,7 @@ def token_logprobs(logits, targets=None, k=0, out=None, workspace=None, stream=N
     if workspace is None:
         need = call("ie_token_logprobs_workspace_bytes", rows, n, k)
         if need:
-            workspace = _empty(need // 4, dtype=_f32, device=logits.device)
-            _made(stream, workspace)
+            workspace = _new(stream, need // 4, _f32, logits.device)
     elif workspace.dtype is not _f32 or workspace.get_device() != at or not workspace.is_contiguous():
         _refuse("token_logprobs", workspace)
     lp, rk, en, tv, ti = out

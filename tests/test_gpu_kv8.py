@@ -457,6 +457,29 @@ def test_graph_and_stream(ie, dev):
         (Q[i] * 2).sum().item()
 
 
+def test_results_made_for_another_stream(ie, dev):
+    """What a call on a given stream allocates comes from that stream's memory: work of the current stream that is still
+    under way on memory freed there cannot meet it."""
+    import torch
+
+    cache, tab = ie.Kv8Cache.empty(4, 2, 64, 16, dev), torch.arange(4, dtype=torch.int32, device=dev)[None]
+    K = torch.ones(1, 40, 2, 64, device=dev)
+    ie.kv8_cache_write(K, K, cache, tab, 0)
+    lens, x = torch.full((1,), 40, dtype=torch.int32, device=dev), torch.ones(64, 2 * 64, device=dev)
+    side = torch.cuda.Stream()
+    calls = [lambda s: ie.decode_attn_kv8(K[:, 0], cache, tab, lens, 64, stream=s),
+             lambda s: ie.prefill_attn_kv8(K, cache, tab, 0, stream=s),
+             lambda s: ie.kv8_cache_read(cache, tab, lens * 0, lens, 40, stream=s)[1],
+             lambda s: ie.token_logprobs(x, None, 3, stream=s).top_logprobs]
+    torch.cuda.synchronize()
+    for call in calls:
+        used = {call(None).data_ptr() for _ in range(4)}  # freed at once, ready for the current stream's next
+        got = call(side)
+        side.synchronize()
+        assert got.data_ptr() not in used
+        assert torch.equal(got, call(None))
+
+
 def test_binding_refusals(ie, dev):
     import torch
 
