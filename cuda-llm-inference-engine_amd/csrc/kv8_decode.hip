@@ -378,6 +378,53 @@ __global__ __launch_bounds__(256) void kv8_merge_kernel(int S, const float* __re
     }
 }
 
+// The same for at most MOST splits: a wave a row, without LDS.  With MOST 2 to 8 it
+// takes 0.6 us less (1 x 12 x 64, ctx 2048 in eight splits 6.05 against 6.65 in all;
+// 6144 rows of two 12.5 against 16.5); with 16, one wave's loads, 9.2 against 9.0.
+template <int D, int MOST>
+__global__ __launch_bounds__(256) void kv8_merge_few_kernel(int rows, int S, const float* __restrict__ ws, float* __restrict__ O) {
+    constexpr int C = D / 64;
+    const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (row >= rows) return;
+    const float* w = ws + (size_t)row * S * (D + 2);
+    float x[MOST][C], m[MOST], l[MOST];
+#pragma unroll
+    for (int u = 0; u < MOST; ++u) {
+        const float* p = w + min(u, S - 1) * (D + 2);
+#pragma unroll
+        for (int i = 0; i < C; ++i) x[u][i] = p[64 * i + lane];
+        m[u] = p[D];
+        l[u] = u < S ? p[D + 1] : 0.0f;
+    }
+    float mm = -INFINITY, lt = 0.0f, o[C];
+#pragma unroll
+    for (int u = 0; u < MOST; ++u) mm = l[u] == 0.0f ? mm : fmaxf(mm, m[u]);
+#pragma unroll
+    for (int i = 0; i < C; ++i) o[i] = 0.0f;
+#pragma unroll
+    for (int u = 0; u < MOST; ++u) {
+        const float f = l[u] == 0.0f ? 0.0f : exp2_sm(m[u] - mm);
+        lt = fmaf(l[u], f, lt);
+#pragma unroll
+        for (int i = 0; i < C; ++i) o[i] = fmaf(x[u][i], f, o[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < C; ++i) O[(size_t)row * D + 64 * i + lane] = lt == 0.0f ? 0.0f : o[i] / lt;
+}
+
+template <int D>
+void merge(int rows, int splits, const float* ws, float* O, hipStream_t s) {
+    const unsigned few = (unsigned)(rows + 3) / 4;
+    if (splits <= 2)
+        kv8_merge_few_kernel<D, 2><<<few, 256, 0, s>>>(rows, splits, ws, O);
+    else if (splits <= 4)
+        kv8_merge_few_kernel<D, 4><<<few, 256, 0, s>>>(rows, splits, ws, O);
+    else if (splits <= 8)
+        kv8_merge_few_kernel<D, 8><<<few, 256, 0, s>>>(rows, splits, ws, O);
+    else
+        kv8_merge_kernel<D><<<rows, 256, 0, s>>>(splits, ws, O);
+}
+
 template <int D>
 void launch(const Kv8Attn& a, hipStream_t s) {
     const int G = a.H_q / a.c.H;
@@ -397,9 +444,9 @@ void launch(const Kv8Attn& a, hipStream_t s) {
 
 void launch_kv8_merge(int d, int rows, int splits, const float* ws, float* O, hipStream_t s) {
     if (d == 64)
-        kv8_merge_kernel<64><<<rows, 256, 0, s>>>(splits, ws, O);
+        merge<64>(rows, splits, ws, O, s);
     else
-        kv8_merge_kernel<128><<<rows, 256, 0, s>>>(splits, ws, O);
+        merge<128>(rows, splits, ws, O, s);
 }
 
 void launch_decode_attn_kv8(const Kv8Attn& a, hipStream_t s) {

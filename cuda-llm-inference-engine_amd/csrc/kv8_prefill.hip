@@ -501,19 +501,31 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void kv8_prefill_split_ke
 int row_blocks(int P, int G, int rows) { return (int)(((long long)P * G + rows - 1) / rows); }
 
 // The form by its workgroups of 64 rows (a row: token x query head of a KV head):
-//   below 256 the block form leaves CUs idle, and 16-row workgroups of the split
-//     form fill them: 1 x 1024 x 8 x 128 (128 of them) 19 against 25 us, 1 x 512 x
-//     12 x 64 (96) 8.8 against 12.1; but 2 x 256 x (8 x 4) x 128 (256) 22 against 12.3;
-//   below 1024 two teams of four waves share a block's tiles: 4 x 512 x 12 x 64 (384)
-//     14.6 against 16.2 us on one team, 1 x 512 x (8 x 4) x 128 behind 4000 (256) 96
+//   Up to 32 rows a KV head leave most of the block form's without work: 64 x 4 x 16
+//     x 128 behind 1000 41.9 us in the split form against 101, 16 x 8 x (16 x 4) x 128
+//     (32 rows) 24.3 against 26.3; 48 rows 34.3 against 27.6.
+//   Below 128 the block form leaves CUs idle, and the split form's 16-row workgroups
+//     fill them: 1 x 512 x 12 x 64 (96) 7.9 against 10.2 us.  From 128 the split
+//     form has several a CU, which cost more than the block form's walk where that
+//     is short: 1 x 384 x (8 x 4) x 128 (192, 6 tiles) 20.5 against 13.2, 2 x 640 x
+//     12 x 64 (240, 10 tiles) 13.6 against 12.7, but 2 x 512 x 8 x 128 (128, 8 tiles)
+//     13.9 against 15.4, 1 x 1536 x 8 x 128 (192, 24 tiles) 28.6 against 34.  From 256
+//     the block form is ahead: 2 x 256 x (8 x 4) x 128 (256) 22 against 12.3.
+//   Below 1024 two teams of four waves share a block's tiles: 4 x 512 x 12 x 64 (384)
+//     13.5 against 16.2 us on one team, 1 x 512 x (8 x 4) x 128 behind 4000 (256) 96
 //     against 131;
 //   from there on one team: 4 x 1000 x (8 x 4) x 64 (2016) 52.5 against 60.3 us, and
 //     at d = 128 with 32 rows a wave, which read K and V from LDS half as often:
 //     1 x 4096 x (8 x 4) x 128 270 against 314 us (at d = 64 57 against 52.5).
 // The split form cuts the context so that there is about a workgroup a CU: 1 x 16
-// x (8 x 4) x 128 behind 4000 14.5 us against 31.6 in one piece; 1 x 77 there
-// (160 workgroups) takes 31.6 in one and 33 to 38 in two to eight.
-constexpr long long kBlockGroups = 256, kFullGroups = 1024;
+// x (8 x 4) x 128 behind 4000 13.0 us against 29 in one piece; 1 x 77 there
+// (160 workgroups) takes 29.5 in one and 33 to 38 in two to eight.
+constexpr long long kFullGroups = 1024;
+
+bool split_form(int B, int P, int G, int H_kv, int max_ctx) {
+    const long long groups = (long long)row_blocks(P, G, 64) * B * H_kv;
+    return row_blocks(P, G, 16) <= 2 || groups < 128 || (groups < 256 && groups < 24ll * ((max_ctx + kTile - 1) / kTile));
+}
 
 template <int D>
 void launch(const Kv8Attn& a, hipStream_t s) {
@@ -521,7 +533,7 @@ void launch(const Kv8Attn& a, hipStream_t s) {
     const int G = a.H_q / a.c.H, bh = a.B * a.c.H;
     const int n16 = row_blocks(a.P, G, 16), n64 = row_blocks(a.P, G, 64), n128 = row_blocks(a.P, G, 128);
     const long long groups = (long long)n64 * bh;
-    if (groups < kBlockGroups) {
+    if (split_form(a.B, a.P, G, a.c.H, a.max_ctx)) {
         kv8_prefill_split_kernel<D><<<(unsigned)n16 * bh * a.splits, 64 * NW, 0, s>>>(a, n16, qscale);
         if (a.splits > 1) launch_kv8_merge(D, a.B * a.P * a.H_q, a.splits, a.ws, a.O, s);
     } else if (groups < kFullGroups) {
@@ -537,7 +549,7 @@ void launch(const Kv8Attn& a, hipStream_t s) {
 
 int kv8_prefill_splits(int B, int P, int H_q, int H_kv, int max_ctx) {
     const int G = H_q / H_kv;
-    if ((long long)row_blocks(P, G, 64) * B * H_kv >= kBlockGroups) return 1;
+    if (!split_form(B, P, G, H_kv, max_ctx)) return 1;
     // a workgroup a CU, and a tile at least for each of its waves
     const long long groups = (long long)row_blocks(P, G, 16) * B * H_kv;
     const int each = (max_ctx + kTile * NW - 1) / (kTile * NW);

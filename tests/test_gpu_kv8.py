@@ -256,9 +256,11 @@ def test_prompt(ie, dev, H, G, d, block, start, P):
 
 
 # ------------------------------------------------------------------ the prompt's forms
-# By workgroups of 64 rows (row: token x query head of a KV head): below 256 the split form, the contexts behind few
-# rows cut; from 256 two teams a block, from 1024 one, with 32 rows a wave where d = 128.
-FORMS = [(2, 3, 2, 64, 16, 300, 9), (1, 2, 3, 128, 64, 4100, 5),
+# By workgroups of 64 rows (row: token x query head of a KV head): for up to 32 rows a head, below 128 and, behind a
+# context of many tiles, below 256 the split form, the contexts behind few rows cut; else two teams a block, from 1024
+# one, with 32 rows a wave where d = 128.
+FORMS = [(2, 3, 2, 64, 16, 300, 9), (1, 2, 3, 128, 64, 4100, 5), (8, 32, 1, 64, 16, 40, 20), (3, 16, 4, 128, 32, 60, 13),
+         (2, 16, 1, 128, 16, 700, 200),
          (4, 16, 1, 64, 16, 0, 250), (4, 16, 1, 128, 32, 37, 251), (2, 16, 3, 128, 64, 5, 177), (16, 16, 4, 64, 256, 0, 13),
          (8, 32, 1, 64, 16, 0, 250), (8, 32, 1, 128, 16, 100, 249), (4, 32, 5, 128, 64, 3, 103), (16, 64, 2, 64, 128, 0, 1)]
 
