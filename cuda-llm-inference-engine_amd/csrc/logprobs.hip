@@ -21,13 +21,16 @@
 // bit, and the least of them is the bound.  After the first tile no wave waits
 // for another before the row's end; then the lists are ranked by counting.
 //
-// Many rows are bound by HBM: 2048 x 50257, k = 20 92 us, 4.5 TB/s (a copy of 1 GiB
-// moves 4.7); k = 0 87 us.  (With the row held in registers, 25 words a thread,
+// Many rows are bound by HBM: 2048 x 50257, k = 20 91 us, 4.5 TB/s (a copy of 1 GiB
+// moves 4.7 to 5.2); k = 0 77 us.  (With the row held in registers, 25 words a thread,
 // 145 us: two rows a CU, which load and compute in step.)  Few rows are bound by
-// one wave's instructions and round trips: 8 x 50257, k = 5 12.5 us, of them 4 the
-// join's; loading a tile ahead changes nothing, 512 or 1024 threads a row gain
-// nothing (8 rows in 8 parts 13.2 and 22.5 against 13.9 us, 2048 rows 126 and 323
-// against 92).
+// one wave's instructions and waits (of a wave's 4.0 thousand issue slots with 64 rows,
+// k = 5, 2.2 are waits and 1.1 instructions): 8 x 50257, k = 5 10.5 us, of them 4 the
+// join's.  Six waves a SIMD at least: with eight, whose 78 scalar registers keep
+// 57 more in vector lanes, 512 x 50257, k = 5 32.7 against 31.1 us, 2048, k = 20
+// 88.6 against 91.4.  Two, six or eight words in flight a thread instead of four: 8 x
+// 50257 11.5, 11.4, 12.2 against 10.9 us; 512 or 1024 threads a row gain nothing
+// (8 rows in 8 parts 13.2 and 22.5 against 13.9 us, 2048 rows 126 and 323 against 92).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -64,19 +67,29 @@ __device__ __forceinline__ uint64_t packed(float v, int i) {
     return ((uint64_t)order_key(v) << 32) | (0xffffffffu - (uint32_t)i);
 }
 
-// Sum over the workgroup, in wave order; every thread gets it.  sh: one word a
-// wave, free for reuse at the next barrier but one.
-template <int T, typename V>
-__device__ __forceinline__ V block_sum(V v, V* sh) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
-    if (T == 64) return v;
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
-    __syncthreads();
-    V s = sh[0];
-#pragma unroll
-    for (int w = 1; w < T / 64; ++w) s += sh[w];
-    return s;
+// Largest over the wave, in every lane; NaN stays.
+__device__ __forceinline__ float wave_most(float v) {
+    v = max_of(v, dpp_row_ror<8>(v));
+    v = max_of(v, dpp_row_ror<4>(v));
+    v = max_of(v, dpp_row_ror<2>(v));
+    v = max_of(v, dpp_row_ror<1>(v));
+    float a, b;
+    pair16(v, a, b);
+    v = max_of(a, b);
+    pair32(v, a, b);
+    return max_of(a, b);
+}
+
+__device__ __forceinline__ uint32_t wave_largest(uint32_t v) {
+    v = max(v, (uint32_t)dpp_row_ror<8>((int)v));
+    v = max(v, (uint32_t)dpp_row_ror<4>((int)v));
+    v = max(v, (uint32_t)dpp_row_ror<2>((int)v));
+    v = max(v, (uint32_t)dpp_row_ror<1>((int)v));
+    float a, b;
+    pair16(__uint_as_float(v), a, b);
+    v = max(__float_as_uint(a), __float_as_uint(b));
+    pair32(__uint_as_float(v), a, b);
+    return max(__float_as_uint(a), __float_as_uint(b));
 }
 
 // Candidates pk[0 .. cnt) ranked (all different), out(rank, packed) for the
@@ -156,8 +169,17 @@ struct Candidates {
     }
 };
 
-// The first 20 bits of the need-th largest of the lanes' keys, need <= 64.
+// The need-th largest of the lanes' keys (need <= 64): exactly for the first few,
+// by taking the largest away, otherwise its first 20 bits, one ballot a bit.
 __device__ __forceinline__ uint32_t wave_bound(uint32_t key, int need) {
+    if (need <= 4) {  // uniform
+        uint32_t b = wave_largest(key);
+        for (int found = __popcll(__ballot(key == b)); found < need; found += __popcll(__ballot(key == b))) {
+            if (key >= b) key = 0;
+            b = wave_largest(key);
+        }
+        return b;
+    }
     uint32_t b = 0;
 #pragma unroll
     for (int bit = 31; bit >= 12; --bit) {
@@ -172,11 +194,11 @@ __device__ __forceinline__ uint32_t wave_bound(uint32_t key, int need) {
 // threads of the first part, those behind the last to threads of the last, one
 // each.  Places without an element hold -inf.
 template <int T>
-__global__ __launch_bounds__(T, 8) void logprobs_kernel(LogprobsArgs a, int parts, int words_per_part) {
+__global__ __launch_bounds__(T, 6) void logprobs_kernel(LogprobsArgs a, int parts, int words_per_part) {
     constexpr int W = T / 64;
     __shared__ __attribute__((aligned(16))) uint64_t pk[W * kList + 2];
-    __shared__ float sh_m[W], sh_e[W], sh_w[W], sh_t[W];
-    __shared__ int sh_a[W], sh_c[W];
+    __shared__ float4 sh_s[W];  // a wave's maximum and sums
+    __shared__ int2 sh_n[W];    // its count ahead of the target, its candidates
     __shared__ uint32_t sh_b[W];
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = (int)(blockIdx.x / (unsigned)parts), part = (int)(blockIdx.x % (unsigned)parts);
@@ -240,7 +262,6 @@ __global__ __launch_bounds__(T, 8) void logprobs_kernel(LogprobsArgs a, int part
         }
 #pragma unroll
         for (int q = 0; q < kWords; ++q) {
-            const float thr = c0 + q * T + tid < tw ? before : xt;
             auto add = [&](float f) {
                 const float d = fmaxf(f - mm, -3.0e38f);  // (finite: 0 times it is 0)
                 const float ev = exp2_sm(d * kLog2e);
@@ -248,12 +269,17 @@ __global__ __launch_bounds__(T, 8) void logprobs_kernel(LogprobsArgs a, int part
                 e += top ? 0.0f : ev;  // (a small rest beside the maximum's own 1 keeps its bits)
                 tops += top ? 1.0f : 0.0f;
                 w = fmaf(ev, d, w);
-                ahead += __popcll(__ballot(f > thr));
             };
             add(v[q].x);
             add(v[q].y);
             add(v[q].z);
             add(v[q].w);
+        }
+#pragma unroll
+        for (int q = 0; q < kWords; ++q) {  // (behind the sums, which do not wait for the target's logit)
+            const float thr = c0 + q * T + tid < tw ? before : xt;
+            ahead += __popcll(__ballot(v[q].x > thr)) + __popcll(__ballot(v[q].y > thr)) + __popcll(__ballot(v[q].z > thr)) +
+                     __popcll(__ballot(v[q].w > thr));
             if (lowest && c0 + q * T <= tw) {  // uniform
                 const bool in = c0 + q * T + tid < tw;
                 above += __popcll(__ballot(in && v[q].x > xt)) + __popcll(__ballot(in && v[q].y > xt)) +
@@ -262,15 +288,14 @@ __global__ __launch_bounds__(T, 8) void logprobs_kernel(LogprobsArgs a, int part
         }
         if (k == 0) continue;
         if (need <= 64) {
-            volatile uint32_t* said = sh_b;
-            if ((tile & (tile + 1)) == 0) {  // uniform
+            if (tile == 0 || ((tile & (tile + 1)) == 0 && c0 + T * kWords < w1)) {  // uniform
                 const uint32_t b = wave_bound(order_key(m), need);
-                if (lane == 0) said[wid] = b;
+                if (lane == 0) __hip_atomic_store(&sh_b[wid], b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
                 if (tile == 0) __syncthreads();
             }
-            uint32_t b = said[0];
+            uint32_t b = ~0u;
 #pragma unroll
-            for (int i = 1; i < W; ++i) b = min(b, said[i]);
+            for (int i = 0; i < W; ++i) b = min(b, __hip_atomic_load(&sh_b[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
             if (b > order_key(-INFINITY)) cand.bound = fmaxf(cand.bound, key_value(b));
         }
         int most_new = 0;
@@ -312,40 +337,50 @@ __global__ __launch_bounds__(T, 8) void logprobs_kernel(LogprobsArgs a, int part
         if (part == parts - 1) mine += max(t - (4 * words + head), 0);
         ahead += (wid == 0 ? mine : 0) - above;
     }
-    if (cand.cnt > 128) cand.cut(k, lane);
+    if (cand.cnt > 128) cand.cut(k, lane);  // (k <= 128)
 
-    // the threads' sums against the row's maximum
-    float rm = m;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) rm = max_of(rm, __shfl_xor(rm, o, 64));
+    // the threads' sums against the wave's maximum, then the waves' against the row's
+    const float wm = wave_most(m);
+    {
+        const float d = fmaxf(m - (wm == -INFINITY ? 0.0f : wm), -3.0e38f), f = exp2_sm(d * kLog2e), s = e + tops;
+        w = wave_sum(fmaf(s * f, d, w * f));
+        e = wave_sum(m == wm ? e : s * f);
+        tops = wave_sum(m == wm ? tops : 0.0f);
+    }
     if (lane == 0) {
-        sh_m[wid] = rm;
-        sh_c[wid] = cand.cnt;
+        sh_s[wid] = make_float4(wm, e, w, tops);
+        sh_n[wid] = make_int2(ahead, cand.cnt);
     }
     __syncthreads();
+    float rm = sh_s[0].x;
 #pragma unroll
-    for (int i = 0; i < W; ++i) rm = max_of(rm, sh_m[i]);
-    {
-        const float d = fmaxf(m - (rm == -INFINITY ? 0.0f : rm), -3.0e38f), f = exp2_sm(d * kLog2e), s = e + tops;
-        w = fmaf(s * f, d, w * f);
-        e = m == rm ? e : s * f;
-        tops = m == rm ? tops : 0.0f;
+    for (int i = 1; i < W; ++i) rm = max_of(rm, sh_s[i].x);
+    e = w = tops = 0.0f;
+    ahead = 0;
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+        const float4 o = sh_s[i];
+        const float d = fmaxf(o.x - (rm == -INFINITY ? 0.0f : rm), -3.0e38f), f = exp2_sm(d * kLog2e), s = o.y + o.w;
+        w += fmaf(s * f, d, o.z * f);
+        e += o.x == rm ? o.y : s * f;
+        tops += o.x == rm ? o.w : 0.0f;
+        ahead += sh_n[i].x;
     }
-    // (each value's words of LDS are its own, so the barriers between are enough)
-    e = block_sum<T>(e, sh_e);
-    w = block_sum<T>(w, sh_w);
-    tops = block_sum<T>(tops, sh_t);
-    ahead = block_sum<T>(lane == 0 ? ahead : 0, sh_a);
+    // What is only written to is read from the arguments here, so that the walk has
+    // its scalar registers (with all of them held, 57 were kept in vector lanes).
+    const __attribute__((address_space(4))) LogprobsArgs* z =
+        (const __attribute__((address_space(4))) LogprobsArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(z));
     const bool empty = rm == -INFINITY;
     const float rest = empty ? 0.0f : e + (tops - 1.0f);
     float L = 0.0f;
-    float* stats = a.ws + ((size_t)r * parts + part) * (kStats + 2 * k);
+    float* stats = z->ws + ((size_t)r * parts + part) * (kStats + 2 * k);
     if (parts == 1) {
         L = log1pf(rest) + (empty ? 0.0f : rm - rm);  // NaN for a row that holds NaN or +inf
         if (tid == 0) {
-            if (a.logprobs) a.logprobs[r] = !asked ? (t == -1 ? 0.0f : NAN) : empty ? -INFINITY : xt - rm - L;
-            if (a.ranks) a.ranks[r] = asked ? ahead + 1 : 0;
-            if (a.entropy) a.entropy[r] = empty ? 0.0f : L - w / (1.0f + rest);
+            if (z->logprobs) z->logprobs[r] = !asked ? (t == -1 ? 0.0f : NAN) : empty ? -INFINITY : xt - rm - L;
+            if (z->ranks) z->ranks[r] = asked ? ahead + 1 : 0;
+            if (z->entropy) z->entropy[r] = empty ? 0.0f : L - w / (1.0f + rest);
         }
     } else if (tid == 0) {
         stats[0] = rm;
@@ -360,8 +395,8 @@ __global__ __launch_bounds__(T, 8) void logprobs_kernel(LogprobsArgs a, int part
         const float val = key_value((uint32_t)(p >> 32));
         const int idx = (int)(0xffffffffu - (uint32_t)p);
         if (parts == 1) {
-            a.top_logprobs[(size_t)r * k + rank] = empty ? -INFINITY : val - rm - L;
-            a.top_idx[(size_t)r * k + rank] = idx;
+            z->top_logprobs[(size_t)r * k + rank] = empty ? -INFINITY : val - rm - L;
+            z->top_idx[(size_t)r * k + rank] = idx;
         } else {
             stats[kStats + rank] = val;
             stats[kStats + k + rank] = __int_as_float(idx);
@@ -372,16 +407,16 @@ __global__ __launch_bounds__(T, 8) void logprobs_kernel(LogprobsArgs a, int part
 #pragma unroll
     for (int i = 0; i < W; ++i) {
         if (i == wid) mine = cnt;
-        cnt += sh_c[i];
+        cnt += sh_n[i].y;
     }
     if (W > 1) {
-        uint64_t held[kList / 64];
+        uint64_t held[2];
 #pragma unroll
-        for (int i = 0; i < kList / 64; ++i)
+        for (int i = 0; i < 2; ++i)
             if (lane + 64 * i < cand.cnt) held[i] = cand.list[lane + 64 * i];
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < kList / 64; ++i)
+        for (int i = 0; i < 2; ++i)
             if (lane + 64 * i < cand.cnt) pk[mine + lane + 64 * i] = held[i];
     }
     if (tid < 2) pk[cnt + tid] = 0;
@@ -389,8 +424,8 @@ __global__ __launch_bounds__(T, 8) void logprobs_kernel(LogprobsArgs a, int part
     for (int i = tid; i < k; i += T)
         if (i >= cnt) {
             if (parts == 1) {
-                a.top_logprobs[(size_t)r * k + i] = NAN;
-                a.top_idx[(size_t)r * k + i] = i;
+                z->top_logprobs[(size_t)r * k + i] = NAN;
+                z->top_idx[(size_t)r * k + i] = i;
             } else {
                 stats[kStats + i] = -INFINITY;
                 stats[kStats + k + i] = __int_as_float(n);
@@ -468,18 +503,22 @@ int row_words(int n) { return std::max(n / 4, 1); }
 
 }  // namespace
 
-// A row's parts: four workgroups a CU, where at least four tiles of one workgroup
-// are shared out (the second launch costs about four tiles' time) and the join
-// ranks at most about 160 candidates.  50257 logits, k = 5: 8 rows 26.7 us in one
-// part, 13.9 in 8, 12.5 in 16; 128 rows 29.7, 20.1 in 8; 512 rows 35.7, 35.1 in 2;
-// k = 20: 16 rows 30.5, 16.5 in 8, 21.3 in 16.  64 x 8000, k = 5 (two tiles): 10.6,
-// 12.0 in 2.
+// A row's parts: up to five workgroups a CU, with as few tiles each as that allows
+// and no more parts than those need, where at least four tiles of one workgroup are
+// shared out (the second launch costs about four tiles' time) and the join ranks at
+// most about 160 candidates.  50257 logits (13 tiles), k = 5: 8 rows 25.1 us in one
+// part, 11.9 in 16, 10.8 in 13; 256 rows 29.8, 25.2 in 4, 24.5 in 5; 512 rows 35.4,
+// 34.3 in 2; k = 20: 16 rows 30.5, 16.5 in 8, 21.3 in 16; 300 x 32001, k = 1 25.2,
+// 22.9 in 3, 22.0 in 4.  64 x 8000, k = 5 (two tiles): 10.6, 12.0 in 2.
 int logprobs_parts(int rows, int n, int k) {
     const int words = row_words(n);
+    const int tiles = (words + kWide * kWords - 1) / (kWide * kWords);
     if (words < 4 * kWide * kWords - kWide) return 1;
-    int p = std::min(1024 / rows, kMostParts);
+    int p = std::min(1280 / rows, kMostParts);
     if (k > 0) p = std::min(p, 160 / k);
-    return std::max(p, 1);
+    p = std::max(p, 1);
+    const int each = (tiles + p - 1) / p;
+    return (tiles + each - 1) / each;
 }
 
 void launch_token_logprobs(const LogprobsArgs& a, hipStream_t s) {
