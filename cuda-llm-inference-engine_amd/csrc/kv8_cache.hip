@@ -10,7 +10,7 @@
 // scale had to grow) the earlier rows' new codes come from one pass over the data.
 //
 // Bound by HBM: 4 x 2000 rows of 8 x 128, K and V (65.5 MB in, 16.4 out) written in
-// 18.8 us, 4.4 TB/s, and read back in 16.5, 5.0 TB/s (a copy of 1 GiB moves 4.7).
+// 17.3 us, 4.7 TB/s, and read back in 15.0, 5.5 TB/s (a copy of 1 GiB moves 4.7 to 5.2).
 // The maximum goes over the wave by DPP and lane swaps: by six LDS permutes, with
 // 16-byte words of codes a lane (64-byte pieces of fp32 rows an instruction), the
 // write took 25.5 us and the read 20.8.
@@ -47,7 +47,6 @@ __device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
 }
 __device__ __forceinline__ int byte_of(uint32_t w, int i) { return (int)(int8_t)(w >> (8 * i)); }
 
-
 // Word j of a lane's four in tile t of a page: K row 4 (lane / 16) + j, V channel
 // 4 (lane % 16) + j.
 template <int D>
@@ -57,7 +56,8 @@ __device__ __forceinline__ int word_of(int t, bool is_v, int lane, int j) {
     return t / HALVES * (4 * D) + (is_v ? (c + j) * 4 + r / 4 : ((r + j) * D + c) / 4);
 }
 
-// blockIdx.x = ((b * npages + page) * H + h) * 2 + (K or V)
+// blockIdx.x = (b * npages + page) * H + h of K, then the same of V (K and V side by
+// side, two streams in and two out at once, took 18.7 us where this takes 17.3)
 template <int D, int T>
 __global__ __launch_bounds__(1024) void kv8_write_kernel(Kv8Write a, int npages) {
     constexpr int HALVES = D / 64;
@@ -65,8 +65,8 @@ __global__ __launch_bounds__(1024) void kv8_write_kernel(Kv8Write a, int npages)
     __shared__ float had_sh;
     const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, nw = blockDim.x >> 6;
     unsigned id = blockIdx.x;
-    const bool is_v = id & 1;
-    id >>= 1;
+    const bool is_v = id >= gridDim.x / 2;
+    if (is_v) id -= gridDim.x / 2;
     const int h = (int)(id % (unsigned)a.c.H);
     id /= (unsigned)a.c.H;
     const int j = (int)(id % (unsigned)npages), b = (int)(id / (unsigned)npages);
