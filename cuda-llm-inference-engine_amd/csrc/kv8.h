@@ -57,6 +57,13 @@ struct Kv8Attn {
     float* O;  // [B, P, H_q, d]
     float* ws;
     int splits;
+    // Decode with at most 4 query heads a KV head in one split may append first:
+    // K and V rows b * kv_ld to positions[b], attention over positions[b] + 1 of
+    // them (lens unused).  positions null: attention alone.
+    const float* K;
+    const float* V;
+    int kv_ld;
+    const int* positions;
 };
 void launch_decode_attn_kv8(const Kv8Attn& a, hipStream_t s);  // kv8_decode.hip
 // O rows [rows, d] from their splits' partials ws [rows, splits, d + 2]: sums, m, l (kv8_decode.hip).

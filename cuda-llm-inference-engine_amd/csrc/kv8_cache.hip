@@ -17,35 +17,10 @@
 #include <algorithm>
 
 #include "device_util.h"
-#include "kv8.h"
+#include "kv8_rule.h"
 
 namespace ie {
 namespace {
-
-constexpr float kFloor = 0x1p-100f;  // least scale (1 / scale stays finite)
-
-__device__ __forceinline__ uint32_t fbits(float x) { return __builtin_bit_cast(uint32_t, x); }
-__device__ __forceinline__ float bitsf(uint32_t x) { return __builtin_bit_cast(float, x); }
-// Larger of two values >= +0, where NaN is the largest.
-__device__ __forceinline__ float max_nan(float a, float b) { return bitsf(max(fbits(a), fbits(b))); }
-// Largest over the wave, in every lane.
-__device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
-    v = max(v, (uint32_t)dpp_row_ror<8>((int)v));
-    v = max(v, (uint32_t)dpp_row_ror<4>((int)v));
-    v = max(v, (uint32_t)dpp_row_ror<2>((int)v));
-    v = max(v, (uint32_t)dpp_row_ror<1>((int)v));
-    float a, b;
-    pair16(bitsf(v), a, b);
-    v = max(fbits(a), fbits(b));
-    pair32(bitsf(v), a, b);
-    return max(fbits(a), fbits(b));
-}
-// rint as an int; NaN gives 0.  |x| <= 127 * (1 + 2^-22) here: need / scale <= 1.
-__device__ __forceinline__ int code(float x) { return (int)rintf(x); }
-__device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
-    return (uint32_t)(a & 255) | (uint32_t)(b & 255) << 8 | (uint32_t)(c & 255) << 16 | (uint32_t)d << 24;
-}
-__device__ __forceinline__ int byte_of(uint32_t w, int i) { return (int)(int8_t)(w >> (8 * i)); }
 
 // Word j of a lane's four in tile t of a page: K row 4 (lane / 16) + j, V channel
 // 4 (lane % 16) + j.
@@ -113,13 +88,10 @@ __global__ __launch_bounds__(1024) void kv8_write_kernel(Kv8Write a, int npages)
     if (lane == 0) wave_mx[wid] = mx;
     __syncthreads();
     for (int w = 0; w < nw; ++w) mx = max(mx, wave_mx[w]);
-    const float had = had_sh;
-    const float need = max_nan(bitsf(mx) / 127.0f, kFloor);
-    const float scale = r0 == 0 ? need : need <= had ? had : max_nan(need, 1.25f * had);
-    const float inv = 1.0f / scale;
-    const bool grew = r0 > 0 && !(scale == had);
-    const float move = had * inv;
-    if (threadIdx.x == 0 && (r0 == 0 || grew)) *scale_at = scale;
+    const PageScale page(mx, r0, had_sh);
+    const bool grew = page.grew;
+    const float inv = page.inv, move = page.move;
+    if (threadIdx.x == 0 && (r0 == 0 || grew)) *scale_at = page.scale;
 #pragma unroll
     for (int i = 0; i < T; ++i) {
         const int t = wid * T + i, row0 = (t / HALVES) * 16;

@@ -149,10 +149,11 @@ int ie_decode_kv8_num_splits(int B, int H_q, int H_kv, int d, int max_context_le
     if (s <= 0) {
         // A workgroup a CU, and a tile at least for each of its four waves; one
         // split where more would spare a wave few tiles (about 0.7 us each at
-        // d = 64, 1.3 at 128, against 2 us of the merge and, past 64 workgroups,
-        // the memory they share): 1 x 12 x 64, ctx 1024 6.9 us in one and in four,
-        // 2048 9.6 and 6.9 in eight; 8 x 12 x 64, ctx 2048 9.9 and 10.8 in two, ctx 8000
-        // 30.2, 23.5 in two, 27.4 in three; 1 x (8 x 4) x 128, ctx 1000 10.7 and 8.7 in four.
+        // d = 64, 1.3 at 128, against the merge and its launch and, past 64
+        // workgroups, the memory they share): 1 x 12 x 64, ctx 1024 6.2 us in one and
+        // 6.1 in four, 2048 8.9 and 6.1 in eight; 8 x 12 x 64, ctx 2048 9.5 in one and
+        // in two, ctx 8000 26.3, 20.5 in two, 25.2 in three; 1 x (8 x 4) x 128, ctx 1000
+        // 9.5 and 8.2 in four.
         const int G = H_q / H_kv, heads = G <= 4 ? 4 : G <= 8 ? 8 : 16;
         const long long units = (long long)B * H_kv * ((G + heads - 1) / heads);
         const int each = (tiles + 3) / 4;

@@ -44,7 +44,7 @@
 #include <cmath>
 
 #include "device_util.h"
-#include "kv8.h"
+#include "kv8_rule.h"
 
 // The lanes of a quad take different digits of one number, so they must come to
 // the same bits: no product is fused into the quad's sums (which would round one
@@ -79,8 +79,50 @@ __device__ __forceinline__ uint32_t gather_bytes(uint32_t x0, uint32_t x1, uint3
     return __builtin_amdgcn_perm(hi, lo, 0x05040100u);
 }
 
-// blockIdx.x = ((b * H + h) * groups + head group) * splits + split
-template <int D, int NT, int HT>
+// One wave: sequence b's new row of K or of V, head h, at position pos of its
+// cache.  A page that grows is rare, so what it holds is read only then.
+template <int D>
+__device__ __forceinline__ void append_row(const Kv8Attn& a, bool is_v, int b, int h, int pos) {
+    constexpr int C = D / 64;  // channels a lane
+    const int lane = threadIdx.x & 63, bs = 1 << a.c.bs_log2, r = pos & (bs - 1);
+    const float* src = (is_v ? a.V : a.K) + (size_t)b * a.kv_ld + (size_t)h * D + C * lane;
+    float x[C];
+    uint32_t mx = 0;
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+        x[i] = src[i];
+        mx = max(mx, fbits(x[i]) & 0x7fffffffu);
+    }
+    const size_t pair = (size_t)a.c.table[(size_t)b * a.c.nbps + (pos >> a.c.bs_log2)] * a.c.H + h;
+    int8_t* codes = (is_v ? a.c.v : a.c.k) + pair * ((size_t)bs * D);
+    float* scale_at = (is_v ? a.c.vs : a.c.ks) + pair;
+    const PageScale page(wave_umax(mx), r, r > 0 ? *scale_at : 0.0f);
+    if (page.grew) {  // uniform
+        // a word: 4 channels of a row of K, 4 tokens of a channel of V
+        for (int i = lane; i < bs * D / 4; i += 64) {
+            const int row = is_v ? i / (4 * D) * 16 + i % 4 * 4 : i / (D / 4);
+            if (row >= r) continue;
+            uint32_t* at = reinterpret_cast<uint32_t*>(codes) + i;
+            const uint32_t was = *at;
+            int q[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                q[e] = byte_of(was, e);
+                if (!is_v || row + e < r) q[e] = code((float)q[e] * page.move);
+            }
+            *at = pack4(q[0], q[1], q[2], q[3]);
+        }
+        __threadfence_block();  // before the row's bytes, which may lie in those words
+    }
+    if (lane == 0 && (r == 0 || page.grew)) *scale_at = page.scale;
+#pragma unroll
+    for (int i = 0; i < C; ++i)
+        codes[is_v ? ((size_t)(r >> 4) * D + C * lane + i) * 16 + (r & 15) : (size_t)r * D + C * lane + i] = (int8_t)code(x[i] * page.inv);
+}
+
+// blockIdx.x = ((b * H + h) * groups + head group) * splits + split.  APPEND (one
+// workgroup a sequence and KV head): the sequence's new row first.
+template <int D, int NT, int HT, bool APPEND>
 __global__ __launch_bounds__(64 * NW, D == 64 ? (NT == 1 ? 4 : 3) : (NT == 1 ? 3 : 2)) void kv8_decode_kernel(Kv8Attn a, int groups, float qscale) {
     constexpr int KB = D / 64, JB = D / 16, HEADS = 4 * NT * HT;
     constexpr int TW = NW / HT;  // waves that share a set of heads
@@ -94,7 +136,11 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? (NT == 1 ? 4 : 3) : (NT == 1 ? 3
     id /= (unsigned)groups;
     const int H = a.c.H, h = (int)(id % (unsigned)H), b = (int)(id / (unsigned)H);
     const int G = a.H_q / H, g0 = hg * HEADS, gn = min(HEADS, G - g0);
-    const int n = max(0, min(a.lens[b], a.max_ctx));
+    const int n = max(0, min(APPEND ? a.positions[b] + 1 : a.lens[b], a.max_ctx));
+    if (APPEND) {
+        if (wid < 2 && n > 0) append_row<D>(a, wid == 1, b, h, n - 1);
+        __syncthreads();
+    }
     const int tiles = (n + kTile - 1) / kTile;
     const int t0 = (int)((unsigned)tiles * split / (unsigned)a.splits), t1 = (int)((unsigned)tiles * (split + 1) / (unsigned)a.splits);
 
@@ -431,12 +477,14 @@ void launch(const Kv8Attn& a, hipStream_t s) {
     const float qscale = (1.0f / sqrtf((float)D)) * 1.4426950408889634f;
     const int heads = G <= 4 ? 4 : G <= 8 ? 8 : 16, groups = (G + heads - 1) / heads;
     const unsigned grid = (unsigned)a.B * a.c.H * groups * a.splits;
-    if (heads == 4)
-        kv8_decode_kernel<D, 1, 1><<<grid, 64 * NW, 0, s>>>(a, groups, qscale);
+    if (a.positions)
+        kv8_decode_kernel<D, 1, 1, true><<<grid, 64 * NW, 0, s>>>(a, groups, qscale);
+    else if (heads == 4)
+        kv8_decode_kernel<D, 1, 1, false><<<grid, 64 * NW, 0, s>>>(a, groups, qscale);
     else if (heads == 8)
-        kv8_decode_kernel<D, 2, 1><<<grid, 64 * NW, 0, s>>>(a, groups, qscale);
+        kv8_decode_kernel<D, 2, 1, false><<<grid, 64 * NW, 0, s>>>(a, groups, qscale);
     else
-        kv8_decode_kernel<D, 2, 2><<<grid, 64 * NW, 0, s>>>(a, groups, qscale);
+        kv8_decode_kernel<D, 2, 2, false><<<grid, 64 * NW, 0, s>>>(a, groups, qscale);
     if (a.splits > 1) launch_kv8_merge(D, a.B * a.H_q, a.splits, a.ws, a.O, s);
 }
 

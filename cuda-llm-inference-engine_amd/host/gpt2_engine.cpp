@@ -496,17 +496,22 @@ struct GPT2Engine::Impl {
     }
 
     // The 8-bit cache: a decode step's K and V rows of qkv [B, 3d] appended at
-    // positions (which sets ctx_lens), then attention of its Q rows.
+    // positions and attention of its Q rows, in one launch where the fused step's
+    // context is in one split, else in two (the first sets ctx_lens).
     void kv8_step(int B, int l) {
         const int d = cfg.d_model;
-        ie::Kv8Write w{};
-        w.B = B; w.P = 1; w.K = qkv + d; w.V = qkv + 2 * d; w.ld = 3 * d;
-        w.c = layer_kv8(l); w.positions = positions; w.ctx_lens = ctx_lens;
-        ie::launch_kv8_write(w, stream);
-        IEC(ie::check_launch("kv8 append"));
         ie::Kv8Attn a{};
-        a.B = B; a.P = 1; a.H_q = cfg.n_heads; a.Q = qkv; a.q_ld = 3 * d; a.c = w.c;
+        a.B = B; a.P = 1; a.H_q = cfg.n_heads; a.Q = qkv; a.q_ld = 3 * d; a.c = layer_kv8(l);
         a.lens = ctx_lens; a.max_ctx = plan.max_ctx; a.O = attn; a.ws = ws; a.splits = plan.splits;
+        if (fused && plan.splits == 1) {
+            a.K = qkv + d; a.V = qkv + 2 * d; a.kv_ld = 3 * d; a.positions = positions;
+        } else {
+            ie::Kv8Write w{};
+            w.B = B; w.P = 1; w.K = qkv + d; w.V = qkv + 2 * d; w.ld = 3 * d;
+            w.c = a.c; w.positions = positions; w.ctx_lens = ctx_lens;
+            ie::launch_kv8_write(w, stream);
+            IEC(ie::check_launch("kv8 append"));
+        }
         ie::launch_decode_attn_kv8(a, stream);
         IEC(ie::check_launch("decode_attn_kv8"));
     }
@@ -763,7 +768,8 @@ struct GPT2Engine::Impl {
     // the output directly.  Computed from the host's position mirror, so the
     // captured graph for that plan can be replayed.
     // The 8-bit cache's attention takes contexts of up to 1024 in one split (one
-    // launch; 12 heads of 64 6.8 us, in four splits 6.9), longer ones by 512.
+    // launch with the append; 12 heads of 64 6.2 us without it, in four splits and
+    // their merge 6.1), longer ones by 512.
     static constexpr int kTokensPerSplit = 384;
     AttnPlan plan_for(int ctx) const {
         AttnPlan p;

@@ -139,6 +139,22 @@ def test_bits_hold_over_graphs_fusion_and_batch(ie, small_dir):
         assert all(np.array_equal(a[b:b + 1], o) for a, o in zip(base, alone))
 
 
+def test_heads_of_128(ie, tmp_path):
+    """The same at 128 channels a head: against the oracle, and the fused step (append and attention in one launch)
+    against the unfused one's two."""
+    ie.write_random_model(tmp_path, seed=24, n_layers=1, n_heads=6, vocab_size=1000, max_seq_len=128)
+    r = np.random.default_rng(8)
+    a, b = (ie.Engine(tmp_path, max_batch=2, kv_dtype=ie.KV_I8, fuse=f) for f in (True, False))
+    om = oracle(tmp_path, 2)
+    prompt = r.integers(0, 1000, (2, 5))
+    near(a.prefill(prompt), om.prompt(prompt))
+    b.prefill(prompt)
+    for t in r.integers(0, 1000, (30, 2)):
+        got = a.step(t)
+        assert np.array_equal(got, b.step(t))
+        near(got, om.step(t))
+
+
 def test_splits_past_1024_tokens(ie, tmp_path):
     """Contexts past 1024 take more than one split: on both sides of the change."""
     cfg = dict(TINY, n_layers=1, max_seq_len=1100)
