@@ -27,11 +27,17 @@
 // part of the context on their own, straight from the cache, and merge in LDS in
 // wave order, the parts in a second launch.
 //
-// The block form is bound by the matrix cores: 1 x 4096 x (8 x 4) x 128 270 us is
-// 509 TFLOP/s of attention, 1018 of half-precision products (a large library product
-// in bf16 reaches 1108 on the same card); with one tile in flight or two it is the
-// same, so not by memory.  The split form is bound by its conversions of K and V
-// (320 of 606 vector instructions a tile at d = 128).
+// The block form is bound by the matrix cores and the vector units together: 1 x
+// 4096 x (8 x 4) x 128 230 us on one card, 261 on a slower one: 597 and 526 TFLOP/s
+// of attention, twice that of half-precision products (a large library product in
+// bf16 reaches 1108 to 1121), matrix cores busy 48%, vector units 46% of the 230.
+// Two waves share a SIMD there, and with the one that has its scores put first
+// (s_setprio) from the weights to the end of the second product the two take turns,
+// one with each unit: without, 264 and 283 us.  (With four waves a SIMD, d = 64, it costs 3%, and is left out.)  Where a
+// launch puts two blocks on some CUs, the shortest go beside the longest: 1 x 2048 x
+// (8 x 4) x 128 96 -> 91 us, 4 x 640 x 12 x 64 15.6 -> 14.1.  With one tile in flight
+// or two it is the same, so not by memory.  The split form is bound by its conversions
+// of K and V (320 of 606 vector instructions a tile at d = 128).
 #include <algorithm>
 #include <cmath>
 
@@ -207,7 +213,7 @@ __device__ __forceinline__ int k_word(int s, int kg, int t, int m) {
     return (s * 4 + kg) * 64 + t * 16 + (m ^ (((t ^ (2 * s + (kg >> 1))) & 3) << 2));
 }
 
-// blockIdx.x = (row blocks, last first) * (B * H) + (sequence, KV head)
+// blockIdx.x = (row blocks, last first) * (B * H) + (sequence, KV head), but see below
 template <int D, int NC, int TM>
 __global__ __launch_bounds__(256 * TM, D == 64 ? (NC == 1 ? 4 : 3) : (NC == 1 ? 3 : 2)) void kv8_prefill_block_kernel(Kv8Attn a, int blocks,
                                                                                              float qscale) {
@@ -218,8 +224,15 @@ __global__ __launch_bounds__(256 * TM, D == 64 ? (NC == 1 ? 4 : 3) : (NC == 1 ? 
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
     const int team = TM == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
     const int H = a.c.H, G = a.H_q / H;
-    const unsigned bh = blockIdx.x % (unsigned)(a.B * H);
-    const int blk = blocks - 1 - (int)(blockIdx.x / (unsigned)(a.B * H));
+    unsigned id = blockIdx.x;
+    if constexpr (D == 64 || NC == 2) {
+        // Two workgroups fit a CU: where those from 256 on are second ones of a CU, the
+        // shortest of them join the longest of the first.  (Bits 0 to 2, the XCD, stay.)
+        const unsigned full = gridDim.x & ~7u;
+        if (gridDim.x <= 512 && id >= 256 && id < full) id = 256 + full - 8 - (id & ~7u) + (id & 7u);
+    }
+    const unsigned bh = id % (unsigned)(a.B * H);
+    const int blk = blocks - 1 - (int)(id / (unsigned)(a.B * H));
     const int h = (int)(bh % (unsigned)H), b = (int)(bh / (unsigned)H);
     const int rows = a.P * G, row0 = blk * ROWS;
     const int n = a.start + min(row0 + ROWS - 1, rows - 1) / G + 1;  // keys that the block sees
@@ -301,12 +314,14 @@ __global__ __launch_bounds__(256 * TM, D == 64 ? (NC == 1 ? 4 : 3) : (NC == 1 ? 
 #pragma unroll
                     for (int t = 0; t < 4; ++t) acc[c][t] = mfma(k[t], q[c].hi[s], acc[c][t]);
             }
+            if (NC == 2) __builtin_amdgcn_s_setprio(1);
             const float2 sc = sh_s[team][buf][q4];
             const bool edge = (tile + 1) * kTile > wmin;
             u32x4 hi[NC][2], lo[NC][2];
 #pragma unroll
             for (int c = 0; c < NC; ++c)
                 weights<D>(acc[c], q[c].scale * sc.x, sc.y, tile * kTile + 16 * q4, q[c].lim, edge, st[c], hi[c], lo[c]);
+            if (NC == 2) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int j = 0; j < J; ++j) {
                 u32x4 v[2];
@@ -321,6 +336,7 @@ __global__ __launch_bounds__(256 * TM, D == 64 ? (NC == 1 ? 4 : 3) : (NC == 1 ? 
 #pragma unroll
                     for (int c = 0; c < NC; ++c) st[c].o[j] = mfma(v[u], hi[c][u], st[c].o[j]);
             }
+            if (NC == 2) __builtin_amdgcn_s_setprio(0);
         }
         if (i + 1 < rounds) stage(buf ^ 1);
         __syncthreads();
@@ -512,11 +528,11 @@ int row_blocks(int P, int G, int rows) { return (int)(((long long)P * G + rows -
 //     13.9 against 15.4, 1 x 1536 x 8 x 128 (192, 24 tiles) 28.6 against 34.  From 256
 //     the block form is ahead: 2 x 256 x (8 x 4) x 128 (256) 22 against 12.3.
 //   Below 1024 two teams of four waves share a block's tiles: 4 x 512 x 12 x 64 (384)
-//     13.5 against 16.2 us on one team, 1 x 512 x (8 x 4) x 128 behind 4000 (256) 96
+//     12.8 against 16.2 us on one team, 1 x 512 x (8 x 4) x 128 behind 4000 (256) 96
 //     against 131;
 //   from there on one team: 4 x 1000 x (8 x 4) x 64 (2016) 52.5 against 60.3 us, and
 //     at d = 128 with 32 rows a wave, which read K and V from LDS half as often:
-//     1 x 4096 x (8 x 4) x 128 270 against 314 us (at d = 64 57 against 52.5).
+//     1 x 4096 x (8 x 4) x 128 264 against 314 us (at d = 64 57 against 52.5).
 // The split form cuts the context so that there is about a workgroup a CU: 1 x 16
 // x (8 x 4) x 128 behind 4000 13.0 us against 29 in one piece; 1 x 77 there
 // (160 workgroups) takes 29.5 in one and 33 to 38 in two to eight.

@@ -29,7 +29,11 @@
  * by at most half a scale; one whose page grew under it by at most 2.5 scales
  * (0.5 / (1 - 1/1.25)), however often it grew.  Rows behind the written ones
  * keep their bytes and count as dropped.  A non-finite value makes its page's
- * scale non-finite, and attention that reads the page returns NaN.
+ * scale non-finite until the page starts anew, and attention of a query that
+ * sees a token of the page returns NaN.
+ *
+ * A workspace serves one call at a time: calls that may run at once (on two
+ * streams, from two replayed graphs) take one each.  No output overlaps an input.
  */
 #ifndef IE_KV8_H
 #define IE_KV8_H

@@ -31,11 +31,14 @@ size_t ie_token_logprobs_workspace_bytes(int rows, int n, int k);
  *   top_logprobs / top_idx [rows, k]: the k largest by value descending, equal
  *     values by index ascending (+0 and -0 are equal), as ie_topk's; 0 <= k <=
  *     min(n, IE_LOGPROBS_TOP_MAX).
- * logprobs, ranks and entropy may each be NULL.  A logit of -inf has probability 0 (log -inf); a row of nothing else
- * has log probabilities -inf and entropy 0; so is one below fp32's range.  A row that holds NaN or +inf has
- * NaN log probabilities and entropy, and its ranks and indices say nothing
- * (the indices lie in [0, n)).  n <= IE_LOGPROBS_N_MAX.  Sums are fp32 over a
- * fixed order: a repeated call repeats its bits. */
+ * logprobs, ranks and entropy may each be NULL.  A logit of -inf has
+ * probability 0 (log probability -inf, as has one below fp32's range); a row
+ * of nothing else has log probabilities -inf and entropy 0.  A row that holds
+ * NaN or +inf has NaN log probabilities and entropy, and its ranks and indices
+ * say nothing (the indices lie in [0, n)).  n <= IE_LOGPROBS_N_MAX.  Sums are
+ * fp32 over a fixed order: a repeated call repeats its bits.  A workspace
+ * serves one call at a time: calls that may run at once (on two streams, from
+ * two replayed graphs) take one each. */
 int ie_token_logprobs(int rows, const float* logits, int row_stride, int n, const int* targets,
                       int k, float* logprobs, int* ranks, float* entropy, float* top_logprobs,
                       int* top_idx, float* workspace, size_t workspace_bytes, ie_stream_t stream);
