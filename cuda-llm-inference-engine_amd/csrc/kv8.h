@@ -69,7 +69,7 @@ void launch_decode_attn_kv8(const Kv8Attn& a, hipStream_t s);  // kv8_decode.hip
 // O rows [rows, d] from their splits' partials ws [rows, splits, d + 2]: sums, m, l (kv8_decode.hip).
 void launch_kv8_merge(int d, int rows, int splits, const float* ws, float* O, hipStream_t s);
 // Splits of the context that launch_prefill_attn_kv8 works with best (above 1 it needs the workspace).
-int kv8_prefill_splits(int B, int P, int H_q, int H_kv, int max_ctx);
+int kv8_prefill_splits(int B, int P, int H_q, int H_kv, int d, int max_ctx);
 void launch_prefill_attn_kv8(const Kv8Attn& a, hipStream_t s);  // kv8_prefill.hip
 
 }  // namespace ie

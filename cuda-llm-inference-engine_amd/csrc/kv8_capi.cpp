@@ -202,10 +202,10 @@ int ie_decode_attn_kv8(int B, int H_q, int H_kv, int d, const float* Q, const vo
 }
 
 size_t ie_prefill_kv8_workspace_bytes(int B, int P, int H_q, int H_kv, int d, int start_pos) {
-    if (B <= 0 || P <= 0 || H_kv <= 0 || H_q <= 0 || H_q % H_kv || d <= 0 || start_pos < 0 ||
+    if (B <= 0 || P <= 0 || H_kv <= 0 || H_q <= 0 || H_q % H_kv || (d != 64 && d != 128) || start_pos < 0 ||
         (long long)start_pos + P > kMaxContext || (long long)((P + 15) / 16) * H_q * B > kMaxGroups)
         return 0;
-    const int S = ie::kv8_prefill_splits(B, P, H_q, H_kv, start_pos + P);
+    const int S = ie::kv8_prefill_splits(B, P, H_q, H_kv, d, start_pos + P);
     return S > 1 ? (size_t)B * P * H_q * S * (d + 2) * sizeof(float) : 0;
 }
 
@@ -231,7 +231,7 @@ int ie_prefill_attn_kv8(int B, int P, int H_q, int H_kv, int d, const float* Q, 
     a.B = B; a.P = P; a.H_q = H_q; a.Q = Q; a.q_ld = H_q * d;
     a.c = cache(k_cache, v_cache, k_scales, v_scales, block_table, num_blocks_per_seq, H_kv, d, block_size);
     a.start = start_pos; a.max_ctx = start_pos + P; a.O = O;
-    a.splits = workspace ? ie::kv8_prefill_splits(B, P, H_q, H_kv, start_pos + P) : 1;
+    a.splits = workspace ? ie::kv8_prefill_splits(B, P, H_q, H_kv, d, start_pos + P) : 1;
     if (a.splits > 1) {
         const size_t need = ie_prefill_kv8_workspace_bytes(B, P, H_q, H_kv, d, start_pos);
         if (!aligned(workspace, 8)) return fail(IE_ERR_INVALID, "%s: workspace must be 8-byte aligned", fn);

@@ -25,7 +25,7 @@
 // of two such teams each takes every other tile and they merge at the end.
 // split: the rows of a workgroup are 16, its waves take every NW-th tile of its
 // part of the context on their own, straight from the cache, and merge in LDS in
-// wave order, the parts in a second launch.
+// wave order.  Either takes a context in parts, joined in a second launch.
 //
 // The block form is bound by the matrix cores and the vector units together: 1 x
 // 4096 x (8 x 4) x 128 230 us on one card, 261 on a slower one: 597 and 526 TFLOP/s
@@ -213,10 +213,10 @@ __device__ __forceinline__ int k_word(int s, int kg, int t, int m) {
     return (s * 4 + kg) * 64 + t * 16 + (m ^ (((t ^ (2 * s + (kg >> 1))) & 3) << 2));
 }
 
-// blockIdx.x = (row blocks, last first) * (B * H) + (sequence, KV head), but see below
-template <int D, int NC, int TM>
-__global__ __launch_bounds__(256 * TM, D == 64 ? (NC == 1 ? 4 : 3) : (NC == 1 ? 3 : 2)) void kv8_prefill_block_kernel(Kv8Attn a, int blocks,
-                                                                                             float qscale) {
+// blockIdx.x = (row blocks, last first) * (B * H) + (sequence, KV head), but see
+// below; CUT: that * splits + split, and partial results to the workspace.
+template <int D, int NC, int TM, bool CUT>
+__global__ __launch_bounds__(256 * TM, D == 64 ? 4 : 2) void kv8_prefill_block_kernel(Kv8Attn a, int blocks, float qscale) {
     constexpr int S = D / 32, J = D / 16, CH = D / 64, ROWS = 64 * NC;
     // the teams' halves of K and V; at the end the other teams' outputs
     __shared__ u32x4 sh_kv[TM][2][2][8 * D];
@@ -224,8 +224,9 @@ __global__ __launch_bounds__(256 * TM, D == 64 ? (NC == 1 ? 4 : 3) : (NC == 1 ? 
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
     const int team = TM == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
     const int H = a.c.H, G = a.H_q / H;
-    unsigned id = blockIdx.x;
-    if constexpr (D == 64 || NC == 2) {
+    const int splits = CUT ? a.splits : 1, split = CUT ? (int)(blockIdx.x % (unsigned)splits) : 0;
+    unsigned id = CUT ? blockIdx.x / (unsigned)splits : blockIdx.x;
+    if constexpr (!CUT && (D == 64 || NC == 2)) {
         // Two workgroups fit a CU: where those from 256 on are second ones of a CU, the
         // shortest of them join the longest of the first.  (Bits 0 to 2, the XCD, stay.)
         const unsigned full = gridDim.x & ~7u;
@@ -236,7 +237,9 @@ __global__ __launch_bounds__(256 * TM, D == 64 ? (NC == 1 ? 4 : 3) : (NC == 1 ? 
     const int h = (int)(bh % (unsigned)H), b = (int)(bh / (unsigned)H);
     const int rows = a.P * G, row0 = blk * ROWS;
     const int n = a.start + min(row0 + ROWS - 1, rows - 1) / G + 1;  // keys that the block sees
-    const int tiles = (n + kTile - 1) / kTile, last = (n - 1) >> 4;
+    const int all = (n + kTile - 1) / kTile, last = (n - 1) >> 4;
+    const int t0 = CUT ? (int)((unsigned)all * split / (unsigned)splits) : 0;
+    const int tiles = CUT ? (int)((unsigned)all * (split + 1) / (unsigned)splits) : all;  // (the end of this part)
     const int lgg = a.c.bs_log2 - 4, gmask = (1 << lgg) - 1;
     const int* table = a.c.table + (size_t)b * a.c.nbps;
 
@@ -269,7 +272,7 @@ __global__ __launch_bounds__(256 * TM, D == 64 ? (NC == 1 ? 4 : 3) : (NC == 1 ? 
         if (lane == 0) sh_s[team][buf][wid] = make_float2(ks + ((ks - ks) + (vs - vs)), vs);
     };
     // the i-th tile of this team (past the last one: the last again)
-    auto nth = [&](int i) { return min(team + i * TM, tiles - 1); };
+    auto nth = [&](int i) { return max(min(t0 + team + i * TM, tiles - 1), 0); };
     int page = entry(nth(0));
     fetch(nth(0), page);
     page = entry(nth(1));
@@ -287,9 +290,9 @@ __global__ __launch_bounds__(256 * TM, D == 64 ? (NC == 1 ? 4 : 3) : (NC == 1 ? 
     const int q4 = lane >> 4, m16 = lane & 15;
     stage(0);
     __syncthreads();
-    const int rounds = (tiles + TM - 1) / TM;  // (every wave makes every round: the barriers are the workgroup's)
+    const int rounds = (tiles - t0 + TM - 1) / TM;  // (every wave makes every round: the barriers are the workgroup's)
     for (int i = 0; i < rounds; ++i) {
-        const int tile = team + i * TM, buf = i & 1;
+        const int tile = t0 + team + i * TM, buf = i & 1;
         if (i + 1 < rounds) {
             fetch(nth(i + 1), page);
             page = entry(nth(i + 2));
@@ -370,7 +373,25 @@ __global__ __launch_bounds__(256 * TM, D == 64 ? (NC == 1 ? 4 : 3) : (NC == 1 ? 
                 st[c].o[j] = st[c].o[j] * u0 + f32x4{o.x, o.y, o.z, o.w} * u1;
             }
             st[c].ub = 127;
+            st[c].m = mm;
         }
+    }
+    if constexpr (CUT) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int row = wrow + 16 * c + m16;
+            if (row < rows) {
+                const float f = pow2(st[c].ub);
+                float* out = a.ws + ((((size_t)b * a.P + row / G) * a.H_q + (size_t)h * G + row % G) * splits + split) * (D + 2);
+#pragma unroll
+                for (int j = 0; j < J; ++j) {  // (8-byte aligned)
+                    *reinterpret_cast<float2*>(out + 16 * j + 4 * q4) = make_float2(st[c].o[j][0] * f, st[c].o[j][1] * f);
+                    *reinterpret_cast<float2*>(out + 16 * j + 4 * q4 + 2) = make_float2(st[c].o[j][2] * f, st[c].o[j][3] * f);
+                }
+                if (q4 == 0) *reinterpret_cast<float2*>(out + D) = make_float2(st[c].m, st[c].l);
+            }
+        }
+        return;
     }
     // lane: row lane & 15 of each 16, channels 16 j + 4 q4 + r
 #pragma unroll
@@ -516,61 +537,100 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void kv8_prefill_split_ke
 
 int row_blocks(int P, int G, int rows) { return (int)(((long long)P * G + rows - 1) / rows); }
 
-// The form by its workgroups of 64 rows (a row: token x query head of a KV head):
+// The form of a call and the parts of its contexts.  A row is a token x query head
+// of a KV head; g16, g64, g128 are the workgroups of that many rows.
+//
+// Contexts in one piece:
 //   Up to 32 rows a KV head leave most of the block form's without work: 64 x 4 x 16
 //     x 128 behind 1000 41.9 us in the split form against 101, 16 x 8 x (16 x 4) x 128
 //     (32 rows) 24.3 against 26.3; 48 rows 34.3 against 27.6.
-//   Below 128 the block form leaves CUs idle, and the split form's 16-row workgroups
-//     fill them: 1 x 512 x 12 x 64 (96) 7.9 against 10.2 us.  From 128 the split
-//     form has several a CU, which cost more than the block form's walk where that
-//     is short: 1 x 384 x (8 x 4) x 128 (192, 6 tiles) 20.5 against 13.2, 2 x 640 x
-//     12 x 64 (240, 10 tiles) 13.6 against 12.7, but 2 x 512 x 8 x 128 (128, 8 tiles)
-//     13.9 against 15.4, 1 x 1536 x 8 x 128 (192, 24 tiles) 28.6 against 34.  From 256
-//     the block form is ahead: 2 x 256 x (8 x 4) x 128 (256) 22 against 12.3.
+//   Below g64 = 128 the block form leaves CUs idle, and the split form's 16-row
+//     workgroups fill them: 1 x 512 x 12 x 64 (96) 7.9 against 10.2 us.  From 128 the
+//     split form has several a CU, which cost more than the block form's walk where
+//     that is short: 1 x 384 x (8 x 4) x 128 (192, 6 tiles) 20.5 against 13.2, 2 x 640
+//     x 12 x 64 (240, 10 tiles) 13.6 against 12.7, but 2 x 512 x 8 x 128 (128, 8
+//     tiles) 13.9 against 15.4, 1 x 1536 x 8 x 128 (192, 24 tiles) 28.6 against 34.
+//     From 256 the block form is ahead: 2 x 256 x (8 x 4) x 128 (256) 22 against 12.3.
 //   Below 1024 two teams of four waves share a block's tiles: 4 x 512 x 12 x 64 (384)
-//     12.8 against 16.2 us on one team, 1 x 512 x (8 x 4) x 128 behind 4000 (256) 96
-//     against 131;
-//   from there on one team: 4 x 1000 x (8 x 4) x 64 (2016) 52.5 against 60.3 us, and
-//     at d = 128 with 32 rows a wave, which read K and V from LDS half as often:
-//     1 x 4096 x (8 x 4) x 128 264 against 314 us (at d = 64 57 against 52.5).
-// The split form cuts the context so that there is about a workgroup a CU: 1 x 16
-// x (8 x 4) x 128 behind 4000 13.0 us against 29 in one piece; 1 x 77 there
-// (160 workgroups) takes 29.5 in one and 33 to 38 in two to eight.
-constexpr long long kFullGroups = 1024;
+//     12.8 against 16.2 us on one team; from there on one team: 4 x 1000 x (8 x 4) x
+//     64 (2016) 52.5 against 60.3 us, and at d = 128 with 32 rows a wave, which read K
+//     and V from LDS half as often: 1 x 4096 x (8 x 4) x 128 264 against 314 us (at d
+//     = 64 57 against 52.5).
+//
+// Cut contexts (their parts joined by a second launch):
+//   The split form up to g16 = 128, for about a workgroup a CU: 1 x 16 x (8 x 4) x 128
+//     behind 4000 13.0 us against 29 in one piece.
+//   Up to 208 (the split form uncut leaves CUs idle, and cut has some with two): two
+//     teams, a block a CU (two at d = 64): 1 x 77 x (8 x 4) x 128 behind 4001 (160) 26.2
+//     in six parts against 29.8, at d = 64 17.6 against 19.8.
+//   From 256 on, behind a context of the chunk's length at least and for parts of 8
+//     to 10 tiles or more.  d = 128: 32 rows a wave, two blocks a CU: 1 x 300 x (8 x 4)
+//     behind 4000 55.2 in six parts against 74.7 uncut, 1 x 512 77.8 against 85.7, 1 x
+//     1000 behind 8000 245 against 316 (behind 1000, 1 x 512 in four parts 39.7 against
+//     35.1); with more blocks than 256 two rounds of them: 1 x 1200 behind 4000 183
+//     against 253, 1 x 8192 x 8 behind none 254 against 332.  Where those parts would
+//     be too short, two teams: 1 x 150 behind 4000 36.6 against 50.3.  d = 64: two teams
+//     for at least four parts, 1 x 512 x 12 behind 4000 29.7 against 34.1, else one: 1
+//     x 1500 x 12 behind 4000 74.8 against 94.9, 1 x 400 x (8 x 4) 47.5 against 57.7.
+enum Form { kRows16, kTwoTeams, kOneTeam };
+struct Plan {
+    Form form;
+    int splits;
+};
 
-bool split_form(int B, int P, int G, int H_kv, int max_ctx) {
-    const long long groups = (long long)row_blocks(P, G, 64) * B * H_kv;
-    return row_blocks(P, G, 16) <= 2 || groups < 128 || (groups < 256 && groups < 24ll * ((max_ctx + kTile - 1) / kTile));
+Plan plan(int B, int P, int G, int H_kv, int d, int max_ctx, bool cut) {
+    const long long bh = (long long)B * H_kv;
+    const int n16 = row_blocks(P, G, 16), n128 = row_blocks(P, G, 128), tiles = (max_ctx + kTile - 1) / kTile;
+    const long long g16 = n16 * bh, g64 = row_blocks(P, G, 64) * bh, g128 = n128 * bh;
+    if (n16 <= 2 || g16 <= 128) {
+        const int each = (tiles + NW - 1) / NW;  // a tile at least for each wave
+        const int s = cut ? (int)std::min<long long>({256 / g16, each, IE_KV8_MAX_SPLITS}) : 1;
+        return {kRows16, std::max(s, 1)};
+    }
+    if (cut) {
+        const bool behind = max_ctx - P >= P;
+        if (d == 128 && g16 > 256 && g128 <= 512 && 4ll * P * G >= 3 * 128ll * n128 && (behind || g128 > 256)) {
+            const int s = (int)((g128 <= 256 ? 512 : 1024) / g128);
+            if (s >= 2 && 8 * s <= tiles) return {kOneTeam, s};
+        }
+        if (behind && (g16 <= 208 || (d == 128 && g16 > 256))) {
+            const int s = (int)std::min<long long>((d == 128 ? 256 : 512) / g64, tiles / 10);
+            if (s >= 2) return {kTwoTeams, s};
+        } else if (behind && g16 > 256) {
+            const int two = (int)(512 / g64), one = g64 <= 448 ? (int)(1024 / g64) : 1;
+            if (two >= 4 && 10 * two <= tiles) return {kTwoTeams, two};
+            if (one >= 2 && 10 * one <= tiles) return {kOneTeam, one};
+        }
+    }
+    if (g64 < 128 || (g64 < 256 && g64 < 24ll * tiles)) return {kRows16, 1};
+    return {g64 < 1024 ? kTwoTeams : kOneTeam, 1};
 }
 
 template <int D>
 void launch(const Kv8Attn& a, hipStream_t s) {
     const float qscale = (1.0f / sqrtf((float)D)) * 1.4426950408889634f;
-    const int G = a.H_q / a.c.H, bh = a.B * a.c.H;
-    const int n16 = row_blocks(a.P, G, 16), n64 = row_blocks(a.P, G, 64), n128 = row_blocks(a.P, G, 128);
-    const long long groups = (long long)n64 * bh;
-    if (split_form(a.B, a.P, G, a.c.H, a.max_ctx)) {
-        kv8_prefill_split_kernel<D><<<(unsigned)n16 * bh * a.splits, 64 * NW, 0, s>>>(a, n16, qscale);
-        if (a.splits > 1) launch_kv8_merge(D, a.B * a.P * a.H_q, a.splits, a.ws, a.O, s);
-    } else if (groups < kFullGroups) {
-        kv8_prefill_block_kernel<D, 1, 2><<<(unsigned)n64 * bh, 512, 0, s>>>(a, n64, qscale);
-    } else if constexpr (D == 64) {
-        kv8_prefill_block_kernel<D, 1, 1><<<(unsigned)n64 * bh, 256, 0, s>>>(a, n64, qscale);
-    } else {
-        kv8_prefill_block_kernel<D, 2, 1><<<(unsigned)n128 * bh, 256, 0, s>>>(a, n128, qscale);
-    }
+    const int G = a.H_q / a.c.H, n16 = row_blocks(a.P, G, 16), n64 = row_blocks(a.P, G, 64), n128 = row_blocks(a.P, G, 128);
+    const unsigned bh = (unsigned)a.B * a.c.H, parts = bh * a.splits;
+    const Form form = plan(a.B, a.P, G, a.c.H, D, a.max_ctx, a.splits > 1).form;
+    constexpr int NC = D == 64 ? 1 : 2;  // of one team
+    const int n = D == 64 ? n64 : n128;
+    if (form == kRows16)
+        kv8_prefill_split_kernel<D><<<n16 * parts, 64 * NW, 0, s>>>(a, n16, qscale);
+    else if (form == kTwoTeams && a.splits == 1)
+        kv8_prefill_block_kernel<D, 1, 2, false><<<n64 * bh, 512, 0, s>>>(a, n64, qscale);
+    else if (form == kTwoTeams)
+        kv8_prefill_block_kernel<D, 1, 2, true><<<n64 * parts, 512, 0, s>>>(a, n64, qscale);
+    else if (a.splits == 1)
+        kv8_prefill_block_kernel<D, NC, 1, false><<<n * bh, 256, 0, s>>>(a, n, qscale);
+    else
+        kv8_prefill_block_kernel<D, NC, 1, true><<<n * parts, 256, 0, s>>>(a, n, qscale);
+    if (a.splits > 1) launch_kv8_merge(D, a.B * a.P * a.H_q, a.splits, a.ws, a.O, s);
 }
 
 }  // namespace
 
-int kv8_prefill_splits(int B, int P, int H_q, int H_kv, int max_ctx) {
-    const int G = H_q / H_kv;
-    if (!split_form(B, P, G, H_kv, max_ctx)) return 1;
-    // a workgroup a CU, and a tile at least for each of its waves
-    const long long groups = (long long)row_blocks(P, G, 16) * B * H_kv;
-    const int each = (max_ctx + kTile * NW - 1) / (kTile * NW);
-    const int s = (int)std::min<long long>({256 / groups, each, IE_KV8_MAX_SPLITS});
-    return s < 1 ? 1 : s;
+int kv8_prefill_splits(int B, int P, int H_q, int H_kv, int d, int max_ctx) {
+    return plan(B, P, H_q / H_kv, H_kv, d, max_ctx, true).splits;
 }
 
 void launch_prefill_attn_kv8(const Kv8Attn& a, hipStream_t s) {

@@ -527,7 +527,7 @@ struct GPT2Engine::Impl {
         ie::Kv8Attn a{};
         a.B = B; a.P = Pc; a.H_q = H; a.Q = pf.qkv; a.q_ld = 3 * d; a.c = w.c;
         a.start = pos; a.max_ctx = pos + Pc; a.O = pf.attn; a.ws = ws;
-        a.splits = ie::kv8_prefill_splits(B, Pc, H, H, pos + Pc);
+        a.splits = ie::kv8_prefill_splits(B, Pc, H, H, cfg.d_head, pos + Pc);
         if ((size_t)B * Pc * H * a.splits * (cfg.d_head + 2) * sizeof(float) > ws_bytes) a.splits = 1;
         ie::launch_prefill_attn_kv8(a, stream);
         IEC(ie::check_launch("prefill_attn_kv8"));

@@ -97,7 +97,8 @@ int ie_decode_attn_kv8(int B, int H_q, int H_kv, int d, const float* Q, const vo
                        size_t workspace_bytes, int num_splits, ie_stream_t stream);
 
 /* Bytes of workspace with which ie_prefill_attn_kv8 can split the context of a
- * call of this size (few rows behind a long one); 0 where it would not. */
+ * call of this size (rows that do not fill the GPU, behind a long one); 0 where
+ * it would not. */
 size_t ie_prefill_kv8_workspace_bytes(int B, int P, int H_q, int H_kv, int d, int start_pos);
 
 /* Causal attention of a prompt chunk over the cache, as ie_prefill_attn: Q, O

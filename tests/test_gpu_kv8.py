@@ -261,6 +261,10 @@ def test_prompt(ie, dev, H, G, d, block, start, P):
 # one, with 32 rows a wave where d = 128.
 FORMS = [(2, 3, 2, 64, 16, 300, 9), (1, 2, 3, 128, 64, 4100, 5), (8, 32, 1, 64, 16, 40, 20), (3, 16, 4, 128, 32, 60, 13),
          (2, 16, 1, 128, 16, 700, 200),
+         # cut contexts: two teams (two and five parts), one team, 32 rows a wave in ten and four parts, two rounds
+         (1, 8, 4, 128, 16, 1300, 77), (1, 12, 1, 64, 32, 1400, 200), (1, 12, 4, 64, 16, 3200, 120), (2, 12, 2, 64, 64, 1700, 400),
+         (1, 16, 4, 128, 16, 5300, 80), (1, 8, 4, 128, 32, 2200, 500), (2, 16, 2, 128, 16, 1000, 600),
+         (2, 12, 1, 128, 32, 0, 1536),  # (its first blocks have fewer tiles than parts)
          (4, 16, 1, 64, 16, 0, 250), (4, 16, 1, 128, 32, 37, 251), (2, 16, 3, 128, 64, 5, 177), (16, 16, 4, 64, 256, 0, 13),
          (8, 32, 1, 64, 16, 0, 250), (8, 32, 1, 128, 16, 100, 249), (4, 32, 5, 128, 64, 3, 103), (16, 64, 2, 64, 128, 0, 1)]
 
