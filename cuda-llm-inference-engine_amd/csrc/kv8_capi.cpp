@@ -69,6 +69,12 @@ int check_attn(const char* fn, int H_q, int H_kv, int d, long long rows, const f
     if (overlap(Q, bytes, O, bytes)) return fail(IE_ERR_INVALID, "%s: O overlaps Q", fn);
     return IE_OK;
 }
+
+// A prompt's workgroups of 16 tokens (each product is below 2^63).
+bool too_many(int B, int P, int H_q) {
+    const long long n = (long long)((P + 15) / 16) * H_q;
+    return n > kMaxGroups || n * B > kMaxGroups;
+}
 }  // namespace
 
 extern "C" {
@@ -143,7 +149,7 @@ int ie_kv8_cache_read(int B, int n, const int* starts, const int* context_lens, 
 }
 
 int ie_decode_kv8_num_splits(int B, int H_q, int H_kv, int d, int max_context_len, int num_splits) {
-    if (B <= 0 || H_q <= 0 || H_kv <= 0 || max_context_len <= 0) return 1;
+    if (B <= 0 || H_q <= 0 || H_kv <= 0 || H_q % H_kv || max_context_len <= 0) return 1;
     const int tiles = (int)(((long long)max_context_len + 63) / 64);
     int s = num_splits;
     if (s <= 0) {
@@ -180,6 +186,7 @@ int ie_decode_attn_kv8(int B, int H_q, int H_kv, int d, const float* Q, const vo
                     num_blocks_per_seq, block_size);
     if (max_context_len > kMaxContext) return fail(IE_ERR_UNSUPPORTED, "%s: max_context_len past 2^30", fn);
     if (B == 0) return IE_OK;
+    if ((long long)B * H_q > kMaxGroups) return fail(IE_ERR_UNSUPPORTED, "%s: B x H_q above 2^21", fn);
     if ((st = check_attn(fn, H_q, H_kv, d, B, Q, O)) != IE_OK) return st;
     if (!context_lens) return fail(IE_ERR_INVALID, "%s: null pointer", fn);
     if (max_context_len > 0 && (st = check_cache(fn, k_cache, v_cache, k_scales, v_scales, block_table)) != IE_OK) return st;
@@ -203,7 +210,7 @@ int ie_decode_attn_kv8(int B, int H_q, int H_kv, int d, const float* Q, const vo
 
 size_t ie_prefill_kv8_workspace_bytes(int B, int P, int H_q, int H_kv, int d, int start_pos) {
     if (B <= 0 || P <= 0 || H_kv <= 0 || H_q <= 0 || H_q % H_kv || (d != 64 && d != 128) || start_pos < 0 ||
-        (long long)start_pos + P > kMaxContext || (long long)((P + 15) / 16) * H_q * B > kMaxGroups)
+        (long long)start_pos + P > kMaxContext || too_many(B, P, H_q))
         return 0;
     const int S = ie::kv8_prefill_splits(B, P, H_q, H_kv, d, start_pos + P);
     return S > 1 ? (size_t)B * P * H_q * S * (d + 2) * sizeof(float) : 0;
@@ -223,10 +230,10 @@ int ie_prefill_attn_kv8(int B, int P, int H_q, int H_kv, int d, const float* Q, 
                     num_blocks_per_seq, block_size);
     if ((long long)start_pos + P > kMaxContext) return fail(IE_ERR_UNSUPPORTED, "%s: positions past 2^30", fn);
     if (B == 0 || P == 0) return IE_OK;
+    if (too_many(B, P, H_q))
+        return fail(IE_ERR_UNSUPPORTED, "%s: grid too large (ceil(P/16) x H_q x B > 2^21)", fn);
     if ((st = check_attn(fn, H_q, H_kv, d, (long long)B * P, Q, O)) != IE_OK) return st;
     if ((st = check_cache(fn, k_cache, v_cache, k_scales, v_scales, block_table)) != IE_OK) return st;
-    if ((long long)((P + 15) / 16) * H_q * B > kMaxGroups)
-        return fail(IE_ERR_UNSUPPORTED, "%s: grid too large (ceil(P/16) x H_q x B > 2^21)", fn);
     ie::Kv8Attn a{};
     a.B = B; a.P = P; a.H_q = H_q; a.Q = Q; a.q_ld = H_q * d;
     a.c = cache(k_cache, v_cache, k_scales, v_scales, block_table, num_blocks_per_seq, H_kv, d, block_size);

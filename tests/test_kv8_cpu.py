@@ -103,6 +103,21 @@ def test_num_splits(ie):
             assert 1 <= f(B, 32, 8, 128, ctx) <= min(ie.KV8_MAX_SPLITS, -(-ctx // 64))
 
 
+BIG = 2**31 - 1
+
+
+def test_sizes_whose_products_pass_64_bits(ie):
+    """Refused like any other that is too large; head counts that do not divide choose nothing."""
+    assert ie.decode_kv8_num_splits(1, 1, 2, 64, 1000) == 1 and ie.decode_kv8_num_splits(1, 12, 8, 64, 1000) == 1
+    assert ie.decode_kv8_num_splits(BIG, BIG, BIG, 128, BIG) >= 1
+    assert ie.call("ie_prefill_kv8_workspace_bytes", BIG, 2**30, BIG, 1, 64, 0) == 0
+    far = dict(nbps=2**22, bs=256, O=1 << 63)
+    for B, n, Hq in ((BIG, 2**29, BIG - 1), (2**26, 2**16, 2**26), (2**31 - 16, 2**30, 2**29)):
+        assert prompt(ie, B=B, n=n, Hq=Hq, **far) == UNSUPPORTED
+    for B, Hq in ((BIG, BIG - 1), (2**30, 2**30), (2**29, 2**30)):
+        assert decode(ie, B=B, Hq=Hq, mx=2**30, splits=64, **far) == UNSUPPORTED
+
+
 def test_prompt_workspace(ie):
     """Few rows behind a long context can be split, and then the workspace has to hold it."""
     f = ie.call
