@@ -245,6 +245,25 @@ def test_score_over_the_8_bit_cache(ie, small_dir):
     assert np.array_equal(a.step(nxt), b.step(nxt))
 
 
+def test_score_in_any_order(ie, tiny_dir):
+    """Calls of other sizes on one engine, in the middle of a session, and with arrays left out."""
+    r = np.random.default_rng(11)
+    toks = r.integers(0, 1000, (2, 40)).astype(np.int32)
+    one, many = (ie.Engine(tiny_dir, max_batch=2, kv_dtype=ie.KV_I8) for _ in range(2))
+    whole = one.score(toks, 8)
+    at = 0
+    for P, k in ((3, 0), (20, 8), (1, 2), (16, 8)):
+        s = many.score(toks[:, at:at + P], k)
+        for got, want in ((s.logprobs, whole.logprobs), (s.entropy, whole.entropy)):  # (a chunk's last token has no next one in it)
+            assert np.abs(got[:, :P - 1] - want[:, at:at + P - 1]).max(initial=0) <= 3e-2 * np.abs(want).max()
+        assert s.top_indices.shape == (2, P, k) and many.session_tokens() == at + P
+        at += P
+    lp = np.full((2, 40), 7, np.float32)
+    one.reset()
+    ie.check("ie_engine_score", one.h, 2, 40, toks.ctypes.data, 0, lp.ctypes.data, None, None, None, None)
+    assert np.array_equal(lp, whole.logprobs)
+
+
 def test_score_refusals(ie, tiny_dir):
     eng = ie.Engine(tiny_dir, max_batch=1)
     for toks, k in (([[1, 2]], -1), ([[1, 2]], ie.LOGPROBS_TOP_MAX + 1), ([[1, 1000]], 0), ([[1] * 65], 0), ([[1], [2]], 0)):

@@ -486,6 +486,35 @@ def test_results_made_for_another_stream(ie, dev):
         assert torch.equal(got, call(None))
 
 
+def test_two_streams_at_once(ie, dev):
+    """Calls under way on two streams, each with its cache and what the binding makes for it: the bits of one alone."""
+    import torch
+
+    r = rng(41)
+    H, G, d, block, n, P = 2, 4, 128, 16, 2000, 40
+    work = []
+    for i in range(2):
+        c, table = filled(r, [n], H, d, block)
+        q = on(dev, rows(r, 1, P, H * G, d))
+        work.append((q, q[:, 0].contiguous(), c.tensors(ie, dev), on(dev, table), on(dev, np.array([n], np.int32))))
+
+    def both(w, stream=None):
+        q, q1, cache, tab, lens = w
+        return ie.prefill_attn_kv8(q, cache, tab, n - P, stream=stream), ie.decode_attn_kv8(q1, cache, tab, lens, n, splits=8, stream=stream)
+
+    want = [both(w) for w in work]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in work]
+    got = [[], []]
+    for _ in range(20):
+        for i, w in enumerate(work):
+            got[i].append(both(w, streams[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for a, b in got[i]:
+            assert torch.equal(a, want[i][0]) and torch.equal(b, want[i][1])
+
+
 def test_binding_refusals(ie, dev):
     import torch
 
