@@ -401,16 +401,23 @@ def _refuse(what, *tensors):
 
 
 _device_index = None  # () -> index of the current device
+_raw_stream_of = None  # device index -> handle of its current stream
 _f32 = _i32 = _i8 = _empty = None
 
 
 def _bind_torch():
-    global _device_index, _f32, _i32, _i8, _empty
+    global _device_index, _raw_stream_of, _f32, _i32, _i8, _empty
     import torch
 
+    load()  # fills _fns
     torch.cuda.current_stream()
     _f32, _i32, _i8, _empty = torch.float32, torch.int32, torch.int8, torch.empty
+    _raw_stream_of = torch._C._cuda_getCurrentRawStream
     _device_index = torch._C._cuda_getDevice
+
+
+def _failed(name, status):
+    raise IeError(name, status, last_error())
 
 
 def _new(stream, shape, dtype, device):
@@ -447,11 +454,12 @@ class Kv8Cache(NamedTuple):
         return sum(t.numel() * t.element_size() for t in self)
 
 
-# The wrappers' checks are spelled out flat: an attribute of a tensor costs 50 to
-# 85 ns, a helper call or a loop over tensors as much again, and a decode step's
-# calls are about as long on the GPU as here.
+# The wrappers' checks and calls are spelled out flat: an attribute of a tensor costs
+# 50 to 85 ns, its shape, a helper call, a loop over tensors or a call by *args two to
+# five times that, and a decode step's calls are about as long on the GPU as here.
+# Contiguous tensors are compared by their numbers of elements.
 def _kv8(what, cache, table):
-    """(heads, block size, d, device) of a cache whose tensors fit each other."""
+    """(heads, block size, d, device, table's rows and columns) of a cache whose tensors fit each other."""
     if _device_index is None:
         _bind_torch()
     k, v, ks, vs = cache
@@ -460,10 +468,11 @@ def _kv8(what, cache, table):
     if not (k.dtype is _i8 and v.dtype is _i8 and ks.dtype is _f32 and vs.dtype is _f32 and table.dtype is _i32
             and k.get_device() == at and v.get_device() == at and ks.get_device() == at and vs.get_device() == at
             and table.get_device() == at and k.is_contiguous() and v.is_contiguous() and ks.is_contiguous()
-            and vs.is_contiguous() and table.is_contiguous() and v.shape == (pages, H, bs // 16, d, 16)
-            and ks.shape == (pages, H) and vs.shape == (pages, H) and table.dim() == 2):
+            and vs.is_contiguous() and table.is_contiguous() and v.numel() == pages * H * bs * d
+            and ks.numel() == pages * H and vs.numel() == pages * H and table.dim() == 2):
         _refuse(what, k, v, ks, vs, table)
-    return H, bs, d, at
+    rows, nbps = table.shape
+    return H, bs, d, at, rows, nbps
 
 
 def _kv8_rows(what, K, V, lead, H, d, at):
@@ -486,48 +495,56 @@ def _kv8_rows(what, K, V, lead, H, d, at):
 def kv8_cache_write(K, V, cache, block_table, start_pos, stream=None):
     """Rows K, V [B, P, heads, d] fp32 (views into a QKV projection serve as they
     lie) to positions start_pos .. of the sequences of block_table [B, nbps]."""
-    H, bs, d, at = _kv8("kv8_cache_write", cache, block_table)
+    H, bs, d, at, rows, nbps = _kv8("kv8_cache_write", cache, block_table)
     B, P = K.shape[:2]
-    if block_table.shape[0] != B:
+    if rows != B:
         raise ValueError("kv8_cache_write: block_table has other sequences than K")
     ld = _kv8_rows("kv8_cache_write", K, V, (B, P), H, d, at) if B * P else H * d
     k, v, ks, vs = cache
-    check("ie_kv8_cache_write", B, P, K.data_ptr(), V.data_ptr(), ld, k.data_ptr(), v.data_ptr(), ks.data_ptr(),
-          vs.data_ptr(), block_table.data_ptr(), block_table.shape[1], start_pos, H, d, bs, _stream(stream))
+    st = _fns["ie_kv8_cache_write"](
+        B, P, K.data_ptr(), V.data_ptr(), ld, k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(),
+        block_table.data_ptr(), nbps, start_pos, H, d, bs, _raw_stream_of(at) if stream is None else stream.cuda_stream)
+    if st:
+        _failed("ie_kv8_cache_write", st)
 
 
 def kv8_cache_append_batch(K, V, cache, block_table, positions, stream=None):
     """One row of each sequence, K, V [B, heads, d], to positions[b] (int32)."""
-    H, bs, d, at = _kv8("kv8_cache_append_batch", cache, block_table)
-    B = K.shape[0]
-    if (block_table.shape[0] != B or positions.shape != (B,) or positions.dtype is not _i32
-            or positions.get_device() != at or not positions.is_contiguous()):
+    H, bs, d, at, B, nbps = _kv8("kv8_cache_append_batch", cache, block_table)
+    if (positions.numel() != B or positions.dtype is not _i32 or positions.get_device() != at
+            or not positions.is_contiguous()):
         _refuse("kv8_cache_append_batch", K, block_table, positions)
     ld = _kv8_rows("kv8_cache_append_batch", K, V, (B,), H, d, at) if B else H * d
     k, v, ks, vs = cache
-    check("ie_kv8_cache_append_batch", B, K.data_ptr(), V.data_ptr(), ld, k.data_ptr(), v.data_ptr(), ks.data_ptr(),
-          vs.data_ptr(), block_table.data_ptr(), block_table.shape[1], positions.data_ptr(), H, d, bs, _stream(stream))
+    st = _fns["ie_kv8_cache_append_batch"](
+        B, K.data_ptr(), V.data_ptr(), ld, k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(),
+        block_table.data_ptr(), nbps, positions.data_ptr(), H, d, bs,
+        _raw_stream_of(at) if stream is None else stream.cuda_stream)
+    if st:
+        _failed("ie_kv8_cache_append_batch", st)
 
 
 def kv8_cache_read(cache, block_table, starts, context_lens, n, out=None, stream=None):
     """(K, V) [B, n, heads, d] fp32: positions starts[b] .. starts[b] + n - 1 of each
     sequence, zeros from context_lens[b] on (None: no limit)."""
-    H, bs, d, at = _kv8("kv8_cache_read", cache, block_table)
-    B = block_table.shape[0]
+    H, bs, d, at, B, nbps = _kv8("kv8_cache_read", cache, block_table)
     if out is None:
         out = tuple(_new(stream, (B, n, H, d), _f32, cache[0].device) for _ in range(2))
     K, V = out
-    want = (B, n, H, d)
-    if not (starts.shape == (B,) and starts.dtype is _i32 and starts.get_device() == at and starts.is_contiguous()
-            and (context_lens is None or (context_lens.shape == (B,) and context_lens.dtype is _i32
+    size = B * n * H * d
+    if not (starts.numel() == B and starts.dtype is _i32 and starts.get_device() == at and starts.is_contiguous()
+            and (context_lens is None or (context_lens.numel() == B and context_lens.dtype is _i32
                                           and context_lens.get_device() == at and context_lens.is_contiguous()))
-            and K.shape == want and V.shape == want and K.dtype is _f32 and V.dtype is _f32 and K.get_device() == at
+            and K.numel() == size and V.numel() == size and K.dtype is _f32 and V.dtype is _f32 and K.get_device() == at
             and V.get_device() == at and K.is_contiguous() and V.is_contiguous()):
         _refuse("kv8_cache_read", starts, *(() if context_lens is None else (context_lens,)), K, V)
     k, v, ks, vs = cache
-    check("ie_kv8_cache_read", B, n, starts.data_ptr(), _ptr(context_lens), k.data_ptr(), v.data_ptr(), ks.data_ptr(),
-          vs.data_ptr(), block_table.data_ptr(), block_table.shape[1], H, d, bs, K.data_ptr(), V.data_ptr(),
-          _stream(stream))
+    st = _fns["ie_kv8_cache_read"](
+        B, n, starts.data_ptr(), None if context_lens is None else context_lens.data_ptr(), k.data_ptr(), v.data_ptr(),
+        ks.data_ptr(), vs.data_ptr(), block_table.data_ptr(), nbps, H, d, bs, K.data_ptr(), V.data_ptr(),
+        _raw_stream_of(at) if stream is None else stream.cuda_stream)
+    if st:
+        _failed("ie_kv8_cache_read", st)
     return K, V
 
 
@@ -538,11 +555,11 @@ def decode_kv8_num_splits(B, H_q, H_kv, d, max_ctx, splits=0):
 def decode_attn_kv8(Q, cache, block_table, context_lens, max_ctx, splits=0, out=None, workspace=None, stream=None):
     """Q [B, H_q, d] fp32, one token a sequence, over the first context_lens[b]
     <= max_ctx cached positions; returns O [B, H_q, d]."""
-    H, bs, d, at = _kv8("decode_attn_kv8", cache, block_table)
+    H, bs, d, at, rows, nbps = _kv8("decode_attn_kv8", cache, block_table)
     B, H_q, dq = Q.shape
     if out is None:
         out = _new(stream, (B, H_q, d), _f32, Q.device)
-    if not (dq == d and block_table.shape[0] == B and context_lens.shape == (B,) and out.shape == Q.shape
+    if not (dq == d and rows == B and context_lens.numel() == B and out.numel() == B * H_q * d
             and Q.dtype is _f32 and out.dtype is _f32 and context_lens.dtype is _i32 and Q.get_device() == at
             and out.get_device() == at and context_lens.get_device() == at and Q.is_contiguous() and out.is_contiguous()
             and context_lens.is_contiguous()):
@@ -554,9 +571,13 @@ def decode_attn_kv8(Q, cache, block_table, context_lens, max_ctx, splits=0, out=
     elif workspace.dtype is not _f32 or workspace.get_device() != at or not workspace.is_contiguous():
         _refuse("decode_attn_kv8", workspace)
     k, v, ks, vs = cache
-    check("ie_decode_attn_kv8", B, H_q, H, d, Q.data_ptr(), k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(),
-          block_table.data_ptr(), context_lens.data_ptr(), max_ctx, bs, block_table.shape[1], out.data_ptr(),
-          _ptr(workspace), 0 if workspace is None else 4 * workspace.numel(), splits, _stream(stream))
+    st = _fns["ie_decode_attn_kv8"](
+        B, H_q, H, d, Q.data_ptr(), k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), block_table.data_ptr(),
+        context_lens.data_ptr(), max_ctx, bs, nbps, out.data_ptr(), None if workspace is None else workspace.data_ptr(),
+        0 if workspace is None else 4 * workspace.numel(), splits,
+        _raw_stream_of(at) if stream is None else stream.cuda_stream)
+    if st:
+        _failed("ie_decode_attn_kv8", st)
     return out
 
 
@@ -564,23 +585,26 @@ def prefill_attn_kv8(Q, cache, block_table, start_pos, out=None, workspace=None,
     """Q [B, P, H_q, d] fp32, token t at position start_pos + t with its rows
     cached; returns causal O [B, P, H_q, d].  workspace: fp32, at least
     ie_prefill_kv8_workspace_bytes (made here where the call has use for one)."""
-    H, bs, d, at = _kv8("prefill_attn_kv8", cache, block_table)
+    H, bs, d, at, rows, nbps = _kv8("prefill_attn_kv8", cache, block_table)
     B, P, H_q, dq = Q.shape
     if out is None:
         out = _new(stream, (B, P, H_q, d), _f32, Q.device)
-    if not (dq == d and block_table.shape[0] == B and out.shape == Q.shape and Q.dtype is _f32 and out.dtype is _f32
+    if not (dq == d and rows == B and out.numel() == B * P * H_q * d and Q.dtype is _f32 and out.dtype is _f32
             and Q.get_device() == at and out.get_device() == at and Q.is_contiguous() and out.is_contiguous()):
         _refuse("prefill_attn_kv8", Q, out, block_table)
     if workspace is None:
-        need = call("ie_prefill_kv8_workspace_bytes", B, P, H_q, H, d, start_pos)
+        need = _fns["ie_prefill_kv8_workspace_bytes"](B, P, H_q, H, d, start_pos)
         if need:
             workspace = _new(stream, need // 4, _f32, Q.device)
     elif workspace.dtype is not _f32 or workspace.get_device() != at or not workspace.is_contiguous():
         _refuse("prefill_attn_kv8", workspace)
     k, v, ks, vs = cache
-    check("ie_prefill_attn_kv8", B, P, H_q, H, d, Q.data_ptr(), k.data_ptr(), v.data_ptr(), ks.data_ptr(),
-          vs.data_ptr(), block_table.data_ptr(), block_table.shape[1], bs, start_pos, out.data_ptr(), _ptr(workspace),
-          0 if workspace is None else 4 * workspace.numel(), _stream(stream))
+    st = _fns["ie_prefill_attn_kv8"](
+        B, P, H_q, H, d, Q.data_ptr(), k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), block_table.data_ptr(),
+        nbps, bs, start_pos, out.data_ptr(), None if workspace is None else workspace.data_ptr(),
+        0 if workspace is None else 4 * workspace.numel(), _raw_stream_of(at) if stream is None else stream.cuda_stream)
+    if st:
+        _failed("ie_prefill_attn_kv8", st)
     return out
 
 
@@ -605,32 +629,35 @@ def token_logprobs(logits, targets=None, k=0, out=None, workspace=None, stream=N
     if logits.get_device() != at or logits.dtype is not _f32 or (n > 1 and step != 1) or (rows > 1 and ld < n):
         raise ValueError(f"token_logprobs: logits need to be fp32 rows on cuda:{at}, got {logits.dtype} strides "
                          f"{(ld, step)} on {logits.device}")
-    if targets is not None and not (targets.shape == (rows,) and targets.dtype is _i32 and targets.get_device() == at
+    if targets is not None and not (targets.numel() == rows and targets.dtype is _i32 and targets.get_device() == at
                                     and targets.is_contiguous()):
         _refuse("token_logprobs", targets)
     if out is None:
         dev = logits.device
         out = (_new(stream, rows, _f32, dev), _new(stream, rows, _i32, dev), _new(stream, rows, _f32, dev),
                _new(stream, (rows, k), _f32, dev), _new(stream, (rows, k), _i32, dev))
+        lp, rk, en, tv, ti = out
     else:
         lp, rk, en, tv, ti = out
-        if not (lp.shape == (rows,) and rk.shape == (rows,) and en.shape == (rows,) and tv.shape == (rows, k)
-                and ti.shape == (rows, k) and lp.dtype is _f32 and rk.dtype is _i32 and en.dtype is _f32
+        if not (lp.numel() == rows and rk.numel() == rows and en.numel() == rows and tv.numel() == rows * k
+                and ti.numel() == rows * k and lp.dtype is _f32 and rk.dtype is _i32 and en.dtype is _f32
                 and tv.dtype is _f32 and ti.dtype is _i32 and lp.get_device() == at and rk.get_device() == at
                 and en.get_device() == at and tv.get_device() == at and ti.get_device() == at and lp.is_contiguous()
                 and rk.is_contiguous() and en.is_contiguous() and tv.is_contiguous() and ti.is_contiguous()):
             _refuse("token_logprobs", lp, rk, en, tv, ti)
     if workspace is None:
-        need = call("ie_token_logprobs_workspace_bytes", rows, n, k)
+        need = _fns["ie_token_logprobs_workspace_bytes"](rows, n, k)
         if need:
             workspace = _new(stream, need // 4, _f32, logits.device)
     elif workspace.dtype is not _f32 or workspace.get_device() != at or not workspace.is_contiguous():
         _refuse("token_logprobs", workspace)
-    lp, rk, en, tv, ti = out
-    check("ie_token_logprobs", rows, logits.data_ptr(), ld if rows > 1 else n, n, _ptr(targets), k, lp.data_ptr(),
-          rk.data_ptr(), en.data_ptr(), tv.data_ptr(), ti.data_ptr(), _ptr(workspace),
-          0 if workspace is None else 4 * workspace.numel(), _stream(stream))
-    return TokenLogprobs(*out)
+    st = _fns["ie_token_logprobs"](
+        rows, logits.data_ptr(), ld if rows > 1 else n, n, None if targets is None else targets.data_ptr(), k, lp.data_ptr(),
+        rk.data_ptr(), en.data_ptr(), tv.data_ptr(), ti.data_ptr(), None if workspace is None else workspace.data_ptr(),
+        0 if workspace is None else 4 * workspace.numel(), _raw_stream_of(at) if stream is None else stream.cuda_stream)
+    if st:
+        _failed("ie_token_logprobs", st)
+    return TokenLogprobs(lp, rk, en, tv, ti)
 
 
 # ---------------------------------------------------------------- engine
