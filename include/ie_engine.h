@@ -31,8 +31,9 @@ typedef struct {
 
 /* model_dir != NULL loads the reference on-disk format and ignores the
  * shape arguments; model_dir == NULL builds a random model of that shape.
- * kv_dtype is IE_KV_F32, IE_KV_BF16 or IE_KV_I8 (ie_kv8.h); fuse selects the fused decode step, prefill / prefill_chunk the prompt path,
- * backend IE_BACKEND_INT8 or IE_BACKEND_FP32 (GPT2EngineOptions). */
+ * kv_dtype is IE_KV_F32, IE_KV_BF16 or IE_KV_I8 (ie_kv8.h); fuse selects the
+ * fused decode step, prefill / prefill_chunk the prompt path, backend
+ * IE_BACKEND_INT8 or IE_BACKEND_FP32 (GPT2EngineOptions). */
 int ie_engine_create(ie_engine** out, const char* model_dir, int n_layers, int n_heads,
                      int d_model, int d_ff, int vocab_size, int max_seq_len,
                      unsigned long long seed, int max_batch, int kv_dtype,
