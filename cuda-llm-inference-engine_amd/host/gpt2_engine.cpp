@@ -943,7 +943,14 @@ struct GPT2Engine::Impl {
     // and positions at pos + P.  The reference prefills only a fresh session
     // and feeds a continuation through decode steps; here both prefill.
     // With a score, the log probability of every chunk row's next token too.
-    struct Score;
+    struct Score {  // into the caller's host arrays [B, P] (and [B, P, k])
+        int k;
+        float* logprobs;
+        int* ranks;
+        float* entropy;
+        float* top_logprobs;
+        int* top_idx;
+    };
     void prefill(const int* toks, int B, int P, Score* score = nullptr) {
         if (B < 1 || B > opt.max_batch) throw std::runtime_error("batch out of range");
         if (P < 1) throw std::runtime_error("empty prompt");
@@ -953,6 +960,7 @@ struct GPT2Engine::Impl {
         const int d = cfg.d_model, H = cfg.n_heads, dh = cfg.d_head;
         const int chunk = std::min(P, prefill_chunk(B));
         ensure_prefill(B * chunk);
+        if (score) ensure_score(B * chunk, score->k);  // (what may fail, before the cache is written)
         ie_stream_t st = (ie_stream_t)stream;
         int Pc = 0;
         for (int c0 = 0; c0 < P; c0 += Pc) {
@@ -993,16 +1001,6 @@ struct GPT2Engine::Impl {
         enqueue_head(B, false);
     }
 
-    // Log probabilities of a prompt's tokens into the caller's host arrays [B, P]
-    // (and [B, P, k]).
-    struct Score {
-        int k;
-        float* logprobs;
-        int* ranks;
-        float* entropy;
-        float* top_logprobs;
-        int* top_idx;
-    };
     struct ScoreBufs {
         int rows = 0, k = 0;
         float *xn = nullptr, *logits = nullptr, *out = nullptr, *ws = nullptr;
@@ -1043,9 +1041,12 @@ struct GPT2Engine::Impl {
             sc.act_q = (int32_t*)get(R * d);
             sc.act_s = (float*)get(R * 4);
         }
+        // what any call of up to so many rows and alternatives needs: a row with
+        // fewer alternatives may be cut into more parts
         sc.ws_bytes = 0;
         for (int r = 1; r <= G; ++r)
-            for (int kk : {0, k}) sc.ws_bytes = std::max(sc.ws_bytes, ie_token_logprobs_workspace_bytes(r, (int)V, kk));
+            for (int kk = 0; kk <= k; ++kk)
+                sc.ws_bytes = std::max(sc.ws_bytes, ie_token_logprobs_workspace_bytes(r, (int)V, kk));
         sc.ws = (float*)get(std::max<size_t>(sc.ws_bytes, 4));
         sc.rows = rows;
         sc.k = k;
@@ -1058,7 +1059,6 @@ struct GPT2Engine::Impl {
     void score_rows(Score& s, int B, int Pc, int c0, int P, const int* toks) {
         const int d = cfg.d_model, V = cfg.vocab_size, M = B * Pc, k = s.k;
         ie_stream_t st = (ie_stream_t)stream;
-        ensure_score(M, k);
         // device results, each array M rows: log probabilities, entropies, alternatives, then the two of integers
         float *lp = sc.out, *en = lp + M, *tv = en + M;
         int *rk = reinterpret_cast<int*>(tv + (size_t)M * k), *ti = rk + M;

@@ -271,3 +271,20 @@ def test_score_refusals(ie, tiny_dir):
             eng.score(np.array(toks), k)
     assert eng.session_tokens() == 0
     eng.close()
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(int8_lm_head=True)])
+def test_score_with_fewer_alternatives_than_before(ie, kw):
+    """At GPT-2's vocabulary, where rows are cut and fewer alternatives allow more parts (and a larger workspace): any
+    order of k, and rows that grow between, give the bits of an engine that is asked once."""
+    cfg = dict(TINY, n_layers=1, vocab_size=50257, seed=5, kv_dtype=ie.KV_I8, max_batch=2, **kw)
+    r = np.random.default_rng(13)
+    many = ie.Engine(**cfg)
+    for P, k in ((8, 100), (8, 20), (8, 10), (8, 128), (8, 5), (8, 0), (3, 1), (30, 81), (30, 7), (60, 12)):
+        toks = r.integers(0, 50257, (2, P)).astype(np.int32)
+        many.reset()
+        got = many.score(toks, k)
+        once = ie.Engine(**cfg)
+        assert all(np.array_equal(a, b) for a, b in zip(got, once.score(toks, k))), (P, k)
+        once.close()
+    many.close()
