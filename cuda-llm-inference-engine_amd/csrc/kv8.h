@@ -19,6 +19,16 @@ struct Kv8Cache {
     int bs_log2;       // pages of 1 << bs_log2 tokens
 };
 
+// What an append of one token a sequence changed of the rows before it, so that the
+// step can be undone: for each (sequence, K or V, head), at index (b * 2 + is_v) *
+// heads + h, the position whose append made the page's scale grow (-1: the last one
+// did not), the scale before it and the page's words before it.  Null: not kept.
+struct Kv8Undo {
+    int* at;
+    float* scale;
+    uint32_t* codes;  // block_size * d / 4 words each
+};
+
 // Rows of B sequences into the cache (kv8_cache.hip): P each from start on, or
 // with positions one each at positions[b].
 struct Kv8Write {
@@ -30,8 +40,12 @@ struct Kv8Write {
     int start;
     const int* positions;
     int* ctx_lens;  // with positions: ctx_lens[b] = positions[b] + 1 (may be null)
+    Kv8Undo undo;   // with positions
 };
 void launch_kv8_write(const Kv8Write& a, hipStream_t s);
+// The rows before position pos of B sequences as they were before the append at pos,
+// which has to be the last one that kept this undo.  The row itself counts as dropped.
+void launch_kv8_undo(int B, int pos, const Kv8Cache& c, const Kv8Undo& u, hipStream_t s);
 
 struct Kv8Read {
     int B, n;
@@ -64,6 +78,7 @@ struct Kv8Attn {
     const float* V;
     int kv_ld;
     const int* positions;
+    Kv8Undo undo;  // with positions
 };
 void launch_decode_attn_kv8(const Kv8Attn& a, hipStream_t s);  // kv8_decode.hip
 // O rows [rows, d] from their splits' partials ws [rows, splits, d + 2]: sums, m, l (kv8_decode.hip).

@@ -92,6 +92,12 @@ __global__ __launch_bounds__(1024) void kv8_write_kernel(Kv8Write a, int npages)
     const bool grew = page.grew;
     const float inv = page.inv, move = page.move;
     if (threadIdx.x == 0 && (r0 == 0 || grew)) *scale_at = page.scale;
+    const bool keep = a.undo.at != nullptr;  // uniform
+    const size_t entry = ((size_t)b * 2 + is_v) * a.c.H + h;
+    if (keep && threadIdx.x == 0) {
+        a.undo.at[entry] = grew ? start : -1;
+        a.undo.scale[entry] = had_sh;
+    }
 #pragma unroll
     for (int i = 0; i < T; ++i) {
         const int t = wid * T + i, row0 = (t / HALVES) * 16;
@@ -100,6 +106,10 @@ __global__ __launch_bounds__(1024) void kv8_write_kernel(Kv8Write a, int npages)
         if (row0 + 16 <= r0)
 #pragma unroll
             for (int k = 0; k < 4; ++k) was[i][k] = codes[word_of<D>(t, is_v, lane, k)];
+        if (keep && grew && row0 < r0)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                a.undo.codes[entry * ((size_t)bs * D / 4) + word_of<D>(t, is_v, lane, k)] = was[i][k];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             int q[4];
@@ -115,6 +125,20 @@ __global__ __launch_bounds__(1024) void kv8_write_kernel(Kv8Write a, int npages)
             codes[word_of<D>(t, is_v, lane, k)] = pack4(q[0], q[1], q[2], q[3]);
         }
     }
+}
+
+// One wave per (sequence, K or V, head), blockIdx.x: the words that hold rows before
+// the undone one, and the page's scale.
+__global__ __launch_bounds__(64) void kv8_undo_kernel(int pos, Kv8Cache c, Kv8Undo u) {
+    const size_t entry = blockIdx.x;
+    const int h = (int)(entry % (unsigned)c.H), is_v = (int)(entry / (unsigned)c.H) & 1, b = (int)(entry / (2u * (unsigned)c.H));
+    if (u.at[entry] != pos) return;  // uniform
+    const int bs = 1 << c.bs_log2, r = pos & (bs - 1), words = bs * c.d / 4;
+    const size_t pair = (size_t)c.table[(size_t)b * c.nbps + (pos >> c.bs_log2)] * c.H + h;
+    uint32_t* codes = reinterpret_cast<uint32_t*>((is_v ? c.v : c.k) + pair * ((size_t)bs * c.d));
+    for (int i = threadIdx.x; i < words; i += 64)
+        if (first_row(i, is_v, c.d) < r) codes[i] = u.codes[entry * words + i];
+    if (threadIdx.x == 0) (is_v ? c.vs : c.ks)[pair] = u.scale[entry];
 }
 
 // One wave per (sequence, 16-token group, head, 64 channels) of K and of V.
@@ -197,6 +221,10 @@ void launch_kv8_read(const Kv8Read& a, hipStream_t s) {
         kv8_read_kernel<64><<<grid, 256, 0, s>>>(a, groups, waves);
     else
         kv8_read_kernel<128><<<grid, 256, 0, s>>>(a, groups, waves);
+}
+
+void launch_kv8_undo(int B, int pos, const Kv8Cache& c, const Kv8Undo& u, hipStream_t s) {
+    if (B > 0) kv8_undo_kernel<<<(unsigned)B * 2 * c.H, 64, 0, s>>>(pos, c, u);
 }
 
 }  // namespace ie

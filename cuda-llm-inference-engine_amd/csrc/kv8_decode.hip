@@ -96,14 +96,21 @@ __device__ __forceinline__ void append_row(const Kv8Attn& a, bool is_v, int b, i
     const size_t pair = (size_t)a.c.table[(size_t)b * a.c.nbps + (pos >> a.c.bs_log2)] * a.c.H + h;
     int8_t* codes = (is_v ? a.c.v : a.c.k) + pair * ((size_t)bs * D);
     float* scale_at = (is_v ? a.c.vs : a.c.ks) + pair;
-    const PageScale page(wave_umax(mx), r, r > 0 ? *scale_at : 0.0f);
+    const float had = r > 0 ? *scale_at : 0.0f;
+    const PageScale page(wave_umax(mx), r, had);
+    const bool keep = a.undo.at != nullptr;  // uniform
+    const size_t entry = ((size_t)b * 2 + is_v) * a.c.H + h;
+    if (keep && lane == 0) {
+        a.undo.at[entry] = page.grew ? pos : -1;
+        a.undo.scale[entry] = had;
+    }
     if (page.grew) {  // uniform
-        // a word: 4 channels of a row of K, 4 tokens of a channel of V
         for (int i = lane; i < bs * D / 4; i += 64) {
-            const int row = is_v ? i / (4 * D) * 16 + i % 4 * 4 : i / (D / 4);
+            const int row = first_row(i, is_v, D);
             if (row >= r) continue;
             uint32_t* at = reinterpret_cast<uint32_t*>(codes) + i;
             const uint32_t was = *at;
+            if (keep) a.undo.codes[entry * (bs * D / 4) + i] = was;
             int q[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {

@@ -33,6 +33,11 @@ __device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
 }
 __device__ __forceinline__ int byte_of(uint32_t w, int i) { return (int)(int8_t)(w >> (8 * i)); }
 
+// Word i of a page's codes: 4 channels of a row of K, 4 tokens of a channel of V; its (first) row.
+__device__ __forceinline__ int first_row(int i, bool is_v, int d) {
+    return is_v ? i / (4 * d) * 16 + i % 4 * 4 : i / (d / 4);
+}
+
 // The scale of a page after a call that writes rows from r0 on, whose largest
 // magnitude has the bits mx; had: the scale before (read only where r0 > 0).
 struct PageScale {

@@ -284,6 +284,7 @@ struct GPT2Engine::Impl {
     size_t layer_elems = 0;
     char *kc = nullptr, *vc = nullptr;
     float *kv8_ks = nullptr, *kv8_vs = nullptr;  // IE_KV_I8: scales [n_layers, P, H]
+    ie::Kv8Undo kv8_kept{};  // what the last step's append made coarser, [n_layers, max_batch, 2, H]
     int *block_table = nullptr, *positions = nullptr, *ctx_lens = nullptr, *tokens = nullptr;
     float* ws = nullptr;
     size_t ws_bytes = 0;
@@ -420,6 +421,10 @@ struct GPT2Engine::Impl {
         if (kv8()) {
             kv8_ks = dev<float>((size_t)cfg.n_layers * phys_blocks * cfg.n_heads);
             kv8_vs = dev<float>((size_t)cfg.n_layers * phys_blocks * cfg.n_heads);
+            const size_t kept = (size_t)cfg.n_layers * B * 2 * cfg.n_heads;
+            kv8_kept.at = dev<int>(kept);
+            kv8_kept.scale = dev<float>(kept);
+            kv8_kept.codes = dev<uint32_t>(kept * kBlock * cfg.d_head / 4);
         }
         std::vector<int> table((size_t)B * nbps);
         std::iota(table.begin(), table.end(), 0);
@@ -495,6 +500,11 @@ struct GPT2Engine::Impl {
         return c;
     }
 
+    ie::Kv8Undo layer_undo(int l) {
+        const size_t e = (size_t)opt.max_batch * 2 * cfg.n_heads * l;
+        return {kv8_kept.at + e, kv8_kept.scale + e, kv8_kept.codes + e * (kBlock * cfg.d_head / 4)};
+    }
+
     // The 8-bit cache: a decode step's K and V rows of qkv [B, 3d] appended at
     // positions and attention of its Q rows, in one launch where the fused step's
     // context is in one split, else in two (the first sets ctx_lens).
@@ -504,11 +514,11 @@ struct GPT2Engine::Impl {
         a.B = B; a.P = 1; a.H_q = cfg.n_heads; a.Q = qkv; a.q_ld = 3 * d; a.c = layer_kv8(l);
         a.lens = ctx_lens; a.max_ctx = plan.max_ctx; a.O = attn; a.ws = ws; a.splits = plan.splits;
         if (fused && plan.splits == 1) {
-            a.K = qkv + d; a.V = qkv + 2 * d; a.kv_ld = 3 * d; a.positions = positions;
+            a.K = qkv + d; a.V = qkv + 2 * d; a.kv_ld = 3 * d; a.positions = positions; a.undo = layer_undo(l);
         } else {
             ie::Kv8Write w{};
             w.B = B; w.P = 1; w.K = qkv + d; w.V = qkv + 2 * d; w.ld = 3 * d;
-            w.c = a.c; w.positions = positions; w.ctx_lens = ctx_lens;
+            w.c = a.c; w.positions = positions; w.ctx_lens = ctx_lens; w.undo = layer_undo(l);
             ie::launch_kv8_write(w, stream);
             IEC(ie::check_launch("kv8 append"));
         }
@@ -841,7 +851,8 @@ struct GPT2Engine::Impl {
     // undoes a step that was enqueued past the stop: the position mirror and
     // the device positions go back one, and the device token buffer gets the
     // ids the host kept (the cache row that step wrote is overwritten by the
-    // next step or prompt at that position).
+    // next step or prompt at that position; in the 8-bit cache, where it may
+    // have made its page's scale grow, the rows before it go back too).
     struct GreedyPipe {
         Impl& I;
         int B;
@@ -868,7 +879,12 @@ struct GPT2Engine::Impl {
         void finish(const int* last_ids) {
             if (launched == waited) return;
             HIPC(hipStreamSynchronize(I.stream));
-            I.pos -= (int)(launched - waited);
+            I.pos -= (int)(launched - waited);  // one step: the last
+            if (I.kv8())
+                for (int l = 0; l < I.cfg.n_layers; ++l) {
+                    ie::launch_kv8_undo(B, I.pos, I.layer_kv8(l), I.layer_undo(l), I.stream);
+                    IEC(ie::check_launch("kv8 undo"));
+                }
             ie::launch_set_positions(B, I.pos, I.positions, I.ctx_lens, I.stream);
             IEC(ie::check_launch("set_positions"));
             std::memcpy(I.host_tokens, last_ids, sizeof(int) * B);

@@ -288,3 +288,58 @@ def test_score_with_fewer_alternatives_than_before(ie, kw):
         assert all(np.array_equal(a, b) for a, b in zip(got, once.score(toks, k))), (P, k)
         once.close()
     many.close()
+
+
+# ------------------------------------------------------------------ a step past the end of text
+EOS = 50256
+WIDE = dict(n_layers=2, vocab_size=EOS + 1, max_seq_len=1100)  # GPT-2 Small's widths: the fused step
+
+
+@pytest.fixture(scope="module")
+def wide_dir(tmp_path_factory, ie):
+    d = tmp_path_factory.mktemp("gpt2_wide_kv8")
+    ie.write_random_model(d, seed=23, **WIDE)
+    return d
+
+
+def end_after(ie, model_dir, prompts, scale):
+    """Makes <|endoftext|> the token that follows each of the prompts: its embedding becomes scale times the sum of their
+    last hidden rows (found from their logits by least squares), whose logits stand far above the others'.  Larger ones
+    than the prompt's, they give the key and value rows of the step that is fed with it."""
+    wte = np.fromfile(model_dir / "wte.bin", np.float32).reshape(EOS + 1, -1)
+    eng = ie.Engine(model_dir, max_batch=len(prompts), kv_dtype=ie.KV_I8)
+    logits = eng.prefill(prompts).astype(np.float64)
+    eng.close()
+    w = wte[:EOS].astype(np.float64)
+    hidden = np.linalg.solve(w.T @ w, w.T @ logits[:, :EOS].T)  # [d, prompts]
+    wte[EOS] = scale * hidden.sum(axis=1)
+    wte.tofile(model_dir / "wte.bin")
+
+
+@pytest.mark.parametrize("B,P,kw", [(1, 17, dict()), (1, 18, dict(fuse=False)), (1, 21, dict(use_graph=False)), (1, 16, dict()),
+                                    (2, 31, dict()), (2, 19, dict(fuse=False)), (1, 1026, dict()), (2, 1035, dict()),
+                                    (1, 1030, dict(fuse=False, use_graph=False))])
+def test_a_step_past_the_end_leaves_no_trace(ie, wide_dir, B, P, kw):
+    """Greedy decoding has the step behind <|endoftext|> under way before the host reads that token.  The session that goes
+    on from there has the bits of one that was never fed it, where the step's rows made pages' scales grow too: in the
+    middle of a page, at its first row, in one launch with the attention and in two, and past the change to split contexts."""
+    r = np.random.default_rng(P)
+    prompts = r.integers(0, EOS, (B, P)).astype(np.int32)
+    end_after(ie, wide_dir, prompts, 0.02)
+    a, b = (ie.Engine(wide_dir, max_batch=2, kv_dtype=ie.KV_I8, **kw) for _ in range(2))
+    for _ in range(2):  # (the second time over pages that hold the first one's)
+        if B == 1:
+            ids, _ = a.generate_one(prompts[0], 9, greedy=True)
+            assert ids == []
+        else:
+            out, _ = a.generate(prompts, 9)
+            assert (out == -1).all()
+        b.reset()
+        b.prefill(prompts)
+        assert a.session_tokens() == b.session_tokens() == P
+        for t in r.integers(0, EOS, (4, B)).astype(np.int32):
+            assert np.array_equal(a.step(t), b.step(t))
+        more = r.integers(0, EOS, (B, 5)).astype(np.int32)
+        assert np.array_equal(a.prefill(more), b.prefill(more))
+    a.close()
+    b.close()
