@@ -72,8 +72,9 @@ struct Kv8Attn {
     float* ws;
     int splits;
     // Decode with at most 4 query heads a KV head in one split may append first:
-    // K and V rows b * kv_ld to positions[b], attention over positions[b] + 1 of
-    // them (lens unused).  positions null: attention alone.
+    // K and V rows b * kv_ld to positions[b] (a sequence whose position is negative or
+    // past its table's row is left out, its output zero), attention over the first
+    // min(positions[b] + 1, max_ctx) (lens unused).  positions null: attention alone.
     const float* K;
     const float* V;
     int kv_ld;

@@ -143,10 +143,15 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? (NT == 1 ? 4 : 3) : (NT == 1 ? 3
     id /= (unsigned)groups;
     const int H = a.c.H, h = (int)(id % (unsigned)H), b = (int)(id / (unsigned)H);
     const int G = a.H_q / H, g0 = hg * HEADS, gn = min(HEADS, G - g0);
-    const int n = max(0, min(APPEND ? a.positions[b] + 1 : a.lens[b], a.max_ctx));
+    int n;
     if (APPEND) {
-        if (wid < 2 && n > 0) append_row<D>(a, wid == 1, b, h, n - 1);
+        const int pos = a.positions[b];
+        const bool in = pos >= 0 && pos < (long long)a.c.nbps << a.c.bs_log2;  // (else the sequence is left out)
+        if (wid < 2 && in) append_row<D>(a, wid == 1, b, h, pos);
         __syncthreads();
+        n = in ? min(pos, a.max_ctx - 1) + 1 : 0;
+    } else {
+        n = max(0, min(a.lens[b], a.max_ctx));
     }
     const int tiles = (n + kTile - 1) / kTile;
     const int t0 = (int)((unsigned)tiles * split / (unsigned)a.splits), t1 = (int)((unsigned)tiles * (split + 1) / (unsigned)a.splits);

@@ -1,5 +1,7 @@
 """The 8-bit KV cache on the GPU: its bytes against the rule in fp32 steps,
 attention over it against 64 bits."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -545,3 +547,50 @@ def test_binding_refusals(ie, dev):
     Q = K[:, 0].contiguous()
     with pytest.raises(ie.IeError):
         ie.decode_attn_kv8(Q, cache, tab, lens, 64, splits=1, out=Q)
+
+
+# ------------------------------------------------------------------ append and attention in one launch
+class CacheArgs(ctypes.Structure):  # Kv8Cache of csrc/kv8.h
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "ks", "vs", "table")] + [(n, ctypes.c_int) for n in ("nbps", "H", "d", "bs_log2")]
+
+
+class AttnArgs(ctypes.Structure):  # Kv8Attn
+    _fields_ = [("B", ctypes.c_int), ("P", ctypes.c_int), ("H_q", ctypes.c_int), ("Q", ctypes.c_void_p), ("q_ld", ctypes.c_int),
+                ("c", CacheArgs), ("lens", ctypes.c_void_p), ("max_ctx", ctypes.c_int), ("start", ctypes.c_int),
+                ("O", ctypes.c_void_p), ("ws", ctypes.c_void_p), ("splits", ctypes.c_int), ("K", ctypes.c_void_p),
+                ("V", ctypes.c_void_p), ("kv_ld", ctypes.c_int), ("positions", ctypes.c_void_p)] + [
+                (n, ctypes.c_void_p) for n in ("undo_at", "undo_scale", "undo_codes")]
+
+
+@pytest.mark.parametrize("H,G,d,block", [(12, 1, 64, 16), (2, 4, 128, 16), (3, 2, 64, 64)])
+def test_append_and_attention_in_one_launch(ie, dev, H, G, d, block):
+    """The launch of the engine's fused step against the two entry points: rows within the limit, at it and past it, past
+    the table's end and at no position (the sequence is left out, its output zero)."""
+    import torch
+
+    r = rng(H + G + block)
+    max_ctx, room = 90, 128
+    pos = [0, 1, block - 1, block, 40, max_ctx - 1, max_ctx, max_ctx + 20, room - 1, room, 2**31 - 1, -1, -(2**31)]
+    B = len(pos)
+    table, pages = ko.tables(r, [room] * B, block)
+    c = ko.Cache(pages, H, d, block, r)
+    for b, p in enumerate(pos):
+        n = min(max(p, 0), room)
+        c.write(rows(r, n, H, d), rows(r, n, H, d), table[b], 0)
+    K, V, Q = (on(dev, rows(r, B, n, d)) for n in (H, H, H * G))
+    tab, p = on(dev, table), on(dev, np.array(pos, np.int32))
+    two, one = c.tensors(ie, dev), c.tensors(ie, dev)
+    ie.kv8_cache_append_batch(K, V, two, tab, p)
+    lens = on(dev, np.array([q + 1 if 0 <= q < room else 0 for q in pos], np.int32))
+    want = ie.decode_attn_kv8(Q, two, tab, lens, max_ctx, splits=1)
+    got = torch.full_like(want, 7)
+    a = AttnArgs(B=B, P=1, H_q=H * G, Q=Q.data_ptr(), q_ld=H * G * d, max_ctx=max_ctx, O=got.data_ptr(), splits=1,
+                 K=K.data_ptr(), V=V.data_ptr(), kv_ld=H * d, positions=p.data_ptr(),
+                 c=CacheArgs(*(t.data_ptr() for t in one), tab.data_ptr(), tab.shape[1], H, d, block.bit_length() - 1))
+    launch = ctypes.CDLL(ie.LIB_PATH)["_ZN2ie22launch_decode_attn_kv8ERKNS_7Kv8AttnEP12ihipStream_t"]
+    launch(ctypes.byref(a), ctypes.c_void_p(ie._stream()))
+    torch.cuda.synchronize()
+    for x, y in zip(one, two):
+        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+    assert torch.equal(got, want)
+    assert not got[-4:].any()
