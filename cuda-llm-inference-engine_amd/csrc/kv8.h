@@ -1,5 +1,7 @@
 // kv8.h — the 8-bit paged KV cache: launchers (arguments validated by
-// kv8_capi.cpp) and what its kernels share.  Layout: include/ie_kv8.h.
+// kv8_capi.cpp) and what its kernels share.  Layout: include/ie_kv8.h.  The two
+// attention launchers return a status: they refuse what no kernel is there for
+// (parts without a workspace, an append with parts or many heads).
 #pragma once
 
 #include "ie_internal.h"
@@ -81,11 +83,11 @@ struct Kv8Attn {
     const int* positions;
     Kv8Undo undo;  // with positions
 };
-void launch_decode_attn_kv8(const Kv8Attn& a, hipStream_t s);  // kv8_decode.hip
+int launch_decode_attn_kv8(const Kv8Attn& a, hipStream_t s);  // kv8_decode.hip
 // O rows [rows, d] from their splits' partials ws [rows, splits, d + 2]: sums, m, l (kv8_decode.hip).
 void launch_kv8_merge(int d, int rows, int splits, const float* ws, float* O, hipStream_t s);
 // Splits of the context that launch_prefill_attn_kv8 works with best (above 1 it needs the workspace).
 int kv8_prefill_splits(int B, int P, int H_q, int H_kv, int d, int max_ctx);
-void launch_prefill_attn_kv8(const Kv8Attn& a, hipStream_t s);  // kv8_prefill.hip
+int launch_prefill_attn_kv8(const Kv8Attn& a, hipStream_t s);  // kv8_prefill.hip
 
 }  // namespace ie

@@ -204,8 +204,8 @@ int ie_decode_attn_kv8(int B, int H_q, int H_kv, int d, const float* Q, const vo
     a.B = B; a.P = 1; a.H_q = H_q; a.Q = Q; a.q_ld = H_q * d;
     a.c = cache(k_cache, v_cache, k_scales, v_scales, block_table, num_blocks_per_seq, H_kv, d, block_size);
     a.lens = context_lens; a.max_ctx = max_context_len; a.O = O; a.ws = workspace; a.splits = S;
-    ie::launch_decode_attn_kv8(a, (hipStream_t)stream);
-    return ie::check_launch(fn);
+    st = ie::launch_decode_attn_kv8(a, (hipStream_t)stream);
+    return st != IE_OK ? st : ie::check_launch(fn);
 }
 
 size_t ie_prefill_kv8_workspace_bytes(int B, int P, int H_q, int H_kv, int d, int start_pos) {
@@ -246,8 +246,8 @@ int ie_prefill_attn_kv8(int B, int P, int H_q, int H_kv, int d, const float* Q, 
             return fail(IE_ERR_WORKSPACE, "%s: workspace %zu bytes < %zu for %d splits", fn, workspace_bytes, need, a.splits);
         a.ws = workspace;
     }
-    ie::launch_prefill_attn_kv8(a, (hipStream_t)stream);
-    return ie::check_launch(fn);
+    st = ie::launch_prefill_attn_kv8(a, (hipStream_t)stream);
+    return st != IE_OK ? st : ie::check_launch(fn);
 }
 
 }  // extern "C"

@@ -509,11 +509,16 @@ void launch_kv8_merge(int d, int rows, int splits, const float* ws, float* O, hi
         merge<128>(rows, splits, ws, O, s);
 }
 
-void launch_decode_attn_kv8(const Kv8Attn& a, hipStream_t s) {
+int launch_decode_attn_kv8(const Kv8Attn& a, hipStream_t s) {
+    if (a.splits < 1 || a.splits > IE_KV8_MAX_SPLITS || (a.splits > 1 && !a.ws))
+        return fail(IE_ERR_INVALID, "decode_attn_kv8: %d splits, workspace %p", a.splits, (void*)a.ws);
+    if (a.positions && (a.splits > 1 || a.H_q > 4 * a.c.H))
+        return fail(IE_ERR_INVALID, "decode_attn_kv8: no append with %d splits, %d heads on %d", a.splits, a.H_q, a.c.H);
     if (a.c.d == 64)
         launch<64>(a, s);
     else
         launch<128>(a, s);
+    return IE_OK;
 }
 
 }  // namespace ie

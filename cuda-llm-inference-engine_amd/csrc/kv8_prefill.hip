@@ -633,11 +633,14 @@ int kv8_prefill_splits(int B, int P, int H_q, int H_kv, int d, int max_ctx) {
     return plan(B, P, H_q / H_kv, H_kv, d, max_ctx, true).splits;
 }
 
-void launch_prefill_attn_kv8(const Kv8Attn& a, hipStream_t s) {
+int launch_prefill_attn_kv8(const Kv8Attn& a, hipStream_t s) {
+    if (a.splits < 1 || a.splits > IE_KV8_MAX_SPLITS || (a.splits > 1 && !a.ws))
+        return fail(IE_ERR_INVALID, "prefill_attn_kv8: %d splits, workspace %p", a.splits, (void*)a.ws);
     if (a.c.d == 64)
         launch<64>(a, s);
     else
         launch<128>(a, s);
+    return IE_OK;
 }
 
 }  // namespace ie

@@ -522,7 +522,7 @@ struct GPT2Engine::Impl {
             ie::launch_kv8_write(w, stream);
             IEC(ie::check_launch("kv8 append"));
         }
-        ie::launch_decode_attn_kv8(a, stream);
+        IEC(ie::launch_decode_attn_kv8(a, stream));
         IEC(ie::check_launch("decode_attn_kv8"));
     }
 
@@ -539,7 +539,7 @@ struct GPT2Engine::Impl {
         a.start = pos; a.max_ctx = pos + Pc; a.O = pf.attn; a.ws = ws;
         a.splits = ie::kv8_prefill_splits(B, Pc, H, H, cfg.d_head, pos + Pc);
         if ((size_t)B * Pc * H * a.splits * (cfg.d_head + 2) * sizeof(float) > ws_bytes) a.splits = 1;
-        ie::launch_prefill_attn_kv8(a, stream);
+        IEC(ie::launch_prefill_attn_kv8(a, stream));
         IEC(ie::check_launch("prefill_attn_kv8"));
     }
 

@@ -1,10 +1,9 @@
 """The 8-bit KV cache on the GPU: its bytes against the rule in fp32 steps,
 attention over it against 64 bits."""
-import ctypes
-
 import numpy as np
 import pytest
 
+import kv8_launch as kl
 import kv8_oracle as ko
 from conftest import rng
 
@@ -550,18 +549,6 @@ def test_binding_refusals(ie, dev):
 
 
 # ------------------------------------------------------------------ append and attention in one launch
-class CacheArgs(ctypes.Structure):  # Kv8Cache of csrc/kv8.h
-    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "ks", "vs", "table")] + [(n, ctypes.c_int) for n in ("nbps", "H", "d", "bs_log2")]
-
-
-class AttnArgs(ctypes.Structure):  # Kv8Attn
-    _fields_ = [("B", ctypes.c_int), ("P", ctypes.c_int), ("H_q", ctypes.c_int), ("Q", ctypes.c_void_p), ("q_ld", ctypes.c_int),
-                ("c", CacheArgs), ("lens", ctypes.c_void_p), ("max_ctx", ctypes.c_int), ("start", ctypes.c_int),
-                ("O", ctypes.c_void_p), ("ws", ctypes.c_void_p), ("splits", ctypes.c_int), ("K", ctypes.c_void_p),
-                ("V", ctypes.c_void_p), ("kv_ld", ctypes.c_int), ("positions", ctypes.c_void_p)] + [
-                (n, ctypes.c_void_p) for n in ("undo_at", "undo_scale", "undo_codes")]
-
-
 @pytest.mark.parametrize("H,G,d,block", [(12, 1, 64, 16), (2, 4, 128, 16), (3, 2, 64, 64)])
 def test_append_and_attention_in_one_launch(ie, dev, H, G, d, block):
     """The launch of the engine's fused step against the two entry points: rows within the limit, at it and past it, past
@@ -584,11 +571,10 @@ def test_append_and_attention_in_one_launch(ie, dev, H, G, d, block):
     lens = on(dev, np.array([q + 1 if 0 <= q < room else 0 for q in pos], np.int32))
     want = ie.decode_attn_kv8(Q, two, tab, lens, max_ctx, splits=1)
     got = torch.full_like(want, 7)
-    a = AttnArgs(B=B, P=1, H_q=H * G, Q=Q.data_ptr(), q_ld=H * G * d, max_ctx=max_ctx, O=got.data_ptr(), splits=1,
-                 K=K.data_ptr(), V=V.data_ptr(), kv_ld=H * d, positions=p.data_ptr(),
-                 c=CacheArgs(*(t.data_ptr() for t in one), tab.data_ptr(), tab.shape[1], H, d, block.bit_length() - 1))
-    launch = ctypes.CDLL(ie.LIB_PATH)["_ZN2ie22launch_decode_attn_kv8ERKNS_7Kv8AttnEP12ihipStream_t"]
-    launch(ctypes.byref(a), ctypes.c_void_p(ie._stream()))
+    a = kl.AttnArgs(B=B, P=1, H_q=H * G, Q=Q.data_ptr(), q_ld=H * G * d, max_ctx=max_ctx, O=got.data_ptr(), splits=1,
+                    K=K.data_ptr(), V=V.data_ptr(), kv_ld=H * d, positions=p.data_ptr(),
+                    c=kl.CacheArgs(*(t.data_ptr() for t in one), tab.data_ptr(), tab.shape[1], H, d, block.bit_length() - 1))
+    assert kl.launch(ie, "decode", a, ie._stream()) == 0
     torch.cuda.synchronize()
     for x, y in zip(one, two):
         assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))

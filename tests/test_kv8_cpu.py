@@ -7,6 +7,7 @@ import re
 import numpy as np
 import pytest
 
+import kv8_launch as kl
 import kv8_oracle as ko
 from conftest import ROOT, rng
 
@@ -149,3 +150,21 @@ def test_oracle_rule_bounds():
     c.write(X, X, [0], 0)
     err = np.abs(c.k[0].transpose(1, 0, 2) * c.ks[0].astype(np.float64)[None, :, None] - X)
     assert (err <= 0.50001 * c.ks[0][None, :, None]).all()
+
+
+def launcher_args(**kw):
+    a = dict(B=1, P=1, H_q=4, Q=P, q_ld=256, lens=P, max_ctx=64, O=1 << 20, ws=P, splits=1, c=kl.CacheArgs(P, P, P, P, P, 4, 4, 64, 4))
+    return kl.AttnArgs(**{**a, **kw})
+
+
+@pytest.mark.parametrize("which,args", [
+    ("decode", dict(splits=2, ws=None)), ("decode", dict(splits=0)), ("decode", dict(splits=65)),
+    ("decode", dict(positions=P, K=P, V=P, kv_ld=256, splits=2)),
+    ("decode", dict(positions=P, K=P, V=P, kv_ld=256, H_q=20, q_ld=1280)),
+    ("prefill", dict(splits=2, ws=None)), ("prefill", dict(splits=0)), ("prefill", dict(splits=65))])
+def test_launchers_refuse_what_no_kernel_is_there_for(ie, which, args):
+    """Parts without a place for them, and an append with parts or with more heads a KV head than one workgroup has."""
+    ie.call("ie_kv8_cache_write", 1, -1, *[None] * 2, 0, *[None] * 5, 0, 0, 0, 0, 0, None)  # (an older message)
+    before = ie.last_error()
+    assert kl.launch(ie, which, launcher_args(**args)) == INVALID
+    assert ie.last_error() != before
