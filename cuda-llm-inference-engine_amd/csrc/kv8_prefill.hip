@@ -173,7 +173,10 @@ __device__ __forceinline__ void weights(const f32x4 (&acc)[4], float sw, float v
         const float mn = moved ? fmaxf(st.m, rtop) : st.m;
         const float f = moved ? exp2_sm(st.m - mn) : 1.0f;
         const float wm = max_xor32(max_xor16(top - mn + vexp));
-        const int ub = moved ? (int)fminf(fmaxf(ceilf(wm) + (127.0f + 3.0f - 15.0f), 1.0f), 224.0f) : st.ub;
+        // 8 times the tile's largest weight, and not below the unit that the output has
+        // so far (which may be of far larger values): o moves by at most a factor of 2
+        const float unit = fmaxf(ceilf(wm) + (127.0f + 3.0f - 15.0f), ceilf((float)st.ub + (st.m - mn)));
+        const int ub = moved ? (int)fminf(fmaxf(unit, 1.0f), 224.0f) : st.ub;
         const float fo = f * pow2(127 + min(max(st.ub - ub, -126), 127));
 #pragma unroll
         for (int j = 0; j < D / 16; ++j) st.o[j] *= fo;

@@ -548,6 +548,35 @@ def test_binding_refusals(ie, dev):
         ie.decode_attn_kv8(Q, cache, tab, lens, 64, splits=1, out=Q)
 
 
+@pytest.mark.parametrize("B,H,G,d,start,P", [(1, 1, 1, 64, 500, 1), (8, 32, 1, 64, 330, 20), (2, 12, 1, 64, 330, 300),
+                                             (2, 16, 2, 128, 330, 100), (4, 32, 1, 64, 330, 510), (4, 32, 2, 128, 330, 260)])
+def test_large_values_behind_a_page_of_zeros(ie, dev, B, H, G, d, start, P):
+    """Values of 1e20 at keys of score 0, zeros (whose page has the least scale) at one of score about 70: the large ones
+    are all that the output has, e^-70 of them.  Values are positive, so the output is off by twice its weights' relative
+    error (kv8_oracle.attend), whatever its size; before and behind the jump, in each of the prompt's forms and for one
+    token."""
+    r = rng(d + P)
+    n, high = start + P, 4 * 64 + 5
+    table, pages = ko.tables(r, [n] * B, 16)
+    c = ko.Cache(pages, H, d, 16, r)
+    q = rows(r, 1, H, 1, d, spread=0.0).repeat(G, 2)  # one query a KV head
+    K, V = np.zeros((n, H, d), np.float32), np.zeros((n, H, d), np.float32)
+    K[high] = 70 * d**0.5 * q[0, :, 0] / (q[0, :, 0] ** 2).sum(-1, keepdims=True)
+    V[:64] = (1e20 * np.abs(1 + 0.1 * r.standard_normal((64, H, d)))).astype(np.float32)
+    for b in range(B):
+        c.write(K, V, table[b], 0)
+    Q = np.broadcast_to(q.reshape(1, 1, H * G, d), (B, P, H * G, d)).copy()
+    want, _ = prompt_in_64_bits(dev, c, table, start, Q)
+    tol = (46 * 71 + 24 + n / 16) * ko.U
+    cache, tab = c.tensors(ie, dev), on(dev, table)
+    got = ie.prefill_attn_kv8(on(dev, Q), cache, tab, start).cpu().numpy()
+    assert (np.abs(got - want) <= tol * want).all(), (got / want).min()
+    lens = on(dev, np.full(B, n, np.int32))
+    for splits in (1, 2):
+        got = ie.decode_attn_kv8(on(dev, Q[:, 0]), cache, tab, lens, n, splits=splits).cpu().numpy()
+        assert (np.abs(got - want[:, -1]) <= tol * want[:, -1]).all()
+
+
 # ------------------------------------------------------------------ append and attention in one launch
 @pytest.mark.parametrize("H,G,d,block", [(12, 1, 64, 16), (2, 4, 128, 16), (3, 2, 64, 64)])
 def test_append_and_attention_in_one_launch(ie, dev, H, G, d, block):
