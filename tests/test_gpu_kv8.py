@@ -609,3 +609,27 @@ def test_append_and_attention_in_one_launch(ie, dev, H, G, d, block):
         assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
     assert torch.equal(got, want)
     assert not got[-4:].any()
+
+
+def test_rows_farther_apart_than_the_entry_points_take(ie, dev):
+    """Distances between rows past 32 bits, and positions past them, are refused, not taken modulo 2^32."""
+    import torch
+
+    far = 2**32 + 512
+    buf = torch.zeros(far + 512, device=dev)
+    cache, tab = ie.Kv8Cache.empty(4, 2, 64, 16, dev), torch.arange(4, dtype=torch.int32, device=dev)[None]
+    K = buf.as_strided((1, 2, 2, 64), (2 * far, far, 64, 1))
+    with pytest.raises(ValueError):
+        ie.kv8_cache_write(K, K, cache, tab, 0)
+    with pytest.raises(ValueError):
+        ie.kv8_cache_append_batch(K[0], K[0], cache, tab.expand(2, 4).contiguous(), torch.zeros(2, dtype=torch.int32, device=dev))
+    with pytest.raises(ValueError):
+        ie.token_logprobs(buf.as_strided((2, 500), (far, 1)), None, 3)
+    x, lens = torch.zeros(1, 2, 2, 64, device=dev), torch.ones(1, dtype=torch.int32, device=dev)
+    for f in (lambda: ie.kv8_cache_write(x, x, cache, tab, 2**32), lambda: ie.prefill_attn_kv8(x, cache, tab, 2**32),
+              lambda: ie.decode_attn_kv8(x[:, 0].contiguous(), cache, tab, lens, 2**32 + 1)):
+        with pytest.raises(ValueError):
+            f()
+    # (a single row's distance to the next one counts for nothing)
+    ie.kv8_cache_write(K[:, :1], K[:, :1], cache, tab, 0)
+    assert ie.token_logprobs(buf.as_strided((1, 500), (far, 1)), None, 3).top_indices.tolist() == [[0, 1, 2]]
