@@ -168,6 +168,43 @@ def test_splits_past_1024_tokens(ie, tmp_path):
     eng.close()
 
 
+@pytest.mark.parametrize("B", [1, 3])
+def test_fused_step_past_1024_tokens(ie, tmp_path, B):
+    """The same at GPT-2 Small's widths, where the fused step goes from one launch of append and attention to an append,
+    split attention and a merge: against the oracle, and the same bits fused or not, replayed or not."""
+    cfg = dict(n_layers=1, vocab_size=1000, max_seq_len=1100)
+    ie.write_random_model(tmp_path, seed=31, **cfg)
+    r = np.random.default_rng(17)
+    engines = [ie.Engine(tmp_path, max_batch=B, kv_dtype=ie.KV_I8, **kw) for kw in (dict(), dict(fuse=False), dict(use_graph=False))]
+    om = oracle(tmp_path, B)
+    prompt = r.integers(0, 1000, (B, 1020))
+    want = om.prompt(prompt)
+    for e in engines:
+        near(e.prefill(prompt), want)
+    for t in r.integers(0, 1000, (9, B)):
+        got = [e.step(t) for e in engines]
+        assert np.array_equal(got[0], got[1]) and np.array_equal(got[0], got[2])
+        near(got[0], om.step(t))
+    for e in engines:
+        e.close()
+
+
+def test_sixteen_sequences(ie, small_dir):
+    """The largest batch: a prompt and steps against the oracle, and each sequence's bits as in a batch of its own."""
+    r = np.random.default_rng(18)
+    eng, om, few = ie.Engine(small_dir, max_batch=16, kv_dtype=ie.KV_I8), oracle(small_dir, 16), ie.Engine(small_dir, max_batch=3, kv_dtype=ie.KV_I8)
+    toks = r.integers(0, 1000, (20, 16))
+    for t in toks:
+        got = eng.step(t)
+        near(got, om.step(t))
+        assert np.array_equal(few.step(t[5:8]), got[5:8])
+    prompt = r.integers(0, 1000, (16, 7))
+    near(eng.prefill(prompt), om.prompt(prompt))
+    near(eng.step(toks[0]), om.step(toks[0]))
+    eng.close()
+    few.close()
+
+
 def test_generates_and_holds_a_quarter_of_the_bytes(ie):
     eng = ie.Engine(max_batch=2, kv_dtype=ie.KV_I8, n_layers=2, vocab_size=2000)
     out, m = eng.generate(np.arange(20).reshape(2, 10), 12, ignore_eos=True)

@@ -54,3 +54,12 @@ def test_nothing_to_do(ie):
 def test_score_refuses_a_null_engine(ie):
     tokens = (ctypes.c_int * 4)()
     assert ie.call("ie_engine_score", None, 1, 4, ctypes.addressof(tokens), 0, None, None, None, None, None) == 1
+
+
+@pytest.mark.parametrize("rows,n,k", [(1, 1 << 19, 5), (8, 50257, 5), (16, 50257, 80), (300, 32001, 1)])
+def test_cut_rows_need_a_workspace(ie, rows, n, k):
+    need = ie.call("ie_token_logprobs_workspace_bytes", rows, n, k)
+    assert need > 0
+    assert call(ie, rows=rows, n=n, ld=n, k=k, ws=None) == 1
+    assert call(ie, rows=rows, n=n, ld=n, k=k, ws=P + 4, wsb=need) == 1
+    assert call(ie, rows=rows, n=n, ld=n, k=k, wsb=need - 1) == 3
