@@ -44,12 +44,25 @@
 namespace ie {
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLog2eRest = 1.92596298909e-8f;  // log2(e) in two parts
 constexpr int kStats = 8;   // words of a part's statistics in the workspace
 constexpr int kWide = 256;  // threads of a workgroup (64 for short rows)
 constexpr int kMostParts = 16;
 constexpr int kWords = 4;   // 16-byte words a thread has in flight: a tile
 constexpr int kList = 512;  // candidates of a wave
+
+// e^d, d <= 0, of what many elements share (a thread's, a wave's and a part's sums
+// against the row's maximum): the exponent in two parts, so that its rounding
+// (d 2^-24 of the result) and log2(e)'s own (1.3e-8 d) do not stay in all of them.
+// An element's, and a thread's as its maximum moves, are exp2_sm(d * kLog2e): their
+// roundings average out.  -log p under 50257 others lower by 78 to 82: off by 1.4e-7 at
+// most, 2.3e-6 with all of them so; 8 x 50257, k = 5 10.75 against 10.6 us.
+__device__ __forceinline__ float exp_of(float d) {
+    d = fmaxf(d, -200.0f);  // (0 from -127 log 2 on)
+    const float t = d * kLog2e, rest = fmaf(d, kLog2eRest, fmaf(d, kLog2e, -t));
+    const float p = exp2_sm(t);
+    return fmaf(p * 0.6931471805599453f, rest, p);
+}
 
 // Unsigned key with the order of the floats, -0 as +0.
 __device__ __forceinline__ uint32_t order_key(float x) {
@@ -342,7 +355,7 @@ __global__ __launch_bounds__(T, 6) void logprobs_kernel(LogprobsArgs a, int part
     // the threads' sums against the wave's maximum, then the waves' against the row's
     const float wm = wave_most(m);
     {
-        const float d = fmaxf(m - (wm == -INFINITY ? 0.0f : wm), -3.0e38f), f = exp2_sm(d * kLog2e), s = e + tops;
+        const float d = fmaxf(m - (wm == -INFINITY ? 0.0f : wm), -3.0e38f), f = exp_of(d), s = e + tops;
         w = wave_sum(fmaf(s * f, d, w * f));
         e = wave_sum(m == wm ? e : s * f);
         tops = wave_sum(m == wm ? tops : 0.0f);
@@ -360,7 +373,7 @@ __global__ __launch_bounds__(T, 6) void logprobs_kernel(LogprobsArgs a, int part
 #pragma unroll
     for (int i = 0; i < W; ++i) {
         const float4 o = sh_s[i];
-        const float d = fmaxf(o.x - (rm == -INFINITY ? 0.0f : rm), -3.0e38f), f = exp2_sm(d * kLog2e), s = o.y + o.w;
+        const float d = fmaxf(o.x - (rm == -INFINITY ? 0.0f : rm), -3.0e38f), f = exp_of(d), s = o.y + o.w;
         w += fmaf(s * f, d, o.z * f);
         e += o.x == rm ? o.y : s * f;
         tops += o.x == rm ? o.w : 0.0f;
@@ -470,7 +483,7 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(LogprobsArgs a, int 
     for (int p = 0; p < kMostParts; ++p) {
         const float d = fmaxf(pm[p] - m, -3.0e38f);  // (finite, as above)
         if (pm[p] == -INFINITY) continue;  // (nothing there; NaN is looked at below)
-        const float f = exp2_sm(d * kLog2e);
+        const float f = exp_of(d);
         const bool it = d == 0.0f && first;
         first = first && !it;
         const float total = f + f * pr[p];

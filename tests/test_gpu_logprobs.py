@@ -215,3 +215,22 @@ def test_binding_refusals(ie, dev):
             f()
     with pytest.raises(ie.IeError):
         ie.token_logprobs(x, t, 41)
+
+
+@pytest.mark.parametrize("n", [3000, 50257])
+def test_no_error_of_one_sign(ie, dev, n):
+    """-log p of a token under which n others lie by 78 to 82: the sum of their exponentials, whose errors average out.
+    Each exponent (up to 119 in base 2) rounds once, by at most 82 u of the exponential with no preferred sign: over n >=
+    2999 elements 82 / sqrt(3 n) u, at six times that 5.2 u; the exponential is off by 1 in its last place, 2 u; of at most
+    n / 256 + 32 additions, half a step each at random in 256 chains of their own, (n / 256 + 32)^0.5 / (3^0.5 16) u, at six
+    times that 3.3 u; log1p keeps it.  So an exponential that many elements share (a thread's sums against the row's
+    maximum) has to be exact to its last places: one that is rounded as an element's is would put up to 82 u into all of
+    them, and a factor of the exponent that is off by 1.3e-8 adds 80 * 1.3e-8 = 18 u in every row."""
+    r = rng(n)
+    x = r.uniform(-82, -78, (32, n)).astype(np.float32)
+    t = r.integers(0, n, 32).astype(np.int32)
+    x[np.arange(32), t] = 0
+    lp = ie.token_logprobs(on(dev, x), on(dev, t), 0)[0].cpu().numpy().astype(np.float64)
+    want = np.array([plain(x[i], t[i], 0)[0] for i in range(32)])
+    assert (want < 0).all()
+    assert np.abs(lp / want - 1).max() <= (82 * 6 / (3 * n) ** 0.5 + 2 + 6 * (n / 256 + 32) ** 0.5 / (3**0.5 * 16)) * U
