@@ -100,24 +100,29 @@ __device__ __forceinline__ void append_row(const Kv8Attn& a, bool is_v, int b, i
     const PageScale page(wave_umax(mx), r, had);
     const bool keep = a.undo.at != nullptr;  // uniform
     const size_t entry = ((size_t)b * 2 + is_v) * a.c.H + h;
-    if (keep && lane == 0) {
-        a.undo.at[entry] = page.grew ? pos : -1;
-        a.undo.scale[entry] = had;
-    }
+    if (keep && lane == 0) a.undo.at[entry] = page.grew ? pos : -1;
     if (page.grew) {  // uniform
-        for (int i = lane; i < bs * D / 4; i += 64) {
-            const int row = first_row(i, is_v, D);
-            if (row >= r) continue;
-            uint32_t* at = reinterpret_cast<uint32_t*>(codes) + i;
-            const uint32_t was = *at;
-            if (keep) a.undo.codes[entry * (bs * D / 4) + i] = was;
-            int q[4];
+        if (keep && lane == 0) a.undo.scale[entry] = had;
+        uint32_t* words = reinterpret_cast<uint32_t*>(codes);
+        uint32_t* kept = a.undo.codes + entry * (bs * D / 4);
+        for (int i0 = lane; i0 < bs * D / 4; i0 += 4 * 64) {  // (a page is 256 words at least)
+            uint32_t was[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                q[e] = byte_of(was, e);
-                if (!is_v || row + e < r) q[e] = code((float)q[e] * page.move);
+            for (int u = 0; u < 4; ++u)
+                if (first_row(i0 + 64 * u, is_v, D) < r) was[u] = words[i0 + 64 * u];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int i = i0 + 64 * u, row = first_row(i, is_v, D);
+                if (row >= r) continue;
+                if (keep) kept[i] = was[u];
+                int q[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    q[e] = byte_of(was[u], e);
+                    if (!is_v || row + e < r) q[e] = code((float)q[e] * page.move);
+                }
+                words[i] = pack4(q[0], q[1], q[2], q[3]);
             }
-            *at = pack4(q[0], q[1], q[2], q[3]);
         }
         __threadfence_block();  // before the row's bytes, which may lie in those words
     }
