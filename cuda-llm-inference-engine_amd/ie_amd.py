@@ -400,7 +400,6 @@ def _refuse(what, *tensors):
                      + ", ".join(f"{t.dtype} {tuple(t.shape)} strides {tuple(t.stride())} on {t.device}" for t in tensors))
 
 
-_INT_MAX = 2**31 - 1  # ctypes takes an int's lowest 32 bits and says nothing
 _device_index = None  # () -> index of the current device
 _raw_stream_of = None  # device index -> handle of its current stream
 _f32 = _i32 = _i8 = _empty = None
@@ -421,7 +420,7 @@ def _failed(name, status):
     raise IeError(name, status, last_error())
 
 
-def _past_int(what, name, value):
+def _past_int(what, name, value):  # (ctypes takes an int's lowest 32 bits and says nothing)
     raise ValueError(f"{what}: {name}={value} lies outside 32 bits")
 
 
@@ -490,7 +489,7 @@ def _kv8_rows(what, K, V, lead, H, d, at):
         ld = st[0] if lead[0] > 1 else H * d
     want = (*lead, H, d)
     if (K.shape != want or V.shape != want or K.dtype is not _f32 or V.dtype is not _f32 or K.get_device() != at
-            or V.get_device() != at or V.stride() != st or st[-1] != 1 or (H > 1 and st[-2] != d) or ld > _INT_MAX
+            or V.get_device() != at or V.stride() != st or st[-1] != 1 or (H > 1 and st[-2] != d) or ld > 0x7FFFFFFF
             or (len(lead) == 2 and lead[0] > 1 and lead[1] > 1 and st[0] != lead[1] * ld)):
         raise ValueError(f"{what}: K and V need to be fp32 {want} on cuda:{at} with equal strides, rows whole and evenly "
                          f"spaced; got {tuple(K.shape)} strides {st}, {tuple(V.shape)} strides {V.stride()}")
@@ -504,7 +503,7 @@ def kv8_cache_write(K, V, cache, block_table, start_pos, stream=None):
     B, P = K.shape[:2]
     if rows != B:
         raise ValueError("kv8_cache_write: block_table has other sequences than K")
-    if not -_INT_MAX <= start_pos <= _INT_MAX:
+    if not -0x80000000 <= start_pos <= 0x7FFFFFFF:
         _past_int("kv8_cache_write", "start_pos", start_pos)
     ld = _kv8_rows("kv8_cache_write", K, V, (B, P), H, d, at) if B * P else H * d
     k, v, ks, vs = cache
@@ -564,7 +563,7 @@ def decode_attn_kv8(Q, cache, block_table, context_lens, max_ctx, splits=0, out=
     <= max_ctx cached positions; returns O [B, H_q, d]."""
     H, bs, d, at, rows, nbps = _kv8("decode_attn_kv8", cache, block_table)
     B, H_q, dq = Q.shape
-    if not -_INT_MAX <= max_ctx <= _INT_MAX:
+    if not -0x80000000 <= max_ctx <= 0x7FFFFFFF:
         _past_int("decode_attn_kv8", "max_ctx", max_ctx)
     if out is None:
         out = _new(stream, (B, H_q, d), _f32, Q.device)
@@ -596,7 +595,7 @@ def prefill_attn_kv8(Q, cache, block_table, start_pos, out=None, workspace=None,
     ie_prefill_kv8_workspace_bytes (made here where the call has use for one)."""
     H, bs, d, at, rows, nbps = _kv8("prefill_attn_kv8", cache, block_table)
     B, P, H_q, dq = Q.shape
-    if not -_INT_MAX <= start_pos <= _INT_MAX:
+    if not -0x80000000 <= start_pos <= 0x7FFFFFFF:
         _past_int("prefill_attn_kv8", "start_pos", start_pos)
     if out is None:
         out = _new(stream, (B, P, H_q, d), _f32, Q.device)
@@ -638,7 +637,7 @@ def token_logprobs(logits, targets=None, k=0, out=None, workspace=None, stream=N
     at = _device_index()
     ld, step = logits.stride()
     if (logits.get_device() != at or logits.dtype is not _f32 or (n > 1 and step != 1)
-            or (rows > 1 and not n <= ld <= _INT_MAX)):
+            or (rows > 1 and not n <= ld <= 0x7FFFFFFF)):
         raise ValueError(f"token_logprobs: logits need to be fp32 rows on cuda:{at}, got {logits.dtype} strides "
                          f"{(ld, step)} on {logits.device}")
     if targets is not None and not (targets.numel() == rows and targets.dtype is _i32 and targets.get_device() == at
