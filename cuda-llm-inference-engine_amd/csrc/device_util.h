@@ -95,6 +95,24 @@ __device__ __forceinline__ float row16_max(float v) {
 __device__ __forceinline__ float wave_max(float v) { return max_xor32(max_xor16(row16_max(v))); }
 __device__ __forceinline__ float wave_sum(float v) { return sum_xor32(sum_xor16(row16_sum(v))); }
 
+// The larger; NaN stays (one instruction, where fmaxf first quiets its operands).
+__device__ __forceinline__ float max_of(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+// Largest over the wave, in every lane.
+__device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
+    v = max(v, (uint32_t)dpp_row_ror<8>((int)v));
+    v = max(v, (uint32_t)dpp_row_ror<4>((int)v));
+    v = max(v, (uint32_t)dpp_row_ror<2>((int)v));
+    v = max(v, (uint32_t)dpp_row_ror<1>((int)v));
+    float a, b;
+    pair16(__builtin_bit_cast(float, v), a, b);
+    v = max(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b));
+    pair32(__builtin_bit_cast(float, v), a, b);
+    return max(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b));
+}
+// 2^(biased - 127), 1 <= biased <= 254, and a number's biased exponent.
+__device__ __forceinline__ float pow2(int biased) { return __builtin_bit_cast(float, (uint32_t)biased << 23); }
+__device__ __forceinline__ int biased_exp(float v) { return (int)((__builtin_bit_cast(uint32_t, v) >> 23) & 255u); }
+
 __device__ __forceinline__ float bf16_to_f32(uint16_t h) {
     return __builtin_bit_cast(float, (uint32_t)h << 16);
 }

@@ -67,8 +67,6 @@ __device__ __forceinline__ float quad_sum(float v) {
     v += dpp_quad<0x4E>(v);  // lanes 2, 3, 0, 1
     return v;
 }
-__device__ __forceinline__ float pow2(int biased) { return __builtin_bit_cast(float, (uint32_t)biased << 23); }
-__device__ __forceinline__ int biased_exp(float v) { return (int)((__builtin_bit_cast(uint32_t, v) >> 23) & 255u); }
 // Biased digits: byte i of the result is the signed digit i of x plus 128.
 __device__ __forceinline__ uint32_t biased_digits(int x) { return (uint32_t)x + 0x80808080u; }
 

@@ -14,18 +14,6 @@ __device__ __forceinline__ uint32_t fbits(float x) { return __builtin_bit_cast(u
 __device__ __forceinline__ float bitsf(uint32_t x) { return __builtin_bit_cast(float, x); }
 // Larger of two values >= +0, where NaN is the largest.
 __device__ __forceinline__ float max_nan(float a, float b) { return bitsf(max(fbits(a), fbits(b))); }
-// Largest over the wave, in every lane.
-__device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
-    v = max(v, (uint32_t)dpp_row_ror<8>((int)v));
-    v = max(v, (uint32_t)dpp_row_ror<4>((int)v));
-    v = max(v, (uint32_t)dpp_row_ror<2>((int)v));
-    v = max(v, (uint32_t)dpp_row_ror<1>((int)v));
-    float a, b;
-    pair16(bitsf(v), a, b);
-    v = max(fbits(a), fbits(b));
-    pair32(bitsf(v), a, b);
-    return max(fbits(a), fbits(b));
-}
 // rint as an int; NaN gives 0.  |x| <= 127 * (1 + 2^-22) here: need / scale <= 1.
 __device__ __forceinline__ int code(float x) { return (int)rintf(x); }
 __device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {

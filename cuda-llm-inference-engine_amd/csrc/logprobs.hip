@@ -73,8 +73,6 @@ __device__ __forceinline__ uint32_t order_key(float x) {
 __device__ __forceinline__ float key_value(uint32_t k) {
     return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
 }
-__device__ __forceinline__ float max_of(float a, float b) { return __builtin_elementwise_maximum(a, b); }  // NaN stays
-
 // Element of a workgroup's candidates: larger value first, then lower index.
 __device__ __forceinline__ uint64_t packed(float v, int i) {
     return ((uint64_t)order_key(v) << 32) | (0xffffffffu - (uint32_t)i);
@@ -91,18 +89,6 @@ __device__ __forceinline__ float wave_most(float v) {
     v = max_of(a, b);
     pair32(v, a, b);
     return max_of(a, b);
-}
-
-__device__ __forceinline__ uint32_t wave_largest(uint32_t v) {
-    v = max(v, (uint32_t)dpp_row_ror<8>((int)v));
-    v = max(v, (uint32_t)dpp_row_ror<4>((int)v));
-    v = max(v, (uint32_t)dpp_row_ror<2>((int)v));
-    v = max(v, (uint32_t)dpp_row_ror<1>((int)v));
-    float a, b;
-    pair16(__uint_as_float(v), a, b);
-    v = max(__float_as_uint(a), __float_as_uint(b));
-    pair32(__uint_as_float(v), a, b);
-    return max(__float_as_uint(a), __float_as_uint(b));
 }
 
 // Candidates pk[0 .. cnt) ranked (all different), out(rank, packed) for the
@@ -186,10 +172,10 @@ struct Candidates {
 // by taking the largest away, otherwise its first 20 bits, one ballot a bit.
 __device__ __forceinline__ uint32_t wave_bound(uint32_t key, int need) {
     if (need <= 4) {  // uniform
-        uint32_t b = wave_largest(key);
+        uint32_t b = wave_umax(key);
         for (int found = __popcll(__ballot(key == b)); found < need; found += __popcll(__ballot(key == b))) {
             if (key >= b) key = 0;
-            b = wave_largest(key);
+            b = wave_umax(key);
         }
         return b;
     }
