@@ -569,6 +569,10 @@ int row_blocks(int P, int G, int rows) { return (int)(((long long)P * G + rows -
 //     be too short, two teams: 1 x 150 behind 4000 36.6 against 50.3.  d = 64: two teams
 //     for at least four parts, 1 x 512 x 12 behind 4000 29.7 against 34.1, else one: 1
 //     x 1500 x 12 behind 4000 74.8 against 94.9, 1 x 400 x (8 x 4) 47.5 against 57.7.
+//   Left in one piece, and not measured cut: 209 to 256, and lengths for which the
+//     fixed number of parts above would give parts that are too short, though fewer
+//     parts would not (8 x 4 heads behind 4000: 105 to 144 tokens at d = 64, 105 to 128
+//     at d = 128).
 enum Form { kRows16, kTwoTeams, kOneTeam };
 struct Plan {
     Form form;

@@ -25,7 +25,7 @@
 // moves 4.7 to 5.2); k = 0 77 us.  (With the row held in registers, 25 words a thread,
 // 145 us: two rows a CU, which load and compute in step.)  Few rows are bound by
 // one wave's instructions and waits (of a wave's 4.0 thousand issue slots with 64 rows,
-// k = 5, 2.2 are waits and 1.1 instructions): 8 x 50257, k = 5 10.5 us, of them 4 the
+// k = 5, 2.2 are waits and 1.1 instructions): 8 x 50257, k = 5 10.7 us, of them 4 the
 // join's.  Six waves a SIMD at least: with eight, whose 78 scalar registers keep
 // 57 more in vector lanes, 512 x 50257, k = 5 32.7 against 31.1 us, 2048, k = 20
 // 88.6 against 91.4.  Two, six or eight words in flight a thread instead of four: 8 x

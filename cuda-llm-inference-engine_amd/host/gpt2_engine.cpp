@@ -527,6 +527,8 @@ struct GPT2Engine::Impl {
     }
 
     // The same for a prompt chunk's rows pf.qkv [B * Pc, 3d] at positions pos ..
+    // (its context cut into parts where the decode step's workspace holds them:
+    // chunks of a few tokens).
     void kv8_prompt(int B, int Pc, int l) {
         const int d = cfg.d_model, H = cfg.n_heads;
         ie::Kv8Write w{};
