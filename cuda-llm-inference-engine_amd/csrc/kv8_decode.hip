@@ -338,11 +338,18 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? (NT == 1 ? 4 : 3) : (NT == 1 ? 3
                 float p[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) p[i] = exp2_sm(sc[i] - m[c]);
-                const float wc = vscale * pow2(254 - ub[c]);
+                float wc = vscale * pow2(254 - ub[c]);
                 float sum = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) sum += p[i];
                 l[c] += sum;
+                if (__ballot(wc == INFINITY) != 0) {  // uniform; a scale more than 2^127 times W's: its weights in two steps
+                    asm volatile("");
+                    const bool over = wc == INFINITY;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) p[i] *= over ? vscale : 1.0f;
+                    wc = over ? pow2(254 - ub[c]) : wc;
+                }
                 i32x4 wd;
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {

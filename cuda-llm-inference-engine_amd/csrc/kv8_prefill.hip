@@ -16,8 +16,10 @@
 // heads that share K and V share its staging.
 //
 // The running maximum m and the weights' unit move only when a weight would
-// pass the unit (set to 8 times the largest of a tile); then the output is
-// rescaled.  Weights more than 29 powers of two below the unit lose bits.
+// pass the unit (set to 8 times the largest of a tile), or a scale 2^126 units
+// (which costs 4 x 512 x 12 x 64 12.5 -> 12.7 us, and without which it is infinite where its
+// weight is not); then the output is rescaled.  Weights more than 29 powers of two
+// below the unit lose bits.
 //
 // Two forms.  block: four waves of 16 NC rows each walk the tiles together;
 // wave w brings group w of the next tile (global bytes in registers during the
@@ -158,18 +160,26 @@ __device__ __forceinline__ void weights(const f32x4 (&acc)[4], float sw, float v
         for (int i = 1; i < 16; ++i) top = max_of(top, acc[i >> 2][i & 3]);
     }
     top = top == -INFINITY ? top : top * sw;
-    // log2 of the lane's largest weight, rounded up, against m
-    const float vexp = (float)(biased_exp(vscale) - 126);
-    bool moved = fmaxf(top - st.m + vexp - (float)(st.ub - 127), top - st.m - 70.0f) > 15.0f;
+    // log2 of the lane's largest weight, rounded up, against m; and a scale has to be a
+    // number of units that fp32 holds (so as if no weight were less than 2^-111 of it)
+    float vexp = (float)(biased_exp(vscale) - 126);
+    const float ahead = top - st.m;
+    bool moved = fmaxf(fmaxf(ahead, -111.0f) + (vexp - (float)(st.ub - 127)), ahead - 70.0f) > 15.0f;
     if (__ballot(moved) != 0) {  // uniform
+        if (key0 >= lim) {  // (a page that the row sees nothing of)
+            moved = false;
+            vexp = -126.0f;
+        }
         moved = max_xor32(max_xor16(moved ? 1.0f : 0.0f)) > 0.0f;  // over the row
         const float rtop = max_xor32(max_xor16(top));
         const float mn = moved ? fmaxf(st.m, rtop) : st.m;
         const float f = moved ? exp2_sm(st.m - mn) : 1.0f;
         const float wm = max_xor32(max_xor16(top - mn + vexp));
-        // 8 times the tile's largest weight, and not below the unit that the output has
-        // so far (which may be of far larger values): o moves by at most a factor of 2
-        const float unit = fmaxf(ceilf(wm) + (127.0f + 3.0f - 15.0f), ceilf((float)st.ub + (st.m - mn)));
+        // 8 times the tile's largest weight, not below the unit that the output has so far
+        // (which may be of far larger values: o moves by at most a factor of 2), and not
+        // below 2^-126 of the tile's largest scale (of which no weight is less)
+        const float most = max_xor32(max_xor16(vexp));
+        const float unit = fmaxf(fmaxf(ceilf(wm) + (127.0f + 3.0f - 15.0f), ceilf((float)st.ub + (st.m - mn))), most + 1.0f);
         const int ub = moved ? (int)fminf(fmaxf(unit, 1.0f), 224.0f) : st.ub;
         const float fo = f * pow2(127 + min(max(st.ub - ub, -126), 127));
 #pragma unroll

@@ -577,6 +577,34 @@ def test_large_values_behind_a_page_of_zeros(ie, dev, B, H, G, d, start, P):
         assert (np.abs(got - want[:, -1]) <= tol * want[:, -1]).all()
 
 
+@pytest.mark.parametrize("value", [1e5, 1e9, 1e20, 1e33])
+@pytest.mark.parametrize("B,H,G,d,start,P", [(1, 1, 1, 64, 100, 1), (8, 32, 1, 64, 130, 20), (2, 12, 1, 64, 130, 300),
+                                             (2, 16, 2, 128, 130, 100), (4, 32, 2, 128, 130, 260)])
+def test_large_values_beside_a_page_of_zeros(ie, dev, B, H, G, d, start, P, value):
+    """The same within a tile, at a distance of 81: a weight is e^-81, the large values' scale is more than 2^127 units of
+    the weights, their product is a number like any other."""
+    r = rng(d + P)
+    n, high = start + P, 20
+    table, pages = ko.tables(r, [n] * B, 16)
+    c = ko.Cache(pages, H, d, 16, r)
+    q = rows(r, 1, H, 1, d, spread=0.0).repeat(G, 2)
+    K, V = np.zeros((n, H, d), np.float32), np.zeros((n, H, d), np.float32)
+    K[high] = 81 * d**0.5 * q[0, :, 0] / (q[0, :, 0] ** 2).sum(-1, keepdims=True)
+    V[:16] = (value * np.abs(1 + 0.1 * r.standard_normal((16, H, d)))).astype(np.float32)
+    for b in range(B):
+        c.write(K, V, table[b], 0)
+    Q = np.broadcast_to(q.reshape(1, 1, H * G, d), (B, P, H * G, d)).copy()
+    want, _ = prompt_in_64_bits(dev, c, table, start, Q)
+    tol = (46 * 82 + 24 + n / 16) * ko.U
+    cache, tab = c.tensors(ie, dev), on(dev, table)
+    got = ie.prefill_attn_kv8(on(dev, Q), cache, tab, start).cpu().numpy()
+    assert (np.abs(got - want) <= tol * want).all(), (got / want).min()
+    lens = on(dev, np.full(B, n, np.int32))
+    for splits in (1, 2):
+        got = ie.decode_attn_kv8(on(dev, Q[:, 0]), cache, tab, lens, n, splits=splits).cpu().numpy()
+        assert (np.abs(got - want[:, -1]) <= tol * want[:, -1]).all(), (got / want[:, -1]).max()
+
+
 # ------------------------------------------------------------------ append and attention in one launch
 @pytest.mark.parametrize("H,G,d,block", [(12, 1, 64, 16), (2, 4, 128, 16), (3, 2, 64, 64)])
 def test_append_and_attention_in_one_launch(ie, dev, H, G, d, block):
