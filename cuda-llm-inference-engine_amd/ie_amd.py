@@ -76,6 +76,20 @@ LOGPROBS_SIGNATURES = {
 }
 LOGPROBS_TOP_MAX = 128
 
+# include/ie_paged.h
+PAGED_SIGNATURES = {
+    "ie_rope_kv_write": (_I, [_I, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _I, _P, _I, _I, _P]),
+    "ie_paged_attn_num_splits": (_I, [_I] * 9),
+    "ie_paged_attn_workspace_bytes": (_Z, [_I] * 5),
+    "ie_paged_attn": (_I, [_I, _I, _I, _I, _I, _P, _P, _P, _I, _P, _I, _I, _P, _P, _I, _P, _P, _I, _F, _F, _P, _P, _P, _Z,
+                           _I, _P]),
+    "ie_tree_attn": (_I, [_I, _I, _I, _I, _I, _P, _P, _P, _I, _P, _I, _I, _P, _P, _P, _I, _I, _F, _F, _P, _P, _P, _Z, _I,
+                          _P]),
+    "ie_kv_cache_keep": (_I, [_I, _I, _I, _P, _P, _I, _P, _I, _I, _I, _I, _P, _P, _P, _P]),
+}
+PAGED_MAX_SPLITS = 64
+TREE_MAX = 256
+
 # include/ie_engine.h
 ENGINE_SIGNATURES = {
     "ie_engine_create": (_I, [ctypes.POINTER(_P), ctypes.c_char_p, _I, _I, _I, _I, _I, _I,
@@ -146,7 +160,7 @@ def load() -> ctypes.CDLL:
         lib = ctypes.CDLL(LIB_PATH)
         for name, (res, args) in (list(SIGNATURES.items()) + list(ENGINE_SIGNATURES.items())
                                   + list(TOKENIZER_SIGNATURES.items()) + list(KV8_SIGNATURES.items())
-                                  + list(LOGPROBS_SIGNATURES.items())):
+                                  + list(LOGPROBS_SIGNATURES.items()) + list(PAGED_SIGNATURES.items())):
             fn = getattr(lib, name)
             fn.restype = res
             fn.argtypes = args
@@ -402,16 +416,16 @@ def _refuse(what, *tensors):
 
 _device_index = None  # () -> index of the current device
 _raw_stream_of = None  # device index -> handle of its current stream
-_f32 = _i32 = _i8 = _empty = None
+_f32 = _i32 = _i8 = _bf16 = _empty = None
 
 
 def _bind_torch():
-    global _device_index, _raw_stream_of, _f32, _i32, _i8, _empty
+    global _device_index, _raw_stream_of, _f32, _i32, _i8, _bf16, _empty
     import torch
 
     load()  # fills _fns
     torch.cuda.current_stream()
-    _f32, _i32, _i8, _empty = torch.float32, torch.int32, torch.int8, torch.empty
+    _f32, _i32, _i8, _bf16, _empty = torch.float32, torch.int32, torch.int8, torch.bfloat16, torch.empty
     _raw_stream_of = torch._C._cuda_getCurrentRawStream
     _device_index = torch._C._cuda_getDevice
 
@@ -669,6 +683,165 @@ def token_logprobs(logits, targets=None, k=0, out=None, workspace=None, stream=N
     if st:
         _failed("ie_token_logprobs", st)
     return TokenLogprobs(lp, rk, en, tv, ti)
+
+
+# ---------------------------------------------------------------- rotary and drafted tokens (include/ie_paged.h)
+def _paged(what, k, v, table):
+    """(heads, block size, d, kv_dtype, device, table's rows and columns) of fp32 or
+    bf16 caches [pages, block, heads, d] that fit each other."""
+    if _device_index is None:
+        _bind_torch()
+    at = _device_index()
+    kind = k.dtype
+    if not ((kind is _f32 or kind is _bf16) and v.dtype is kind and table.dtype is _i32 and k.dim() == 4 and v.shape == k.shape
+            and k.get_device() == at and v.get_device() == at and table.get_device() == at and k.is_contiguous()
+            and v.is_contiguous() and table.is_contiguous() and table.dim() == 2):
+        _refuse(what, k, v, table)
+    _, bs, H, d = k.shape
+    rows, nbps = table.shape
+    return H, bs, d, KV_F32 if kind is _f32 else KV_BF16, at, rows, nbps
+
+
+def _ints(what, t, n, at):
+    """Address of n int32 (None: none)."""
+    if t is None:
+        return None
+    if t.numel() != n or t.dtype is not _i32 or t.get_device() != at or not t.is_contiguous():
+        _refuse(what, t)
+    return t.data_ptr()
+
+
+def _paged_rows(what, x, B, P, d, at):
+    """Distance between the rows of x [B, P, heads, d] fp32, which may lie apart but evenly so (None: one row)."""
+    st = x.stride()
+    if (x.dtype is not _f32 or x.get_device() != at or x.dim() != 4 or x.shape[0] != B or x.shape[1] != P or x.shape[3] != d
+            or st[3] != 1 or (x.shape[2] > 1 and st[2] != d) or (B > 1 and P > 1 and st[0] != P * st[1])):
+        raise ValueError(f"{what}: Q, K and V need to be fp32 [{B}, {P}, heads, {d}] on cuda:{at}, rows whole and evenly "
+                         f"spaced; got {x.dtype} {tuple(x.shape)} strides {st} on {x.device}")
+    return st[1] if P > 1 else st[0] if B > 1 else None
+
+
+def rope_kv_write(Q, K, V, inv_freq, starts, k_cache, v_cache, block_table, positions=None, lens=None, interleaved=False,
+                  out=None, stream=None):
+    """Rows Q [B, P, H_q, d] (None: none), K, V [B, P, heads, d] fp32 (views into a QKV
+    projection serve as they lie) rotated by positions [B, P] (None: starts[b] + t)
+    times inv_freq [rot / 2]; K and V go to cache positions starts[b] + t, t <
+    lens[b].  Returns the rotated Q."""
+    H, bs, d, kind, at, rows, nbps = _paged("rope_kv_write", k_cache, v_cache, block_table)
+    B, P = K.shape[:2]
+    if rows != B or inv_freq.dtype is not _f32 or inv_freq.get_device() != at or not inv_freq.is_contiguous():
+        _refuse("rope_kv_write", K, block_table, inv_freq)
+    H_q, q, o, q_ld, ld = 0, None, None, None, None
+    if B * P:
+        ld = _paged_rows("rope_kv_write", K, B, P, d, at)
+        if K.shape[2] != H or V.shape != K.shape or _paged_rows("rope_kv_write", V, B, P, d, at) != ld:
+            raise ValueError(f"rope_kv_write: K and V need {H} heads and equal strides, got {tuple(K.shape)} strides "
+                             f"{K.stride()}, {tuple(V.shape)} strides {V.stride()}")
+    if Q is not None:
+        H_q = Q.shape[2]
+        if B * P:
+            q_ld = _paged_rows("rope_kv_write", Q, B, P, d, at)
+        if out is None:
+            out = _new(stream, (B, P, H_q, d), _f32, Q.device)
+        elif (out.numel() != B * P * H_q * d or out.dtype is not _f32 or out.get_device() != at or not out.is_contiguous()):
+            _refuse("rope_kv_write", out)
+        q, o = Q.data_ptr(), out.data_ptr()
+    q_ld, ld = H_q * d if q_ld is None else q_ld, H * d if ld is None else ld
+    if max(q_ld, ld) > 0x7FFFFFFF:
+        _past_int("rope_kv_write", "row distance", max(q_ld, ld))
+    st = _fns["ie_rope_kv_write"](
+        B, P, q, K.data_ptr(), V.data_ptr(), q_ld, ld, H_q, H, d, 2 * inv_freq.numel(), int(interleaved), inv_freq.data_ptr(),
+        _ints("rope_kv_write", starts, B, at), _ints("rope_kv_write", lens, B, at),
+        _ints("rope_kv_write", positions, B * P, at), o, k_cache.data_ptr(), v_cache.data_ptr(), kind,
+        block_table.data_ptr(), nbps, bs, _raw_stream_of(at) if stream is None else stream.cuda_stream)
+    if st:
+        _failed("ie_rope_kv_write", st)
+    return out
+
+
+def paged_attn_num_splits(B, P, H_q, H_kv, d, kv_dtype, max_keys, window=0, splits=0):
+    return call("ie_paged_attn_num_splits", B, P, H_q, H_kv, d, kv_dtype, max_keys, window, splits)
+
+
+def _attend(what, name, Q, k_cache, v_cache, block_table, starts, lens, extra, max_ctx, keys, window, scale, cap, slopes, splits,
+            out, workspace, stream):
+    H, bs, d, kind, at, rows, nbps = _paged(what, k_cache, v_cache, block_table)
+    B, P, H_q, dq = Q.shape
+    if not -0x80000000 <= max_ctx <= 0x7FFFFFFF:
+        _past_int(what, "max_ctx", max_ctx)
+    if not -0x80000000 <= window <= 0x7FFFFFFF:
+        _past_int(what, "window", window)
+    if out is None:
+        out = _new(stream, (B, P, H_q, d), _f32, Q.device)
+    if not (dq == d and rows == B and out.numel() == B * P * H_q * d and Q.dtype is _f32 and out.dtype is _f32
+            and Q.get_device() == at and out.get_device() == at and Q.is_contiguous() and out.is_contiguous()
+            and (slopes is None or (slopes.numel() == H_q and slopes.dtype is _f32 and slopes.get_device() == at
+                                    and slopes.is_contiguous()))):
+        _refuse(what, Q, out, block_table, *(() if slopes is None else (slopes,)))
+    if workspace is None:
+        if keys <= 0x7FFFFFFF:
+            S = _fns["ie_paged_attn_num_splits"](B, P, H_q, H, d, kind, keys, window, splits)
+            if S > 1:
+                workspace = _new(stream, B * P * H_q * S * (d + 2), _f32, Q.device)
+    elif workspace.dtype is not _f32 or workspace.get_device() != at or not workspace.is_contiguous():
+        _refuse(what, workspace)
+    st = _fns[name](
+        B, P, H_q, H, d, Q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), kind, block_table.data_ptr(), nbps, bs,
+        _ints(what, starts, B, at), _ints(what, lens, B, at), *extra(B * P, at), window, 0.0 if scale is None else scale, cap,
+        None if slopes is None else slopes.data_ptr(), out.data_ptr(), None if workspace is None else workspace.data_ptr(),
+        0 if workspace is None else 4 * workspace.numel(), splits, _raw_stream_of(at) if stream is None else stream.cuda_stream)
+    if st:
+        _failed(name, st)
+    return out
+
+
+def paged_attn(Q, k_cache, v_cache, block_table, starts, max_ctx, lens=None, first=None, end=None, window=0, scale=None,
+               cap=0.0, slopes=None, splits=0, out=None, workspace=None, stream=None):
+    """Q [B, P, H_q, d] fp32, token t of sequence b at position starts[b] + t, over caches
+    [pages, block, heads, d]; lens [B] tokens count, keys [first, end) of each ([B, P];
+    None: from 0, to itself) inside the window; scores scale q.k capped by cap * tanh and
+    less slopes[h] times the distance.  max_ctx >= starts[b] + lens[b].  Returns O
+    [B, P, H_q, d] (rows past lens[b] are not written)."""
+    def extra(n, at):
+        return max_ctx, _ints("paged_attn", first, n, at), _ints("paged_attn", end, n, at)
+    return _attend("paged_attn", "ie_paged_attn", Q, k_cache, v_cache, block_table, starts, lens, extra, max_ctx, max_ctx,
+                   window, scale, cap, slopes, splits, out, workspace, stream)
+
+
+def tree_attn(Q, k_cache, v_cache, block_table, context_lens, parents, max_ctx, lens=None, window=0, scale=None, cap=0.0,
+              slopes=None, splits=0, out=None, workspace=None, stream=None):
+    """Q [B, T, H_q, d] fp32 of drafted nodes at cache positions context_lens[b] + t, each
+    behind node parents[b, t] < t (-1: the context); over the context, its ancestors and
+    itself.  max_ctx >= context_lens[b].  Scores, lens and result as paged_attn."""
+    def extra(n, at):
+        return _ints("tree_attn", parents, n, at), max_ctx
+    return _attend("tree_attn", "ie_tree_attn", Q, k_cache, v_cache, block_table, context_lens, lens, extra, max_ctx,
+                   max_ctx + Q.shape[1], window, scale, cap, slopes, splits, out, workspace, stream)
+
+
+def kv_cache_keep(k_caches, v_caches, block_table, context_lens, paths, counts, stream=None):
+    """Rows context_lens[b] + paths[b, j] of every layer's caches to context_lens[b] + j, j <
+    counts[b]; paths [B, n] ascending."""
+    n = len(k_caches)
+    if len(v_caches) != n:
+        raise ValueError(f"kv_cache_keep: {n} K caches and {len(v_caches)} V caches")
+    if not n:
+        return
+    H, bs, d, kind, at, B, nbps = _paged("kv_cache_keep", k_caches[0], v_caches[0], block_table)
+    shape, dtype = k_caches[0].shape, k_caches[0].dtype
+    for t in (*k_caches, *v_caches):
+        if t.shape != shape or t.dtype is not dtype or t.get_device() != at or not t.is_contiguous():
+            _refuse("kv_cache_keep", k_caches[0], t)
+    if paths.dim() != 2 or paths.shape[0] != B:
+        _refuse("kv_cache_keep", block_table, paths)
+    most = paths.shape[1]
+    k, v = ((ctypes.c_void_p * n)(*(t.data_ptr() for t in c)) for c in (k_caches, v_caches))
+    st = _fns["ie_kv_cache_keep"](
+        B, most, n, k, v, kind, block_table.data_ptr(), nbps, bs, H, d, _ints("kv_cache_keep", context_lens, B, at),
+        _ints("kv_cache_keep", paths, B * most, at), _ints("kv_cache_keep", counts, B, at),
+        _raw_stream_of(at) if stream is None else stream.cuda_stream)
+    if st:
+        _failed("ie_kv_cache_keep", st)
 
 
 # ---------------------------------------------------------------- engine
