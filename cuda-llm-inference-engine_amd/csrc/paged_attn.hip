@@ -1,5 +1,19 @@
 // paged_attn.hip — attention over the paged cache with capped, biased and ranged
 // scores, and of drafted trees (include/ie_paged.h).
+//
+// The rows of a (sequence, KV head) are its tokens times the query heads that share
+// the KV head, row t * G + g, so a tile of rows reads a key once for all of them.
+// Both products run on v_mfma_f32_32x32x16_bf16 with every fp32 operand as the sum of
+// three bf16 (8 bits apiece, so the sum is the fp32 value): S^T = K Q^T, 32 keys x 32
+// rows, leaves lane l (i = l % 32, h = l / 32) with row i and keys 8 (v / 4) + 4 h +
+// v % 4, v < 16, of a block, so a softmax step is 16 values of the lane's own and one
+// swap between the halves; the weights, split again, are as they lie the B operand of
+// O^T += V^T P^T, whose A operand takes the same keys: 4 h .. 4 h + 3 and 8 + 4 h .. of
+// each 16, read transposed from V's rows (ds_read_b64_tr_b16).  A bf16 cache is one
+// part and takes three products, an fp32 cache six of the nine (the rest are below
+// 2^-24).  Statistics and outputs are fp32.
+#include <type_traits>
+
 #include "device_util.h"
 #include "paged.h"
 
@@ -7,6 +21,14 @@ namespace ie {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
+typedef __attribute__((address_space(3))) void* lds_ptr;
+typedef const __attribute__((address_space(1))) void* gbl_ptr;
 
 __device__ __forceinline__ uint32_t cache_row(const PageMap& m, const int* table, int p) {
     const int page = m.mul ? (int)(__umulhi((uint32_t)p, m.mul) >> m.shift) : p;
@@ -19,90 +41,221 @@ __device__ __forceinline__ float as_float(KV x) {
     else return bf16_to_f32(x);
 }
 
-// A query row: token t of sequence b, its position and the keys it may see.
-// Ranges: lo <= j < hi.  A tree: lo <= j < ctx, and ctx + u for u itself and its
-// ancestors whose position is at least lo.
+// The largest and smallest of non-negative ints over the wave.
+__device__ __forceinline__ int wave_imax(int v) { return (int)wave_umax((uint32_t)v); }
+__device__ __forceinline__ int wave_imin(int v) { return (int)~wave_umax(~(uint32_t)v); }
+
+// ---- operands in three parts
+__device__ __forceinline__ uint32_t round_pair(float x0, float x1) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{x0, x1}), bf16x2));
+}
+__device__ __forceinline__ float low_of(uint32_t w) { return __builtin_bit_cast(float, w << 16); }
+__device__ __forceinline__ float high_of(uint32_t w) { return __builtin_bit_cast(float, w & 0xffff0000u); }
+// x0 and x1 as three parts each, the largest first, x0's in the low halves.
+__device__ __forceinline__ void split_pair(float x0, float x1, uint32_t& a, uint32_t& b, uint32_t& c) {
+    a = round_pair(x0, x1);
+    const float r0 = x0 - low_of(a), r1 = x1 - high_of(a);
+    b = round_pair(r0, r1);
+    c = round_pair(r0 - low_of(b), r1 - high_of(b));
+}
+template <int N>
+struct Parts {
+    uint4 p[N];
+};
+__device__ __forceinline__ Parts<3> split8(const float* x) {
+    Parts<3> r;
+    split_pair(x[0], x[1], r.p[0].x, r.p[1].x, r.p[2].x);
+    split_pair(x[2], x[3], r.p[0].y, r.p[1].y, r.p[2].y);
+    split_pair(x[4], x[5], r.p[0].z, r.p[1].z, r.p[2].z);
+    split_pair(x[6], x[7], r.p[0].w, r.p[1].w, r.p[2].w);
+    return r;
+}
+__device__ __forceinline__ f32x16 mfma(uint4 a, uint4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+// The products of a's N parts and b's three, the small ones first.
+template <int N>
+__device__ __forceinline__ f32x16 product(const Parts<N>& a, const Parts<3>& b, f32x16 c) {
+    if constexpr (N == 3) {
+        c = mfma(a.p[2], b.p[0], c);
+        c = mfma(a.p[0], b.p[2], c);
+        c = mfma(a.p[1], b.p[1], c);
+        c = mfma(a.p[1], b.p[0], c);
+    } else {
+        c = mfma(a.p[0], b.p[2], c);
+    }
+    c = mfma(a.p[0], b.p[1], c);
+    return mfma(a.p[0], b.p[0], c);
+}
+
+// ---- scores
+// tanh: below 0.55 x + x^3 p(x^2), p the polynomial nearest to (tanh(x) / x - 1) / x^2 there
+// (weighted least squares, 1.2e-9 of the value off); above it 1 - 2 / (1 + e^2x), whose rounding is that of a value near 1.
+__device__ __forceinline__ float tanh_of(float x) {
+    const float a = fabsf(x), y = x * x;
+    const float e = __builtin_amdgcn_exp2f(2.0f * kLog2e * fminf(a, 20.0f));
+    const float big = __builtin_copysignf(fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + e), 1.0f), x);
+    float p = -0.0062074303f;
+    p = fmaf(p, y, 0.021027219f);
+    p = fmaf(p, y, -0.053842276f);
+    p = fmaf(p, y, 0.133325f);
+    p = fmaf(p, y, -0.33333316f);
+    const float small = fmaf(x * y, p, x);
+    return a < 0.55f ? small : x == x ? big : x;
+}
+
+// What turns a product q.k into a score of base 2: the factor folded into q, the
+// cap's factor behind tanh, and the distance's factor.
+struct Scores {
+    float q, cap, slope;
+};
+__device__ __forceinline__ Scores scores_of(const PagedAttn& a, int head) {
+    Scores s;
+    s.q = a.cap > 0.0f ? a.scale / a.cap : a.scale * kLog2e;
+    s.cap = a.cap * kLog2e;
+    s.slope = a.slopes ? a.slopes[head] * kLog2e : 0.0f;
+    return s;
+}
+
+// ---- a tree's ancestors, by node: bit u of line[t] says that t sees node u, depth
+// the number of its ancestors (inside or outside the window).
+constexpr int kLine = IE_TREE_MAX / 32 + 1;  // (odd: 32 rows' words lie in different banks)
+struct TreeLds {
+    uint32_t line[IE_TREE_MAX][kLine];
+    int depth[IE_TREE_MAX];
+    int up[IE_TREE_MAX];
+};
+struct NoTree {};
+
+// By pointer doubling: after round k a node has its 2^k nearest ancestors.
+__device__ __forceinline__ void grow_tree(TreeLds& s, const int* parents, int T, int window) {
+    const int t = threadIdx.x;
+    constexpr int W = kLine - 1;
+    uint32_t w[W];
+#pragma unroll
+    for (int k = 0; k < W; ++k) w[k] = t >> 5 == k ? 1u << (t & 31) : 0u;
+    int up = t < T ? parents[t] : -1;
+    if (up >= t) up = -1;
+    for (;;) {
+        s.up[t] = up;
+#pragma unroll
+        for (int k = 0; k < W; ++k) s.line[t][k] = w[k];
+        if (!__syncthreads_or(up >= 0)) break;
+        if (up >= 0) {
+#pragma unroll
+            for (int k = 0; k < W; ++k) w[k] |= s.line[up][k];
+            up = s.up[up];
+        }
+        __syncthreads();
+    }
+    int deep = -1;
+#pragma unroll
+    for (int k = 0; k < W; ++k) deep += __builtin_popcount(w[k]);
+    s.depth[t] = deep;
+    __syncthreads();
+    if (window > 0 && deep >= window) {
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+            uint32_t keep = w[k];
+            for (uint32_t left = w[k]; left; left &= left - 1) {
+                const int u = __builtin_ctz(left);
+                if (s.depth[32 * k + u] <= deep - window) keep &= ~(1u << u);
+            }
+            s.line[t][k] = keep;
+        }
+    }
+    __syncthreads();
+}
+
+// ---- rows
+// A row sees keys lo <= j < hi; of a tree's, j >= ctx only if its line has them.
 struct Row {
-    int b, t, lo, hi, pos, ctx;
+    int t, head;  // of the sequence; query head
+    int lo, hi, pos;
     bool live;
 };
 
-__device__ __forceinline__ int depth_of(const int* parents, int t) {
-    int n = 0;
-    for (int a = parents[t], c = t; a >= 0 && a < c; c = a, a = parents[a]) ++n;
-    return n;
-}
-
-__device__ __forceinline__ Row row_at(const PagedAttn& a, int b, int t) {
-    Row r;
-    r.b = b;
-    r.t = t;
-    const int len = a.lens ? min(a.lens[b], a.P) : a.P;
-    const int start = min(max(a.starts[b], 0), 1 << 30);
-    r.live = t < len;
-    r.lo = 0;
-    if (a.parents) {
-        r.ctx = min(start, a.max_ctx);
-        r.pos = r.ctx + (r.live ? depth_of(a.parents + (size_t)b * a.P, t) : 0);
-        r.hi = r.ctx + t + 1;
+template <bool TREE, typename Tree>
+__device__ __forceinline__ Row row_of(const PagedAttn& a, const Tree& tree, int r, int b, int kvh, int start, int len) {
+    const int G = a.H_q / a.H_kv;
+    Row x;
+    const int rc = min(r, a.P * G - 1);
+    x.t = rc / G;
+    x.head = kvh * G + (rc - x.t * G);
+    x.live = r < a.P * G && x.t < len;
+    x.lo = 0;
+    if constexpr (TREE) {
+        x.pos = start + tree.depth[x.t];
+        x.hi = start + x.t + 1;
     } else {
-        const size_t i = (size_t)b * a.P + t;
-        r.pos = start + t;
-        r.hi = min(min(start + len, a.max_ctx), a.end ? a.end[i] : r.pos + 1);
-        if (a.first) r.lo = max(0, a.first[i]);
-        r.ctx = 1 << 30;
+        const size_t i = (size_t)b * a.P + x.t;
+        x.pos = start + x.t;
+        x.hi = max(0, min(min(start + len, a.max_ctx), a.end ? a.end[i] : x.pos + 1));
+        if (a.first) x.lo = max(0, a.first[i]);
     }
-    if (a.window) r.lo = max(r.lo, r.pos - a.window + 1);
-    return r;
+    if (a.window) x.lo = max(x.lo, x.pos - a.window + 1);
+    return x;
 }
 
-// Whether a row sees key j of [lo, hi), and how far off it is.
-__device__ __forceinline__ bool sees(const PagedAttn& a, const Row& r, int j, float& gap) {
-    gap = fabsf((float)(r.pos - j));
-    if (j < r.ctx) return j >= r.lo;
-    const int* parents = a.parents + (size_t)r.b * a.P;
-    const int u = j - r.ctx;
-    int n = r.t, up = 0;
-    while (n > u) {
-        const int p = parents[n];
-        n = p >= 0 && p < n ? p : -1;
-        ++up;
+// The bits of a block of 32 keys from c0 on that a row sees.
+template <bool TREE, typename Tree>
+__device__ __forceinline__ uint32_t seen_bits(const Tree& tree, const Row& r, int c0, int ctx) {
+    const int from = min(max(r.lo - c0, 0), 32), to = min(max(r.hi - c0, 0), 32);
+    uint32_t bits = (uint32_t)((1ull << to) - 1) & (uint32_t)(~0ull << from);
+    if constexpr (TREE) {
+        const int o = c0 - ctx;  // node of the block's first key
+        if (o > -32) {
+            // nodes o .. o + 31; what lies before the tree counts as seen
+            const int w = max(o, 0) >> 5, sh = max(o, 0) & 31;
+            const uint32_t lo = w < kLine - 1 ? tree.line[r.t][w] : 0u, hi = w < kLine - 2 ? tree.line[r.t][w + 1] : 0u;
+            uint32_t nodes = (uint32_t)((((uint64_t)hi << 32) | lo) >> sh);
+            if (o < 0) nodes = (lo << -o) | ((1u << -o) - 1);
+            // (a node's position is past ctx, so lo, which is about positions, cannot cut it here)
+            const uint32_t before = o < 0 ? (1u << -o) - 1 : 0u;
+            const uint32_t past = (uint32_t)((1ull << to) - 1);
+            bits = (bits & before) | (nodes & past & ~before);
+        }
     }
-    gap = (float)up;
-    return n == u && r.pos - up >= r.lo;
+    return bits;
 }
 
-// A wave a row: a lane a key for the scores, two or one channel a lane for the
-// sums.  Keys that are not seen are never multiplied.
-template <int D, typename KV>
-__global__ __launch_bounds__(256) void paged_row_kernel(PagedAttn a) {
-    const int lane = threadIdx.x & 63;
-    const int row = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
-    if (row >= a.B * a.P * a.H_q) return;
-    const int h = row % a.H_q, bt = row / a.H_q;
-    const Row r = row_at(a, bt / a.P, bt % a.P);
-    if (!r.live) return;
-    const int* table = a.pages.table + (size_t)r.b * a.pages.nbps;
-    const size_t stride = (size_t)a.H_kv * D, at = (size_t)(h / (a.H_q / a.H_kv)) * D;
-    const KV *K = static_cast<const KV*>(a.k) + at, *V = static_cast<const KV*>(a.v) + at;
-    const float* q = a.Q + (size_t)row * D;
-    const float slope = a.slopes ? a.slopes[h] : 0.0f;
+// ---- one row by one wave, a lane a key: what the matrix cores have no three-part
+// form for (see attend's `bad`), over keys k0 .. k1 - 1.  Keys that the row does not
+// see are not multiplied.  Leaves lane l with channels N l .. of the sum.
+template <int D, typename KV, bool TREE, typename Tree>
+__device__ __forceinline__ void exact_row(const PagedAttn& a, const Tree& tree, const Row& r, int b, int kvh, int ctx, int k0,
+                                          int k1, float& m, float& l, float (&o)[D / 64]) {
     constexpr int N = D / 64;
-    float m = -INFINITY, l = 0.0f, o[N] = {};
-    for (int c0 = min(r.lo, r.ctx); c0 < r.hi; c0 += 64) {
+    const int lane = threadIdx.x & 63;
+    const int* table = a.pages.table + (size_t)b * a.pages.nbps;
+    const size_t stride = (size_t)a.H_kv * D;
+    const KV *K = static_cast<const KV*>(a.k) + (size_t)kvh * D, *V = static_cast<const KV*>(a.v) + (size_t)kvh * D;
+    const float* q = a.Q + (((size_t)b * a.P + r.t) * a.H_q + r.head) * D;
+    const float slope = a.slopes ? a.slopes[r.head] : 0.0f;
+    m = -INFINITY;
+    l = 0.0f;
+    for (int i = 0; i < N; ++i) o[i] = 0.0f;
+    k0 = max(k0, TREE ? min(r.lo, ctx) : r.lo);
+    k1 = min(k1, r.hi);
+#pragma unroll 1
+    for (int c0 = k0; c0 < k1; c0 += 64) {
         const int j = c0 + lane;
-        float gap = 0.0f, s = -INFINITY;
-        const bool seen = j < r.hi && sees(a, r, j, gap);
+        const bool seen = j < k1 && (seen_bits<TREE>(tree, r, c0 + (lane & 32), ctx) >> (lane & 31) & 1);
+        float s = -INFINITY;
         uint32_t slot = 0;
         if (seen) {
             slot = cache_row(a.pages, table, j);
             const KV* k = K + slot * stride;
             float acc[4] = {};
+#pragma unroll 4
             for (int e = 0; e < D; e += 4)
                 for (int i = 0; i < 4; ++i) acc[i] = fmaf(q[e + i], as_float(k[e + i]), acc[i]);
             s = a.scale * ((acc[0] + acc[1]) + (acc[2] + acc[3]));
-            if (a.cap > 0.0f) s = a.cap * tanhf(s / a.cap);
-            if (a.slopes) s = fmaf(-slope, gap, s);
+            if (a.cap > 0.0f) s = a.cap * tanh_of(s / a.cap);
+            int at = j;
+            if constexpr (TREE) at = j < ctx ? j : ctx + tree.depth[j - ctx];
+            if (a.slopes) s = fmaf(-slope, fabsf((float)(r.pos - at)), s);
             s *= kLog2e;
         }
         const float mn = fmaxf(m, wave_max(s)), mu = mn == -INFINITY ? 0.0f : mn;
@@ -110,6 +263,7 @@ __global__ __launch_bounds__(256) void paged_row_kernel(PagedAttn a) {
         l = fmaf(l, alpha, wave_sum(p));
         m = mn;
         for (int i = 0; i < N; ++i) o[i] *= alpha;
+#pragma unroll 1
         for (uint64_t left = __ballot(seen); left; left &= left - 1) {
             const int k = __builtin_ctzll(left);
             const float w = __shfl(p, k);
@@ -117,21 +271,453 @@ __global__ __launch_bounds__(256) void paged_row_kernel(PagedAttn a) {
             for (int i = 0; i < N; ++i) o[i] = fmaf(w, as_float(v[i]), o[i]);
         }
     }
+}
+
+// ---- the tile kernel
+// A workgroup of four waves: WR of them take 32 rows each, 4 / WR groups of them
+// different keys.  A stage holds SK keys' K and V in LDS, NB blocks of 32 for each
+// group of waves; rows past the tile's keys are its last key again.
+template <int D, int NP, int WR>
+struct Tile {
+    static constexpr int WK = 4 / WR;
+    static constexpr int NB = NP == 1 && WR == 4 ? 2 : 1;
+    static constexpr int SK = 32 * NB * WK;
+    static constexpr int ROW = 2 * D;          // bytes of a part's row
+    static constexpr int PART = SK * ROW;      // of a stage's K or V
+    static constexpr int STAGE = 2 * NP * PART;
+    static constexpr int BUFS = NP == 1 ? 2 : 1;
+    static constexpr int MERGE = (WK - 1) * WR * 64 * (D / 2 + 2) * 4;  // the other key groups' states
+    static constexpr int LDS = BUFS * STAGE > MERGE ? BUFS * STAGE : MERGE;
+    static constexpr int CH = ROW / 16;        // 16-byte chunks of a row
+    // Chunk c of row r lies at c ^ swizzle: K's rows are read 32 at a time at one chunk, V's four at a
+    // time at four chunks side by side; so each read touches every bank alike.
+    __device__ static __forceinline__ int kswz(int r) { return D == 128 ? r & 15 : (r >> 1) & 7; }
+    __device__ static __forceinline__ int vswz(int r) { return D == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1); }
+};
+
+template <int D, int NP, int WR, bool TREE>
+__global__ __launch_bounds__(256, NP == 1 && WR == 4 ? 2 : 1) void paged_tile_kernel(PagedAttn a, int tiles) {
+    using T = Tile<D, NP, WR>;
+    using KV = std::conditional_t<NP == 1, uint16_t, float>;
+    using Tree = std::conditional_t<TREE, TreeLds, NoTree>;
+    constexpr int NT = D / 32, KS = D / 16;
+    __shared__ __attribute__((aligned(1024))) int8_t lds[T::LDS];
+    __shared__ uint32_t slots[2][T::SK];
+    __shared__ int bounds[4][4];
+    __shared__ Tree tree;
+    const int tid = threadIdx.x, lane = tid & 63, i = lane & 31, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), rw = wave % WR, kw = wave / WR;
+    // workgroup u: pair (sequence, KV head) u % pairs, so that a pair's tiles run on one XCD where pairs
+    // are a multiple of 8; then the tile, the last (a prompt's longest) first, then the split
+    const int pairs = a.B * a.H_kv;
+    const int u = blockIdx.x / pairs, pair = blockIdx.x - u * pairs;
+    const int split = u / tiles, tile = tiles - 1 - (u - split * tiles);
+    const int b = pair / a.H_kv, kvh = pair - b * a.H_kv;
+    const int start = TREE ? min(max(a.starts[b], 0), a.max_ctx) : min(max(a.starts[b], 0), 1 << 30);
+    const int len = a.lens ? min(a.lens[b], a.P) : a.P;
+    if constexpr (TREE) grow_tree(tree, a.parents + (size_t)b * a.P, a.P, a.window);
+    const Row row = row_of<TREE>(a, tree, tile * 32 * WR + rw * 32 + i, b, kvh, start, len);
+    const int ctx = start;
+
+    // Keys that some row of the tile sees, and, of this wave's rows, between which every row sees all.
+    const bool some = row.live && row.lo < row.hi;
+    const int w_lo = wave_imin(some ? row.lo : 0x7fffffff), w_hi = wave_imax(some ? row.hi : 0);
+    const int all_lo = wave_imax(row.live ? row.lo : 0);
+    const int all_hi = wave_imin(row.live ? (TREE ? min(row.hi, ctx) : row.hi) : 0x7fffffff);
+    if (lane == 0) {
+        bounds[wave][0] = w_lo;
+        bounds[wave][1] = w_hi;
+    }
+    __syncthreads();
+    int kbeg = 0x7fffffff, kend = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        kbeg = min(kbeg, bounds[w][0]);
+        kend = max(kend, bounds[w][1]);
+    }
+    if (kbeg > kend) kbeg = kend;
+    // this split's stages
+    const int all = (kend - kbeg + T::SK - 1) / T::SK, per = (all + a.splits - 1) / a.splits;
+    const int s0 = min(split * per, all), s1 = min(s0 + per, all);
+    const int k0 = kbeg + s0 * T::SK, k1 = min(kbeg + s1 * T::SK, kend);
+
+    const int* table = a.pages.table + (size_t)b * a.pages.nbps;
+    const size_t row_bytes = (size_t)a.H_kv * D * sizeof(KV);
+    const int8_t* kbase = reinterpret_cast<const int8_t*>(static_cast<const KV*>(a.k) + (size_t)kvh * D);
+    const int8_t* vbase = reinterpret_cast<const int8_t*>(static_cast<const KV*>(a.v) + (size_t)kvh * D);
+    auto find = [&](int s) { return cache_row(a.pages, table, min(kbeg + s * T::SK + tid, k1 - 1)); };
+
+    // bf16: a stage's rows straight into LDS; a wave's load fills 1 KiB, its lanes' addresses are
+    // permuted so that the chunks land swizzled.
+    constexpr int RPL = 1024 / T::ROW, LOADS = T::SK / RPL / 4;
+    auto copy = [&](int s, int buf) {
+        if constexpr (NP == 1) {
+#pragma unroll
+            for (int j = 0; j < LOADS; ++j) {
+                const int r0 = (wave + 4 * j) * RPL, r = r0 + lane / T::CH, c = lane % T::CH;
+                const size_t at = slots[s & 1][r] * row_bytes;
+                int8_t* to = lds + buf * T::STAGE + r0 * T::ROW;
+                __builtin_amdgcn_global_load_lds((gbl_ptr)(kbase + at + 16 * (c ^ T::kswz(r))), (lds_ptr)to, 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((gbl_ptr)(vbase + at + 16 * (c ^ T::vswz(r))), (lds_ptr)(to + T::PART), 16, 0, 0);
+            }
+        }
+    };
+    // fp32: through registers, split on the way.
+    constexpr int CPT = NP == 1 ? 1 : T::SK * T::CH / 256;  // chunks of eight values a thread
+    float4 raw[2][CPT][2];
+    auto load = [&](int s) {
+        if constexpr (NP == 3) {
+#pragma unroll
+            for (int j = 0; j < CPT; ++j) {
+                const int id = tid + 256 * j, r = id / T::CH, c = id % T::CH;
+                const size_t at = slots[s & 1][r] * row_bytes + 32 * c;
+                raw[0][j][0] = *reinterpret_cast<const float4*>(kbase + at);
+                raw[0][j][1] = *reinterpret_cast<const float4*>(kbase + at + 16);
+                raw[1][j][0] = *reinterpret_cast<const float4*>(vbase + at);
+                raw[1][j][1] = *reinterpret_cast<const float4*>(vbase + at + 16);
+            }
+        }
+    };
+    auto store = [&] {
+        if constexpr (NP == 3) {
+#pragma unroll
+            for (int j = 0; j < CPT; ++j) {
+                const int id = tid + 256 * j, r = id / T::CH, c = id % T::CH;
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const float4 p = raw[x][j][0], q = raw[x][j][1];
+                    const float y[8] = {p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
+                    const Parts<3> parts = split8(y);
+                    const int at = x * NP * T::PART + r * T::ROW + 16 * (c ^ (x ? T::vswz(r) : T::kswz(r)));
+#pragma unroll
+                    for (int n = 0; n < 3; ++n) *reinterpret_cast<uint4*>(lds + at + n * T::PART) = parts.p[n];
+                }
+            }
+        }
+    };
+
+    if (s0 < s1 && tid < T::SK) {
+        slots[s0 & 1][tid] = find(s0);
+        slots[(s0 + 1) & 1][tid] = find(s0 + 1);
+    }
+    __syncthreads();
+    if (s0 < s1) {
+        if constexpr (NP == 1) copy(s0, 0);
+        else load(s0);
+    }
+
+    // The query rows in parts, and whether one of a row's values has none that serve: a value
+    // below 2^-98 once scaled, whose parts bf16 may not hold, or one from 2^64 on.
+    const Scores sc = scores_of(a, row.head);
+    const float* qrow = a.Q + (((size_t)b * a.P + row.t) * a.H_q + row.head) * D;
+    Parts<3> q[KS];
+    bool q_bad = false;
+    {
+        float least = INFINITY, most = 0.0f;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const float4 x = *reinterpret_cast<const float4*>(qrow + 16 * s + 8 * h);
+            const float4 y = *reinterpret_cast<const float4*>(qrow + 16 * s + 8 * h + 4);
+            float z[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                z[e] *= sc.q;
+                least = fminf(least, fabsf(z[e]));
+                most = fmaxf(most, fabsf(z[e]));
+            }
+            q[s] = split8(z);
+        }
+        if (__ballot(!(least >= 0x1p-98f && most < 0x1p64f))) {  // (seldom; zeros among them)
+#pragma unroll 1
+            for (int e = 0; e < D; ++e) {
+                const float x = qrow[e], y = fabsf(x * sc.q);
+                q_bad |= x != 0.0f && !(y >= 0x1p-98f && y < 0x1p64f);
+            }
+        }
+    }
+
+    float m = -INFINITY, l = 0.0f;
+    f32x16 o[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) o[t] = f32x16{};
+
+    // LDS places of a lane's operands: chunk 2 s + h of key i; of V, 8 bytes of keys 4 h + (lane % 16) / 4
+    // on at channels 16 (lane / 16 % 2) + 4 (lane % 4) of tile t.
+    const int krow = i * T::ROW, kx = 16 * (h ^ T::kswz(i));
+    const int vkey = 4 * h + (lane & 15) / 4, vrow = vkey * T::ROW;
+    const int vc = 2 * (lane >> 4 & 1) + (lane >> 1 & 1), vsub = 8 * (lane & 1);
+
+    auto attend = [&](const int8_t* stage, int blk, int c0) {
+        const int8_t* kp = stage + blk * 32 * T::ROW;
+        const int8_t* vp = stage + NP * T::PART + blk * 32 * T::ROW;
+        f32x16 s{};
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            Parts<NP> x;
+#pragma unroll
+            for (int n = 0; n < NP; ++n) x.p[n] = *reinterpret_cast<const uint4*>(kp + n * T::PART + krow + (kx ^ (32 * k)));
+            s = product<NP>(x, q[k], s);
+        }
+        if (a.cap > 0.0f) {
+#pragma unroll
+            for (int v = 0; v < 16; ++v) s[v] = sc.cap * tanh_of(s[v]);
+        }
+        const bool edge = c0 < all_lo || c0 + 32 > all_hi;
+        if (a.slopes) {
+            if (TREE && c0 + 32 > ctx) {
+                if constexpr (TREE) {
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) {
+                        const int j = c0 + 8 * (v >> 2) + 4 * h + (v & 3);
+                        const int at = j < ctx ? j : ctx + tree.depth[min(j - ctx, IE_TREE_MAX - 1)];
+                        s[v] = fmaf(-sc.slope, fabsf((float)(row.pos - at)), s[v]);
+                    }
+                }
+            } else {
+                const int base = row.pos - c0 - 4 * h;
+#pragma unroll
+                for (int v = 0; v < 16; ++v) s[v] = fmaf(-sc.slope, fabsf((float)(base - 8 * (v >> 2) - (v & 3))), s[v]);
+            }
+        }
+        if (edge) {
+            const uint32_t bits = seen_bits<TREE>(tree, row, c0, ctx) >> (4 * h);
+#pragma unroll
+            for (int v = 0; v < 16; ++v)
+                if (!(bits >> (8 * (v >> 2) + (v & 3)) & 1)) s[v] = -INFINITY;
+        }
+        float top = s[0];
+#pragma unroll
+        for (int v = 1; v < 16; ++v) top = fmaxf(top, s[v]);
+        const float mn = fmaxf(m, max_xor32(top));
+        const float mu = mn == -INFINITY ? 0.0f : mn;  // no key yet: keep o, l at 0
+        const float alpha = exp2_sm(m - mu);
+        m = mn;
+        float p[16], sum = 0.0f;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+            p[v] = exp2_sm(s[v] - mu);
+            sum += p[v];
+        }
+        l = fmaf(l, alpha, sum);  // (a lane's own 16 keys; the halves are added at the end)
+        if (__ballot(alpha != 1.0f)) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t) o[t] *= alpha;
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const Parts<3> w = split8(p + 8 * k);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                Parts<NP> x;
+#pragma unroll
+                for (int n = 0; n < NP; ++n) {
+                    const int8_t* at = vp + n * T::PART + vrow + 16 * k * T::ROW + 16 * ((4 * t + vc) ^ T::vswz(vkey)) + vsub;
+                    const s16x4 u0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)at);
+                    const s16x4 u1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + 8 * T::ROW));
+                    const uint2 y0 = __builtin_bit_cast(uint2, u0), y1 = __builtin_bit_cast(uint2, u1);
+                    x.p[n] = make_uint4(y0.x, y0.y, y1.x, y1.y);
+                }
+                o[t] = product<NP>(x, w, o[t]);
+            }
+        }
+    };
+
+#pragma unroll 1
+    for (int s = s0; s < s1; ++s) {
+        int buf = 0;
+        if constexpr (NP == 1) {
+            buf = (s - s0) & 1;
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();  // stage s is there, and the other buffer read
+            if (s + 1 < s1) copy(s + 1, buf ^ 1);
+        } else {
+            __syncthreads();  // the last stage has been read
+            store();
+            __syncthreads();
+            if (s + 1 < s1) load(s + 1);
+        }
+        uint32_t next = 0;
+        if (s + 2 < s1 && tid < T::SK) next = find(s + 2);
+        const int8_t* stage = lds + buf * T::STAGE;
+#pragma unroll
+        for (int n = 0; n < T::NB; ++n) {
+            const int blk = kw * T::NB + n, c0 = kbeg + s * T::SK + 32 * blk;
+            if (c0 < w_hi && c0 + 32 > w_lo) attend(stage, blk, c0);
+        }
+        if (s + 2 < s1 && tid < T::SK) slots[s & 1][tid] = next;
+    }
+    l = sum_xor32(l);
+
+    // The key groups' states into the first one's.
+    if constexpr (T::WK > 1) {
+        __syncthreads();
+        float4* mo = reinterpret_cast<float4*>(lds);
+        float2* ml = reinterpret_cast<float2*>(lds + (T::WK - 1) * WR * 64 * (D / 2) * 4);
+        if (kw > 0) {
+            const int g = (kw - 1) * WR + rw;
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int v = 0; v < 4; ++v)
+                    mo[(g * NT * 4 + t * 4 + v) * 64 + lane] = make_float4(o[t][4 * v], o[t][4 * v + 1], o[t][4 * v + 2], o[t][4 * v + 3]);
+            ml[g * 64 + lane] = make_float2(m, l);
+        }
+        __syncthreads();
+        if (kw > 0) return;
+#pragma unroll 1
+        for (int k = 1; k < T::WK; ++k) {
+            const int g = (k - 1) * WR + rw;
+            const float2 x = ml[g * 64 + lane];
+            const float mn = fmaxf(m, x.x), mu = mn == -INFINITY ? 0.0f : mn;
+            const float fa = exp2_sm(m - mu), fb = exp2_sm(x.x - mu);
+            m = mn;
+            l = l * fa + x.y * fb;
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                    const float4 y = mo[(g * NT * 4 + t * 4 + v) * 64 + lane];
+                    o[t][4 * v] = o[t][4 * v] * fa + y.x * fb;
+                    o[t][4 * v + 1] = o[t][4 * v + 1] * fa + y.y * fb;
+                    o[t][4 * v + 2] = o[t][4 * v + 2] * fa + y.z * fb;
+                    o[t][4 * v + 3] = o[t][4 * v + 3] * fa + y.w * fb;
+                }
+        }
+    }
+
+    // Rows whose result is not finite, or whose query has no parts, again one by one.
+    float bad = l * 0.0f;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) bad = fmaf(o[t][v], 0.0f, bad);
+    const uint64_t lanes = __ballot(row.live && (q_bad || !(bad == 0.0f)));
+    uint32_t again = (uint32_t)lanes | (uint32_t)(lanes >> 32);
+    const size_t rows = (size_t)a.B * a.P * a.H_q, mine = ((size_t)b * a.P + row.t) * a.H_q + row.head;
+    if (row.live && !(again >> i & 1)) {
+        float* out;
+        float inv = 1.0f;
+        if (a.splits == 1) {
+            inv = l > 0.0f ? 1.0f / l : 0.0f;
+            out = a.O + mine * D;
+        } else {
+            out = a.ws + (split * rows + mine) * D;
+            if (h == 0) *reinterpret_cast<float2*>(a.ws + a.splits * rows * D + 2 * (split * rows + mine)) = make_float2(m, l);
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int v = 0; v < 4; ++v)
+                *reinterpret_cast<float4*>(out + 32 * t + 8 * v + 4 * h) =
+                    make_float4(o[t][4 * v] * inv, o[t][4 * v + 1] * inv, o[t][4 * v + 2] * inv, o[t][4 * v + 3] * inv);
+    }
+#pragma unroll 1
+    for (; again; again &= again - 1) {
+        const int x = __builtin_ctz(again);
+        Row r;
+        r.t = __shfl(row.t, x);
+        r.head = __shfl(row.head, x);
+        r.lo = __shfl(row.lo, x);
+        r.hi = __shfl(row.hi, x);
+        r.pos = __shfl(row.pos, x);
+        r.live = true;
+        float rm, rl, ro[D / 64];
+        exact_row<D, KV, TREE>(a, tree, r, b, kvh, ctx, k0, k1, rm, rl, ro);
+        const size_t at = ((size_t)b * a.P + r.t) * a.H_q + r.head;
+        float* out = a.O + at * D;
+        float inv = 1.0f;
+        if (a.splits == 1) {
+            inv = rl == 0.0f ? 0.0f : 1.0f / rl;
+        } else {
+            out = a.ws + (split * rows + at) * D;
+            if (lane == 0) *reinterpret_cast<float2*>(a.ws + a.splits * rows * D + 2 * (split * rows + at)) = make_float2(rm, rl);
+        }
+        for (int e = 0; e < D / 64; ++e) out[lane * (D / 64) + e] = ro[e] * inv;
+    }
+}
+
+// O rows from their splits' partials, D / 4 lanes a row.
+template <int D>
+__global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn a) {
+    constexpr int L = D / 4;
+    const size_t rows = (size_t)a.B * a.P * a.H_q;
+    const size_t r = (size_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+    if (r >= rows) return;
+    if (a.lens && (int)(r / a.H_q % a.P) >= a.lens[r / a.H_q / a.P]) return;
+    const float2* ml = reinterpret_cast<const float2*>(a.ws + a.splits * rows * D);
+    float m = -INFINITY;
+    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, ml[s * rows + r].x);
+    const float mu = m == -INFINITY ? 0.0f : m;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float l = 0.0f;
+    const int c = threadIdx.x % L;
+    for (int s = 0; s < a.splits; ++s) {
+        const float2 x = ml[s * rows + r];
+        if (x.y == 0.0f) continue;
+        const float f = exp2_sm(x.x - mu);
+        const float4 y = reinterpret_cast<const float4*>(a.ws + (s * rows + r) * D)[c];
+        l = fmaf(f, x.y, l);
+        o.x = fmaf(f, y.x, o.x);
+        o.y = fmaf(f, y.y, o.y);
+        o.z = fmaf(f, y.z, o.z);
+        o.w = fmaf(f, y.w, o.w);
+    }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    float* out = a.O + (size_t)row * D + lane * N;
-    for (int i = 0; i < N; ++i) out[i] = o[i] * inv;
+    reinterpret_cast<float4*>(a.O + r * D)[c] = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+}
+
+// Waves of a workgroup that take different rows.
+int row_waves(int P, int G, int kv_dtype) {
+    const long long rows = (long long)P * G;
+    if (kv_dtype == IE_KV_BF16 && rows <= 32) return 1;
+    return rows <= 64 ? 2 : 4;
+}
+
+template <int D, int NP, int WR>
+void launch_tile(const PagedAttn& a, hipStream_t s) {
+    const int G = a.H_q / a.H_kv, tiles = (int)(((long long)a.P * G + 32 * WR - 1) / (32 * WR));
+    const unsigned grid = (unsigned)((long long)a.B * a.H_kv * tiles * a.splits);
+    auto* k = a.parents ? paged_tile_kernel<D, NP, WR, true> : paged_tile_kernel<D, NP, WR, false>;
+    k<<<grid, 256, 0, s>>>(a, tiles);
+}
+
+template <int D>
+void launch_d(const PagedAttn& a, hipStream_t s) {
+    const int wr = row_waves(a.P, a.H_q / a.H_kv, a.kv_dtype);
+    if (a.kv_dtype == IE_KV_BF16) {
+        if (wr == 1) launch_tile<D, 1, 1>(a, s);
+        else if (wr == 2) launch_tile<D, 1, 2>(a, s);
+        else launch_tile<D, 1, 4>(a, s);
+    } else {
+        if (wr == 2) launch_tile<D, 3, 2>(a, s);
+        else launch_tile<D, 3, 4>(a, s);
+    }
+    if (a.splits > 1) {
+        const long long rows = (long long)a.B * a.P * a.H_q;
+        paged_merge_kernel<D><<<(unsigned)((rows * (D / 4) + 255) / 256), 256, 0, s>>>(a);
+    }
 }
 
 }  // namespace
 
-int paged_attn_splits(int, int, int, int, int, int, int, int, int) { return 1; }
+int paged_attn_splits(int B, int P, int H_q, int H_kv, int, int kv_dtype, int max_keys, int window, int asked) {
+    const int G = H_q / H_kv, wr = row_waves(P, G, kv_dtype);
+    const long long walked = window && (long long)window + P < max_keys ? (long long)window + P : max_keys;
+    const int stages = (int)((walked + 127) / 128);
+    int s = asked;
+    if (s <= 0) {
+        const long long groups = (long long)B * H_kv * (((long long)P * G + 32 * wr - 1) / (32 * wr));
+        s = (int)(512 / groups);
+        s = s < 1 ? 1 : s > stages / 2 ? stages / 2 : s;
+        if (s < 1) s = 1;
+    }
+    if (s > IE_PAGED_MAX_SPLITS) s = IE_PAGED_MAX_SPLITS;
+    return s < stages ? s : stages;
+}
 
 void launch_paged_attn(const PagedAttn& a, hipStream_t s) {
-    const bool half = a.kv_dtype == IE_KV_BF16;
-    const unsigned grid = (unsigned)(((long long)a.B * a.P * a.H_q + 3) / 4);
-    auto* k = a.d == 64 ? (half ? paged_row_kernel<64, uint16_t> : paged_row_kernel<64, float>)
-                        : (half ? paged_row_kernel<128, uint16_t> : paged_row_kernel<128, float>);
-    k<<<grid, 256, 0, s>>>(a);
+    if (a.d == 64) launch_d<64>(a, s);
+    else launch_d<128>(a, s);
 }
 
 }  // namespace ie
