@@ -27,11 +27,20 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
-typedef __attribute__((address_space(3))) void* lds_ptr;
-typedef const __attribute__((address_space(1))) void* gbl_ptr;
+typedef __attribute__((address_space(3))) int8_t* lds_i8;
 
+// 16 bytes a lane from global memory straight into LDS, 1 KiB from `to` on (uniform).  Written out because the
+// compiler waits for such copies before any LDS read that follows; here the loop's own wait
+// is where the stage is first read.  (m0 is the compiler's own: it sets it before each use, and has none here.)
+__device__ __forceinline__ void copy16(const int8_t* from, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(to) : "memory");
+}
+
+__device__ __forceinline__ int page_of(const PageMap& m, int p) {
+    return m.mul ? (int)(__umulhi((uint32_t)p, m.mul) >> m.shift) : p;
+}
 __device__ __forceinline__ uint32_t cache_row(const PageMap& m, const int* table, int p) {
-    const int page = m.mul ? (int)(__umulhi((uint32_t)p, m.mul) >> m.shift) : p;
+    const int page = page_of(m, p);
     return (uint32_t)table[page] * (uint32_t)m.block + (uint32_t)(p - page * m.block);
 }
 
@@ -302,7 +311,7 @@ __global__ __launch_bounds__(256, NP == 1 && WR == 4 ? 2 : 1) void paged_tile_ke
     using Tree = std::conditional_t<TREE, TreeLds, NoTree>;
     constexpr int NT = D / 32, KS = D / 16;
     __shared__ __attribute__((aligned(1024))) int8_t lds[T::LDS];
-    __shared__ uint32_t slots[2][T::SK];
+    __shared__ uint32_t slots[2][256];  // a thread's each, SK of them keys of the stage
     __shared__ int bounds[4][4];
     __shared__ Tree tree;
     const int tid = threadIdx.x, lane = tid & 63, i = lane & 31, h = lane >> 5;
@@ -345,20 +354,21 @@ __global__ __launch_bounds__(256, NP == 1 && WR == 4 ? 2 : 1) void paged_tile_ke
     const size_t row_bytes = (size_t)a.H_kv * D * sizeof(KV);
     const int8_t* kbase = reinterpret_cast<const int8_t*>(static_cast<const KV*>(a.k) + (size_t)kvh * D);
     const int8_t* vbase = reinterpret_cast<const int8_t*>(static_cast<const KV*>(a.v) + (size_t)kvh * D);
-    auto find = [&](int s) { return cache_row(a.pages, table, min(kbeg + s * T::SK + tid, k1 - 1)); };
+    auto pos_of = [&](int s) { return min(kbeg + s * T::SK + tid, k1 - 1); };  // of a stage's key tid
 
     // bf16: a stage's rows straight into LDS; a wave's load fills 1 KiB, its lanes' addresses are
     // permuted so that the chunks land swizzled.
     constexpr int RPL = 1024 / T::ROW, LOADS = T::SK / RPL / 4;
+    const uint32_t lds_at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_i8)lds);
     auto copy = [&](int s, int buf) {
         if constexpr (NP == 1) {
 #pragma unroll
             for (int j = 0; j < LOADS; ++j) {
                 const int r0 = (wave + 4 * j) * RPL, r = r0 + lane / T::CH, c = lane % T::CH;
                 const size_t at = slots[s & 1][r] * row_bytes;
-                int8_t* to = lds + buf * T::STAGE + r0 * T::ROW;
-                __builtin_amdgcn_global_load_lds((gbl_ptr)(kbase + at + 16 * (c ^ T::kswz(r))), (lds_ptr)to, 16, 0, 0);
-                __builtin_amdgcn_global_load_lds((gbl_ptr)(vbase + at + 16 * (c ^ T::vswz(r))), (lds_ptr)(to + T::PART), 16, 0, 0);
+                const uint32_t to = lds_at + buf * T::STAGE + r0 * T::ROW;
+                copy16(kbase + at + 16 * (c ^ T::kswz(r)), to);
+                copy16(vbase + at + 16 * (c ^ T::vswz(r)), to + T::PART);
             }
         }
     };
@@ -396,9 +406,9 @@ __global__ __launch_bounds__(256, NP == 1 && WR == 4 ? 2 : 1) void paged_tile_ke
         }
     };
 
-    if (s0 < s1 && tid < T::SK) {
-        slots[s0 & 1][tid] = find(s0);
-        slots[(s0 + 1) & 1][tid] = find(s0 + 1);
+    if (s0 < s1) {
+        slots[s0 & 1][tid] = cache_row(a.pages, table, pos_of(s0));
+        slots[(s0 + 1) & 1][tid] = cache_row(a.pages, table, pos_of(s0 + 1));
     }
     __syncthreads();
     if (s0 < s1) {
@@ -536,15 +546,18 @@ __global__ __launch_bounds__(256, NP == 1 && WR == 4 ? 2 : 1) void paged_tile_ke
             __syncthreads();
             if (s + 1 < s1) load(s + 1);
         }
-        uint32_t next = 0;
-        if (s + 2 < s1 && tid < T::SK) next = find(s + 2);
+        // The page of this thread's key of stage s + 2: asked for here, used behind the products.  By every
+        // thread, and at the end too, where it is k1 - 1's: a register loaded or used under a condition makes
+        // the compiler wait for the copies here.
+        const int p2 = pos_of(s + 2), in2 = page_of(a.pages, p2);
+        const uint32_t page = (uint32_t)table[in2];
         const int8_t* stage = lds + buf * T::STAGE;
 #pragma unroll
         for (int n = 0; n < T::NB; ++n) {
             const int blk = kw * T::NB + n, c0 = kbeg + s * T::SK + 32 * blk;
             if (c0 < w_hi && c0 + 32 > w_lo) attend(stage, blk, c0);
         }
-        if (s + 2 < s1 && tid < T::SK) slots[s & 1][tid] = next;
+        slots[s & 1][tid] = page * (uint32_t)a.pages.block + (uint32_t)(p2 - in2 * a.pages.block);
     }
     l = sum_xor32(l);
 
