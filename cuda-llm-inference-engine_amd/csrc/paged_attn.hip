@@ -83,46 +83,64 @@ __device__ __forceinline__ Parts<3> split8(const float* x) {
 __device__ __forceinline__ f32x16 mfma(uint4 a, uint4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
-// The products of a's N parts and b's three, the small ones first.
-template <int N>
-__device__ __forceinline__ f32x16 product(const Parts<N>& a, const Parts<3>& b, f32x16 c) {
+// c[t] += a[t] b, of a's N parts and b's three, the small products first; an accumulator's own are not back to back.
+template <int N, int NT>
+__device__ __forceinline__ void product(const Parts<N> (&a)[NT], const Parts<3>& b, f32x16 (&c)[NT]) {
+    auto all = [&](int i, int j) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) c[t] = mfma(a[t].p[i], b.p[j], c[t]);
+    };
     if constexpr (N == 3) {
-        c = mfma(a.p[2], b.p[0], c);
-        c = mfma(a.p[0], b.p[2], c);
-        c = mfma(a.p[1], b.p[1], c);
-        c = mfma(a.p[1], b.p[0], c);
+        all(2, 0);
+        all(0, 2);
+        all(1, 1);
+        all(1, 0);
     } else {
-        c = mfma(a.p[0], b.p[2], c);
+        all(0, 2);
     }
-    c = mfma(a.p[0], b.p[1], c);
-    return mfma(a.p[0], b.p[0], c);
+    all(0, 1);
+    all(0, 0);
 }
 
 // ---- scores
-// tanh: below 0.55 x + x^3 p(x^2), p the polynomial nearest to (tanh(x) / x - 1) / x^2 there
-// (weighted least squares, 1.2e-9 of the value off); above it 1 - 2 / (1 + e^2x), whose rounding is that of a value near 1.
-__device__ __forceinline__ float tanh_of(float x) {
-    const float a = fabsf(x), y = x * x;
-    const float e = __builtin_amdgcn_exp2f(2.0f * kLog2e * fminf(a, 20.0f));
-    const float big = __builtin_copysignf(fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + e), 1.0f), x);
-    float p = -0.0062074303f;
-    p = fmaf(p, y, 0.021027219f);
-    p = fmaf(p, y, -0.053842276f);
-    p = fmaf(p, y, 0.133325f);
-    p = fmaf(p, y, -0.33333316f);
-    const float small = fmaf(x * y, p, x);
-    return a < 0.55f ? small : x == x ? big : x;
+// cap * tanh(x), cap with the factor to base 2.  Below 1 x (cap + y P(y)), y = x^2, P the polynomial nearest to
+// cap (tanh(x) / x - 1) / y there (weighted least squares: 4.6e-9 of the value off, with fp32's
+// steps 7e-8): nine instructions, which is all that a block takes whose scores lie there.  Above it 1 - 2 / (1 +
+// e^2x), whose rounding is that of a value near 1.
+struct Cap {
+    float cap, p[7];
+};
+// The same value of every lane, in a scalar register.
+__device__ __forceinline__ float uniform(float x) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
+}
+__device__ __forceinline__ Cap cap_of(float cap) {
+    const float c = cap * kLog2e;
+    return {uniform(c),
+            {uniform(c * -0.33333295583724976f), uniform(c * 0.13332344591617584f), uniform(c * -0.05387980118393898f),
+             uniform(c * 0.021486656740307808f), uniform(c * -0.007946106605231762f), uniform(c * 0.0023013646714389324f),
+             uniform(c * -0.00035845203092321754f)}};
+}
+__device__ __forceinline__ float capped_small(float x, const Cap& c) {
+    const float y = x * x;
+    float p = c.p[6];
+#pragma unroll
+    for (int i = 5; i >= 0; --i) p = fmaf(p, y, c.p[i]);
+    return x * fmaf(p, y, c.cap);
+}
+__device__ __forceinline__ float capped(float x, const Cap& c) {
+    const float e = __builtin_amdgcn_exp2f(2.0f * kLog2e * fabsf(x));
+    const float big = c.cap * __builtin_copysignf(fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + e), 1.0f), x);
+    return fabsf(x) < 1.0f ? capped_small(x, c) : big;
 }
 
-// What turns a product q.k into a score of base 2: the factor folded into q, the
-// cap's factor behind tanh, and the distance's factor.
+// What turns a product q.k into a score of base 2: the factor folded into q, and the distance's factor.
 struct Scores {
-    float q, cap, slope;
+    float q, slope;
 };
 __device__ __forceinline__ Scores scores_of(const PagedAttn& a, int head) {
     Scores s;
     s.q = a.cap > 0.0f ? a.scale / a.cap : a.scale * kLog2e;
-    s.cap = a.cap * kLog2e;
     s.slope = a.slopes ? a.slopes[head] * kLog2e : 0.0f;
     return s;
 }
@@ -241,7 +259,8 @@ __device__ __forceinline__ void exact_row(const PagedAttn& a, const Tree& tree, 
     const size_t stride = (size_t)a.H_kv * D;
     const KV *K = static_cast<const KV*>(a.k) + (size_t)kvh * D, *V = static_cast<const KV*>(a.v) + (size_t)kvh * D;
     const float* q = a.Q + (((size_t)b * a.P + r.t) * a.H_q + r.head) * D;
-    const float slope = a.slopes ? a.slopes[r.head] : 0.0f;
+    const float slope = a.slopes ? a.slopes[r.head] * kLog2e : 0.0f;
+    const Cap cap = cap_of(a.cap);
     m = -INFINITY;
     l = 0.0f;
     for (int i = 0; i < N; ++i) o[i] = 0.0f;
@@ -261,11 +280,10 @@ __device__ __forceinline__ void exact_row(const PagedAttn& a, const Tree& tree, 
             for (int e = 0; e < D; e += 4)
                 for (int i = 0; i < 4; ++i) acc[i] = fmaf(q[e + i], as_float(k[e + i]), acc[i]);
             s = a.scale * ((acc[0] + acc[1]) + (acc[2] + acc[3]));
-            if (a.cap > 0.0f) s = a.cap * tanh_of(s / a.cap);
+            s = a.cap > 0.0f ? capped(s / a.cap, cap) : s * kLog2e;
             int at = j;
             if constexpr (TREE) at = j < ctx ? j : ctx + tree.depth[j - ctx];
             if (a.slopes) s = fmaf(-slope, fabsf((float)(r.pos - at)), s);
-            s *= kLog2e;
         }
         const float mn = fmaxf(m, wave_max(s)), mu = mn == -INFINITY ? 0.0f : mn;
         const float alpha = exp2_sm(m - mu), p = seen ? exp2_sm(s - mu) : 0.0f;
@@ -419,6 +437,7 @@ __global__ __launch_bounds__(256, NP == 1 && WR == 4 ? 2 : 1) void paged_tile_ke
     // The query rows in parts, and whether one of a row's values has none that serve: a value
     // below 2^-98 once scaled, whose parts bf16 may not hold, or one from 2^64 on.
     const Scores sc = scores_of(a, row.head);
+    const Cap cap = cap_of(a.cap);
     const float* qrow = a.Q + (((size_t)b * a.P + row.t) * a.H_q + row.head) * D;
     Parts<3> q[KS];
     bool q_bad = false;
@@ -460,17 +479,26 @@ __global__ __launch_bounds__(256, NP == 1 && WR == 4 ? 2 : 1) void paged_tile_ke
     auto attend = [&](const int8_t* stage, int blk, int c0) {
         const int8_t* kp = stage + blk * 32 * T::ROW;
         const int8_t* vp = stage + NP * T::PART + blk * 32 * T::ROW;
-        f32x16 s{};
+        f32x16 sa[1] = {};
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
-            Parts<NP> x;
+            Parts<NP> x[1];
 #pragma unroll
-            for (int n = 0; n < NP; ++n) x.p[n] = *reinterpret_cast<const uint4*>(kp + n * T::PART + krow + (kx ^ (32 * k)));
-            s = product<NP>(x, q[k], s);
+            for (int n = 0; n < NP; ++n) x[0].p[n] = *reinterpret_cast<const uint4*>(kp + n * T::PART + krow + (kx ^ (32 * k)));
+            product<NP, 1>(x, q[k], sa);
         }
+        f32x16& s = sa[0];
         if (a.cap > 0.0f) {
+            float most = 0.0f;
 #pragma unroll
-            for (int v = 0; v < 16; ++v) s[v] = sc.cap * tanh_of(s[v]);
+            for (int v = 0; v < 16; ++v) most = fmaxf(most, fabsf(s[v]));
+            if (__ballot(!(most < 1.0f))) {
+#pragma unroll
+                for (int v = 0; v < 16; ++v) s[v] = capped(s[v], cap);
+            } else {
+#pragma unroll
+                for (int v = 0; v < 16; ++v) s[v] = capped_small(s[v], cap);
+            }
         }
         const bool edge = c0 < all_lo || c0 + 32 > all_hi;
         if (a.slopes) {
@@ -498,37 +526,40 @@ __global__ __launch_bounds__(256, NP == 1 && WR == 4 ? 2 : 1) void paged_tile_ke
         float top = s[0];
 #pragma unroll
         for (int v = 1; v < 16; ++v) top = fmaxf(top, s[v]);
-        const float mn = fmaxf(m, max_xor32(top));
-        const float mu = mn == -INFINITY ? 0.0f : mn;  // no key yet: keep o, l at 0
-        const float alpha = exp2_sm(m - mu);
-        m = mn;
+        // The weights' unit m follows the largest score once that is 2^8 above it: up to there they only grow, and
+        // fp32 holds them as well.  (With 32 rows a wave some row's largest grows in most blocks.)
+        top = max_xor32(top);
+        if (__ballot(top > m + 8.0f)) {
+            const float mn = fmaxf(m, top);
+            const float alpha = mn == -INFINITY ? 0.0f : exp2_sm(m - mn);
+            m = mn;
+            l *= alpha;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) o[t] *= alpha;
+        }
+        const float mu = m == -INFINITY ? 0.0f : m;  // no key yet: keep o, l at 0
         float p[16], sum = 0.0f;
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
             p[v] = exp2_sm(s[v] - mu);
             sum += p[v];
         }
-        l = fmaf(l, alpha, sum);  // (a lane's own 16 keys; the halves are added at the end)
-        if (__ballot(alpha != 1.0f)) {
-#pragma unroll
-            for (int t = 0; t < NT; ++t) o[t] *= alpha;
-        }
+        l += sum;  // (a lane's own 16 keys; the halves are added at the end)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             const Parts<3> w = split8(p + 8 * k);
+            Parts<NP> x[NT];
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                Parts<NP> x;
+            for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int n = 0; n < NP; ++n) {
                     const int8_t* at = vp + n * T::PART + vrow + 16 * k * T::ROW + 16 * ((4 * t + vc) ^ T::vswz(vkey)) + vsub;
                     const s16x4 u0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)at);
                     const s16x4 u1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + 8 * T::ROW));
                     const uint2 y0 = __builtin_bit_cast(uint2, u0), y1 = __builtin_bit_cast(uint2, u1);
-                    x.p[n] = make_uint4(y0.x, y0.y, y1.x, y1.y);
+                    x[t].p[n] = make_uint4(y0.x, y0.y, y1.x, y1.y);
                 }
-                o[t] = product<NP>(x, w, o[t]);
-            }
+            product<NP, NT>(x, w, o);
         }
     };
 
