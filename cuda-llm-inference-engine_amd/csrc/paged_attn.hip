@@ -51,8 +51,8 @@ __device__ __forceinline__ float as_float(KV x) {
 }
 
 // The largest and smallest of non-negative ints over the wave.
-__device__ __forceinline__ int wave_imax(int v) { return (int)wave_umax((uint32_t)v); }
-__device__ __forceinline__ int wave_imin(int v) { return (int)~wave_umax(~(uint32_t)v); }
+__device__ __forceinline__ int wave_imax(int v) { return __builtin_amdgcn_readfirstlane((int)wave_umax((uint32_t)v)); }
+__device__ __forceinline__ int wave_imin(int v) { return __builtin_amdgcn_readfirstlane((int)~wave_umax(~(uint32_t)v)); }
 
 // ---- operands in three parts
 __device__ __forceinline__ uint32_t round_pair(float x0, float x1) {
@@ -203,6 +203,13 @@ struct Row {
     bool live;
 };
 
+// Row r of a (sequence, KV head): its query.
+template <int D>
+__device__ __forceinline__ const float* query_row(const PagedAttn& a, int r, int b, int kvh) {
+    const int G = a.H_q / a.H_kv, rc = min(r, a.P * G - 1), t = rc / G;
+    return a.Q + (((size_t)b * a.P + t) * a.H_q + kvh * G + (rc - t * G)) * D;
+}
+
 template <bool TREE, typename Tree>
 __device__ __forceinline__ Row row_of(const PagedAttn& a, const Tree& tree, int r, int b, int kvh, int start, int len) {
     const int G = a.H_q / a.H_kv;
@@ -300,6 +307,259 @@ __device__ __forceinline__ void exact_row(const PagedAttn& a, const Tree& tree, 
     }
 }
 
+// ---- what a wave keeps of its 32 rows
+template <int D>
+struct State {
+    float m, l;         // the weights' unit, and a lane's own keys' sum of them
+    f32x16 o[D / 32];   // o[t][v]: channel 32 t + 8 (v / 4) + 4 h + v % 4
+    __device__ __forceinline__ void clear() {
+        m = -INFINITY;
+        l = 0.0f;
+#pragma unroll
+        for (int t = 0; t < D / 32; ++t) o[t] = f32x16{};
+    }
+    __device__ __forceinline__ void scale(float f) {
+        l *= f;
+#pragma unroll
+        for (int t = 0; t < D / 32; ++t) o[t] *= f;
+    }
+};
+
+// What a wave's rows have in common: keys below all_lo or from all_hi on are not seen by all of them.
+struct Limits {
+    int lo, hi, all_lo, all_hi;
+};
+template <bool TREE>
+__device__ __forceinline__ Limits limits_of(const Row& row, int ctx) {
+    const bool some = row.live && row.lo < row.hi;
+    Limits x;
+    x.lo = wave_imin(some ? row.lo : 0x7fffffff);
+    x.hi = wave_imax(some ? row.hi : 0);
+    x.all_lo = wave_imax(row.live ? row.lo : 0);
+    x.all_hi = wave_imin(row.live ? (TREE ? min(row.hi, ctx) : row.hi) : 0x7fffffff);
+    return x;
+}
+
+// The products s of a block's keys from c0 on to weights p; st.o scaled where their unit moves.
+template <int D, bool TREE, typename Tree>
+__device__ __forceinline__ void weigh(const PagedAttn& a, const Tree& tree, const Row& row, const Limits& lim, const Scores& sc,
+                                      const Cap& cap, int c0, int ctx, f32x16& s, State<D>& st, float (&p)[16]) {
+    const int h = (threadIdx.x >> 5) & 1;
+    if (a.cap > 0.0f) {
+        float most = 0.0f;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) most = fmaxf(most, fabsf(s[v]));
+        if (__ballot(!(most < 1.0f))) {
+#pragma unroll
+            for (int v = 0; v < 16; ++v) s[v] = capped(s[v], cap);
+        } else {
+#pragma unroll
+            for (int v = 0; v < 16; ++v) s[v] = capped_small(s[v], cap);
+        }
+    }
+    if (a.slopes) {
+        if (TREE && c0 + 32 > ctx) {
+            if constexpr (TREE) {
+#pragma unroll
+                for (int v = 0; v < 16; ++v) {
+                    const int j = c0 + 8 * (v >> 2) + 4 * h + (v & 3);
+                    const int at = j < ctx ? j : ctx + tree.depth[min(j - ctx, IE_TREE_MAX - 1)];
+                    s[v] = fmaf(-sc.slope, fabsf((float)(row.pos - at)), s[v]);
+                }
+            }
+        } else {
+            const int base = row.pos - c0 - 4 * h;
+#pragma unroll
+            for (int v = 0; v < 16; ++v) s[v] = fmaf(-sc.slope, fabsf((float)(base - 8 * (v >> 2) - (v & 3))), s[v]);
+        }
+    }
+    if (c0 < lim.all_lo || c0 + 32 > lim.all_hi) {
+        const uint32_t bits = seen_bits<TREE>(tree, row, c0, ctx) >> (4 * h);
+#pragma unroll
+        for (int v = 0; v < 16; ++v)
+            if (!(bits >> (8 * (v >> 2) + (v & 3)) & 1)) s[v] = -INFINITY;
+    }
+    float top = s[0];
+#pragma unroll
+    for (int v = 1; v < 16; ++v) top = fmaxf(top, s[v]);
+    // The weights' unit m follows the largest score once that is 2^8 above it: up to there they only grow, and
+    // fp32 holds them as well.  (With 32 rows a wave some row's largest grows in most blocks.)
+    top = max_xor32(top);
+    if (__ballot(top > st.m + 8.0f)) {
+        const float mn = fmaxf(st.m, top);
+        const float alpha = mn == -INFINITY ? 0.0f : exp2_sm(st.m - mn);
+        st.m = mn;
+        st.scale(alpha);
+    }
+    const float mu = st.m == -INFINITY ? 0.0f : st.m;  // no key yet: keep o, l at 0
+    float sum = 0.0f;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+        p[v] = exp2_sm(s[v] - mu);
+        sum += p[v];
+    }
+    st.l += sum;
+}
+
+// A lane's share of its row of Q: channels 16 s + 8 h on.
+template <int D>
+struct RawQuery {
+    float4 x[D / 16][2];
+};
+template <int D>
+__device__ __forceinline__ RawQuery<D> load_query(const float* row, int h) {
+    RawQuery<D> r;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) r.x[s][k] = *reinterpret_cast<const float4*>(row + 16 * s + 8 * h + 4 * k);
+    return r;
+}
+// Its parts, and whether one of the values has none that serve: one below 2^-98 once scaled, whose parts bf16 may
+// not hold, or one from 2^64 on.
+template <int D>
+__device__ __forceinline__ bool split_query(const float* row, const RawQuery<D>& r, float scale, Parts<3> (&q)[D / 16]) {
+    float least = INFINITY, most = 0.0f;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) {
+        float z[8] = {r.x[s][0].x, r.x[s][0].y, r.x[s][0].z, r.x[s][0].w, r.x[s][1].x, r.x[s][1].y, r.x[s][1].z, r.x[s][1].w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            z[e] *= scale;
+            least = fminf(least, fabsf(z[e]));
+            most = fmaxf(most, fabsf(z[e]));
+        }
+        q[s] = split8(z);
+    }
+    bool bad = false;
+    if (__ballot(!(least >= 0x1p-98f && most < 0x1p64f))) {  // (seldom; zeros among them)
+#pragma unroll 1
+        for (int e = 0; e < D; ++e) {
+            const float x = row[e], y = fabsf(x * scale);
+            bad |= x != 0.0f && !(y >= 0x1p-98f && y < 0x1p64f);
+        }
+    }
+    return bad;
+}
+
+// Results of a wave's rows: outputs, or with splits partial sums.  Rows whose result is not finite, or whose query
+// has no parts, again one by one over keys k0 .. k1 - 1.
+template <int D, typename KV, bool TREE, typename Tree>
+__device__ __forceinline__ void finish(const PagedAttn& a, const Tree& tree, const Row& row, int b, int kvh, int ctx, int split,
+                                       int k0, int k1, bool q_bad, const State<D>& st, float l) {
+    constexpr int NT = D / 32;
+    const int lane = threadIdx.x & 63, i = lane & 31, h = lane >> 5;
+    float bad = l * 0.0f;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) bad = fmaf(st.o[t][v], 0.0f, bad);
+    const uint64_t lanes = __ballot(row.live && (q_bad || !(bad == 0.0f)));
+    uint32_t again = (uint32_t)lanes | (uint32_t)(lanes >> 32);
+    const size_t rows = (size_t)a.B * a.P * a.H_q, mine = ((size_t)b * a.P + row.t) * a.H_q + row.head;
+    if (row.live && !(again >> i & 1)) {
+        float* out;
+        float inv = 1.0f;
+        if (a.splits == 1) {
+            inv = l > 0.0f ? 1.0f / l : 0.0f;
+            out = a.O + mine * D;
+        } else {
+            out = a.ws + (split * rows + mine) * D;
+            if (h == 0) *reinterpret_cast<float2*>(a.ws + a.splits * rows * D + 2 * (split * rows + mine)) = make_float2(st.m, l);
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int v = 0; v < 4; ++v)
+                *reinterpret_cast<float4*>(out + 32 * t + 8 * v + 4 * h) =
+                    make_float4(st.o[t][4 * v] * inv, st.o[t][4 * v + 1] * inv, st.o[t][4 * v + 2] * inv, st.o[t][4 * v + 3] * inv);
+    }
+#pragma unroll 1
+    for (; again; again &= again - 1) {
+        const int x = __builtin_ctz(again);
+        Row r;
+        r.t = __shfl(row.t, x);
+        r.head = __shfl(row.head, x);
+        r.lo = __shfl(row.lo, x);
+        r.hi = __shfl(row.hi, x);
+        r.pos = __shfl(row.pos, x);
+        r.live = true;
+        float rm, rl, ro[D / 64];
+        exact_row<D, KV, TREE>(a, tree, r, b, kvh, ctx, k0, k1, rm, rl, ro);
+        const size_t at = ((size_t)b * a.P + r.t) * a.H_q + r.head;
+        float* out = a.O + at * D;
+        float inv = 1.0f;
+        if (a.splits == 1) {
+            inv = rl == 0.0f ? 0.0f : 1.0f / rl;
+        } else {
+            out = a.ws + (split * rows + at) * D;
+            if (lane == 0) *reinterpret_cast<float2*>(a.ws + a.splits * rows * D + 2 * (split * rows + at)) = make_float2(rm, rl);
+        }
+        for (int e = 0; e < D / 64; ++e) out[lane * (D / 64) + e] = ro[e] * inv;
+    }
+}
+
+// Key groups' states through LDS into the first group's wave; `slot` numbers the others' and mine. Groups' waves
+// with rows in common call this together; false: the wave is done.
+template <int D, int OTHERS>
+__device__ __forceinline__ bool gather(int8_t* lds, int group, int per, int which, State<D>& st, float& l) {
+    constexpr int NT = D / 32;
+    const int lane = threadIdx.x & 63;
+    float4* mo = reinterpret_cast<float4*>(lds);
+    float2* ml = reinterpret_cast<float2*>(lds + OTHERS * per * 64 * (D / 2) * 4);
+    if (group > 0) {
+        const int g = (group - 1) * per + which;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int v = 0; v < 4; ++v)
+                mo[(g * NT * 4 + t * 4 + v) * 64 + lane] =
+                    make_float4(st.o[t][4 * v], st.o[t][4 * v + 1], st.o[t][4 * v + 2], st.o[t][4 * v + 3]);
+        ml[g * 64 + lane] = make_float2(st.m, l);
+    }
+    __syncthreads();
+    if (group > 0) return false;
+#pragma unroll 1
+    for (int k = 0; k < OTHERS; ++k) {
+        const int g = k * per + which;
+        const float2 x = ml[g * 64 + lane];
+        const float mn = fmaxf(st.m, x.x), mu = mn == -INFINITY ? 0.0f : mn;
+        const float fa = exp2_sm(st.m - mu), fb = exp2_sm(x.x - mu);
+        st.m = mn;
+        l = l * fa + x.y * fb;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                const float4 y = mo[(g * NT * 4 + t * 4 + v) * 64 + lane];
+                st.o[t][4 * v] = st.o[t][4 * v] * fa + y.x * fb;
+                st.o[t][4 * v + 1] = st.o[t][4 * v + 1] * fa + y.y * fb;
+                st.o[t][4 * v + 2] = st.o[t][4 * v + 2] * fa + y.z * fb;
+                st.o[t][4 * v + 3] = st.o[t][4 * v + 3] * fa + y.w * fb;
+            }
+    }
+    return true;
+}
+
+// Which of the grid's workgroups this is: pair (sequence, KV head) u % pairs, so that a pair's tiles run on one
+// XCD where pairs are a multiple of 8; then the tile, the last (a prompt's longest) first, then the split.
+struct Place {
+    int b, kvh, tile, split, start, len;
+};
+template <bool TREE>
+__device__ __forceinline__ Place place_of(const PagedAttn& a, int tiles) {
+    const int pairs = a.B * a.H_kv;
+    const int u = blockIdx.x / pairs, pair = blockIdx.x - u * pairs;
+    Place p;
+    p.split = u / tiles;
+    p.tile = tiles - 1 - (u - p.split * tiles);
+    p.b = pair / a.H_kv;
+    p.kvh = pair - p.b * a.H_kv;
+    p.start = min(max(a.starts[p.b], 0), TREE ? a.max_ctx : 1 << 30);
+    p.len = a.lens ? min(a.lens[p.b], a.P) : a.P;
+    return p;
+}
+
 // ---- the tile kernel
 // A workgroup of four waves: WR of them take 32 rows each, 4 / WR groups of them
 // different keys.  A stage holds SK keys' K and V in LDS, NB blocks of 32 for each
@@ -330,30 +590,22 @@ __global__ __launch_bounds__(256, NP == 1 && WR == 4 ? 2 : 1) void paged_tile_ke
     constexpr int NT = D / 32, KS = D / 16;
     __shared__ __attribute__((aligned(1024))) int8_t lds[T::LDS];
     __shared__ uint32_t slots[2][256];  // a thread's each, SK of them keys of the stage
-    __shared__ int bounds[4][4];
+    __shared__ int bounds[4][2];
     __shared__ Tree tree;
     const int tid = threadIdx.x, lane = tid & 63, i = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), rw = wave % WR, kw = wave / WR;
-    // workgroup u: pair (sequence, KV head) u % pairs, so that a pair's tiles run on one XCD where pairs
-    // are a multiple of 8; then the tile, the last (a prompt's longest) first, then the split
-    const int pairs = a.B * a.H_kv;
-    const int u = blockIdx.x / pairs, pair = blockIdx.x - u * pairs;
-    const int split = u / tiles, tile = tiles - 1 - (u - split * tiles);
-    const int b = pair / a.H_kv, kvh = pair - b * a.H_kv;
-    const int start = TREE ? min(max(a.starts[b], 0), a.max_ctx) : min(max(a.starts[b], 0), 1 << 30);
-    const int len = a.lens ? min(a.lens[b], a.P) : a.P;
+    const Place at = place_of<TREE>(a, tiles);
+    const int b = at.b, kvh = at.kvh, ctx = at.start;
+    const int r = at.tile * 32 * WR + rw * 32 + i;
+    // the query first: it waits for nothing
+    const float* q_row = query_row<D>(a, r, b, kvh);
+    const RawQuery<D> raw_q = load_query<D>(q_row, h);
     if constexpr (TREE) grow_tree(tree, a.parents + (size_t)b * a.P, a.P, a.window);
-    const Row row = row_of<TREE>(a, tree, tile * 32 * WR + rw * 32 + i, b, kvh, start, len);
-    const int ctx = start;
-
-    // Keys that some row of the tile sees, and, of this wave's rows, between which every row sees all.
-    const bool some = row.live && row.lo < row.hi;
-    const int w_lo = wave_imin(some ? row.lo : 0x7fffffff), w_hi = wave_imax(some ? row.hi : 0);
-    const int all_lo = wave_imax(row.live ? row.lo : 0);
-    const int all_hi = wave_imin(row.live ? (TREE ? min(row.hi, ctx) : row.hi) : 0x7fffffff);
+    const Row row = row_of<TREE>(a, tree, r, b, kvh, at.start, at.len);
+    const Limits lim = limits_of<TREE>(row, ctx);
     if (lane == 0) {
-        bounds[wave][0] = w_lo;
-        bounds[wave][1] = w_hi;
+        bounds[wave][0] = lim.lo;
+        bounds[wave][1] = lim.hi;
     }
     __syncthreads();
     int kbeg = 0x7fffffff, kend = 0;
@@ -365,7 +617,7 @@ __global__ __launch_bounds__(256, NP == 1 && WR == 4 ? 2 : 1) void paged_tile_ke
     if (kbeg > kend) kbeg = kend;
     // this split's stages
     const int all = (kend - kbeg + T::SK - 1) / T::SK, per = (all + a.splits - 1) / a.splits;
-    const int s0 = min(split * per, all), s1 = min(s0 + per, all);
+    const int s0 = min(at.split * per, all), s1 = min(s0 + per, all);
     const int k0 = kbeg + s0 * T::SK, k1 = min(kbeg + s1 * T::SK, kend);
 
     const int* table = a.pages.table + (size_t)b * a.pages.nbps;
@@ -373,7 +625,6 @@ __global__ __launch_bounds__(256, NP == 1 && WR == 4 ? 2 : 1) void paged_tile_ke
     const int8_t* kbase = reinterpret_cast<const int8_t*>(static_cast<const KV*>(a.k) + (size_t)kvh * D);
     const int8_t* vbase = reinterpret_cast<const int8_t*>(static_cast<const KV*>(a.v) + (size_t)kvh * D);
     auto pos_of = [&](int s) { return min(kbeg + s * T::SK + tid, k1 - 1); };  // of a stage's key tid
-
     // bf16: a stage's rows straight into LDS; a wave's load fills 1 KiB, its lanes' addresses are
     // permuted so that the chunks land swizzled.
     constexpr int RPL = 1024 / T::ROW, LOADS = T::SK / RPL / 4;
@@ -434,41 +685,12 @@ __global__ __launch_bounds__(256, NP == 1 && WR == 4 ? 2 : 1) void paged_tile_ke
         else load(s0);
     }
 
-    // The query rows in parts, and whether one of a row's values has none that serve: a value
-    // below 2^-98 once scaled, whose parts bf16 may not hold, or one from 2^64 on.
     const Scores sc = scores_of(a, row.head);
     const Cap cap = cap_of(a.cap);
-    const float* qrow = a.Q + (((size_t)b * a.P + row.t) * a.H_q + row.head) * D;
     Parts<3> q[KS];
-    bool q_bad = false;
-    {
-        float least = INFINITY, most = 0.0f;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            const float4 x = *reinterpret_cast<const float4*>(qrow + 16 * s + 8 * h);
-            const float4 y = *reinterpret_cast<const float4*>(qrow + 16 * s + 8 * h + 4);
-            float z[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                z[e] *= sc.q;
-                least = fminf(least, fabsf(z[e]));
-                most = fmaxf(most, fabsf(z[e]));
-            }
-            q[s] = split8(z);
-        }
-        if (__ballot(!(least >= 0x1p-98f && most < 0x1p64f))) {  // (seldom; zeros among them)
-#pragma unroll 1
-            for (int e = 0; e < D; ++e) {
-                const float x = qrow[e], y = fabsf(x * sc.q);
-                q_bad |= x != 0.0f && !(y >= 0x1p-98f && y < 0x1p64f);
-            }
-        }
-    }
-
-    float m = -INFINITY, l = 0.0f;
-    f32x16 o[NT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) o[t] = f32x16{};
+    const bool q_bad = split_query<D>(q_row, raw_q, sc.q, q);
+    State<D> st;
+    st.clear();
 
     // LDS places of a lane's operands: chunk 2 s + h of key i; of V, 8 bytes of keys 4 h + (lane % 16) / 4
     // on at channels 16 (lane / 16 % 2) + 4 (lane % 4) of tile t.
@@ -479,6 +701,7 @@ __global__ __launch_bounds__(256, NP == 1 && WR == 4 ? 2 : 1) void paged_tile_ke
     auto attend = [&](const int8_t* stage, int blk, int c0) {
         const int8_t* kp = stage + blk * 32 * T::ROW;
         const int8_t* vp = stage + NP * T::PART + blk * 32 * T::ROW;
+        __builtin_amdgcn_s_setprio(0);
         f32x16 sa[1] = {};
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
@@ -488,63 +711,10 @@ __global__ __launch_bounds__(256, NP == 1 && WR == 4 ? 2 : 1) void paged_tile_ke
             product<NP, 1>(x, q[k], sa);
         }
         f32x16& s = sa[0];
-        if (a.cap > 0.0f) {
-            float most = 0.0f;
-#pragma unroll
-            for (int v = 0; v < 16; ++v) most = fmaxf(most, fabsf(s[v]));
-            if (__ballot(!(most < 1.0f))) {
-#pragma unroll
-                for (int v = 0; v < 16; ++v) s[v] = capped(s[v], cap);
-            } else {
-#pragma unroll
-                for (int v = 0; v < 16; ++v) s[v] = capped_small(s[v], cap);
-            }
-        }
-        const bool edge = c0 < all_lo || c0 + 32 > all_hi;
-        if (a.slopes) {
-            if (TREE && c0 + 32 > ctx) {
-                if constexpr (TREE) {
-#pragma unroll
-                    for (int v = 0; v < 16; ++v) {
-                        const int j = c0 + 8 * (v >> 2) + 4 * h + (v & 3);
-                        const int at = j < ctx ? j : ctx + tree.depth[min(j - ctx, IE_TREE_MAX - 1)];
-                        s[v] = fmaf(-sc.slope, fabsf((float)(row.pos - at)), s[v]);
-                    }
-                }
-            } else {
-                const int base = row.pos - c0 - 4 * h;
-#pragma unroll
-                for (int v = 0; v < 16; ++v) s[v] = fmaf(-sc.slope, fabsf((float)(base - 8 * (v >> 2) - (v & 3))), s[v]);
-            }
-        }
-        if (edge) {
-            const uint32_t bits = seen_bits<TREE>(tree, row, c0, ctx) >> (4 * h);
-#pragma unroll
-            for (int v = 0; v < 16; ++v)
-                if (!(bits >> (8 * (v >> 2) + (v & 3)) & 1)) s[v] = -INFINITY;
-        }
-        float top = s[0];
-#pragma unroll
-        for (int v = 1; v < 16; ++v) top = fmaxf(top, s[v]);
-        // The weights' unit m follows the largest score once that is 2^8 above it: up to there they only grow, and
-        // fp32 holds them as well.  (With 32 rows a wave some row's largest grows in most blocks.)
-        top = max_xor32(top);
-        if (__ballot(top > m + 8.0f)) {
-            const float mn = fmaxf(m, top);
-            const float alpha = mn == -INFINITY ? 0.0f : exp2_sm(m - mn);
-            m = mn;
-            l *= alpha;
-#pragma unroll
-            for (int t = 0; t < NT; ++t) o[t] *= alpha;
-        }
-        const float mu = m == -INFINITY ? 0.0f : m;  // no key yet: keep o, l at 0
-        float p[16], sum = 0.0f;
-#pragma unroll
-        for (int v = 0; v < 16; ++v) {
-            p[v] = exp2_sm(s[v] - mu);
-            sum += p[v];
-        }
-        l += sum;  // (a lane's own 16 keys; the halves are added at the end)
+        __builtin_amdgcn_s_setprio(1);
+        float p[16];
+        weigh<D, TREE>(a, tree, row, lim, sc, cap, c0, ctx, s, st, p);
+        __builtin_amdgcn_s_setprio(2);
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             const Parts<3> w = split8(p + 8 * k);
@@ -559,8 +729,9 @@ __global__ __launch_bounds__(256, NP == 1 && WR == 4 ? 2 : 1) void paged_tile_ke
                     const uint2 y0 = __builtin_bit_cast(uint2, u0), y1 = __builtin_bit_cast(uint2, u1);
                     x[t].p[n] = make_uint4(y0.x, y0.y, y1.x, y1.y);
                 }
-            product<NP, NT>(x, w, o);
+            product<NP, NT>(x, w, st.o);
         }
+        __builtin_amdgcn_s_setprio(0);
     };
 
 #pragma unroll 1
@@ -583,101 +754,19 @@ __global__ __launch_bounds__(256, NP == 1 && WR == 4 ? 2 : 1) void paged_tile_ke
         const int p2 = pos_of(s + 2), in2 = page_of(a.pages, p2);
         const uint32_t page = (uint32_t)table[in2];
         const int8_t* stage = lds + buf * T::STAGE;
-#pragma unroll
+#pragma unroll 1
         for (int n = 0; n < T::NB; ++n) {
             const int blk = kw * T::NB + n, c0 = kbeg + s * T::SK + 32 * blk;
-            if (c0 < w_hi && c0 + 32 > w_lo) attend(stage, blk, c0);
+            if (c0 < lim.hi && c0 + 32 > lim.lo) attend(stage, blk, c0);
         }
         slots[s & 1][tid] = page * (uint32_t)a.pages.block + (uint32_t)(p2 - in2 * a.pages.block);
     }
-    l = sum_xor32(l);
-
-    // The key groups' states into the first one's.
+    float l = sum_xor32(st.l);
     if constexpr (T::WK > 1) {
         __syncthreads();
-        float4* mo = reinterpret_cast<float4*>(lds);
-        float2* ml = reinterpret_cast<float2*>(lds + (T::WK - 1) * WR * 64 * (D / 2) * 4);
-        if (kw > 0) {
-            const int g = (kw - 1) * WR + rw;
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int v = 0; v < 4; ++v)
-                    mo[(g * NT * 4 + t * 4 + v) * 64 + lane] = make_float4(o[t][4 * v], o[t][4 * v + 1], o[t][4 * v + 2], o[t][4 * v + 3]);
-            ml[g * 64 + lane] = make_float2(m, l);
-        }
-        __syncthreads();
-        if (kw > 0) return;
-#pragma unroll 1
-        for (int k = 1; k < T::WK; ++k) {
-            const int g = (k - 1) * WR + rw;
-            const float2 x = ml[g * 64 + lane];
-            const float mn = fmaxf(m, x.x), mu = mn == -INFINITY ? 0.0f : mn;
-            const float fa = exp2_sm(m - mu), fb = exp2_sm(x.x - mu);
-            m = mn;
-            l = l * fa + x.y * fb;
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int v = 0; v < 4; ++v) {
-                    const float4 y = mo[(g * NT * 4 + t * 4 + v) * 64 + lane];
-                    o[t][4 * v] = o[t][4 * v] * fa + y.x * fb;
-                    o[t][4 * v + 1] = o[t][4 * v + 1] * fa + y.y * fb;
-                    o[t][4 * v + 2] = o[t][4 * v + 2] * fa + y.z * fb;
-                    o[t][4 * v + 3] = o[t][4 * v + 3] * fa + y.w * fb;
-                }
-        }
+        if (!gather<D, T::WK - 1>(lds, kw, WR, rw, st, l)) return;
     }
-
-    // Rows whose result is not finite, or whose query has no parts, again one by one.
-    float bad = l * 0.0f;
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) bad = fmaf(o[t][v], 0.0f, bad);
-    const uint64_t lanes = __ballot(row.live && (q_bad || !(bad == 0.0f)));
-    uint32_t again = (uint32_t)lanes | (uint32_t)(lanes >> 32);
-    const size_t rows = (size_t)a.B * a.P * a.H_q, mine = ((size_t)b * a.P + row.t) * a.H_q + row.head;
-    if (row.live && !(again >> i & 1)) {
-        float* out;
-        float inv = 1.0f;
-        if (a.splits == 1) {
-            inv = l > 0.0f ? 1.0f / l : 0.0f;
-            out = a.O + mine * D;
-        } else {
-            out = a.ws + (split * rows + mine) * D;
-            if (h == 0) *reinterpret_cast<float2*>(a.ws + a.splits * rows * D + 2 * (split * rows + mine)) = make_float2(m, l);
-        }
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int v = 0; v < 4; ++v)
-                *reinterpret_cast<float4*>(out + 32 * t + 8 * v + 4 * h) =
-                    make_float4(o[t][4 * v] * inv, o[t][4 * v + 1] * inv, o[t][4 * v + 2] * inv, o[t][4 * v + 3] * inv);
-    }
-#pragma unroll 1
-    for (; again; again &= again - 1) {
-        const int x = __builtin_ctz(again);
-        Row r;
-        r.t = __shfl(row.t, x);
-        r.head = __shfl(row.head, x);
-        r.lo = __shfl(row.lo, x);
-        r.hi = __shfl(row.hi, x);
-        r.pos = __shfl(row.pos, x);
-        r.live = true;
-        float rm, rl, ro[D / 64];
-        exact_row<D, KV, TREE>(a, tree, r, b, kvh, ctx, k0, k1, rm, rl, ro);
-        const size_t at = ((size_t)b * a.P + r.t) * a.H_q + r.head;
-        float* out = a.O + at * D;
-        float inv = 1.0f;
-        if (a.splits == 1) {
-            inv = rl == 0.0f ? 0.0f : 1.0f / rl;
-        } else {
-            out = a.ws + (split * rows + at) * D;
-            if (lane == 0) *reinterpret_cast<float2*>(a.ws + a.splits * rows * D + 2 * (split * rows + at)) = make_float2(rm, rl);
-        }
-        for (int e = 0; e < D / 64; ++e) out[lane * (D / 64) + e] = ro[e] * inv;
-    }
+    finish<D, KV, TREE>(a, tree, row, b, kvh, ctx, at.split, k0, k1, q_bad, st, l);
 }
 
 // O rows from their splits' partials, D / 4 lanes a row.
