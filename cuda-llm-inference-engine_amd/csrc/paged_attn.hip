@@ -85,7 +85,7 @@ __device__ __forceinline__ f32x16 mfma(uint4 a, uint4 b, f32x16 c) {
 }
 // c[t] += a[t] b, of a's N parts and b's three, the small products first; an accumulator's own are not back to back.
 template <int N, int NT>
-__device__ __forceinline__ void product(const Parts<N> (&a)[NT], const Parts<3>& b, f32x16 (&c)[NT]) {
+__device__ __forceinline__ void product(const Parts<N> (&a)[NT], const Parts<3>& b, f32x16* c) {
     auto all = [&](int i, int j) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) c[t] = mfma(a[t].p[i], b.p[j], c[t]);
@@ -629,15 +629,17 @@ __global__ __launch_bounds__(256, NP == 1 && WR == 4 ? 2 : 1) void paged_tile_ke
     // permuted so that the chunks land swizzled.
     constexpr int RPL = 1024 / T::ROW, LOADS = T::SK / RPL / 4;
     const uint32_t lds_at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_i8)lds);
+    // (a lane's rows are multiples of 16 apart, after which both swizzles repeat: one place in the row each)
+    const int lane_row = wave * RPL + lane / T::CH;
+    const int kcol = 16 * ((lane % T::CH) ^ T::kswz(lane_row)), vcol = 16 * ((lane % T::CH) ^ T::vswz(lane_row));
     auto copy = [&](int s, int buf) {
         if constexpr (NP == 1) {
 #pragma unroll
             for (int j = 0; j < LOADS; ++j) {
-                const int r0 = (wave + 4 * j) * RPL, r = r0 + lane / T::CH, c = lane % T::CH;
-                const size_t at = slots[s & 1][r] * row_bytes;
-                const uint32_t to = lds_at + buf * T::STAGE + r0 * T::ROW;
-                copy16(kbase + at + 16 * (c ^ T::kswz(r)), to);
-                copy16(vbase + at + 16 * (c ^ T::vswz(r)), to + T::PART);
+                const uint64_t at = slots[s & 1][lane_row + 4 * j * RPL] * row_bytes;
+                const uint32_t to = lds_at + buf * T::STAGE + (wave + 4 * j) * 1024;
+                copy16(kbase + (at + kcol), to);
+                copy16(vbase + (at + vcol), to + T::PART);
             }
         }
     };
@@ -718,18 +720,21 @@ __global__ __launch_bounds__(256, NP == 1 && WR == 4 ? 2 : 1) void paged_tile_ke
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             const Parts<3> w = split8(p + 8 * k);
-            Parts<NP> x[NT];
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
+            for (int t0 = 0; t0 < NT; t0 += 2) {
+                Parts<NP> x[2];
 #pragma unroll
-                for (int n = 0; n < NP; ++n) {
-                    const int8_t* at = vp + n * T::PART + vrow + 16 * k * T::ROW + 16 * ((4 * t + vc) ^ T::vswz(vkey)) + vsub;
-                    const s16x4 u0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)at);
-                    const s16x4 u1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + 8 * T::ROW));
-                    const uint2 y0 = __builtin_bit_cast(uint2, u0), y1 = __builtin_bit_cast(uint2, u1);
-                    x[t].p[n] = make_uint4(y0.x, y0.y, y1.x, y1.y);
-                }
-            product<NP, NT>(x, w, st.o);
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int n = 0; n < NP; ++n) {
+                        const int8_t* at = vp + n * T::PART + vrow + 16 * k * T::ROW + 16 * ((4 * (t0 + t) + vc) ^ T::vswz(vkey)) + vsub;
+                        const s16x4 u0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)at);
+                        const s16x4 u1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + 8 * T::ROW));
+                        const uint2 y0 = __builtin_bit_cast(uint2, u0), y1 = __builtin_bit_cast(uint2, u1);
+                        x[t].p[n] = make_uint4(y0.x, y0.y, y1.x, y1.y);
+                    }
+                product<NP, 2>(x, w, st.o + t0);
+            }
         }
         __builtin_amdgcn_s_setprio(0);
     };
