@@ -36,6 +36,18 @@ __device__ __forceinline__ void copy16(const int8_t* from, uint32_t to) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(to) : "memory");
 }
 
+// 4 bytes a lane, 256 from `to` on.
+__device__ __forceinline__ void copy4(const int* from, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(to) : "memory");
+}
+// Waits until at most N of the wave's copies are under way (the oldest end first).
+template <int N>
+__device__ __forceinline__ void copies_left() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// Waits for the wave's LDS reads: what copies overwrite has been read.
+__device__ __forceinline__ void reads_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
 __device__ __forceinline__ int page_of(const PageMap& m, int p) {
     return m.mul ? (int)(__umulhi((uint32_t)p, m.mul) >> m.shift) : p;
 }
@@ -342,7 +354,7 @@ __device__ __forceinline__ Limits limits_of(const Row& row, int ctx) {
 
 // The products s of a block's keys from c0 on to weights p; st.o scaled where their unit moves.
 template <int D, bool TREE, typename Tree>
-__device__ __forceinline__ void weigh(const PagedAttn& a, const Tree& tree, const Row& row, const Limits& lim, const Scores& sc,
+__device__ __forceinline__ void weigh(const PagedAttn& a, const Tree& tree, const Row& row, const Limits& lim, float slope,
                                       const Cap& cap, int c0, int ctx, f32x16& s, State<D>& st, float (&p)[16]) {
     const int h = (threadIdx.x >> 5) & 1;
     if (a.cap > 0.0f) {
@@ -364,13 +376,13 @@ __device__ __forceinline__ void weigh(const PagedAttn& a, const Tree& tree, cons
                 for (int v = 0; v < 16; ++v) {
                     const int j = c0 + 8 * (v >> 2) + 4 * h + (v & 3);
                     const int at = j < ctx ? j : ctx + tree.depth[min(j - ctx, IE_TREE_MAX - 1)];
-                    s[v] = fmaf(-sc.slope, fabsf((float)(row.pos - at)), s[v]);
+                    s[v] = fmaf(-slope, fabsf((float)(row.pos - at)), s[v]);
                 }
             }
         } else {
             const int base = row.pos - c0 - 4 * h;
 #pragma unroll
-            for (int v = 0; v < 16; ++v) s[v] = fmaf(-sc.slope, fabsf((float)(base - 8 * (v >> 2) - (v & 3))), s[v]);
+            for (int v = 0; v < 16; ++v) s[v] = fmaf(-slope, fabsf((float)(base - 8 * (v >> 2) - (v & 3))), s[v]);
         }
     }
     if (c0 < lim.all_lo || c0 + 32 > lim.all_hi) {
@@ -560,6 +572,18 @@ __device__ __forceinline__ Place place_of(const PagedAttn& a, int tiles) {
     return p;
 }
 
+// V's operand: tile t of keys k0 + 4 h .. and k0 + 8 + 4 h .. of a block's bf16 rows at `rows`.
+template <typename T>
+__device__ __forceinline__ uint4 read_v(const int8_t* rows, int k0, int t) {
+    // this lane's 8 bytes: keys 4 h + (lane % 16) / 4 on, channels 16 (lane / 16 % 2) + 4 (lane % 4) of the tile
+    const int lane = threadIdx.x & 63, key = 4 * (lane >> 5) + (lane & 15) / 4;
+    const int c = 2 * (lane >> 4 & 1) + (lane >> 1 & 1);
+    const int8_t* at = rows + key * T::ROW + 16 * ((4 * t + c) ^ T::vswz(key)) + 8 * (lane & 1) + k0 * T::ROW;
+    const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)at));
+    const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + 8 * T::ROW)));
+    return make_uint4(x.x, x.y, y.x, y.y);
+}
+
 // ---- the tile kernel
 // A workgroup of four waves: WR of them take 32 rows each, 4 / WR groups of them
 // different keys.  A stage holds SK keys' K and V in LDS, NB blocks of 32 for each
@@ -694,12 +718,7 @@ __global__ __launch_bounds__(256, NP == 1 && WR == 4 ? 2 : 1) void paged_tile_ke
     State<D> st;
     st.clear();
 
-    // LDS places of a lane's operands: chunk 2 s + h of key i; of V, 8 bytes of keys 4 h + (lane % 16) / 4
-    // on at channels 16 (lane / 16 % 2) + 4 (lane % 4) of tile t.
-    const int krow = i * T::ROW, kx = 16 * (h ^ T::kswz(i));
-    const int vkey = 4 * h + (lane & 15) / 4, vrow = vkey * T::ROW;
-    const int vc = 2 * (lane >> 4 & 1) + (lane >> 1 & 1), vsub = 8 * (lane & 1);
-
+    const int krow = i * T::ROW, kx = 16 * (h ^ T::kswz(i));  // chunk 2 s + h of key i
     auto attend = [&](const int8_t* stage, int blk, int c0) {
         const int8_t* kp = stage + blk * 32 * T::ROW;
         const int8_t* vp = stage + NP * T::PART + blk * 32 * T::ROW;
@@ -715,7 +734,7 @@ __global__ __launch_bounds__(256, NP == 1 && WR == 4 ? 2 : 1) void paged_tile_ke
         f32x16& s = sa[0];
         __builtin_amdgcn_s_setprio(1);
         float p[16];
-        weigh<D, TREE>(a, tree, row, lim, sc, cap, c0, ctx, s, st, p);
+        weigh<D, TREE>(a, tree, row, lim, sc.slope, cap, c0, ctx, s, st, p);
         __builtin_amdgcn_s_setprio(2);
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
@@ -726,13 +745,7 @@ __global__ __launch_bounds__(256, NP == 1 && WR == 4 ? 2 : 1) void paged_tile_ke
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
-                    for (int n = 0; n < NP; ++n) {
-                        const int8_t* at = vp + n * T::PART + vrow + 16 * k * T::ROW + 16 * ((4 * (t0 + t) + vc) ^ T::vswz(vkey)) + vsub;
-                        const s16x4 u0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)at);
-                        const s16x4 u1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + 8 * T::ROW));
-                        const uint2 y0 = __builtin_bit_cast(uint2, u0), y1 = __builtin_bit_cast(uint2, u1);
-                        x[t].p[n] = make_uint4(y0.x, y0.y, y1.x, y1.y);
-                    }
+                    for (int n = 0; n < NP; ++n) x[t].p[n] = read_v<T>(vp + n * T::PART, 16 * k, t0 + t);
                 product<NP, 2>(x, w, st.o + t0);
             }
         }
@@ -774,6 +787,183 @@ __global__ __launch_bounds__(256, NP == 1 && WR == 4 ? 2 : 1) void paged_tile_ke
     finish<D, KV, TREE>(a, tree, row, b, kvh, ctx, at.split, k0, k1, q_bad, st, l);
 }
 
+// ---- the kernel for at most 32 rows
+// Four waves, all of the same 32 rows, take the keys' blocks of 32 in turn, each by itself: its K and V come into LDS
+// of its own as they lie in the cache, DEEP blocks ahead, so the loop has no barrier and a block's products
+// run beside the next ones' copies.  Of a bf16 cache K's and V's rows are operands as in the tile kernel; fp32 rows
+// are split as they are read, V's a channel a lane (32 lanes read 128 bytes).  A page's number comes the same way,
+// DEEP blocks ahead of its rows.
+template <int D, int NP>
+struct Few {
+    static constexpr int ROW = D * (NP == 1 ? 2 : 4);  // bytes of a row
+    static constexpr int PART = 32 * ROW;              // of a block's K or V
+    static constexpr int DEEP = PART > 8192 ? 1 : 2;
+    static constexpr int WAVE = 2 * DEEP * PART;
+    static constexpr int COPIES = PART / 1024;         // a wave's copies of K or V
+    static constexpr int MERGE = 3 * 64 * (D / 2 + 2) * 4;
+    static constexpr int LDS = 4 * WAVE;
+    static constexpr int CH = ROW / 16;
+    static_assert(LDS >= MERGE && 3 * COPIES + 2 < 63, "a wave's ring");
+    // As Tile's; fp32 rows' chunks of four values, of which K's operand takes two.
+    __device__ static __forceinline__ int kswz(int r) {
+        return NP == 3 ? (r & 7) << 1 : D == 128 ? r & 15 : (r >> 1) & 7;
+    }
+    __device__ static __forceinline__ int vswz(int r) { return NP == 3 ? 0 : D == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1); }
+};
+
+template <int D, int NP, bool TREE>
+__global__ __launch_bounds__(256, 1) void paged_few_kernel(PagedAttn a, int tiles) {
+    using T = Few<D, NP>;
+    using KV = std::conditional_t<NP == 1, uint16_t, float>;
+    using Tree = std::conditional_t<TREE, TreeLds, NoTree>;
+    constexpr int NT = D / 32, KS = D / 16, DEEP = T::DEEP, C = T::COPIES;
+    __shared__ __attribute__((aligned(1024))) int8_t lds_all[T::LDS];
+    __shared__ __attribute__((aligned(256))) int pages_all[4][2 * DEEP][64];  // pages of a block's keys
+    __shared__ uint32_t slots_all[4][32];
+    __shared__ Tree tree;
+    const int lane = threadIdx.x & 63, i = lane & 31, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Place at = place_of<TREE>(a, tiles);
+    const int b = at.b, kvh = at.kvh, ctx = at.start;
+    const int r = at.tile * 32 + i;
+    const float* q_row = query_row<D>(a, r, b, kvh);
+    RawQuery<D> raw_q = load_query<D>(q_row, h);
+    if constexpr (TREE) grow_tree(tree, a.parents + (size_t)b * a.P, a.P, a.window);
+    const Row row = row_of<TREE>(a, tree, r, b, kvh, at.start, at.len);
+    const Limits lim = limits_of<TREE>(row, ctx);
+    const int kbeg = min(lim.lo, lim.hi), kend = lim.hi;
+    // this split's blocks, and this wave's: numbers wave, wave + 4, ...
+    const int all = (kend - kbeg + 127) / 128, per = (all + a.splits - 1) / a.splits;
+    const int s0 = min(at.split * per, all), s1 = min(s0 + per, all);
+    const int k0 = kbeg + s0 * 128, k1 = min(kbeg + s1 * 128, kend);
+    const int n = ((k1 - k0 + 31) / 32 - wave + 3) / 4;
+
+    const int* table = a.pages.table + (size_t)b * a.pages.nbps;
+    const size_t row_bytes = (size_t)a.H_kv * D * sizeof(KV);
+    const int8_t* kbase = reinterpret_cast<const int8_t*>(static_cast<const KV*>(a.k) + (size_t)kvh * D);
+    const int8_t* vbase = reinterpret_cast<const int8_t*>(static_cast<const KV*>(a.v) + (size_t)kvh * D);
+    int8_t* const lds = lds_all + wave * T::WAVE;
+    const uint32_t lds_at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_i8)lds);
+    const uint32_t pages_at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_i8)(int8_t*)pages_all[wave]);
+    uint32_t* const slots = slots_all[wave];
+    auto first = [&](int j) { return k0 + 32 * (4 * j + wave); };           // key of block j
+    auto pos_of = [&](int j) { return min(first(j) + i, k1 - 1); };         // of this lane's key
+    auto ask_pages = [&](int j) { copy4(table + page_of(a.pages, pos_of(j)), pages_at + (j & (2 * DEEP - 1)) * 256); };
+    constexpr int RPC = 1024 / T::ROW;  // rows of a copy
+    const int lane_row = lane / T::CH;
+    auto col = [&](int j, bool v) {  // of this lane's 16 bytes in its row of copy j
+        const int rr = lane_row + j * RPC;
+        return 16 * ((lane % T::CH) ^ (v ? T::vswz(rr) : T::kswz(rr)));
+    };
+    // K of block j (its pages have come), and the pages of block j + DEEP
+    auto ask_k = [&](int j) {
+        const int p = pos_of(j), in = page_of(a.pages, p);
+        const uint32_t page = (uint32_t)pages_all[wave][j & (2 * DEEP - 1)][i];
+        slots[i] = page * (uint32_t)a.pages.block + (uint32_t)(p - in * a.pages.block);
+        ask_pages(j + DEEP);
+        reads_done();
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+            copy16(kbase + (slots[lane_row + c * RPC] * row_bytes + col(c, false)), lds_at + (j & (DEEP - 1)) * T::PART + c * 1024);
+    };
+    auto ask_v = [&](int j) {  // (after ask_k(j))
+        reads_done();
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+            copy16(vbase + (slots[lane_row + c * RPC] * row_bytes + col(c, true)),
+                   lds_at + (DEEP + (j & (DEEP - 1))) * T::PART + c * 1024);
+    };
+
+    if (n > 0) {
+#pragma unroll
+        for (int j = 0; j < DEEP; ++j) ask_pages(j);
+    }
+    // (the query is there before the copies start: the compiler's wait for it would be one for them)
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            asm volatile("" : "+v"(raw_q.x[s][k].x), "+v"(raw_q.x[s][k].y), "+v"(raw_q.x[s][k].z), "+v"(raw_q.x[s][k].w));
+    const Scores sc = scores_of(a, row.head);
+    const Cap cap = cap_of(a.cap);
+    float slope = sc.slope;
+    asm volatile("" : "+v"(slope));
+    if (n > 0) {
+        copies_left<0>();
+        ask_k(0);
+        ask_v(0);
+        if (DEEP == 2 && n > 1) {
+            ask_k(1);
+            ask_v(1);
+        }
+    }
+    Parts<3> q[KS];
+    const bool q_bad = split_query<D>(q_row, raw_q, sc.q, q);
+    State<D> st;
+    st.clear();
+
+#pragma unroll 1
+    for (int j = 0; j < n; ++j) {
+        // what may be under way while block j's K is read: V of j, and of j + 1 its successor's pages, K and V
+        if (DEEP == 2 && j + 1 < n) copies_left<3 * C + 1>();
+        else copies_left<C>();
+        const int c0 = first(j);
+        const int8_t* kp = lds + (j & (DEEP - 1)) * T::PART;
+        const int8_t* vp = lds + (DEEP + (j & (DEEP - 1))) * T::PART;
+        f32x16 sa[1] = {};
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            Parts<NP> x[1];
+            if constexpr (NP == 1) {
+                x[0].p[0] = *reinterpret_cast<const uint4*>(kp + i * T::ROW + 16 * ((2 * k + h) ^ T::kswz(i)));
+            } else {
+                float y[8];
+                const float4 u = *reinterpret_cast<const float4*>(kp + i * T::ROW + 16 * ((4 * k + 2 * h) ^ T::kswz(i)));
+                const float4 w = *reinterpret_cast<const float4*>(kp + i * T::ROW + 16 * ((4 * k + 2 * h + 1) ^ T::kswz(i)));
+                y[0] = u.x, y[1] = u.y, y[2] = u.z, y[3] = u.w, y[4] = w.x, y[5] = w.y, y[6] = w.z, y[7] = w.w;
+                x[0] = split8(y);
+            }
+            product<NP, 1>(x, q[k], sa);
+        }
+        if (j + DEEP < n) ask_k(j + DEEP);
+        float p[16];
+        weigh<D, TREE>(a, tree, row, lim, slope, cap, c0, ctx, sa[0], st, p);
+        // V of block j: behind it came K of j + DEEP and the pages behind that, and with two blocks under way the
+        // same and V of j + 1
+        if (j + DEEP < n) copies_left<DEEP == 2 ? 3 * C + 2 : C + 1>();
+        else if (DEEP == 2 && j + 1 < n) copies_left<2 * C + 1>();
+        else copies_left<0>();
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const Parts<3> w = split8(p + 8 * k);
+#pragma unroll
+            for (int t0 = 0; t0 < NT; t0 += 2) {
+                Parts<NP> x[2];
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    if constexpr (NP == 1) {
+                        x[t].p[0] = read_v<T>(vp, 16 * k, t0 + t);
+                    } else {
+                        float y[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            y[e] = *reinterpret_cast<const float*>(vp + (16 * k + 4 * h + (e & 3) + 8 * (e >> 2)) * T::ROW +
+                                                                   128 * (t0 + t) + 4 * i);
+                        x[t] = split8(y);
+                    }
+                }
+                product<NP, 2>(x, w, st.o + t0);
+            }
+        }
+        if (j + DEEP < n) ask_v(j + DEEP);
+    }
+    float l = sum_xor32(st.l);
+    copies_left<0>();
+    __syncthreads();
+    if (!gather<D, 3>(lds_all, wave, 1, 0, st, l)) return;
+    finish<D, KV, TREE>(a, tree, row, b, kvh, ctx, at.split, k0, k1, q_bad, st, l);
+}
+
 // O rows from their splits' partials, D / 4 lanes a row.
 template <int D>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn a) {
@@ -804,32 +994,37 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn a) {
     reinterpret_cast<float4*>(a.O + r * D)[c] = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
-// Waves of a workgroup that take different rows.
+// Waves of a workgroup that take different rows; 1: paged_few_kernel's.
 int row_waves(int P, int G, int kv_dtype) {
     const long long rows = (long long)P * G;
-    if (kv_dtype == IE_KV_BF16 && rows <= 32) return 1;
-    return rows <= 64 ? 2 : 4;
+    return rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
 }
 
 template <int D, int NP, int WR>
 void launch_tile(const PagedAttn& a, hipStream_t s) {
     const int G = a.H_q / a.H_kv, tiles = (int)(((long long)a.P * G + 32 * WR - 1) / (32 * WR));
     const unsigned grid = (unsigned)((long long)a.B * a.H_kv * tiles * a.splits);
-    auto* k = a.parents ? paged_tile_kernel<D, NP, WR, true> : paged_tile_kernel<D, NP, WR, false>;
-    k<<<grid, 256, 0, s>>>(a, tiles);
+    if constexpr (WR == 1) {
+        auto* k = a.parents ? paged_few_kernel<D, NP, true> : paged_few_kernel<D, NP, false>;
+        k<<<grid, 256, 0, s>>>(a, tiles);
+    } else {
+        auto* k = a.parents ? paged_tile_kernel<D, NP, WR, true> : paged_tile_kernel<D, NP, WR, false>;
+        k<<<grid, 256, 0, s>>>(a, tiles);
+    }
+}
+
+template <int D, int NP>
+void launch_np(const PagedAttn& a, hipStream_t s) {
+    const int wr = row_waves(a.P, a.H_q / a.H_kv, a.kv_dtype);
+    if (wr == 1) launch_tile<D, NP, 1>(a, s);
+    else if (wr == 2) launch_tile<D, NP, 2>(a, s);
+    else launch_tile<D, NP, 4>(a, s);
 }
 
 template <int D>
 void launch_d(const PagedAttn& a, hipStream_t s) {
-    const int wr = row_waves(a.P, a.H_q / a.H_kv, a.kv_dtype);
-    if (a.kv_dtype == IE_KV_BF16) {
-        if (wr == 1) launch_tile<D, 1, 1>(a, s);
-        else if (wr == 2) launch_tile<D, 1, 2>(a, s);
-        else launch_tile<D, 1, 4>(a, s);
-    } else {
-        if (wr == 2) launch_tile<D, 3, 2>(a, s);
-        else launch_tile<D, 3, 4>(a, s);
-    }
+    if (a.kv_dtype == IE_KV_BF16) launch_np<D, 1>(a, s);
+    else launch_np<D, 3>(a, s);
     if (a.splits > 1) {
         const long long rows = (long long)a.B * a.P * a.H_q;
         paged_merge_kernel<D><<<(unsigned)((rows * (D / 4) + 255) / 256), 256, 0, s>>>(a);
