@@ -167,19 +167,23 @@ struct TreeLds {
 };
 struct NoTree {};
 
-// By pointer doubling: after round k a node has its 2^k nearest ancestors.
+// By pointer doubling: after round k a node has its 2^k nearest ancestors.  For any workgroup of at least IE_TREE_MAX
+// threads, the first of which have a node each.
 __device__ __forceinline__ void grow_tree(TreeLds& s, const int* parents, int T, int window) {
     const int t = threadIdx.x;
+    const bool node = t < IE_TREE_MAX;
     constexpr int W = kLine - 1;
     uint32_t w[W];
 #pragma unroll
     for (int k = 0; k < W; ++k) w[k] = t >> 5 == k ? 1u << (t & 31) : 0u;
-    int up = t < T ? parents[t] : -1;
-    if (up >= t) up = -1;
-    for (;;) {
-        s.up[t] = up;
+    int up = node && t < T ? parents[t] : -1;
+    if (up >= t || up < 0) up = -1;
+    for (int round = 0; round <= 8; ++round) {  // (2^8 ancestors at most)
+        if (node) {
+            s.up[t] = up;
 #pragma unroll
-        for (int k = 0; k < W; ++k) s.line[t][k] = w[k];
+            for (int k = 0; k < W; ++k) s.line[t][k] = w[k];
+        }
         if (!__syncthreads_or(up >= 0)) break;
         if (up >= 0) {
 #pragma unroll
@@ -191,9 +195,9 @@ __device__ __forceinline__ void grow_tree(TreeLds& s, const int* parents, int T,
     int deep = -1;
 #pragma unroll
     for (int k = 0; k < W; ++k) deep += __builtin_popcount(w[k]);
-    s.depth[t] = deep;
+    if (node) s.depth[t] = deep;
     __syncthreads();
-    if (window > 0 && deep >= window) {
+    if (node && window > 0 && deep >= window) {
 #pragma unroll
         for (int k = 0; k < W; ++k) {
             uint32_t keep = w[k];
@@ -964,6 +968,314 @@ __global__ __launch_bounds__(256, 1) void paged_few_kernel(PagedAttn a, int tile
     finish<D, KV, TREE>(a, tree, row, b, kvh, ctx, at.split, k0, k1, q_bad, st, l);
 }
 
+// ---- the kernel for up to four rows: vector units
+// At so few rows a matrix tile of 32 is mostly empty and its softmax costs as much as a full one's.  Here eight waves
+// take the keys' batches in turn, in fp32 as they are: LPK lanes hold a key's row, 16 bytes each, so a copy
+// brings KPI whole rows; a score is a lane's products summed over its LPK lanes, which then have the key's weight for
+// their channels of V.  Each group of LPK lanes keeps its own unit, sum and output, joined at the end.  K and V come
+// into LDS of the wave's own, 8 KiB each: the next batch's K while the weights are made, its V behind the products, its
+// pages a batch earlier.  (Loaded into registers
+// instead, four rows of 32 x 8 heads x 8192 x 128 bf16 took 450 us against 182: the loads' addresses and targets waited
+// for one another's.)
+template <int D, typename KV>
+struct Lanes {
+    static constexpr int E = 16 / (int)sizeof(KV);  // values a lane
+    static constexpr int LPK = D / E;               // lanes a key
+    static constexpr int KPI = 64 / LPK;            // keys a load
+    static constexpr int U = 8;                     // copies of a batch's K or V
+    static constexpr int PART = U * 1024;
+    static constexpr int BK = U * KPI;              // its keys
+};
+// Sum over the N lanes that hold a key.
+template <int N>
+__device__ __forceinline__ float lanes_sum(float v) {
+    if constexpr (N == 8) {
+        v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0xB1, 0xf, 0xf, false));   // l ^ 1
+        v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x4E, 0xf, 0xf, false));   // l ^ 2
+        v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x141, 0xf, 0xf, false));  // 7 - l
+        return v;
+    } else if constexpr (N == 16) {
+        return row16_sum(v);
+    } else {
+        return sum_xor16(row16_sum(v));
+    }
+}
+// Over the groups of lanes that hold different keys.
+template <int N>
+__device__ __forceinline__ float groups_sum(float v) {
+    if constexpr (N == 8) v += dpp_row_ror<8>(v);
+    if constexpr (N <= 16) v = sum_xor16(v);
+    return sum_xor32(v);
+}
+template <int N>
+__device__ __forceinline__ float groups_max(float v) {
+    if constexpr (N == 8) v = fmaxf(v, dpp_row_ror<8>(v));
+    if constexpr (N <= 16) v = max_xor16(v);
+    return max_xor32(v);
+}
+template <typename KV>
+__device__ __forceinline__ void values(uint4 w, float (&x)[16 / sizeof(KV)]) {
+    if constexpr (sizeof(KV) == 4) {
+        x[0] = __builtin_bit_cast(float, w.x), x[1] = __builtin_bit_cast(float, w.y);
+        x[2] = __builtin_bit_cast(float, w.z), x[3] = __builtin_bit_cast(float, w.w);
+    } else {
+        x[0] = low_of(w.x), x[1] = high_of(w.x), x[2] = low_of(w.y), x[3] = high_of(w.y);
+        x[4] = low_of(w.z), x[5] = high_of(w.z), x[6] = low_of(w.w), x[7] = high_of(w.w);
+    }
+}
+
+constexpr int kRowWaves = 8;
+static_assert(64 * kRowWaves >= IE_TREE_MAX, "grow_tree has a thread a node");
+template <int D, typename KV, int R, bool TREE>
+__global__ __launch_bounds__(64 * kRowWaves, 2) void paged_row_kernel(PagedAttn a, int tiles) {
+    using T = Lanes<D, KV>;
+    using Tree = std::conditional_t<TREE, TreeLds, NoTree>;
+    constexpr int E = T::E, U = T::U, W = kRowWaves;
+    __shared__ Tree tree;
+    __shared__ __attribute__((aligned(1024))) int8_t lds_all[W * 2 * T::PART];
+    __shared__ __attribute__((aligned(256))) int pages_all[W][2][64];
+    __shared__ uint32_t slots_all[W][64];
+    __shared__ float sm_m[W][R], sm_l[W][R];
+    static_assert(sizeof(lds_all) >= sizeof(float) * W * R * D, "the join");
+    const int tid = threadIdx.x, lane = tid & 63, sub = lane % T::LPK, grp = lane / T::LPK;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const Place at = place_of<TREE>(a, tiles);
+    const int b = at.b, kvh = at.kvh, ctx = at.start;
+    float q[R][E];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const float* row = query_row<D>(a, at.tile * R + r, b, kvh) + E * sub;
+#pragma unroll
+        for (int e = 0; e < E; e += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(row + e);
+            q[r][e] = x.x, q[r][e + 1] = x.y, q[r][e + 2] = x.z, q[r][e + 3] = x.w;
+        }
+    }
+    if constexpr (TREE) grow_tree(tree, a.parents + (size_t)b * a.P, a.P, a.window);
+    // a row's bounds in lane r, and in scalar registers
+    const Row mine = row_of<TREE>(a, tree, at.tile * R + (lane & (R - 1)), b, kvh, at.start, at.len);
+    const Limits lim = limits_of<TREE>(mine, ctx);
+    Row rows[R];
+    float slope[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        rows[r].t = __builtin_amdgcn_readlane(mine.t, r);
+        rows[r].head = __builtin_amdgcn_readlane(mine.head, r);
+        rows[r].lo = __builtin_amdgcn_readlane(mine.lo, r);
+        rows[r].hi = __builtin_amdgcn_readlane(mine.hi, r);
+        rows[r].pos = __builtin_amdgcn_readlane(mine.pos, r);
+        slope[r] = a.slopes ? a.slopes[rows[r].head] * kLog2e : 0.0f;
+    }
+    const int kbeg = min(lim.lo, lim.hi), kend = lim.hi;
+    const int all = (kend - kbeg + 127) / 128, per = (all + a.splits - 1) / a.splits;
+    const int s0 = min(at.split * per, all), s1 = min(s0 + per, all);
+    const int k0 = kbeg + s0 * 128, k1 = min(kbeg + s1 * 128, kend);
+
+    const int* table = a.pages.table + (size_t)b * a.pages.nbps;
+    const size_t row_bytes = (size_t)a.H_kv * D * sizeof(KV);
+    const int8_t* kbase = reinterpret_cast<const int8_t*>(static_cast<const KV*>(a.k) + (size_t)kvh * D) + 16 * sub;
+    const int8_t* vbase = reinterpret_cast<const int8_t*>(static_cast<const KV*>(a.v) + (size_t)kvh * D) + 16 * sub;
+    const Cap cap = cap_of(a.cap);
+    const float factor = a.cap > 0.0f ? a.scale / a.cap : a.scale * kLog2e;
+
+    float m[R], l[R], o[R][E];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        m[r] = -INFINITY;
+        l[r] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[r][e] = 0.0f;
+    }
+    // batch n of this wave: keys first(n) on
+    auto first = [&](int n) { return k0 + T::BK * (W * n + wave); };
+    auto pos_of = [&](int n) { return min(first(n) + (lane & (T::BK - 1)), k1 - 1); };
+    const int n1 = k1 > k0 ? ((k1 - k0 + T::BK - 1) / T::BK - wave + W - 1) / W : 0;
+    int8_t* const lds = lds_all + wave * 2 * T::PART;
+    const uint32_t lds_at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_i8)lds);
+    const uint32_t pages_at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_i8)(int8_t*)pages_all[wave]);
+    uint32_t* const slots = slots_all[wave];
+    auto ask_pages = [&](int n) { copy4(table + page_of(a.pages, pos_of(n)), pages_at + (n & 1) * 256); };
+    auto ask_k = [&](int n) {  // (its pages have come)
+        const int p = pos_of(n);
+        slots[lane] = (uint32_t)pages_all[wave][n & 1][lane] * (uint32_t)a.pages.block + (uint32_t)(p - page_of(a.pages, p) * a.pages.block);
+        ask_pages(n + 1);
+        reads_done();
+#pragma unroll
+        for (int u = 0; u < U; ++u) copy16(kbase + slots[u * T::KPI + grp] * row_bytes, lds_at + u * 1024);
+    };
+    auto ask_v = [&] {  // (after ask_k of the same batch)
+        reads_done();
+#pragma unroll
+        for (int u = 0; u < U; ++u) copy16(vbase + slots[u * T::KPI + grp] * row_bytes, lds_at + T::PART + u * 1024);
+    };
+    if (n1 > 0) ask_pages(0);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {  // (here before the copies start: a wait of the compiler's would be one for them)
+        asm volatile("" : "+v"(slope[r]));
+#pragma unroll
+        for (int e = 0; e < E; ++e) asm volatile("" : "+v"(q[r][e]));
+    }
+    if (n1 > 0) {
+        copies_left<0>();
+        ask_k(0);
+        ask_v();
+    }
+#pragma unroll 1
+    for (int n = 0; n < n1; ++n) {
+        const int c0 = first(n);
+        float s[R][U];
+        copies_left<U>();  // K of batch n; V of it may be under way
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            float x[E];
+            values<KV>(*reinterpret_cast<const uint4*>(lds + u * 1024 + 16 * lane), x);
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                float d0 = q[r][0] * x[0], d1 = q[r][1] * x[1];
+#pragma unroll
+                for (int e = 2; e < E; e += 2) {
+                    d0 = fmaf(q[r][e], x[e], d0);
+                    d1 = fmaf(q[r][e + 1], x[e + 1], d1);
+                }
+                s[r][u] = lanes_sum<T::LPK>(d0 + d1) * factor;
+            }
+        }
+        if (n + 1 < n1) ask_k(n + 1);
+        const bool edge = c0 < lim.all_lo || c0 + T::BK > lim.all_hi;
+        uint32_t seen[R];  // bit u: this lane's key of load u
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            if (a.cap > 0.0f) {
+                float most = 0.0f;
+#pragma unroll
+                for (int u = 0; u < U; ++u) most = fmaxf(most, fabsf(s[r][u]));
+                if (__ballot(!(most < 1.0f))) {
+#pragma unroll
+                    for (int u = 0; u < U; ++u) s[r][u] = capped(s[r][u], cap);
+                } else {
+#pragma unroll
+                    for (int u = 0; u < U; ++u) s[r][u] = capped_small(s[r][u], cap);
+                }
+            }
+            if (a.slopes) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    int j = c0 + u * T::KPI + grp;
+                    if constexpr (TREE) j = j < ctx ? j : ctx + tree.depth[min(j - ctx, IE_TREE_MAX - 1)];
+                    s[r][u] = fmaf(-slope[r], fabsf((float)(rows[r].pos - j)), s[r][u]);
+                }
+            }
+            seen[r] = 0xffffffffu;
+            if (edge) {
+                seen[r] = 0;
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int j = c0 + u * T::KPI + grp;
+                    bool in = j >= rows[r].lo && j < rows[r].hi;
+                    if constexpr (TREE) {
+                        const int x = min(max(j - ctx, 0), IE_TREE_MAX - 1);
+                        if (j >= ctx) in = j < rows[r].hi && (tree.line[rows[r].t][x >> 5] >> (x & 31) & 1);
+                    }
+                    if (in) seen[r] |= 1u << u;
+                    else s[r][u] = -INFINITY;
+                }
+            }
+            float top = s[r][0];
+#pragma unroll
+            for (int u = 1; u < U; ++u) top = fmaxf(top, s[r][u]);
+            if (__ballot(top > m[r] + 8.0f)) {  // (as weigh)
+                const float mn = fmaxf(m[r], top), alpha = mn == -INFINITY ? 0.0f : exp2_sm(m[r] - mn);
+                m[r] = mn;
+                l[r] *= alpha;
+#pragma unroll
+                for (int e = 0; e < E; ++e) o[r][e] *= alpha;
+            }
+            const float mu = m[r] == -INFINITY ? 0.0f : m[r];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                s[r][u] = exp2_sm(s[r][u] - mu);
+                l[r] += s[r][u];
+            }
+        }
+        if (n + 1 < n1) copies_left<U + 1>();  // V of batch n; behind it K of the next and the pages after that
+        else copies_left<0>();
+        const int8_t* vp = lds + T::PART + 16 * lane;
+        if (edge) {  // (what a row does not see may be anything)
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                float x[E];
+                values<KV>(*reinterpret_cast<const uint4*>(vp + u * 1024), x);
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) o[r][e] = fmaf(s[r][u], seen[r] >> u & 1 ? x[e] : 0.0f, o[r][e]);
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                float x[E];
+                values<KV>(*reinterpret_cast<const uint4*>(vp + u * 1024), x);
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) o[r][e] = fmaf(s[r][u], x[e], o[r][e]);
+            }
+        }
+        if (n + 1 < n1) ask_v();
+    }
+    copies_left<0>();
+    __syncthreads();  // (the waves' buffers serve the join)
+    float (*sm_o)[R][D] = reinterpret_cast<float (*)[R][D]>(lds_all);
+    // The wave's groups, then the waves.
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const float mx = groups_max<T::LPK>(m[r]), f = mx == -INFINITY ? 0.0f : exp2_sm(m[r] - mx);
+        const float sum = groups_sum<T::LPK>(l[r] * f);
+        float x[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = groups_sum<T::LPK>(o[r][e] * f);
+        if (grp == 0) {
+#pragma unroll
+            for (int e = 0; e < E; e += 4) *reinterpret_cast<float4*>(&sm_o[wave][r][E * sub + e]) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+        }
+        if (lane == 0) {
+            sm_m[wave][r] = mx;
+            sm_l[wave][r] = sum;
+        }
+    }
+    __syncthreads();
+    const size_t total = (size_t)a.B * a.P * a.H_q;
+#pragma unroll 1
+    for (int x = tid; x < R * D / 4; x += 64 * W) {
+        const int r = x / (D / 4), c = 4 * (x % (D / 4));
+        const Row row = row_of<TREE>(a, tree, at.tile * R + r, b, kvh, at.start, at.len);
+        if (!row.live) continue;
+        float mx = sm_m[0][r];
+#pragma unroll
+        for (int w = 1; w < W; ++w) mx = fmaxf(mx, sm_m[w][r]);
+        const float mu = mx == -INFINITY ? 0.0f : mx;
+        float sum = 0.0f;
+        float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const float f = exp2_sm(sm_m[w][r] - mu);
+            const float4 z = *reinterpret_cast<const float4*>(&sm_o[w][r][c]);
+            sum = fmaf(f, sm_l[w][r], sum);
+            y.x = fmaf(f, z.x, y.x), y.y = fmaf(f, z.y, y.y), y.z = fmaf(f, z.z, y.z), y.w = fmaf(f, z.w, y.w);
+        }
+        const size_t to = ((size_t)b * a.P + row.t) * a.H_q + row.head;
+        float* out = a.O + to * D;
+        float inv = 1.0f;
+        if (a.splits == 1) {
+            inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        } else {
+            out = a.ws + (at.split * total + to) * D;
+            if (c == 0) *reinterpret_cast<float2*>(a.ws + a.splits * total * D + 2 * (at.split * total + to)) = make_float2(mx, sum);
+        }
+        *reinterpret_cast<float4*>(out + c) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+    }
+}
+
 // O rows from their splits' partials, D / 4 lanes a row.
 template <int D>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn a) {
@@ -994,31 +1306,44 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn a) {
     reinterpret_cast<float4*>(a.O + r * D)[c] = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
-// Waves of a workgroup that take different rows; 1: paged_few_kernel's.
-int row_waves(int P, int G, int kv_dtype) {
+// Rows of a tile: up to 4 are paged_row_kernel's, 32 paged_few_kernel's, 64 and 128 paged_tile_kernel's.
+// Row against few kernel (us, 8 KV heads, one sequence of 2000 keys; 32 of 4000): fp32 d 64 one row 15.8 and
+// 45.5; 92 and 101, four 30.8 and 45.6; 99 and 102, eight 53.7 and 45.6; 118 and 103, d 128 four 63.7 and 77.6; 193 and
+// 190; bf16 d 64 two 15.3 and 26.1; 48.9 and 49.0, four 23.8 and 26.2; 54.4 and 49.2, d 128 two 25.8 and 38.7; 96.5 and
+// 98.8, four 40.2 and 38.8; 103 and 99.
+int tile_rows(int P, int G, int kv_dtype) {
     const long long rows = (long long)P * G;
-    return rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
+    if (rows <= (kv_dtype == IE_KV_BF16 ? 2 : 4)) return rows <= 2 ? (int)rows : 4;
+    return rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
 }
 
-template <int D, int NP, int WR>
+template <int D, int NP, int ROWS, bool TREE>
 void launch_tile(const PagedAttn& a, hipStream_t s) {
-    const int G = a.H_q / a.H_kv, tiles = (int)(((long long)a.P * G + 32 * WR - 1) / (32 * WR));
+    const int G = a.H_q / a.H_kv, tiles = (int)(((long long)a.P * G + ROWS - 1) / ROWS);
     const unsigned grid = (unsigned)((long long)a.B * a.H_kv * tiles * a.splits);
-    if constexpr (WR == 1) {
-        auto* k = a.parents ? paged_few_kernel<D, NP, true> : paged_few_kernel<D, NP, false>;
-        k<<<grid, 256, 0, s>>>(a, tiles);
-    } else {
-        auto* k = a.parents ? paged_tile_kernel<D, NP, WR, true> : paged_tile_kernel<D, NP, WR, false>;
-        k<<<grid, 256, 0, s>>>(a, tiles);
+    using KV = std::conditional_t<NP == 1, uint16_t, float>;
+    if constexpr (ROWS <= 4) paged_row_kernel<D, KV, ROWS, TREE><<<grid, 64 * kRowWaves, 0, s>>>(a, tiles);
+    else if constexpr (ROWS == 32) paged_few_kernel<D, NP, TREE><<<grid, 256, 0, s>>>(a, tiles);
+    else paged_tile_kernel<D, NP, ROWS / 32, TREE><<<grid, 256, 0, s>>>(a, tiles);
+}
+
+template <int D, int NP, bool TREE>
+void launch_rows(const PagedAttn& a, hipStream_t s) {
+    switch (tile_rows(a.P, a.H_q / a.H_kv, a.kv_dtype)) {
+        case 1: return launch_tile<D, NP, 1, TREE>(a, s);
+        case 2: return launch_tile<D, NP, 2, TREE>(a, s);
+        case 4:
+            if constexpr (NP == 3) return launch_tile<D, NP, 4, TREE>(a, s);
+        case 32: return launch_tile<D, NP, 32, TREE>(a, s);
+        case 64: return launch_tile<D, NP, 64, TREE>(a, s);
+        default: return launch_tile<D, NP, 128, TREE>(a, s);
     }
 }
 
 template <int D, int NP>
 void launch_np(const PagedAttn& a, hipStream_t s) {
-    const int wr = row_waves(a.P, a.H_q / a.H_kv, a.kv_dtype);
-    if (wr == 1) launch_tile<D, NP, 1>(a, s);
-    else if (wr == 2) launch_tile<D, NP, 2>(a, s);
-    else launch_tile<D, NP, 4>(a, s);
+    if (a.parents) launch_rows<D, NP, true>(a, s);
+    else launch_rows<D, NP, false>(a, s);
 }
 
 template <int D>
@@ -1034,13 +1359,13 @@ void launch_d(const PagedAttn& a, hipStream_t s) {
 }  // namespace
 
 int paged_attn_splits(int B, int P, int H_q, int H_kv, int, int kv_dtype, int max_keys, int window, int asked) {
-    const int G = H_q / H_kv, wr = row_waves(P, G, kv_dtype);
+    const int G = H_q / H_kv, rows = tile_rows(P, G, kv_dtype);
     const long long walked = window && (long long)window + P < max_keys ? (long long)window + P : max_keys;
     const int stages = (int)((walked + 127) / 128);
     int s = asked;
     if (s <= 0) {
-        const long long groups = (long long)B * H_kv * (((long long)P * G + 32 * wr - 1) / (32 * wr));
-        s = (int)(512 / groups);
+        const long long groups = (long long)B * H_kv * (((long long)P * G + rows - 1) / rows);
+        s = (int)((rows <= 32 ? 256 : 512) / groups);
         s = s < 1 ? 1 : s > stages / 2 ? stages / 2 : s;
         if (s < 1) s = 1;
     }
