@@ -22,6 +22,7 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -92,12 +93,41 @@ __device__ __forceinline__ Parts<3> split8(const float* x) {
     split_pair(x[6], x[7], r.p[0].w, r.p[1].w, r.p[2].w);
     return r;
 }
+
+// ---- the matrix instructions' shapes: M rows a wave (lane l: row i = l % M, group g = l / M)
+// M = 32: v_mfma_f32_32x32x16_bf16; M = 16: v_mfma_f32_16x16x32_bf16.  A lane has 8 values of an operand, of channels (or
+// keys' slots) 8 g on of each step; of a product AV values, its column the lane's row.  Of a block of 32 keys it ends
+// with the scores of keys STEP (v / 4) + 4 g + v % 4, v < NS, whose weights p[8 k ..] are step k's operand of the
+// second product.
+template <int M>
+struct Shape {
+    static constexpr int AV = M * M / 64, TILES = 32 / M, NS = TILES * AV, STEP = M == 32 ? 8 : 16;
+    static constexpr int KC = 512 / M;  // channels (keys) of a step
+    typedef float Acc __attribute__((ext_vector_type(AV)));
+    __device__ static __forceinline__ float rows_max(float x) {
+        if constexpr (M == 16) x = max_xor16(x);
+        return max_xor32(x);
+    }
+    __device__ static __forceinline__ float rows_sum(float x) {
+        if constexpr (M == 16) x = sum_xor16(x);
+        return sum_xor32(x);
+    }
+    // rows (bit i) that have a lane among `lanes`
+    __device__ static __forceinline__ uint32_t rows_of(uint64_t lanes) {
+        uint32_t x = (uint32_t)lanes | (uint32_t)(lanes >> 32);
+        if constexpr (M == 16) x = (x | x >> 16) & 0xffffu;
+        return x;
+    }
+};
 __device__ __forceinline__ f32x16 mfma(uint4 a, uint4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
+__device__ __forceinline__ f32x4 mfma(uint4 a, uint4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
 // c[t] += a[t] b, of a's N parts and b's three, the small products first; an accumulator's own are not back to back.
-template <int N, int NT>
-__device__ __forceinline__ void product(const Parts<N> (&a)[NT], const Parts<3>& b, f32x16* c) {
+template <int N, int NT, typename Acc>
+__device__ __forceinline__ void product(const Parts<N> (&a)[NT], const Parts<3>& b, Acc* c) {
     auto all = [&](int i, int j) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) c[t] = mfma(a[t].p[i], b.p[j], c[t]);
@@ -323,21 +353,23 @@ __device__ __forceinline__ void exact_row(const PagedAttn& a, const Tree& tree, 
     }
 }
 
-// ---- what a wave keeps of its 32 rows
-template <int D>
+// ---- what a wave keeps of its M rows
+template <int D, int M>
 struct State {
-    float m, l;         // the weights' unit, and a lane's own keys' sum of them
-    f32x16 o[D / 32];   // o[t][v]: channel 32 t + 8 (v / 4) + 4 h + v % 4
+    using Sh = Shape<M>;
+    static constexpr int NT = D / M;
+    float m, l;              // the weights' unit, and a lane's own keys' sum of them
+    typename Sh::Acc o[NT];  // o[t][v]: channel M t + 8 (v / 4) + 4 g + v % 4
     __device__ __forceinline__ void clear() {
         m = -INFINITY;
         l = 0.0f;
 #pragma unroll
-        for (int t = 0; t < D / 32; ++t) o[t] = f32x16{};
+        for (int t = 0; t < NT; ++t) o[t] = typename Sh::Acc{};
     }
     __device__ __forceinline__ void scale(float f) {
         l *= f;
 #pragma unroll
-        for (int t = 0; t < D / 32; ++t) o[t] *= f;
+        for (int t = 0; t < NT; ++t) o[t] *= f;
     }
 };
 
@@ -356,51 +388,52 @@ __device__ __forceinline__ Limits limits_of(const Row& row, int ctx) {
     return x;
 }
 
-// The products s of a block's keys from c0 on to weights p; st.o scaled where their unit moves.
-template <int D, bool TREE, typename Tree>
+// The products s of a block's keys from c0 on become their weights; st.o is scaled where their unit moves.
+template <int D, int M, bool TREE, typename Tree>
 __device__ __forceinline__ void weigh(const PagedAttn& a, const Tree& tree, const Row& row, const Limits& lim, float slope,
-                                      const Cap& cap, int c0, int ctx, f32x16& s, State<D>& st, float (&p)[16]) {
-    const int h = (threadIdx.x >> 5) & 1;
+                                      const Cap& cap, int c0, int ctx, float (&s)[Shape<M>::NS], State<D, M>& st) {
+    constexpr int NS = Shape<M>::NS, STEP = Shape<M>::STEP;
+    const int g = (threadIdx.x & 63) / M;
     if (a.cap > 0.0f) {
         float most = 0.0f;
 #pragma unroll
-        for (int v = 0; v < 16; ++v) most = fmaxf(most, fabsf(s[v]));
+        for (int v = 0; v < NS; ++v) most = fmaxf(most, fabsf(s[v]));
         if (__ballot(!(most < 1.0f))) {
 #pragma unroll
-            for (int v = 0; v < 16; ++v) s[v] = capped(s[v], cap);
+            for (int v = 0; v < NS; ++v) s[v] = capped(s[v], cap);
         } else {
 #pragma unroll
-            for (int v = 0; v < 16; ++v) s[v] = capped_small(s[v], cap);
+            for (int v = 0; v < NS; ++v) s[v] = capped_small(s[v], cap);
         }
     }
     if (a.slopes) {
         if (TREE && c0 + 32 > ctx) {
             if constexpr (TREE) {
 #pragma unroll
-                for (int v = 0; v < 16; ++v) {
-                    const int j = c0 + 8 * (v >> 2) + 4 * h + (v & 3);
+                for (int v = 0; v < NS; ++v) {
+                    const int j = c0 + STEP * (v >> 2) + 4 * g + (v & 3);
                     const int at = j < ctx ? j : ctx + tree.depth[min(j - ctx, IE_TREE_MAX - 1)];
                     s[v] = fmaf(-slope, fabsf((float)(row.pos - at)), s[v]);
                 }
             }
         } else {
-            const int base = row.pos - c0 - 4 * h;
+            const int base = row.pos - c0 - 4 * g;
 #pragma unroll
-            for (int v = 0; v < 16; ++v) s[v] = fmaf(-slope, fabsf((float)(base - 8 * (v >> 2) - (v & 3))), s[v]);
+            for (int v = 0; v < NS; ++v) s[v] = fmaf(-slope, fabsf((float)(base - STEP * (v >> 2) - (v & 3))), s[v]);
         }
     }
     if (c0 < lim.all_lo || c0 + 32 > lim.all_hi) {
-        const uint32_t bits = seen_bits<TREE>(tree, row, c0, ctx) >> (4 * h);
+        const uint32_t bits = seen_bits<TREE>(tree, row, c0, ctx) >> (4 * g);
 #pragma unroll
-        for (int v = 0; v < 16; ++v)
-            if (!(bits >> (8 * (v >> 2) + (v & 3)) & 1)) s[v] = -INFINITY;
+        for (int v = 0; v < NS; ++v)
+            if (!(bits >> (STEP * (v >> 2) + (v & 3)) & 1)) s[v] = -INFINITY;
     }
     float top = s[0];
 #pragma unroll
-    for (int v = 1; v < 16; ++v) top = fmaxf(top, s[v]);
+    for (int v = 1; v < NS; ++v) top = fmaxf(top, s[v]);
     // The weights' unit m follows the largest score once that is 2^8 above it: up to there they only grow, and
     // fp32 holds them as well.  (With 32 rows a wave some row's largest grows in most blocks.)
-    top = max_xor32(top);
+    top = Shape<M>::rows_max(top);
     if (__ballot(top > st.m + 8.0f)) {
         const float mn = fmaxf(st.m, top);
         const float alpha = mn == -INFINITY ? 0.0f : exp2_sm(st.m - mn);
@@ -410,34 +443,36 @@ __device__ __forceinline__ void weigh(const PagedAttn& a, const Tree& tree, cons
     const float mu = st.m == -INFINITY ? 0.0f : st.m;  // no key yet: keep o, l at 0
     float sum = 0.0f;
 #pragma unroll
-    for (int v = 0; v < 16; ++v) {
-        p[v] = exp2_sm(s[v] - mu);
-        sum += p[v];
+    for (int v = 0; v < NS; ++v) {
+        s[v] = exp2_sm(s[v] - mu);
+        sum += s[v];
     }
     st.l += sum;
 }
 
-// A lane's share of its row of Q: channels 16 s + 8 h on.
-template <int D>
+// A lane's share of its row of Q: channels KC s + 8 g on.
+template <int D, int M>
 struct RawQuery {
-    float4 x[D / 16][2];
+    static constexpr int KS = D / Shape<M>::KC;
+    float4 x[KS][2];
 };
-template <int D>
-__device__ __forceinline__ RawQuery<D> load_query(const float* row, int h) {
-    RawQuery<D> r;
+template <int D, int M>
+__device__ __forceinline__ RawQuery<D, M> load_query(const float* row, int g) {
+    RawQuery<D, M> r;
 #pragma unroll
-    for (int s = 0; s < D / 16; ++s)
+    for (int s = 0; s < r.KS; ++s)
 #pragma unroll
-        for (int k = 0; k < 2; ++k) r.x[s][k] = *reinterpret_cast<const float4*>(row + 16 * s + 8 * h + 4 * k);
+        for (int k = 0; k < 2; ++k) r.x[s][k] = *reinterpret_cast<const float4*>(row + Shape<M>::KC * s + 8 * g + 4 * k);
     return r;
 }
 // Its parts, and whether one of the values has none that serve: one below 2^-98 once scaled, whose parts bf16 may
 // not hold, or one from 2^64 on.
-template <int D>
-__device__ __forceinline__ bool split_query(const float* row, const RawQuery<D>& r, float scale, Parts<3> (&q)[D / 16]) {
+template <int D, int M>
+__device__ __forceinline__ bool split_query(const float* row, const RawQuery<D, M>& r, float scale,
+                                            Parts<3> (&q)[RawQuery<D, M>::KS]) {
     float least = INFINITY, most = 0.0f;
 #pragma unroll
-    for (int s = 0; s < D / 16; ++s) {
+    for (int s = 0; s < r.KS; ++s) {
         float z[8] = {r.x[s][0].x, r.x[s][0].y, r.x[s][0].z, r.x[s][0].w, r.x[s][1].x, r.x[s][1].y, r.x[s][1].z, r.x[s][1].w};
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -460,18 +495,18 @@ __device__ __forceinline__ bool split_query(const float* row, const RawQuery<D>&
 
 // Results of a wave's rows: outputs, or with splits partial sums.  Rows whose result is not finite, or whose query
 // has no parts, again one by one over keys k0 .. k1 - 1.
-template <int D, typename KV, bool TREE, typename Tree>
+template <int D, int M, typename KV, bool TREE, typename Tree>
 __device__ __forceinline__ void finish(const PagedAttn& a, const Tree& tree, const Row& row, int b, int kvh, int ctx, int split,
-                                       int k0, int k1, bool q_bad, const State<D>& st, float l) {
-    constexpr int NT = D / 32;
-    const int lane = threadIdx.x & 63, i = lane & 31, h = lane >> 5;
+                                       int k0, int k1, bool q_bad, const State<D, M>& st, float l) {
+    constexpr int NT = D / M, AV = Shape<M>::AV;
+    const int lane = threadIdx.x & 63, i = lane & (M - 1), g = lane / M;
     float bad = l * 0.0f;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int v = 0; v < 16; ++v) bad = fmaf(st.o[t][v], 0.0f, bad);
+        for (int v = 0; v < AV; ++v) bad = fmaf(st.o[t][v], 0.0f, bad);
     const uint64_t lanes = __ballot(row.live && (q_bad || !(bad == 0.0f)));
-    uint32_t again = (uint32_t)lanes | (uint32_t)(lanes >> 32);
+    uint32_t again = Shape<M>::rows_of(lanes);
     const size_t rows = (size_t)a.B * a.P * a.H_q, mine = ((size_t)b * a.P + row.t) * a.H_q + row.head;
     if (row.live && !(again >> i & 1)) {
         float* out;
@@ -481,13 +516,13 @@ __device__ __forceinline__ void finish(const PagedAttn& a, const Tree& tree, con
             out = a.O + mine * D;
         } else {
             out = a.ws + (split * rows + mine) * D;
-            if (h == 0) *reinterpret_cast<float2*>(a.ws + a.splits * rows * D + 2 * (split * rows + mine)) = make_float2(st.m, l);
+            if (g == 0) *reinterpret_cast<float2*>(a.ws + a.splits * rows * D + 2 * (split * rows + mine)) = make_float2(st.m, l);
         }
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int v = 0; v < 4; ++v)
-                *reinterpret_cast<float4*>(out + 32 * t + 8 * v + 4 * h) =
+            for (int v = 0; v < AV / 4; ++v)
+                *reinterpret_cast<float4*>(out + M * t + 8 * v + 4 * g) =
                     make_float4(st.o[t][4 * v] * inv, st.o[t][4 * v + 1] * inv, st.o[t][4 * v + 2] * inv, st.o[t][4 * v + 3] * inv);
     }
 #pragma unroll 1
@@ -517,19 +552,19 @@ __device__ __forceinline__ void finish(const PagedAttn& a, const Tree& tree, con
 
 // Key groups' states through LDS into the first group's wave; `slot` numbers the others' and mine. Groups' waves
 // with rows in common call this together; false: the wave is done.
-template <int D, int OTHERS>
-__device__ __forceinline__ bool gather(int8_t* lds, int group, int per, int which, State<D>& st, float& l) {
-    constexpr int NT = D / 32;
+template <int D, int M, int OTHERS>
+__device__ __forceinline__ bool gather(int8_t* lds, int group, int per, int which, State<D, M>& st, float& l) {
+    constexpr int NT = D / M, Q = Shape<M>::AV / 4, PER_LANE = D * M / 64;
     const int lane = threadIdx.x & 63;
     float4* mo = reinterpret_cast<float4*>(lds);
-    float2* ml = reinterpret_cast<float2*>(lds + OTHERS * per * 64 * (D / 2) * 4);
+    float2* ml = reinterpret_cast<float2*>(lds + OTHERS * per * 64 * PER_LANE * 4);
     if (group > 0) {
         const int g = (group - 1) * per + which;
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int v = 0; v < 4; ++v)
-                mo[(g * NT * 4 + t * 4 + v) * 64 + lane] =
+            for (int v = 0; v < Q; ++v)
+                mo[((g * NT + t) * Q + v) * 64 + lane] =
                     make_float4(st.o[t][4 * v], st.o[t][4 * v + 1], st.o[t][4 * v + 2], st.o[t][4 * v + 3]);
         ml[g * 64 + lane] = make_float2(st.m, l);
     }
@@ -546,8 +581,8 @@ __device__ __forceinline__ bool gather(int8_t* lds, int group, int per, int whic
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                const float4 y = mo[(g * NT * 4 + t * 4 + v) * 64 + lane];
+            for (int v = 0; v < Q; ++v) {
+                const float4 y = mo[((g * NT + t) * Q + v) * 64 + lane];
                 st.o[t][4 * v] = st.o[t][4 * v] * fa + y.x * fb;
                 st.o[t][4 * v + 1] = st.o[t][4 * v + 1] * fa + y.y * fb;
                 st.o[t][4 * v + 2] = st.o[t][4 * v + 2] * fa + y.z * fb;
@@ -576,15 +611,15 @@ __device__ __forceinline__ Place place_of(const PagedAttn& a, int tiles) {
     return p;
 }
 
-// V's operand: tile t of keys k0 + 4 h .. and k0 + 8 + 4 h .. of a block's bf16 rows at `rows`.
-template <typename T>
+// V's operand, channels M t on: keys k0 + 4 g .. + 3, and as many 8 (M = 32) or 16 on, of a block's bf16 rows.
+template <typename T, int M>
 __device__ __forceinline__ uint4 read_v(const int8_t* rows, int k0, int t) {
-    // this lane's 8 bytes: keys 4 h + (lane % 16) / 4 on, channels 16 (lane / 16 % 2) + 4 (lane % 4) of the tile
-    const int lane = threadIdx.x & 63, key = 4 * (lane >> 5) + (lane & 15) / 4;
-    const int c = 2 * (lane >> 4 & 1) + (lane >> 1 & 1);
-    const int8_t* at = rows + key * T::ROW + 16 * ((4 * t + c) ^ T::vswz(key)) + 8 * (lane & 1) + k0 * T::ROW;
+    // this lane's 8 bytes: key 4 g + (lane % 16) / 4, channels 4 (lane % 4) on of its 16 lanes' 16
+    const int lane = threadIdx.x & 63, key = 4 * (lane / M) + (lane & 15) / 4;
+    const int c = (M == 32 ? 4 * t + 2 * (lane >> 4 & 1) : 2 * t) + (lane >> 1 & 1);
+    const int8_t* at = rows + key * T::ROW + 16 * (c ^ T::vswz(key)) + 8 * (lane & 1) + k0 * T::ROW;
     const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)at));
-    const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + 8 * T::ROW)));
+    const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + (M == 32 ? 8 : 16) * T::ROW)));
     return make_uint4(x.x, x.y, y.x, y.y);
 }
 
@@ -627,7 +662,7 @@ __global__ __launch_bounds__(256, NP == 1 && WR == 4 ? 2 : 1) void paged_tile_ke
     const int r = at.tile * 32 * WR + rw * 32 + i;
     // the query first: it waits for nothing
     const float* q_row = query_row<D>(a, r, b, kvh);
-    const RawQuery<D> raw_q = load_query<D>(q_row, h);
+    const RawQuery<D, 32> raw_q = load_query<D, 32>(q_row, h);
     if constexpr (TREE) grow_tree(tree, a.parents + (size_t)b * a.P, a.P, a.window);
     const Row row = row_of<TREE>(a, tree, r, b, kvh, at.start, at.len);
     const Limits lim = limits_of<TREE>(row, ctx);
@@ -718,8 +753,8 @@ __global__ __launch_bounds__(256, NP == 1 && WR == 4 ? 2 : 1) void paged_tile_ke
     const Scores sc = scores_of(a, row.head);
     const Cap cap = cap_of(a.cap);
     Parts<3> q[KS];
-    const bool q_bad = split_query<D>(q_row, raw_q, sc.q, q);
-    State<D> st;
+    const bool q_bad = split_query<D, 32>(q_row, raw_q, sc.q, q);
+    State<D, 32> st;
     st.clear();
 
     const int krow = i * T::ROW, kx = 16 * (h ^ T::kswz(i));  // chunk 2 s + h of key i
@@ -735,10 +770,11 @@ __global__ __launch_bounds__(256, NP == 1 && WR == 4 ? 2 : 1) void paged_tile_ke
             for (int n = 0; n < NP; ++n) x[0].p[n] = *reinterpret_cast<const uint4*>(kp + n * T::PART + krow + (kx ^ (32 * k)));
             product<NP, 1>(x, q[k], sa);
         }
-        f32x16& s = sa[0];
         __builtin_amdgcn_s_setprio(1);
         float p[16];
-        weigh<D, TREE>(a, tree, row, lim, sc.slope, cap, c0, ctx, s, st, p);
+#pragma unroll
+        for (int v = 0; v < 16; ++v) p[v] = sa[0][v];
+        weigh<D, 32, TREE>(a, tree, row, lim, sc.slope, cap, c0, ctx, p, st);
         __builtin_amdgcn_s_setprio(2);
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
@@ -749,7 +785,7 @@ __global__ __launch_bounds__(256, NP == 1 && WR == 4 ? 2 : 1) void paged_tile_ke
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
-                    for (int n = 0; n < NP; ++n) x[t].p[n] = read_v<T>(vp + n * T::PART, 16 * k, t0 + t);
+                    for (int n = 0; n < NP; ++n) x[t].p[n] = read_v<T, 32>(vp + n * T::PART, 16 * k, t0 + t);
                 product<NP, 2>(x, w, st.o + t0);
             }
         }
@@ -786,61 +822,68 @@ __global__ __launch_bounds__(256, NP == 1 && WR == 4 ? 2 : 1) void paged_tile_ke
     float l = sum_xor32(st.l);
     if constexpr (T::WK > 1) {
         __syncthreads();
-        if (!gather<D, T::WK - 1>(lds, kw, WR, rw, st, l)) return;
+        if (!gather<D, 32, T::WK - 1>(lds, kw, WR, rw, st, l)) return;
     }
-    finish<D, KV, TREE>(a, tree, row, b, kvh, ctx, at.split, k0, k1, q_bad, st, l);
+    finish<D, 32, KV, TREE>(a, tree, row, b, kvh, ctx, at.split, k0, k1, q_bad, st, l);
 }
 
 // ---- the kernel for at most 32 rows
-// Four waves, all of the same 32 rows, take the keys' blocks of 32 in turn, each by itself: its K and V come into LDS
+// Four or eight waves, all of the same 16 or 32 rows, take the keys' blocks of 32 in turn, each by itself: its K and V come into LDS
 // of its own as they lie in the cache, DEEP blocks ahead, so the loop has no barrier and a block's products
 // run beside the next ones' copies.  Of a bf16 cache K's and V's rows are operands as in the tile kernel; fp32 rows
 // are split as they are read, V's a channel a lane (32 lanes read 128 bytes).  A page's number comes the same way,
 // DEEP blocks ahead of its rows.
-template <int D, int NP>
+template <int D, int NP, int M>
 struct Few {
     static constexpr int ROW = D * (NP == 1 ? 2 : 4);  // bytes of a row
     static constexpr int PART = 32 * ROW;              // of a block's K or V
-    static constexpr int DEEP = PART > 8192 ? 1 : 2;
+    static constexpr int WAVES = M == 16 && PART <= 8192 ? 8 : 4;
+    static constexpr int DEEP = WAVES * 4 * PART > 128 * 1024 ? 1 : 2;
     static constexpr int WAVE = 2 * DEEP * PART;
     static constexpr int COPIES = PART / 1024;         // a wave's copies of K or V
-    static constexpr int MERGE = 3 * 64 * (D / 2 + 2) * 4;
-    static constexpr int LDS = 4 * WAVE;
+    static constexpr int MERGE = (WAVES - 1) * 64 * (D * M / 64 + 2) * 4;
+    static constexpr int LDS = WAVES * WAVE;
     static constexpr int CH = ROW / 16;
     static_assert(LDS >= MERGE && 3 * COPIES + 2 < 63, "a wave's ring");
-    // As Tile's; fp32 rows' chunks of four values, of which K's operand takes two.
+    // As Tile's; fp32 rows' chunks of four values, of which K's operand takes two; 16 rows' V is read eight keys at a
+    // time at two chunks.
     __device__ static __forceinline__ int kswz(int r) {
         return NP == 3 ? (r & 7) << 1 : D == 128 ? r & 15 : (r >> 1) & 7;
     }
-    __device__ static __forceinline__ int vswz(int r) { return NP == 3 ? 0 : D == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1); }
+    __device__ static __forceinline__ int vswz(int r) {
+        if (NP == 3) return 0;
+        if (M == 16) return D == 128 ? 2 * (r & 7) : 2 * ((r >> 1) & 3);
+        return D == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1);
+    }
 };
 
-template <int D, int NP, bool TREE>
-__global__ __launch_bounds__(256, 1) void paged_few_kernel(PagedAttn a, int tiles) {
-    using T = Few<D, NP>;
+template <int D, int NP, int M, bool TREE>
+__global__ __launch_bounds__((64 * Few<D, NP, M>::WAVES), (Few<D, NP, M>::WAVES / 4)) void paged_few_kernel(PagedAttn a, int tiles) {
+    using T = Few<D, NP, M>;
+    using Sh = Shape<M>;
     using KV = std::conditional_t<NP == 1, uint16_t, float>;
     using Tree = std::conditional_t<TREE, TreeLds, NoTree>;
-    constexpr int NT = D / 32, KS = D / 16, DEEP = T::DEEP, C = T::COPIES;
+    constexpr int NT = D / M, KS = D / Sh::KC, DEEP = T::DEEP, C = T::COPIES, W = T::WAVES;
     __shared__ __attribute__((aligned(1024))) int8_t lds_all[T::LDS];
-    __shared__ __attribute__((aligned(256))) int pages_all[4][2 * DEEP][64];  // pages of a block's keys
-    __shared__ uint32_t slots_all[4][32];
+    __shared__ __attribute__((aligned(256))) int pages_all[W][2 * DEEP][64];  // pages of a block's keys
+    __shared__ uint32_t slots_all[W][32];
     __shared__ Tree tree;
-    const int lane = threadIdx.x & 63, i = lane & 31, h = lane >> 5;
+    const int lane = threadIdx.x & 63, i = lane & (M - 1), g = lane / M;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Place at = place_of<TREE>(a, tiles);
     const int b = at.b, kvh = at.kvh, ctx = at.start;
-    const int r = at.tile * 32 + i;
+    const int r = at.tile * M + i;
     const float* q_row = query_row<D>(a, r, b, kvh);
-    RawQuery<D> raw_q = load_query<D>(q_row, h);
+    RawQuery<D, M> raw_q = load_query<D, M>(q_row, g);
     if constexpr (TREE) grow_tree(tree, a.parents + (size_t)b * a.P, a.P, a.window);
     const Row row = row_of<TREE>(a, tree, r, b, kvh, at.start, at.len);
     const Limits lim = limits_of<TREE>(row, ctx);
     const int kbeg = min(lim.lo, lim.hi), kend = lim.hi;
-    // this split's blocks, and this wave's: numbers wave, wave + 4, ...
+    // this split's blocks, and this wave's: numbers wave, wave + W, ...
     const int all = (kend - kbeg + 127) / 128, per = (all + a.splits - 1) / a.splits;
     const int s0 = min(at.split * per, all), s1 = min(s0 + per, all);
     const int k0 = kbeg + s0 * 128, k1 = min(kbeg + s1 * 128, kend);
-    const int n = ((k1 - k0 + 31) / 32 - wave + 3) / 4;
+    const int n = ((k1 - k0 + 31) / 32 - wave + W - 1) / W;
 
     const int* table = a.pages.table + (size_t)b * a.pages.nbps;
     const size_t row_bytes = (size_t)a.H_kv * D * sizeof(KV);
@@ -850,8 +893,8 @@ __global__ __launch_bounds__(256, 1) void paged_few_kernel(PagedAttn a, int tile
     const uint32_t lds_at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_i8)lds);
     const uint32_t pages_at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_i8)(int8_t*)pages_all[wave]);
     uint32_t* const slots = slots_all[wave];
-    auto first = [&](int j) { return k0 + 32 * (4 * j + wave); };           // key of block j
-    auto pos_of = [&](int j) { return min(first(j) + i, k1 - 1); };         // of this lane's key
+    auto first = [&](int j) { return k0 + 32 * (W * j + wave); };           // key of block j
+    auto pos_of = [&](int j) { return min(first(j) + (lane & 31), k1 - 1); };  // of this lane's key
     auto ask_pages = [&](int j) { copy4(table + page_of(a.pages, pos_of(j)), pages_at + (j & (2 * DEEP - 1)) * 256); };
     constexpr int RPC = 1024 / T::ROW;  // rows of a copy
     const int lane_row = lane / T::CH;
@@ -862,8 +905,8 @@ __global__ __launch_bounds__(256, 1) void paged_few_kernel(PagedAttn a, int tile
     // K of block j (its pages have come), and the pages of block j + DEEP
     auto ask_k = [&](int j) {
         const int p = pos_of(j), in = page_of(a.pages, p);
-        const uint32_t page = (uint32_t)pages_all[wave][j & (2 * DEEP - 1)][i];
-        slots[i] = page * (uint32_t)a.pages.block + (uint32_t)(p - in * a.pages.block);
+        const uint32_t page = (uint32_t)pages_all[wave][j & (2 * DEEP - 1)][lane & 31];
+        slots[lane & 31] = page * (uint32_t)a.pages.block + (uint32_t)(p - in * a.pages.block);
         ask_pages(j + DEEP);
         reads_done();
 #pragma unroll
@@ -902,8 +945,8 @@ __global__ __launch_bounds__(256, 1) void paged_few_kernel(PagedAttn a, int tile
         }
     }
     Parts<3> q[KS];
-    const bool q_bad = split_query<D>(q_row, raw_q, sc.q, q);
-    State<D> st;
+    const bool q_bad = split_query<D, M>(q_row, raw_q, sc.q, q);
+    State<D, M> st;
     st.clear();
 
 #pragma unroll 1
@@ -914,31 +957,37 @@ __global__ __launch_bounds__(256, 1) void paged_few_kernel(PagedAttn a, int tile
         const int c0 = first(j);
         const int8_t* kp = lds + (j & (DEEP - 1)) * T::PART;
         const int8_t* vp = lds + (DEEP + (j & (DEEP - 1))) * T::PART;
-        f32x16 sa[1] = {};
+        typename Sh::Acc sa[Sh::TILES] = {};
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
-            Parts<NP> x[1];
-            if constexpr (NP == 1) {
-                x[0].p[0] = *reinterpret_cast<const uint4*>(kp + i * T::ROW + 16 * ((2 * k + h) ^ T::kswz(i)));
-            } else {
-                float y[8];
-                const float4 u = *reinterpret_cast<const float4*>(kp + i * T::ROW + 16 * ((4 * k + 2 * h) ^ T::kswz(i)));
-                const float4 w = *reinterpret_cast<const float4*>(kp + i * T::ROW + 16 * ((4 * k + 2 * h + 1) ^ T::kswz(i)));
-                y[0] = u.x, y[1] = u.y, y[2] = u.z, y[3] = u.w, y[4] = w.x, y[5] = w.y, y[6] = w.z, y[7] = w.w;
-                x[0] = split8(y);
+            Parts<NP> x[Sh::TILES];
+#pragma unroll
+            for (int t = 0; t < Sh::TILES; ++t) {
+                const int key = M * t + i;
+                if constexpr (NP == 1) {
+                    x[t].p[0] = *reinterpret_cast<const uint4*>(kp + key * T::ROW + 16 * ((Sh::KC / 8 * k + g) ^ T::kswz(key)));
+                } else {
+                    const int c = (Sh::KC / 4 * k + 2 * g) ^ T::kswz(key);
+                    const float4 u = *reinterpret_cast<const float4*>(kp + key * T::ROW + 16 * c);
+                    const float4 w = *reinterpret_cast<const float4*>(kp + key * T::ROW + 16 * (c + 1));
+                    const float y[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
+                    x[t] = split8(y);
+                }
             }
-            product<NP, 1>(x, q[k], sa);
+            product<NP, Sh::TILES>(x, q[k], sa);
         }
         if (j + DEEP < n) ask_k(j + DEEP);
-        float p[16];
-        weigh<D, TREE>(a, tree, row, lim, slope, cap, c0, ctx, sa[0], st, p);
+        float p[Sh::NS];
+#pragma unroll
+        for (int v = 0; v < Sh::NS; ++v) p[v] = sa[v / Sh::AV][v % Sh::AV];
+        weigh<D, M, TREE>(a, tree, row, lim, slope, cap, c0, ctx, p, st);
         // V of block j: behind it came K of j + DEEP and the pages behind that, and with two blocks under way the
         // same and V of j + 1
         if (j + DEEP < n) copies_left<DEEP == 2 ? 3 * C + 2 : C + 1>();
         else if (DEEP == 2 && j + 1 < n) copies_left<2 * C + 1>();
         else copies_left<0>();
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
+        for (int k = 0; k < Sh::NS / 8; ++k) {
             const Parts<3> w = split8(p + 8 * k);
 #pragma unroll
             for (int t0 = 0; t0 < NT; t0 += 2) {
@@ -946,13 +995,13 @@ __global__ __launch_bounds__(256, 1) void paged_few_kernel(PagedAttn a, int tile
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
                     if constexpr (NP == 1) {
-                        x[t].p[0] = read_v<T>(vp, 16 * k, t0 + t);
+                        x[t].p[0] = read_v<T, M>(vp, 16 * k, t0 + t);
                     } else {
                         float y[8];
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
-                            y[e] = *reinterpret_cast<const float*>(vp + (16 * k + 4 * h + (e & 3) + 8 * (e >> 2)) * T::ROW +
-                                                                   128 * (t0 + t) + 4 * i);
+                            y[e] = *reinterpret_cast<const float*>(vp + (16 * k + 4 * g + (e & 3) + Sh::STEP * (e >> 2)) * T::ROW +
+                                                                   4 * (M * (t0 + t) + i));
                         x[t] = split8(y);
                     }
                 }
@@ -961,11 +1010,11 @@ __global__ __launch_bounds__(256, 1) void paged_few_kernel(PagedAttn a, int tile
         }
         if (j + DEEP < n) ask_v(j + DEEP);
     }
-    float l = sum_xor32(st.l);
+    float l = Sh::rows_sum(st.l);
     copies_left<0>();
     __syncthreads();
-    if (!gather<D, 3>(lds_all, wave, 1, 0, st, l)) return;
-    finish<D, KV, TREE>(a, tree, row, b, kvh, ctx, at.split, k0, k1, q_bad, st, l);
+    if (!gather<D, M, W - 1>(lds_all, wave, 1, 0, st, l)) return;
+    finish<D, M, KV, TREE>(a, tree, row, b, kvh, ctx, at.split, k0, k1, q_bad, st, l);
 }
 
 // ---- the kernel for up to four rows: vector units
@@ -1306,7 +1355,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn a) {
     reinterpret_cast<float4*>(a.O + r * D)[c] = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
-// Rows of a tile: up to 4 are paged_row_kernel's, 32 paged_few_kernel's, 64 and 128 paged_tile_kernel's.
+// Rows of a tile: up to 4 are paged_row_kernel's, 16 and 32 paged_few_kernel's, 64 and 128 paged_tile_kernel's.
 // Row against few kernel (us, 8 KV heads, one sequence of 2000 keys; 32 of 4000): fp32 d 64 one row 15.8 and
 // 45.5; 92 and 101, four 30.8 and 45.6; 99 and 102, eight 53.7 and 45.6; 118 and 103, d 128 four 63.7 and 77.6; 193 and
 // 190; bf16 d 64 two 15.3 and 26.1; 48.9 and 49.0, four 23.8 and 26.2; 54.4 and 49.2, d 128 two 25.8 and 38.7; 96.5 and
@@ -1314,7 +1363,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn a) {
 int tile_rows(int P, int G, int kv_dtype) {
     const long long rows = (long long)P * G;
     if (rows <= (kv_dtype == IE_KV_BF16 ? 2 : 4)) return rows <= 2 ? (int)rows : 4;
-    return rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+    return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
 }
 
 template <int D, int NP, int ROWS, bool TREE>
@@ -1323,7 +1372,7 @@ void launch_tile(const PagedAttn& a, hipStream_t s) {
     const unsigned grid = (unsigned)((long long)a.B * a.H_kv * tiles * a.splits);
     using KV = std::conditional_t<NP == 1, uint16_t, float>;
     if constexpr (ROWS <= 4) paged_row_kernel<D, KV, ROWS, TREE><<<grid, 64 * kRowWaves, 0, s>>>(a, tiles);
-    else if constexpr (ROWS == 32) paged_few_kernel<D, NP, TREE><<<grid, 256, 0, s>>>(a, tiles);
+    else if constexpr (ROWS <= 32) paged_few_kernel<D, NP, ROWS, TREE><<<grid, 64 * Few<D, NP, ROWS>::WAVES, 0, s>>>(a, tiles);
     else paged_tile_kernel<D, NP, ROWS / 32, TREE><<<grid, 256, 0, s>>>(a, tiles);
 }
 
@@ -1334,6 +1383,7 @@ void launch_rows(const PagedAttn& a, hipStream_t s) {
         case 2: return launch_tile<D, NP, 2, TREE>(a, s);
         case 4:
             if constexpr (NP == 3) return launch_tile<D, NP, 4, TREE>(a, s);
+        case 16: return launch_tile<D, NP, 16, TREE>(a, s);
         case 32: return launch_tile<D, NP, 32, TREE>(a, s);
         case 64: return launch_tile<D, NP, 64, TREE>(a, s);
         default: return launch_tile<D, NP, 128, TREE>(a, s);
