@@ -593,7 +593,9 @@ __device__ __forceinline__ bool gather(int8_t* lds, int group, int per, int whic
 }
 
 // Which of the grid's workgroups this is: pair (sequence, KV head) u % pairs, so that a pair's tiles run on one
-// XCD where pairs are a multiple of 8; then the tile, the last (a prompt's longest) first, then the split.
+// XCD where pairs are a multiple of 8; then the tile, the last (a prompt's longest) first, then the split.  Up to 64
+// sequences come by length, the longest first, so that what starts last is short (32 x 8 x 4 x 128 over 4096 to 8192 keys
+// XXX).
 struct Place {
     int b, kvh, tile, split, start, len;
 };
@@ -606,6 +608,16 @@ __device__ __forceinline__ Place place_of(const PagedAttn& a, int tiles) {
     p.tile = tiles - 1 - (u - p.split * tiles);
     p.b = pair / a.H_kv;
     p.kvh = pair - p.b * a.H_kv;
+    if (a.B > 1 && a.B <= 64) {
+        const int k = threadIdx.x & 63;
+        const int len = k < a.B ? a.starts[k] : -0x7fffffff;
+        int rank = 0;
+        for (int j = 0; j < a.B; ++j) {
+            const int other = __builtin_amdgcn_readlane(len, j);
+            rank += other > len || (other == len && j < k);
+        }
+        p.b = __builtin_ctzll(__ballot(k < a.B && rank == p.b));
+    }
     p.start = min(max(a.starts[p.b], 0), TREE ? a.max_ctx : 1 << 30);
     p.len = a.lens ? min(a.lens[p.b], a.P) : a.P;
     return p;
@@ -1017,7 +1029,7 @@ __global__ __launch_bounds__((64 * Few<D, NP, M>::WAVES), (Few<D, NP, M>::WAVES 
     finish<D, M, KV, TREE>(a, tree, row, b, kvh, ctx, at.split, k0, k1, q_bad, st, l);
 }
 
-// ---- the kernel for up to four rows: vector units
+// ---- the kernel for one row, or two of an fp32 cache: vector units
 // At so few rows a matrix tile of 32 is mostly empty and its softmax costs as much as a full one's.  Here eight waves
 // take the keys' batches in turn, in fp32 as they are: LPK lanes hold a key's row, 16 bytes each, so a copy
 // brings KPI whole rows; a score is a lane's products summed over its LPK lanes, which then have the key's weight for
@@ -1355,14 +1367,14 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn a) {
     reinterpret_cast<float4*>(a.O + r * D)[c] = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
-// Rows of a tile: up to 4 are paged_row_kernel's, 16 and 32 paged_few_kernel's, 64 and 128 paged_tile_kernel's.
-// Row against few kernel (us, 8 KV heads, one sequence of 2000 keys; 32 of 4000): fp32 d 64 one row 15.8 and
-// 45.5; 92 and 101, four 30.8 and 45.6; 99 and 102, eight 53.7 and 45.6; 118 and 103, d 128 four 63.7 and 77.6; 193 and
-// 190; bf16 d 64 two 15.3 and 26.1; 48.9 and 49.0, four 23.8 and 26.2; 54.4 and 49.2, d 128 two 25.8 and 38.7; 96.5 and
-// 98.8, four 40.2 and 38.8; 103 and 99.
+// Rows of a tile: up to 2 are paged_row_kernel's, 16 and 32 paged_few_kernel's, 64 and 128 paged_tile_kernel's.
+// Row against few kernel (us, 8 KV heads, one sequence of 2000 keys; 32 of 4000): fp32 d 64 one row 15.8 and 26.9;
+// 92.2 and 96.7, two 20.9 and 26.8; 94.4 and 96.7, four 30.8 and 27.0; 98.9 and 96.4, d 128 two 41.7 and 65.6; 185 and
+// 186, four 63.7 and 65.6; 192 and 186; bf16 d 64 one 11.4 and 14.3; 46.1 and 47.7, two 15.3 and 14.3; 49.0 and 47.9, d 128
+// one 19.5 and 19.6; 93.3 and 94.0, two 25.7 and 19.8; 96.3 and 94.1.
 int tile_rows(int P, int G, int kv_dtype) {
     const long long rows = (long long)P * G;
-    if (rows <= (kv_dtype == IE_KV_BF16 ? 2 : 4)) return rows <= 2 ? (int)rows : 4;
+    if (rows <= (kv_dtype == IE_KV_BF16 ? 1 : 2)) return (int)rows;
     return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
 }
 
@@ -1371,7 +1383,7 @@ void launch_tile(const PagedAttn& a, hipStream_t s) {
     const int G = a.H_q / a.H_kv, tiles = (int)(((long long)a.P * G + ROWS - 1) / ROWS);
     const unsigned grid = (unsigned)((long long)a.B * a.H_kv * tiles * a.splits);
     using KV = std::conditional_t<NP == 1, uint16_t, float>;
-    if constexpr (ROWS <= 4) paged_row_kernel<D, KV, ROWS, TREE><<<grid, 64 * kRowWaves, 0, s>>>(a, tiles);
+    if constexpr (ROWS <= 2) paged_row_kernel<D, KV, ROWS, TREE><<<grid, 64 * kRowWaves, 0, s>>>(a, tiles);
     else if constexpr (ROWS <= 32) paged_few_kernel<D, NP, ROWS, TREE><<<grid, 64 * Few<D, NP, ROWS>::WAVES, 0, s>>>(a, tiles);
     else paged_tile_kernel<D, NP, ROWS / 32, TREE><<<grid, 256, 0, s>>>(a, tiles);
 }
@@ -1380,9 +1392,8 @@ template <int D, int NP, bool TREE>
 void launch_rows(const PagedAttn& a, hipStream_t s) {
     switch (tile_rows(a.P, a.H_q / a.H_kv, a.kv_dtype)) {
         case 1: return launch_tile<D, NP, 1, TREE>(a, s);
-        case 2: return launch_tile<D, NP, 2, TREE>(a, s);
-        case 4:
-            if constexpr (NP == 3) return launch_tile<D, NP, 4, TREE>(a, s);
+        case 2:
+            if constexpr (NP == 3) return launch_tile<D, NP, 2, TREE>(a, s);
         case 16: return launch_tile<D, NP, 16, TREE>(a, s);
         case 32: return launch_tile<D, NP, 32, TREE>(a, s);
         case 64: return launch_tile<D, NP, 64, TREE>(a, s);
