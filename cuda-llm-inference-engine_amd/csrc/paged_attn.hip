@@ -12,6 +12,7 @@
 // each 16, read transposed from V's rows (ds_read_b64_tr_b16).  A bf16 cache is one
 // part and takes three products, an fp32 cache six of the nine (the rest are below
 // 2^-24).  Statistics and outputs are fp32.
+#include <cmath>
 #include <type_traits>
 
 #include "device_util.h"
@@ -594,8 +595,8 @@ __device__ __forceinline__ bool gather(int8_t* lds, int group, int per, int whic
 
 // Which of the grid's workgroups this is: pair (sequence, KV head) u % pairs, so that a pair's tiles run on one
 // XCD where pairs are a multiple of 8; then the tile, the last (a prompt's longest) first, then the split.  Up to 64
-// sequences come by length, the longest first, so that what starts last is short (32 x 8 x 4 x 128 over 4096 to 8192 keys
-// XXX).
+// sequences come by length, the longest first, so that what starts last is short (32 x 8 x 4 x 128 over 4096 to 8192 keys in
+// two splits 154 us, unsorted 177).
 struct Place {
     int b, kvh, tile, split, start, len;
 };
@@ -1337,45 +1338,124 @@ __global__ __launch_bounds__(64 * kRowWaves, 2) void paged_row_kernel(PagedAttn 
     }
 }
 
-// O rows from their splits' partials, D / 4 lanes a row.
-template <int D>
+// O rows from their splits' partials: D / 4 lanes a row, SG times, each of which has every SG-th split; four splits'
+// loads are under way at once, and with SG = 8 (more than four splits) the eight's sums meet in LDS (one sequence of
+// 16000 keys, 8 x 4 x 128 in 16 splits: 31.0 us in all with a row's splits one after another, 20.3 so).
+template <int D, int SG>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn a) {
-    constexpr int L = D / 4;
+    constexpr int L = D / 4, PER = 256 / (L * SG);
     const size_t rows = (size_t)a.B * a.P * a.H_q;
-    const size_t r = (size_t)blockIdx.x * (256 / L) + threadIdx.x / L;
-    if (r >= rows) return;
-    if (a.lens && (int)(r / a.H_q % a.P) >= a.lens[r / a.H_q / a.P]) return;
+    const int c = threadIdx.x % L, sg = threadIdx.x / L % SG, local = threadIdx.x / (L * SG);
+    const size_t r = (size_t)blockIdx.x * PER + local;
+    const bool live = r < rows && !(a.lens && (int)(r / a.H_q % a.P) >= a.lens[r / a.H_q / a.P]);
     const float2* ml = reinterpret_cast<const float2*>(a.ws + a.splits * rows * D);
-    float m = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, ml[s * rows + r].x);
-    const float mu = m == -INFINITY ? 0.0f : m;
+    float m = -INFINITY, l = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float l = 0.0f;
-    const int c = threadIdx.x % L;
-    for (int s = 0; s < a.splits; ++s) {
-        const float2 x = ml[s * rows + r];
-        if (x.y == 0.0f) continue;
-        const float f = exp2_sm(x.x - mu);
-        const float4 y = reinterpret_cast<const float4*>(a.ws + (s * rows + r) * D)[c];
-        l = fmaf(f, x.y, l);
-        o.x = fmaf(f, y.x, o.x);
-        o.y = fmaf(f, y.y, o.y);
-        o.z = fmaf(f, y.z, o.z);
-        o.w = fmaf(f, y.w, o.w);
+    auto add = [&](float xm, float xl, float4 y) {  // (an empty part has xm = -inf, xl = 0 and no y)
+        const float mn = fmaxf(m, xm), mu = mn == -INFINITY ? 0.0f : mn;
+        const float fa = exp2_sm(m - mu), fb = exp2_sm(xm - mu);
+        m = mn;
+        l = l * fa + xl * fb;
+        o.x = o.x * fa + y.x * fb;
+        o.y = o.y * fa + y.y * fb;
+        o.z = o.z * fa + y.z * fb;
+        o.w = o.w * fa + y.w * fb;
+    };
+    if (live) {
+        for (int s0 = sg; s0 < a.splits; s0 += 4 * SG) {
+            float2 x[4];
+            float4 y[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int s = s0 + k * SG;
+                x[k] = make_float2(-INFINITY, 0.0f);
+                y[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (s < a.splits) {
+                    x[k] = ml[s * rows + r];
+                    y[k] = reinterpret_cast<const float4*>(a.ws + (s * rows + r) * D)[c];
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) add(x[k].x, x[k].y, y[k]);
+        }
     }
+    if constexpr (SG > 1) {
+        __shared__ float4 so[256];
+        __shared__ float2 sm[256];
+        so[threadIdx.x] = o;
+        sm[threadIdx.x] = make_float2(m, l);
+        __syncthreads();
+        if (sg > 0) return;
+#pragma unroll
+        for (int k = 1; k < SG; ++k) {
+            const float2 x = sm[threadIdx.x + k * L];
+            add(x.x, x.y, so[threadIdx.x + k * L]);
+        }
+    }
+    if (!live) return;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     reinterpret_cast<float4*>(a.O + r * D)[c] = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
-// Rows of a tile: up to 2 are paged_row_kernel's, 16 and 32 paged_few_kernel's, 64 and 128 paged_tile_kernel's.
-// Row against few kernel (us, 8 KV heads, one sequence of 2000 keys; 32 of 4000): fp32 d 64 one row 15.8 and 26.9;
-// 92.2 and 96.7, two 20.9 and 26.8; 94.4 and 96.7, four 30.8 and 27.0; 98.9 and 96.4, d 128 two 41.7 and 65.6; 185 and
-// 186, four 63.7 and 65.6; 192 and 186; bf16 d 64 one 11.4 and 14.3; 46.1 and 47.7, two 15.3 and 14.3; 49.0 and 47.9, d 128
-// one 19.5 and 19.6; 93.3 and 94.0, two 25.7 and 19.8; 96.3 and 94.1.
-int tile_rows(int P, int G, int kv_dtype) {
-    const long long rows = (long long)P * G;
-    if (rows <= (kv_dtype == IE_KV_BF16 ? 1 : 2)) return (int)rows;
-    return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+// Which kernel, and how many splits: the least estimated time.  A form has tiles of 1 or 2 rows (paged_row_kernel),
+// 16 or 32 (paged_few_kernel), 64 or 128 (paged_tile_kernel); a workgroup of it takes `start` us and `rate` us for every
+// 1000 keys, measured with 8 workgroups on the card (8 KV heads over 512 and 2560 keys), `loaded` with one or two on every
+// CU (32 and 64 sequences; the smallest forms, whose keys come from HBM then: prompts of 1000 tokens).
+struct Form {
+    int rows;
+    float start, rate, loaded;
+};
+constexpr int kForms = 4;
+constexpr Form kTiles[2][2][kForms] = {
+    {{{16, 5.7f, 10.5f, 12.0f}, {32, 5.8f, 19.9f, 22.0f}, {64, 5.2f, 36.1f, 39.5f}, {128, 5.8f, 53.0f, 53.0f}},      // fp32, d 64
+     {{16, 5.7f, 29.3f, 33.0f}, {32, 8.4f, 34.3f, 40.0f}, {64, 8.2f, 62.2f, 76.0f}, {128, 7.9f, 104.0f, 112.0f}}},  // d 128
+    {{{16, 5.7f, 4.4f, 5.5f}, {32, 5.9f, 9.8f, 10.2f}, {64, 5.9f, 18.3f, 18.6f}, {128, 5.7f, 27.0f, 27.0f}},         // bf16, d 64
+     {{16, 7.5f, 6.6f, 8.8f}, {32, 8.8f, 15.5f, 18.0f}, {64, 8.1f, 25.4f, 32.3f}, {128, 7.9f, 42.0f, 45.0f}}}};     // d 128
+// One row, and two of an fp32 cache, have no other form (us, 8 KV heads, one sequence of 2000 keys; 32 of 4000; against 16
+// rows'): fp32 d 64 one 15.8 and 26.9; 92.2 and 96.7, two 20.9 and 26.8; 94.4 and 96.7, four 30.8 and 27.0; 98.9 and
+// 96.4, d 128 two 41.7 and 65.6; 185 and 186, four 63.7 and 65.6; 192 and 186; bf16 d 64 one 11.4 and 14.3; 46.1 and
+// 47.7, two 15.3 and 14.3; 49.0 and 47.9, d 128 one 19.5 and 19.6; 93.3 and 94.0, two 25.7 and 19.8; 96.3 and 94.1.
+constexpr Form kRows[2][2][2] = {{{{1, 4.7f, 5.6f, 5.6f}, {2, 5.5f, 7.8f, 7.8f}}, {{1, 4.7f, 13.8f, 13.8f}, {2, 5.5f, 18.5f, 18.5f}}},
+                                 {{{1, 4.7f, 3.3f, 3.3f}, {}}, {{1, 4.7f, 7.3f, 7.3f}, {}}}};
+
+struct Plan {
+    int rows, splits;
+};
+// asked > 0: the best form for that many splits (clamped); else the best of both.
+Plan plan_of(int B, int P, int H_q, int H_kv, int d, int kv_dtype, int max_keys, int window, int asked) {
+    const int half = kv_dtype == IE_KV_BF16, wide = d == 128;
+    const double rows = (double)P * (H_q / H_kv), pairs = (double)B * H_kv;
+    const double walked = window && (long long)window + P < max_keys ? (double)window + P : max_keys;
+    const int stages = (int)((walked + 127) / 128), most = stages < IE_PAGED_MAX_SPLITS ? stages : IE_PAGED_MAX_SPLITS;
+    const bool few = rows <= (half ? 1 : 2);
+    const Form* forms = few ? &kRows[half][wide][(int)rows - 1] : kTiles[half][wide];
+    Plan best{forms[0].rows, 1};
+    double least = INFINITY;
+    for (int f = 0; f < (few ? 1 : kForms); ++f) {
+        const Form& x = forms[f];
+        const double tiles = (double)(((long long)rows + x.rows - 1) / x.rows), groups = tiles * pairs;
+        for (int s = asked > 0 ? asked : 1; s <= (asked > 0 ? asked : most); ++s) {
+            const int n = s < 1 ? 1 : s > most ? (most < 1 ? 1 : most) : s;
+            const double a_cu = groups * n / 256;
+            // 1000 keys of a workgroup where all CUs read their own from HBM (5.5 TB/s); tiles of a pair share theirs
+            const double memory = 1000.0 * 2 * d * (half ? 2 : 4) / (5.5e6 / 256) / tiles * (a_cu < 1 ? a_cu : 1);
+            const double own = a_cu < 0.5 ? x.rate : x.loaded, rate = (own > memory ? own : memory) / 1000 / n;
+            // Workgroups of like length come in whole rounds; a causal prompt's tiles see half of its own keys on average.
+            // A batch's sequences are taken to hold four fifths of the longest's keys.
+            const bool alike = walked >= 2.0 * P;
+            const double seen = (alike ? walked - (P - 1) / 2.0 : walked > P ? walked - P / 2.0 : walked / 2) * (B > 1 ? 0.8 : 1);
+            const double rounds = a_cu <= 1 ? a_cu : alike ? std::ceil(a_cu) : a_cu + 0.6;
+            const double start = x.rows >= 64 ? 0.6 * x.start : x.start;  // (several of those share a CU)
+            const double longest = x.start + walked * rate, work = rounds * (start + seen * rate);
+            double t = longest > work ? longest : work;
+            if (n > 1) t += 5 + rows * pairs * n * (d + 2) * 8 / 4e6;  // the join: a launch, partial results out and back
+            if (t < least) {
+                least = t;
+                best = {x.rows, n};
+            }
+        }
+    }
+    return best;
 }
 
 template <int D, int NP, int ROWS, bool TREE>
@@ -1390,7 +1470,8 @@ void launch_tile(const PagedAttn& a, hipStream_t s) {
 
 template <int D, int NP, bool TREE>
 void launch_rows(const PagedAttn& a, hipStream_t s) {
-    switch (tile_rows(a.P, a.H_q / a.H_kv, a.kv_dtype)) {
+    const int keys = a.parents ? a.max_ctx + a.P : a.max_ctx;
+    switch (plan_of(a.B, a.P, a.H_q, a.H_kv, a.d, a.kv_dtype, keys, a.window, a.splits).rows) {
         case 1: return launch_tile<D, NP, 1, TREE>(a, s);
         case 2:
             if constexpr (NP == 3) return launch_tile<D, NP, 2, TREE>(a, s);
@@ -1413,25 +1494,16 @@ void launch_d(const PagedAttn& a, hipStream_t s) {
     else launch_np<D, 3>(a, s);
     if (a.splits > 1) {
         const long long rows = (long long)a.B * a.P * a.H_q;
-        paged_merge_kernel<D><<<(unsigned)((rows * (D / 4) + 255) / 256), 256, 0, s>>>(a);
+        constexpr int per = 256 / (D / 4);  // rows of a workgroup, or an eighth of them
+        if (a.splits <= 4) paged_merge_kernel<D, 1><<<(unsigned)((rows + per - 1) / per), 256, 0, s>>>(a);
+        else paged_merge_kernel<D, 8><<<(unsigned)((rows * 8 + per - 1) / per), 256, 0, s>>>(a);
     }
 }
 
 }  // namespace
 
-int paged_attn_splits(int B, int P, int H_q, int H_kv, int, int kv_dtype, int max_keys, int window, int asked) {
-    const int G = H_q / H_kv, rows = tile_rows(P, G, kv_dtype);
-    const long long walked = window && (long long)window + P < max_keys ? (long long)window + P : max_keys;
-    const int stages = (int)((walked + 127) / 128);
-    int s = asked;
-    if (s <= 0) {
-        const long long groups = (long long)B * H_kv * (((long long)P * G + rows - 1) / rows);
-        s = (int)((rows <= 32 ? 256 : 512) / groups);
-        s = s < 1 ? 1 : s > stages / 2 ? stages / 2 : s;
-        if (s < 1) s = 1;
-    }
-    if (s > IE_PAGED_MAX_SPLITS) s = IE_PAGED_MAX_SPLITS;
-    return s < stages ? s : stages;
+int paged_attn_splits(int B, int P, int H_q, int H_kv, int d, int kv_dtype, int max_keys, int window, int asked) {
+    return plan_of(B, P, H_q, H_kv, d, kv_dtype, max_keys, window, asked).splits;
 }
 
 void launch_paged_attn(const PagedAttn& a, hipStream_t s) {
