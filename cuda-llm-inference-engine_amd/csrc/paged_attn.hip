@@ -148,10 +148,10 @@ __device__ __forceinline__ void product(const Parts<N> (&a)[NT], const Parts<3>&
 // ---- scores
 // cap * tanh(x), cap with the factor to base 2.  Below 1 x (cap + y P(y)), y = x^2, P the polynomial nearest to
 // cap (tanh(x) / x - 1) / y there (weighted least squares: 4.6e-9 of the value off, with fp32's
-// steps 7e-8): nine instructions, which is all that a block takes whose scores lie there.  Above it 1 - 2 / (1 +
-// e^2x), whose rounding is that of a value near 1.
+// steps 7e-8), below 0.55 one of degree 3 (3.7e-08, with fp32's steps 1e-7): nine instructions or six, which is all that a block takes whose
+// scores lie there.  Above it 1 - 2 / (1 + e^2x), whose rounding is that of a value near 1.
 struct Cap {
-    float cap, p[7];
+    float cap, p[7], low[4];
 };
 // The same value of every lane, in a scalar register.
 __device__ __forceinline__ float uniform(float x) {
@@ -162,13 +162,21 @@ __device__ __forceinline__ Cap cap_of(float cap) {
     return {uniform(c),
             {uniform(c * -0.33333295583724976f), uniform(c * 0.13332344591617584f), uniform(c * -0.05387980118393898f),
              uniform(c * 0.021486656740307808f), uniform(c * -0.007946106605231762f), uniform(c * 0.0023013646714389324f),
-             uniform(c * -0.00035845203092321754f)}};
+             uniform(c * -0.00035845203092321754f)},
+            {uniform(c * -0.3333294689655304f), uniform(c * 0.13320724666118622f), uniform(c * -0.05267181247472763f), uniform(c * 0.016437580808997154f)}};
 }
 __device__ __forceinline__ float capped_small(float x, const Cap& c) {
     const float y = x * x;
     float p = c.p[6];
 #pragma unroll
     for (int i = 5; i >= 0; --i) p = fmaf(p, y, c.p[i]);
+    return x * fmaf(p, y, c.cap);
+}
+__device__ __forceinline__ float capped_low(float x, const Cap& c) {
+    const float y = x * x;
+    float p = c.low[3];
+#pragma unroll
+    for (int i = 2; i >= 0; --i) p = fmaf(p, y, c.low[i]);
     return x * fmaf(p, y, c.cap);
 }
 __device__ __forceinline__ float capped(float x, const Cap& c) {
@@ -209,6 +217,7 @@ __device__ __forceinline__ void grow_tree(TreeLds& s, const int* parents, int T,
     for (int k = 0; k < W; ++k) w[k] = t >> 5 == k ? 1u << (t & 31) : 0u;
     int up = node && t < T ? parents[t] : -1;
     if (up >= t || up < 0) up = -1;
+#pragma unroll 1
     for (int round = 0; round <= 8; ++round) {  // (2^8 ancestors at most)
         if (node) {
             s.up[t] = up;
@@ -402,6 +411,9 @@ __device__ __forceinline__ void weigh(const PagedAttn& a, const Tree& tree, cons
         if (__ballot(!(most < 1.0f))) {
 #pragma unroll
             for (int v = 0; v < NS; ++v) s[v] = capped(s[v], cap);
+        } else if (!__ballot(!(most < 0.55f))) {
+#pragma unroll
+            for (int v = 0; v < NS; ++v) s[v] = capped_low(s[v], cap);
         } else {
 #pragma unroll
             for (int v = 0; v < NS; ++v) s[v] = capped_small(s[v], cap);
@@ -597,13 +609,20 @@ __device__ __forceinline__ bool gather(int8_t* lds, int group, int per, int whic
 // XCD where pairs are a multiple of 8; then the tile, the last (a prompt's longest) first, then the split.  Up to 64
 // sequences come by length, the longest first, so that what starts last is short (32 x 8 x 4 x 128 over 4096 to 8192 keys in
 // two splits 154 us, unsorted 177).
+//
+// SHARED: two workgroups run on a CU.  Where one round of them fills more than half of the card the second half comes in
+// reverse, so that a CU has a long one and a short one (2048 tokens x 8 x 128 58.1 -> 49.7 us; alone on its CU a
+// workgroup has to come by length: 2048 x 16 x 128 in fp32 143 -> 200).
+constexpr int kCus = 256;
 struct Place {
     int b, kvh, tile, split, start, len;
 };
-template <bool TREE>
+template <bool TREE, bool SHARED>
 __device__ __forceinline__ Place place_of(const PagedAttn& a, int tiles) {
     const int pairs = a.B * a.H_kv;
-    const int u = blockIdx.x / pairs, pair = blockIdx.x - u * pairs;
+    int n = blockIdx.x;
+    if (SHARED && n >= kCus && gridDim.x <= 2 * kCus) n = kCus + gridDim.x - 1 - n;
+    const int u = n / pairs, pair = n - u * pairs;
     Place p;
     p.split = u / tiles;
     p.tile = tiles - 1 - (u - p.split * tiles);
@@ -670,7 +689,7 @@ __global__ __launch_bounds__(256, NP == 1 && WR == 4 ? 2 : 1) void paged_tile_ke
     __shared__ Tree tree;
     const int tid = threadIdx.x, lane = tid & 63, i = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), rw = wave % WR, kw = wave / WR;
-    const Place at = place_of<TREE>(a, tiles);
+    const Place at = place_of<TREE, D == 64 || (NP == 1 && WR == 4)>(a, tiles);
     const int b = at.b, kvh = at.kvh, ctx = at.start;
     const int r = at.tile * 32 * WR + rw * 32 + i;
     // the query first: it waits for nothing
@@ -690,7 +709,8 @@ __global__ __launch_bounds__(256, NP == 1 && WR == 4 ? 2 : 1) void paged_tile_ke
         kbeg = min(kbeg, bounds[w][0]);
         kend = max(kend, bounds[w][1]);
     }
-    if (kbeg > kend) kbeg = kend;
+    kend = __builtin_amdgcn_readfirstlane(kend);  // (scalars, and all that follows from them)
+    kbeg = min(__builtin_amdgcn_readfirstlane(kbeg), kend);
     // this split's stages
     const int all = (kend - kbeg + T::SK - 1) / T::SK, per = (all + a.splits - 1) / a.splits;
     const int s0 = min(at.split * per, all), s1 = min(s0 + per, all);
@@ -823,14 +843,14 @@ __global__ __launch_bounds__(256, NP == 1 && WR == 4 ? 2 : 1) void paged_tile_ke
         // thread, and at the end too, where it is k1 - 1's: a register loaded or used under a condition makes
         // the compiler wait for the copies here.
         const int p2 = pos_of(s + 2), in2 = page_of(a.pages, p2);
-        const uint32_t page = (uint32_t)table[in2];
+        const uint32_t page = (uint32_t)table[in2], row2 = (uint32_t)(p2 - in2 * a.pages.block);
         const int8_t* stage = lds + buf * T::STAGE;
 #pragma unroll 1
         for (int n = 0; n < T::NB; ++n) {
             const int blk = kw * T::NB + n, c0 = kbeg + s * T::SK + 32 * blk;
             if (c0 < lim.hi && c0 + 32 > lim.lo) attend(stage, blk, c0);
         }
-        slots[s & 1][tid] = page * (uint32_t)a.pages.block + (uint32_t)(p2 - in2 * a.pages.block);
+        slots[s & 1][tid] = page * (uint32_t)a.pages.block + row2;
     }
     float l = sum_xor32(st.l);
     if constexpr (T::WK > 1) {
@@ -883,7 +903,7 @@ __global__ __launch_bounds__((64 * Few<D, NP, M>::WAVES), (Few<D, NP, M>::WAVES 
     __shared__ Tree tree;
     const int lane = threadIdx.x & 63, i = lane & (M - 1), g = lane / M;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const Place at = place_of<TREE>(a, tiles);
+    const Place at = place_of<TREE, false>(a, tiles);
     const int b = at.b, kvh = at.kvh, ctx = at.start;
     const int r = at.tile * M + i;
     const float* q_row = query_row<D>(a, r, b, kvh);
@@ -1101,7 +1121,7 @@ __global__ __launch_bounds__(64 * kRowWaves, 2) void paged_row_kernel(PagedAttn 
     static_assert(sizeof(lds_all) >= sizeof(float) * W * R * D, "the join");
     const int tid = threadIdx.x, lane = tid & 63, sub = lane % T::LPK, grp = lane / T::LPK;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const Place at = place_of<TREE>(a, tiles);
+    const Place at = place_of<TREE, false>(a, tiles);
     const int b = at.b, kvh = at.kvh, ctx = at.start;
     float q[R][E];
 #pragma unroll

@@ -179,10 +179,11 @@ __global__ __launch_bounds__(256) void rope_write_any_kernel(RopeWrite a) {
     }
 }
 
-// A workgroup for a (sequence, layer, K or V): a thread moves its 16 bytes of every
-// row of the path, in the path's order.  An entry's row lies at or behind the place it
-// goes to, and every later entry's row behind that place, so in order no row is
-// overwritten before it is read; four are read ahead of four writes.
+// A workgroup for a (sequence, layer): K's 16-byte chunks of a row and V's behind them, a thread the same one of every
+// row, in the path's order.  An entry's row lies at or behind the place it goes to, and every later entry's behind
+// that place, so in order no row is overwritten before it is read; eight are read ahead of eight writes.  Bound by the
+// chain count, path, table, row, not by the bytes: a wave looks up 64 entries side by side (one after another, four
+// rows ahead of four writes: 32 x 32 layers of 8 x 128 bf16 30.2 us, so XXX).
 constexpr int kLayers = 64;
 struct KeepArgs {
     void* cache[2][kLayers];
@@ -191,37 +192,43 @@ struct KeepArgs {
     const int *ctx, *paths, *counts;
 };
 __global__ __launch_bounds__(256) void kv_keep_kernel(KeepArgs a) {
-    const int b = blockIdx.y;
-    uint4* cache = static_cast<uint4*>(a.cache[blockIdx.z][blockIdx.x]);
+    __shared__ uint32_t from[64], to[64];
+    __shared__ int valid;
+    const int b = blockIdx.y, lane = threadIdx.x & 63;
     const int* table = a.pages.table + (size_t)b * a.pages.nbps;
     const int* path = a.paths + (size_t)b * a.most;
     const int ctx = a.ctx[b], n = min(a.counts[b], a.most);
     const long long end = (long long)a.pages.nbps * a.pages.block;
     if (ctx < 0) return;
-    int last = -1;
-    for (int j0 = 0; j0 < n; j0 += 4) {
-        int count = 0;
-        size_t from[4], to[4];
+    for (int j0 = 0; j0 < n; j0 += 64) {
+        if (threadIdx.x < 64) {
+            const int j = j0 + lane, p = j < n ? path[j] : -1, before = j > 0 && j < n ? path[j - 1] : -1;
+            const bool ok = p > before && (long long)ctx + p < end;
+            const uint64_t bad = ~__ballot(ok);
+            const int count = bad ? __builtin_ctzll(bad) : 64;  // (the path ends at the first that is not)
+            if (lane < count) {
+                from[lane] = cache_row(a.pages, table, ctx + p);
+                to[lane] = cache_row(a.pages, table, ctx + j);
+            }
+            if (lane == 0) valid = count;
+        }
+        __syncthreads();
+        const int count = valid;
+        for (int c = threadIdx.x; c < 2 * a.chunks; c += 256) {
+            const bool v = c >= a.chunks;
+            uint4* cache = static_cast<uint4*>(a.cache[v][blockIdx.x]) + (v ? c - a.chunks : c);
+            for (int k0 = 0; k0 < count; k0 += 8) {
+                uint4 x[8];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int p = j0 + k < n ? path[j0 + k] : -1;
-            if (count == k && p > last && (long long)ctx + p < end) {
-                from[k] = (size_t)cache_row(a.pages, table, ctx + p) * a.chunks;
-                to[k] = (size_t)cache_row(a.pages, table, ctx + j0 + k) * a.chunks;
-                last = p;
-                count = k + 1;
+                for (int k = 0; k < 8; ++k)
+                    if (k0 + k < count && from[k0 + k] != to[k0 + k]) x[k] = cache[(size_t)from[k0 + k] * a.chunks];
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (k0 + k < count && from[k0 + k] != to[k0 + k]) cache[(size_t)to[k0 + k] * a.chunks] = x[k];
             }
         }
-        for (int c = threadIdx.x; c < a.chunks; c += 256) {
-            uint4 x[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (k < count && from[k] != to[k]) x[k] = cache[from[k] + c];
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (k < count && from[k] != to[k]) cache[to[k] + c] = x[k];
-        }
-        if (count < 4) return;
+        if (count < 64) return;
+        __syncthreads();
     }
 }
 
@@ -258,7 +265,7 @@ void launch_kv_keep(const KeepRows& a, hipStream_t s) {
         k.ctx = a.ctx;
         k.paths = a.paths;
         k.counts = a.counts;
-        kv_keep_kernel<<<dim3((unsigned)n, (unsigned)a.B, 2), 256, 0, s>>>(k);
+        kv_keep_kernel<<<dim3((unsigned)n, (unsigned)a.B), 256, 0, s>>>(k);
     }
 }
 

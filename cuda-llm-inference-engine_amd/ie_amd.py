@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import numbers
+import operator
 import os
 from typing import NamedTuple
 
@@ -416,16 +417,18 @@ def _refuse(what, *tensors):
 
 _device_index = None  # () -> index of the current device
 _raw_stream_of = None  # device index -> handle of its current stream
-_f32 = _i32 = _i8 = _bf16 = _empty = None
+_f32 = _i32 = _i8 = _bf16 = _empty = _tensor = None
+_dtype_of = operator.attrgetter("dtype")
 
 
 def _bind_torch():
-    global _device_index, _raw_stream_of, _f32, _i32, _i8, _bf16, _empty
+    global _device_index, _raw_stream_of, _f32, _i32, _i8, _bf16, _empty, _tensor
     import torch
 
     load()  # fills _fns
     torch.cuda.current_stream()
     _f32, _i32, _i8, _bf16, _empty = torch.float32, torch.int32, torch.int8, torch.bfloat16, torch.empty
+    _tensor = torch.Tensor
     _raw_stream_of = torch._C._cuda_getCurrentRawStream
     _device_index = torch._C._cuda_getDevice
 
@@ -711,14 +714,10 @@ def _ints(what, t, n, at):
     return t.data_ptr()
 
 
-def _paged_rows(what, x, B, P, d, at):
-    """Distance between the rows of x [B, P, heads, d] fp32, which may lie apart but evenly so (None: one row)."""
-    st = x.stride()
-    if (x.dtype is not _f32 or x.get_device() != at or x.dim() != 4 or x.shape[0] != B or x.shape[1] != P or x.shape[3] != d
-            or st[3] != 1 or (x.shape[2] > 1 and st[2] != d) or (B > 1 and P > 1 and st[0] != P * st[1])):
-        raise ValueError(f"{what}: Q, K and V need to be fp32 [{B}, {P}, heads, {d}] on cuda:{at}, rows whole and evenly "
-                         f"spaced; got {x.dtype} {tuple(x.shape)} strides {st} on {x.device}")
-    return st[1] if P > 1 else st[0] if B > 1 else None
+def _uneven(what, *tensors):
+    raise ValueError(f"{what}: Q, K and V need to be fp32 [B, P, heads, d] on cuda:{_device_index()}, rows whole and evenly spaced, "
+                     "K's and V's alike; got " + ", ".join(f"{t.dtype} {tuple(t.shape)} strides {t.stride()} on {t.device}"
+                                                           for t in tensors))
 
 
 def rope_kv_write(Q, K, V, inv_freq, starts, k_cache, v_cache, block_table, positions=None, lens=None, interleaved=False,
@@ -728,32 +727,39 @@ def rope_kv_write(Q, K, V, inv_freq, starts, k_cache, v_cache, block_table, posi
     times inv_freq [rot / 2]; K and V go to cache positions starts[b] + t, t <
     lens[b].  Returns the rotated Q."""
     H, bs, d, kind, at, rows, nbps = _paged("rope_kv_write", k_cache, v_cache, block_table)
-    B, P = K.shape[:2]
+    shape, kst = K.shape, K.stride()
+    B, P, _, _ = shape
     if rows != B or inv_freq.dtype is not _f32 or inv_freq.get_device() != at or not inv_freq.is_contiguous():
         _refuse("rope_kv_write", K, block_table, inv_freq)
-    H_q, q, o, q_ld, ld = 0, None, None, None, None
-    if B * P:
-        ld = _paged_rows("rope_kv_write", K, B, P, d, at)
-        if K.shape[2] != H or V.shape != K.shape or _paged_rows("rope_kv_write", V, B, P, d, at) != ld:
-            raise ValueError(f"rope_kv_write: K and V need {H} heads and equal strides, got {tuple(K.shape)} strides "
-                             f"{K.stride()}, {tuple(V.shape)} strides {V.stride()}")
+    # (the distance between rows: a view's rows may lie apart, but evenly so)
+    ld = kst[1] if P > 1 else kst[0] if B > 1 else H * d
+    if B * P and (shape != (B, P, H, d) or V.shape != shape or V.stride() != kst or K.dtype is not _f32 or V.dtype is not _f32
+                  or K.get_device() != at or V.get_device() != at or kst[3] != 1 or (H > 1 and kst[2] != d)
+                  or (B > 1 and P > 1 and kst[0] != P * ld)):
+        _uneven("rope_kv_write", K, V)
+    H_q, q, o, q_ld = 0, None, None, 0
     if Q is not None:
-        H_q = Q.shape[2]
-        if B * P:
-            q_ld = _paged_rows("rope_kv_write", Q, B, P, d, at)
+        _, _, H_q, dq = Q.shape
+        qst = Q.stride()
+        q_ld = qst[1] if P > 1 else qst[0] if B > 1 else H_q * d
+        if (Q.shape != (B, P, H_q, d) or Q.dtype is not _f32 or Q.get_device() != at
+                or (B * P and (qst[3] != 1 or (H_q > 1 and qst[2] != d) or (B > 1 and P > 1 and qst[0] != P * q_ld)))):
+            _uneven("rope_kv_write", Q)
         if out is None:
             out = _new(stream, (B, P, H_q, d), _f32, Q.device)
-        elif (out.numel() != B * P * H_q * d or out.dtype is not _f32 or out.get_device() != at or not out.is_contiguous()):
+        elif out.numel() != B * P * H_q * d or out.dtype is not _f32 or out.get_device() != at or not out.is_contiguous():
             _refuse("rope_kv_write", out)
         q, o = Q.data_ptr(), out.data_ptr()
-    q_ld, ld = H_q * d if q_ld is None else q_ld, H * d if ld is None else ld
-    if max(q_ld, ld) > 0x7FFFFFFF:
+    if ld > 0x7FFFFFFF or q_ld > 0x7FFFFFFF:
         _past_int("rope_kv_write", "row distance", max(q_ld, ld))
+    if not (starts.numel() == B and starts.dtype is _i32 and starts.get_device() == at and starts.is_contiguous()):
+        _refuse("rope_kv_write", starts)
     st = _fns["ie_rope_kv_write"](
-        B, P, q, K.data_ptr(), V.data_ptr(), q_ld, ld, H_q, H, d, 2 * inv_freq.numel(), int(interleaved), inv_freq.data_ptr(),
-        _ints("rope_kv_write", starts, B, at), _ints("rope_kv_write", lens, B, at),
-        _ints("rope_kv_write", positions, B * P, at), o, k_cache.data_ptr(), v_cache.data_ptr(), kind,
-        block_table.data_ptr(), nbps, bs, _raw_stream_of(at) if stream is None else stream.cuda_stream)
+        B, P, q, K.data_ptr(), V.data_ptr(), q_ld, ld, H_q, H, d, 2 * inv_freq.numel(), 1 if interleaved else 0,
+        inv_freq.data_ptr(), starts.data_ptr(), None if lens is None else _ints("rope_kv_write", lens, B, at),
+        None if positions is None else _ints("rope_kv_write", positions, B * P, at), o, k_cache.data_ptr(),
+        v_cache.data_ptr(), kind, block_table.data_ptr(), nbps, bs,
+        _raw_stream_of(at) if stream is None else stream.cuda_stream)
     if st:
         _failed("ie_rope_kv_write", st)
     return out
@@ -763,36 +769,28 @@ def paged_attn_num_splits(B, P, H_q, H_kv, d, kv_dtype, max_keys, window=0, spli
     return call("ie_paged_attn_num_splits", B, P, H_q, H_kv, d, kv_dtype, max_keys, window, splits)
 
 
-def _attend(what, name, Q, k_cache, v_cache, block_table, starts, lens, extra, max_ctx, keys, window, scale, cap, slopes, splits,
-            out, workspace, stream):
-    H, bs, d, kind, at, rows, nbps = _paged(what, k_cache, v_cache, block_table)
-    B, P, H_q, dq = Q.shape
-    if not -0x80000000 <= max_ctx <= 0x7FFFFFFF:
-        _past_int(what, "max_ctx", max_ctx)
+def _attend(what, H_q, H, d, kind, at, rows, B, P, dq, Q, out, block_table, starts, lens, keys, window, slopes, splits, workspace,
+            stream):
+    """(out, workspace, lens' address) of an attention call whose tensors fit each other."""
+    if not -0x80000000 <= keys <= 0x7FFFFFFF:
+        _past_int(what, "max_ctx", keys)
     if not -0x80000000 <= window <= 0x7FFFFFFF:
         _past_int(what, "window", window)
     if out is None:
         out = _new(stream, (B, P, H_q, d), _f32, Q.device)
     if not (dq == d and rows == B and out.numel() == B * P * H_q * d and Q.dtype is _f32 and out.dtype is _f32
             and Q.get_device() == at and out.get_device() == at and Q.is_contiguous() and out.is_contiguous()
+            and starts.numel() == B and starts.dtype is _i32 and starts.get_device() == at and starts.is_contiguous()
             and (slopes is None or (slopes.numel() == H_q and slopes.dtype is _f32 and slopes.get_device() == at
                                     and slopes.is_contiguous()))):
-        _refuse(what, Q, out, block_table, *(() if slopes is None else (slopes,)))
+        _refuse(what, Q, out, block_table, starts, *(() if slopes is None else (slopes,)))
     if workspace is None:
-        if keys <= 0x7FFFFFFF:
-            S = _fns["ie_paged_attn_num_splits"](B, P, H_q, H, d, kind, keys, window, splits)
-            if S > 1:
-                workspace = _new(stream, B * P * H_q * S * (d + 2), _f32, Q.device)
+        S = _fns["ie_paged_attn_num_splits"](B, P, H_q, H, d, kind, keys, window, splits)
+        if S > 1:
+            workspace = _new(stream, B * P * H_q * S * (d + 2), _f32, Q.device)
     elif workspace.dtype is not _f32 or workspace.get_device() != at or not workspace.is_contiguous():
         _refuse(what, workspace)
-    st = _fns[name](
-        B, P, H_q, H, d, Q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), kind, block_table.data_ptr(), nbps, bs,
-        _ints(what, starts, B, at), _ints(what, lens, B, at), *extra(B * P, at), window, 0.0 if scale is None else scale, cap,
-        None if slopes is None else slopes.data_ptr(), out.data_ptr(), None if workspace is None else workspace.data_ptr(),
-        0 if workspace is None else 4 * workspace.numel(), splits, _raw_stream_of(at) if stream is None else stream.cuda_stream)
-    if st:
-        _failed(name, st)
-    return out
+    return out, workspace, None if lens is None else _ints(what, lens, B, at)
 
 
 def paged_attn(Q, k_cache, v_cache, block_table, starts, max_ctx, lens=None, first=None, end=None, window=0, scale=None,
@@ -802,10 +800,19 @@ def paged_attn(Q, k_cache, v_cache, block_table, starts, max_ctx, lens=None, fir
     None: from 0, to itself) inside the window; scores scale q.k capped by cap * tanh and
     less slopes[h] times the distance.  max_ctx >= starts[b] + lens[b].  Returns O
     [B, P, H_q, d] (rows past lens[b] are not written)."""
-    def extra(n, at):
-        return max_ctx, _ints("paged_attn", first, n, at), _ints("paged_attn", end, n, at)
-    return _attend("paged_attn", "ie_paged_attn", Q, k_cache, v_cache, block_table, starts, lens, extra, max_ctx, max_ctx,
-                   window, scale, cap, slopes, splits, out, workspace, stream)
+    H, bs, d, kind, at, rows, nbps = _paged("paged_attn", k_cache, v_cache, block_table)
+    B, P, H_q, dq = Q.shape
+    out, ws, len_at = _attend("paged_attn", H_q, H, d, kind, at, rows, B, P, dq, Q, out, block_table, starts, lens, max_ctx, window,
+                              slopes, splits, workspace, stream)
+    st = _fns["ie_paged_attn"](
+        B, P, H_q, H, d, Q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), kind, block_table.data_ptr(), nbps, bs,
+        starts.data_ptr(), len_at, max_ctx, None if first is None else _ints("paged_attn", first, B * P, at),
+        None if end is None else _ints("paged_attn", end, B * P, at), window, 0.0 if scale is None else scale, cap,
+        None if slopes is None else slopes.data_ptr(), out.data_ptr(), None if ws is None else ws.data_ptr(),
+        0 if ws is None else 4 * ws.numel(), splits, _raw_stream_of(at) if stream is None else stream.cuda_stream)
+    if st:
+        _failed("ie_paged_attn", st)
+    return out
 
 
 def tree_attn(Q, k_cache, v_cache, block_table, context_lens, parents, max_ctx, lens=None, window=0, scale=None, cap=0.0,
@@ -813,10 +820,19 @@ def tree_attn(Q, k_cache, v_cache, block_table, context_lens, parents, max_ctx, 
     """Q [B, T, H_q, d] fp32 of drafted nodes at cache positions context_lens[b] + t, each
     behind node parents[b, t] < t (-1: the context); over the context, its ancestors and
     itself.  max_ctx >= context_lens[b].  Scores, lens and result as paged_attn."""
-    def extra(n, at):
-        return _ints("tree_attn", parents, n, at), max_ctx
-    return _attend("tree_attn", "ie_tree_attn", Q, k_cache, v_cache, block_table, context_lens, lens, extra, max_ctx,
-                   max_ctx + Q.shape[1], window, scale, cap, slopes, splits, out, workspace, stream)
+    H, bs, d, kind, at, rows, nbps = _paged("tree_attn", k_cache, v_cache, block_table)
+    B, T, H_q, dq = Q.shape
+    out, ws, len_at = _attend("tree_attn", H_q, H, d, kind, at, rows, B, T, dq, Q, out, block_table, context_lens, lens,
+                              max_ctx + T, window, slopes, splits, workspace, stream)
+    st = _fns["ie_tree_attn"](
+        B, T, H_q, H, d, Q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), kind, block_table.data_ptr(), nbps, bs,
+        context_lens.data_ptr(), len_at, _ints("tree_attn", parents, B * T, at), max_ctx, window,
+        0.0 if scale is None else scale, cap, None if slopes is None else slopes.data_ptr(), out.data_ptr(),
+        None if ws is None else ws.data_ptr(), 0 if ws is None else 4 * ws.numel(), splits,
+        _raw_stream_of(at) if stream is None else stream.cuda_stream)
+    if st:
+        _failed("ie_tree_attn", st)
+    return out
 
 
 def kv_cache_keep(k_caches, v_caches, block_table, context_lens, paths, counts, stream=None):
@@ -827,17 +843,20 @@ def kv_cache_keep(k_caches, v_caches, block_table, context_lens, paths, counts, 
         raise ValueError(f"kv_cache_keep: {n} K caches and {len(v_caches)} V caches")
     if not n:
         return
-    H, bs, d, kind, at, B, nbps = _paged("kv_cache_keep", k_caches[0], v_caches[0], block_table)
-    shape, dtype = k_caches[0].shape, k_caches[0].dtype
-    for t in (*k_caches, *v_caches):
-        if t.shape != shape or t.dtype is not dtype or t.get_device() != at or not t.is_contiguous():
-            _refuse("kv_cache_keep", k_caches[0], t)
+    first = k_caches[0]
+    H, bs, d, kind, at, B, nbps = _paged("kv_cache_keep", first, v_caches[0], block_table)
+    # (by map: a loop's own steps cost as much as the looks at a tensor)
+    every, size, dtype = [*k_caches, *v_caches], first.numel(), first.dtype
+    if not (set(map(_tensor.numel, every)) == {size} and set(map(_tensor.get_device, every)) == {at}
+            and set(map(_dtype_of, every)) == {dtype} and all(map(_tensor.is_contiguous, every))):
+        _refuse("kv_cache_keep", first, *(t for t in every if t.numel() != size or t.dtype is not dtype or t.get_device() != at
+                                          or not t.is_contiguous()))
     if paths.dim() != 2 or paths.shape[0] != B:
         _refuse("kv_cache_keep", block_table, paths)
     most = paths.shape[1]
-    k, v = ((ctypes.c_void_p * n)(*(t.data_ptr() for t in c)) for c in (k_caches, v_caches))
+    pointers = (_P * (2 * n))(*map(_tensor.data_ptr, every))
     st = _fns["ie_kv_cache_keep"](
-        B, most, n, k, v, kind, block_table.data_ptr(), nbps, bs, H, d, _ints("kv_cache_keep", context_lens, B, at),
+        B, most, n, pointers, ctypes.byref(pointers, 8 * n), kind, block_table.data_ptr(), nbps, bs, H, d, _ints("kv_cache_keep", context_lens, B, at),
         _ints("kv_cache_keep", paths, B * most, at), _ints("kv_cache_keep", counts, B, at),
         _raw_stream_of(at) if stream is None else stream.cuda_stream)
     if st:

@@ -60,7 +60,10 @@ SCORES = [(dict(Hq=3), INVALID), (dict(Hq=0), INVALID), (dict(n=-1), INVALID), (
           (dict(scale=float("inf")), INVALID), (dict(cap=-1.0), INVALID), (dict(cap=float("nan")), INVALID),
           (dict(cap=1e-39, scale=1.0), INVALID), (dict(Q=None), INVALID), (dict(O=None), INVALID), (dict(Q=P + 4), INVALID),
           (dict(O=OUT + 4), INVALID), (dict(O=P + 1024), INVALID), (dict(mx=2**30 + 1, nbps=2**27, bs=256), UNSUPPORTED),
-          (dict(B=2**21), UNSUPPORTED)]
+          (dict(B=2**21), UNSUPPORTED), (dict(splits=4, ws=None, nbps=256, mx=2048), INVALID),
+          (dict(splits=4, nbps=256, mx=2048, ws=1 << 50, wsb=4 * 4 * 4 * 66 * 4 - 1), WORKSPACE),
+          (dict(splits=4, nbps=256, mx=2048, ws=(1 << 50) + 4, wsb=1 << 30), INVALID),
+          (dict(splits=4, nbps=256, mx=2048, ws=P, wsb=1 << 30), INVALID)]
 CASES = [(rope, LAYOUT + CACHE + [(dict(n=-1), INVALID), (dict(Hq=-1), INVALID), (dict(rot=63), INVALID), (dict(rot=66), INVALID),
                                   (dict(rot=-2), INVALID), (dict(qld=252), INVALID), (dict(qld=258), INVALID),
                                   (dict(ld=124), INVALID), (dict(ld=130), INVALID), (dict(Q=None), INVALID),
