@@ -32,22 +32,39 @@ __device__ __forceinline__ void rotate(float& x, float& y, float2 cs) {
     y = fmaf(y, cs.x, a * cs.y);
 }
 
-template <typename KV>
-__device__ __forceinline__ void put4(KV* p, float4 v) {
-    if constexpr (sizeof(KV) == 4)
-        *reinterpret_cast<float4*>(p) = v;
-    else
-        *reinterpret_cast<ushort4*>(p) =
-            make_ushort4(f32_to_bf16_rne(v.x), f32_to_bf16_rne(v.y), f32_to_bf16_rne(v.z), f32_to_bf16_rne(v.w));
+// VEC values side by side: sources, which are read once, past the caches (4 x 2000 rows of 48 x 128 38.3 -> 32.9 us).
+template <int VEC>
+struct Values {
+    float v[VEC];
+};
+template <int VEC>
+__device__ __forceinline__ Values<VEC> get(const float* p) {
+    typedef float Raw __attribute__((ext_vector_type(VEC)));
+    Values<VEC> r;
+    if constexpr (VEC == 1) {
+        r.v[0] = __builtin_nontemporal_load(p);
+    } else {
+        const Raw x = __builtin_nontemporal_load(reinterpret_cast<const Raw*>(p));
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) r.v[i] = x[i];
+    }
+    return r;
 }
-template <typename KV>
-__device__ __forceinline__ void put1(KV* p, float v) {
-    if constexpr (sizeof(KV) == 4)
-        *p = v;
-    else
-        *p = f32_to_bf16_rne(v);
+template <typename T, int VEC>
+__device__ __forceinline__ void put(T* p, const Values<VEC>& x) {
+    T y[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+        if constexpr (sizeof(T) == 4) y[i] = x.v[i];
+        else y[i] = f32_to_bf16_rne(x.v[i]);
+    }
+    struct alignas(sizeof(T) * VEC) Whole {
+        T v[VEC];
+    };
+    *reinterpret_cast<Whole*>(p) = __builtin_bit_cast(Whole, y);
 }
 
+constexpr int kUnits = 3;  // of a thread, where there are rows enough
 // A row (b, t): which it is and where it goes.
 struct RowOf {
     int b;
@@ -67,42 +84,44 @@ __device__ __forceinline__ RowOf row_of(const RopeWrite& a, int row) {
     return r;
 }
 
-// TOK rows to a workgroup (blockDim.x / units of them, one where a row has more
-// units than threads; then gridDim.y workgroups share it).  A unit is eight channels
-// of a head: a rotated pair of fours (i .., i + rot / 2 ..), eight side by side where
-// pairs are interleaved, and eight side by side behind the rotated ones and of V.
-// The row's angles are computed once a workgroup, for all of its heads, while the
-// first unit's channels arrive.  Bound by HBM: reads 4 bytes a value, writes 4 of Q
-// and 2 or 4 of K and V.
-template <typename KV>
+// A unit is 2 VEC channels of a head: rotated pairs, VEC of the first half (i ..) and theirs of the second (i + rot / 2
+// ..), or side by side where pairs are interleaved, behind the rotated ones and of V.  VEC is 4 where rot is a multiple of 8,
+// 2 of 4, else 1.  `tok` rows to a workgroup where a row has few units, else gridDim.y workgroups to a row, and N units
+// to a thread.  A row's angles are computed once a workgroup, for all of its heads, while the units' channels arrive.
+// Bound by HBM: reads 4 bytes a value, writes 4 of Q and 2 or 4 of K and V; 4 x 2000 rows of (32 + 16) x 128 into bf16
+// pages take 36 us, 4.2 TB/s (of 196 MB), with one unit a thread 43.
+template <typename KV, int VEC, int N>
 __global__ __launch_bounds__(256) void rope_write_kernel(RopeWrite a, int units, int tok) {
-    __shared__ float2 cs[512];  // (tok * rot / 2: a row has at least d / 4 units)
-    const int half = a.rot / 2, per = a.d / 8, rows = a.B * a.P;
+    __shared__ float2 cs[512];  // (tok * rot / 2: a row has at least d / VEC units)
+    const int half = a.rot / 2, per = a.d / (2 * VEC), rows = a.B * a.P;
     const int lt = tok > 1 ? threadIdx.x / units : 0;
     const int row = blockIdx.x * tok + lt;
-    int u = tok > 1 ? threadIdx.x - lt * units : blockIdx.y * 256 + threadIdx.x;
+    const int u0 = tok > 1 ? threadIdx.x - lt * units : blockIdx.y * (256 * N) + threadIdx.x;
     const bool mine = lt < tok && row < rows;
     RowOf r{};
     if (mine) r = row_of(a, row);
     const size_t q_src = (size_t)row * a.q_ld, kv_src = (size_t)row * a.kv_ld;
+    const bool go = mine && r.live;
 
-    float4 x, y;
-    int head = 0, c = 0, c2 = 0;
-    auto fetch = [&] {
-        head = u / per;
-        const int w = u - head * per;
-        const bool pair = !a.interleaved && head < a.H_q + a.H_kv && 4 * w < half;
-        // (fours of the first half stand for both halves, so the rest begins at rot)
-        c = pair ? 4 * w : 8 * w;
-        c2 = pair ? c + half : c + 4;
-        const float* p = head < a.H_q ? a.Q + q_src + (size_t)head * a.d
-                         : head < a.H_q + a.H_kv ? a.K + kv_src + (size_t)(head - a.H_q) * a.d
-                                                 : a.V + kv_src + (size_t)(head - a.H_q - a.H_kv) * a.d;
-        x = *reinterpret_cast<const float4*>(p + c);
-        y = *reinterpret_cast<const float4*>(p + c2);
-    };
-    const bool go = mine && r.live && u < units;
-    if (go) fetch();
+    Values<VEC> x[N], y[N];
+    int head[N], c[N], c2[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const int u = u0 + 256 * n;
+        head[n] = u / per;
+        const int w = u - head[n] * per;
+        const bool pair = !a.interleaved && head[n] < a.H_q + a.H_kv && VEC * w < half;
+        // (a unit of pairs stands for both halves, so the rest begins at rot)
+        c[n] = pair ? VEC * w : 2 * VEC * w;
+        c2[n] = pair ? c[n] + half : c[n] + VEC;
+        if (go && u < units) {
+            const float* p = head[n] < a.H_q ? a.Q + q_src + (size_t)head[n] * a.d
+                             : head[n] < a.H_q + a.H_kv ? a.K + kv_src + (size_t)(head[n] - a.H_q) * a.d
+                                                        : a.V + kv_src + (size_t)(head[n] - a.H_q - a.H_kv) * a.d;
+            x[n] = get<VEC>(p + c[n]);
+            y[n] = get<VEC>(p + c2[n]);
+        }
+    }
     for (int i = threadIdx.x; i < tok * half; i += 256) {
         const int rr = blockIdx.x * tok + i / half;
         if (rr < rows) {
@@ -114,76 +133,55 @@ __global__ __launch_bounds__(256) void rope_write_kernel(RopeWrite a, int units,
     if (!go) return;
     const float2* t = cs + lt * half;
     const size_t slot = r.stored ? cache_row(a.pages, a.pages.table + (size_t)r.b * a.pages.nbps, r.at) : 0;
-    for (;;) {
-        if (head < a.H_q + a.H_kv && c < a.rot) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        if (u0 + 256 * n >= units) return;
+        const int h = head[n], i = c[n];
+        if (h < a.H_q + a.H_kv && i < a.rot) {
             if (a.interleaved) {
-                rotate(x.x, x.y, t[c / 2]);
-                rotate(x.z, x.w, t[c / 2 + 1]);
-                rotate(y.x, y.y, t[c / 2 + 2]);
-                rotate(y.z, y.w, t[c / 2 + 3]);
-            } else if (c < half) {
-                rotate(x.x, y.x, t[c]);
-                rotate(x.y, y.y, t[c + 1]);
-                rotate(x.z, y.z, t[c + 2]);
-                rotate(x.w, y.w, t[c + 3]);
+                float z[2 * VEC];
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) z[e] = x[n].v[e], z[VEC + e] = y[n].v[e];
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) rotate(z[2 * e], z[2 * e + 1], t[i / 2 + e]);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) x[n].v[e] = z[e], y[n].v[e] = z[VEC + e];
+            } else {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) rotate(x[n].v[e], y[n].v[e], t[i + e]);
             }
         }
-        if (head < a.H_q) {
-            float* o = a.out + ((size_t)row * a.H_q + head) * a.d;
-            *reinterpret_cast<float4*>(o + c) = x;
-            *reinterpret_cast<float4*>(o + c2) = y;
+        if (h < a.H_q) {
+            float* o = a.out + ((size_t)row * a.H_q + h) * a.d;
+            put(o + i, x[n]);
+            put(o + c2[n], y[n]);
         } else if (r.stored) {
-            const bool key = head < a.H_q + a.H_kv;
-            KV* o = static_cast<KV*>(key ? a.k : a.v) + (slot * a.H_kv + (head - a.H_q - (key ? 0 : a.H_kv))) * a.d;
-            put4(o + c, x);
-            put4(o + c2, y);
+            const bool key = h < a.H_q + a.H_kv;
+            KV* o = static_cast<KV*>(key ? a.k : a.v) + (slot * a.H_kv + (h - a.H_q - (key ? 0 : a.H_kv))) * a.d;
+            put(o + i, x[n]);
+            put(o + c2[n], y[n]);
         }
-        if (tok > 1) return;
-        u += gridDim.y * 256;
-        if (u >= units) return;
-        fetch();
     }
 }
 
-// Any rot: a thread takes a value and its partner.
-template <typename KV>
-__global__ __launch_bounds__(256) void rope_write_any_kernel(RopeWrite a) {
-    const int row = blockIdx.x, half = a.rot / 2;
-    const RowOf r = row_of(a, row);
-    if (!r.live) return;
-    const size_t q_src = (size_t)row * a.q_ld, kv_src = (size_t)row * a.kv_ld;
-    const size_t slot = r.stored ? cache_row(a.pages, a.pages.table + (size_t)r.b * a.pages.nbps, r.at) : 0;
-    // of a head: its pairs, then the values behind them; V: its values
-    const int turned = half + (a.d - a.rot), n = (a.H_q + a.H_kv) * turned + a.H_kv * a.d;
-    for (int u = blockIdx.y * 256 + threadIdx.x; u < n; u += gridDim.y * 256) {
-        const int of_v = u - (a.H_q + a.H_kv) * turned;
-        if (of_v >= 0) {
-            if (r.stored) put1(static_cast<KV*>(a.v) + slot * a.H_kv * a.d + of_v, a.V[kv_src + of_v]);
-            continue;
-        }
-        const int head = u / turned, i = u - head * turned;
-        const bool pair = i < half;
-        const int c = pair ? (a.interleaved ? 2 * i : i) : i + half, c2 = a.interleaved ? c + 1 : c + half;
-        const float* p = head < a.H_q ? a.Q + q_src + (size_t)head * a.d : a.K + kv_src + (size_t)(head - a.H_q) * a.d;
-        float x = p[c], y = pair ? p[c2] : 0.0f;
-        if (pair) rotate(x, y, turn(r.pos, a.freq[i]));
-        if (head < a.H_q) {
-            float* o = a.out + ((size_t)row * a.H_q + head) * a.d;
-            o[c] = x;
-            if (pair) o[c2] = y;
-        } else if (r.stored) {
-            KV* o = static_cast<KV*>(a.k) + (slot * a.H_kv + (head - a.H_q)) * a.d;
-            put1(o + c, x);
-            if (pair) put1(o + c2, y);
-        }
-    }
+template <typename KV, int VEC>
+void launch_rope(const RopeWrite& a, hipStream_t s) {
+    const long long units = (long long)(a.H_q + 2 * a.H_kv) * a.d / (2 * VEC);
+    const int rows = a.B * a.P, tok = (int)std::max(1ll, 256 / units);
+    // several units a thread where there are rows enough (a decode step's few are spread over more workgroups), and where
+    // a row has more than a grid's second size times them
+    const bool many = (rows >= 512 && units > 256) || units > 256ll * 65535;
+    const int each = many ? 256 * kUnits : 256;
+    const dim3 grid((unsigned)((rows + tok - 1) / tok), tok > 1 ? 1u : (unsigned)((units + each - 1) / each));
+    auto* k = many ? rope_write_kernel<KV, VEC, kUnits> : rope_write_kernel<KV, VEC, 1>;
+    k<<<grid, 256, 0, s>>>(a, (int)units, tok);
 }
 
 // A workgroup for a (sequence, layer): K's 16-byte chunks of a row and V's behind them, a thread the same one of every
 // row, in the path's order.  An entry's row lies at or behind the place it goes to, and every later entry's behind
 // that place, so in order no row is overwritten before it is read; eight are read ahead of eight writes.  Bound by the
 // chain count, path, table, row, not by the bytes: a wave looks up 64 entries side by side (one after another, four
-// rows ahead of four writes: 32 x 32 layers of 8 x 128 bf16 30.2 us, so XXX).
+// rows ahead of four writes: 32 x 32 layers of 8 x 128 bf16 30.8 us, so 18.2).
 constexpr int kLayers = 64;
 struct KeepArgs {
     void* cache[2][kLayers];
@@ -235,20 +233,14 @@ __global__ __launch_bounds__(256) void kv_keep_kernel(KeepArgs a) {
 }  // namespace
 
 void launch_rope_write(const RopeWrite& a, hipStream_t s) {
-    const bool half = a.kv_dtype == IE_KV_BF16;
-    const int rows = a.B * a.P;
-    // fours of a pair stay whole, and what is not rotated is whole eights
-    if (a.rot % 8 == 0) {
-        const int units = (a.H_q + 2 * a.H_kv) * a.d / 8;
-        const int tok = std::max(1, 256 / units);
-        const dim3 grid((unsigned)((rows + tok - 1) / tok), tok > 1 ? 1u : (unsigned)std::min(65535, (units + 255) / 256));
-        auto* k = half ? rope_write_kernel<uint16_t> : rope_write_kernel<float>;
-        k<<<grid, 256, 0, s>>>(a, units, tok);
-    } else {
-        const long long n = (long long)(a.H_q + 2 * a.H_kv) * a.d;
-        auto* k = half ? rope_write_any_kernel<uint16_t> : rope_write_any_kernel<float>;
-        k<<<dim3((unsigned)rows, (unsigned)std::min(65535ll, (n + 255) / 256)), 256, 0, s>>>(a);
-    }
+    auto go = [&](auto kv) {
+        using KV = decltype(kv);
+        if (a.rot % 8 == 0) launch_rope<KV, 4>(a, s);
+        else if (a.rot % 4 == 0) launch_rope<KV, 2>(a, s);
+        else launch_rope<KV, 1>(a, s);
+    };
+    if (a.kv_dtype == IE_KV_BF16) go(uint16_t{});
+    else go(float{});
 }
 
 void launch_kv_keep(const KeepRows& a, hipStream_t s) {
