@@ -656,12 +656,13 @@ __device__ __forceinline__ uint4 read_v(const int8_t* rows, int k0, int t) {
 }
 
 // ---- the tile kernel
-// A workgroup of four waves: WR of them take 32 rows each, 4 / WR groups of them
+// WR x WK waves: WR of them take 32 rows each, WK groups of them
 // different keys.  A stage holds SK keys' K and V in LDS, NB blocks of 32 for each
 // group of waves; rows past the tile's keys are its last key again.
-template <int D, int NP, int WR>
+template <int D, int NP, int WR, int WK_>
 struct Tile {
-    static constexpr int WK = 4 / WR;
+    static constexpr int WK = WK_, W = WR * WK, THREADS = 64 * W;
+    static constexpr bool SHARED = W == 4 && (D == 64 || (NP == 1 && WR == 4));  // two workgroups run on a CU
     static constexpr int NB = NP == 1 && WR == 4 ? 2 : 1;
     static constexpr int SK = 32 * NB * WK;
     static constexpr int ROW = 2 * D;          // bytes of a part's row
@@ -677,19 +678,19 @@ struct Tile {
     __device__ static __forceinline__ int vswz(int r) { return D == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1); }
 };
 
-template <int D, int NP, int WR, bool TREE>
-__global__ __launch_bounds__(256, NP == 1 && WR == 4 ? 2 : 1) void paged_tile_kernel(PagedAttn a, int tiles) {
-    using T = Tile<D, NP, WR>;
+template <int D, int NP, int WR, int WK, bool TREE>
+__global__ __launch_bounds__(64 * WR * WK, NP == 1 && WR == 4 ? 2 : 1) void paged_tile_kernel(PagedAttn a, int tiles) {
+    using T = Tile<D, NP, WR, WK>;
     using KV = std::conditional_t<NP == 1, uint16_t, float>;
     using Tree = std::conditional_t<TREE, TreeLds, NoTree>;
     constexpr int NT = D / 32, KS = D / 16;
     __shared__ __attribute__((aligned(1024))) int8_t lds[T::LDS];
-    __shared__ uint32_t slots[2][256];  // a thread's each, SK of them keys of the stage
-    __shared__ int bounds[4][2];
+    __shared__ uint32_t slots[2][T::THREADS];  // a thread's each, SK of them keys of the stage
+    __shared__ int bounds[T::W][2];
     __shared__ Tree tree;
     const int tid = threadIdx.x, lane = tid & 63, i = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), rw = wave % WR, kw = wave / WR;
-    const Place at = place_of<TREE, D == 64 || (NP == 1 && WR == 4)>(a, tiles);
+    const Place at = place_of<TREE, T::SHARED>(a, tiles);
     const int b = at.b, kvh = at.kvh, ctx = at.start;
     const int r = at.tile * 32 * WR + rw * 32 + i;
     // the query first: it waits for nothing
@@ -705,7 +706,7 @@ __global__ __launch_bounds__(256, NP == 1 && WR == 4 ? 2 : 1) void paged_tile_ke
     __syncthreads();
     int kbeg = 0x7fffffff, kend = 0;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < T::W; ++w) {
         kbeg = min(kbeg, bounds[w][0]);
         kend = max(kend, bounds[w][1]);
     }
@@ -723,7 +724,7 @@ __global__ __launch_bounds__(256, NP == 1 && WR == 4 ? 2 : 1) void paged_tile_ke
     auto pos_of = [&](int s) { return min(kbeg + s * T::SK + tid, k1 - 1); };  // of a stage's key tid
     // bf16: a stage's rows straight into LDS; a wave's load fills 1 KiB, its lanes' addresses are
     // permuted so that the chunks land swizzled.
-    constexpr int RPL = 1024 / T::ROW, LOADS = T::SK / RPL / 4;
+    constexpr int RPL = 1024 / T::ROW, LOADS = T::SK / RPL / T::W;
     const uint32_t lds_at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_i8)lds);
     // (a lane's rows are multiples of 16 apart, after which both swizzles repeat: one place in the row each)
     const int lane_row = wave * RPL + lane / T::CH;
@@ -732,21 +733,21 @@ __global__ __launch_bounds__(256, NP == 1 && WR == 4 ? 2 : 1) void paged_tile_ke
         if constexpr (NP == 1) {
 #pragma unroll
             for (int j = 0; j < LOADS; ++j) {
-                const uint64_t at = slots[s & 1][lane_row + 4 * j * RPL] * row_bytes;
-                const uint32_t to = lds_at + buf * T::STAGE + (wave + 4 * j) * 1024;
+                const uint64_t at = slots[s & 1][lane_row + T::W * j * RPL] * row_bytes;
+                const uint32_t to = lds_at + buf * T::STAGE + (wave + T::W * j) * 1024;
                 copy16(kbase + (at + kcol), to);
                 copy16(vbase + (at + vcol), to + T::PART);
             }
         }
     };
     // fp32: through registers, split on the way.
-    constexpr int CPT = NP == 1 ? 1 : T::SK * T::CH / 256;  // chunks of eight values a thread
+    constexpr int CPT = NP == 1 ? 1 : T::SK * T::CH / T::THREADS;  // chunks of eight values a thread
     float4 raw[2][CPT][2];
     auto load = [&](int s) {
         if constexpr (NP == 3) {
 #pragma unroll
             for (int j = 0; j < CPT; ++j) {
-                const int id = tid + 256 * j, r = id / T::CH, c = id % T::CH;
+                const int id = tid + T::THREADS * j, r = id / T::CH, c = id % T::CH;
                 const size_t at = slots[s & 1][r] * row_bytes + 32 * c;
                 raw[0][j][0] = *reinterpret_cast<const float4*>(kbase + at);
                 raw[0][j][1] = *reinterpret_cast<const float4*>(kbase + at + 16);
@@ -759,7 +760,7 @@ __global__ __launch_bounds__(256, NP == 1 && WR == 4 ? 2 : 1) void paged_tile_ke
         if constexpr (NP == 3) {
 #pragma unroll
             for (int j = 0; j < CPT; ++j) {
-                const int id = tid + 256 * j, r = id / T::CH, c = id % T::CH;
+                const int id = tid + T::THREADS * j, r = id / T::CH, c = id % T::CH;
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
                     const float4 p = raw[x][j][0], q = raw[x][j][1];
@@ -1424,13 +1425,14 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn a) {
 struct Form {
     int rows;
     float start, rate, loaded;
+    int groups = 1;  // of waves with keys of their own, of 128 rows
 };
-constexpr int kForms = 4;
+constexpr int kForms = 5;
 constexpr Form kTiles[2][2][kForms] = {
-    {{{16, 5.7f, 10.5f, 12.0f}, {32, 5.8f, 19.9f, 22.0f}, {64, 5.2f, 36.1f, 39.5f}, {128, 5.8f, 53.0f, 53.0f}},      // fp32, d 64
-     {{16, 5.7f, 29.3f, 33.0f}, {32, 8.4f, 34.3f, 40.0f}, {64, 8.2f, 62.2f, 76.0f}, {128, 7.9f, 104.0f, 112.0f}}},  // d 128
-    {{{16, 5.7f, 4.4f, 5.5f}, {32, 5.9f, 9.8f, 10.2f}, {64, 5.9f, 18.3f, 18.6f}, {128, 5.7f, 27.0f, 27.0f}},         // bf16, d 64
-     {{16, 7.5f, 6.6f, 8.8f}, {32, 8.8f, 15.5f, 18.0f}, {64, 8.1f, 25.4f, 32.3f}, {128, 7.9f, 42.0f, 45.0f}}}};     // d 128
+    {{{16, 5.7f, 10.5f, 12.0f}, {32, 5.8f, 19.9f, 22.0f}, {64, 5.2f, 36.1f, 39.5f}, {128, 5.8f, 53.0f, 53.0f}, {}},      // fp32, d 64
+     {{16, 5.7f, 29.3f, 33.0f}, {32, 8.4f, 34.3f, 40.0f}, {64, 8.2f, 62.2f, 76.0f}, {128, 7.9f, 104.0f, 112.0f}, {}}},  // d 128
+    {{{16, 5.7f, 4.4f, 5.5f}, {32, 5.9f, 9.8f, 10.2f}, {64, 5.9f, 18.3f, 18.6f}, {128, 5.7f, 27.0f, 27.0f}, {128, 7.4f, 18.4f, 27.0f, 2}},         // bf16, d 64
+     {{16, 7.5f, 6.6f, 8.8f}, {32, 8.8f, 15.5f, 18.0f}, {64, 8.1f, 25.4f, 32.3f}, {128, 7.9f, 41.0f, 42.5f}, {128, 11.0f, 28.8f, 46.4f, 2}}}};     // d 128
 // One row, and two of an fp32 cache, have no other form (us, 8 KV heads, one sequence of 2000 keys; 32 of 4000; against 16
 // rows'): fp32 d 64 one 15.8 and 26.9; 92.2 and 96.7, two 20.9 and 26.8; 94.4 and 96.7, four 30.8 and 27.0; 98.9 and
 // 96.4, d 128 two 41.7 and 65.6; 185 and 186, four 63.7 and 65.6; 192 and 186; bf16 d 64 one 11.4 and 14.3; 46.1 and
@@ -1439,7 +1441,7 @@ constexpr Form kRows[2][2][2] = {{{{1, 4.7f, 5.6f, 5.6f}, {2, 5.5f, 7.8f, 7.8f}}
                                  {{{1, 4.7f, 3.3f, 3.3f}, {}}, {{1, 4.7f, 7.3f, 7.3f}, {}}}};
 
 struct Plan {
-    int rows, splits;
+    int rows, groups, splits;
 };
 // asked > 0: the best form for that many splits (clamped); else the best of both.
 Plan plan_of(int B, int P, int H_q, int H_kv, int d, int kv_dtype, int max_keys, int window, int asked) {
@@ -1449,57 +1451,60 @@ Plan plan_of(int B, int P, int H_q, int H_kv, int d, int kv_dtype, int max_keys,
     const int stages = (int)((walked + 127) / 128), most = stages < IE_PAGED_MAX_SPLITS ? stages : IE_PAGED_MAX_SPLITS;
     const bool few = rows <= (half ? 1 : 2);
     const Form* forms = few ? &kRows[half][wide][(int)rows - 1] : kTiles[half][wide];
-    Plan best{forms[0].rows, 1};
+    Plan best{forms[0].rows, 1, 1};
     double least = INFINITY;
     for (int f = 0; f < (few ? 1 : kForms); ++f) {
         const Form& x = forms[f];
+        if (!x.rows) continue;
         const double tiles = (double)(((long long)rows + x.rows - 1) / x.rows), groups = tiles * pairs;
         for (int s = asked > 0 ? asked : 1; s <= (asked > 0 ? asked : most); ++s) {
             const int n = s < 1 ? 1 : s > most ? (most < 1 ? 1 : most) : s;
             const double a_cu = groups * n / 256;
             // 1000 keys of a workgroup where all CUs read their own from HBM (5.5 TB/s); tiles of a pair share theirs
             const double memory = 1000.0 * 2 * d * (half ? 2 : 4) / (5.5e6 / 256) / tiles * (a_cu < 1 ? a_cu : 1);
-            const double own = a_cu < 0.5 ? x.rate : x.loaded, rate = (own > memory ? own : memory) / 1000 / n;
             // Workgroups of like length come in whole rounds; a causal prompt's tiles see half of its own keys on average.
             // A batch's sequences are taken to hold four fifths of the longest's keys.
             const bool alike = walked >= 2.0 * P;
             const double seen = (alike ? walked - (P - 1) / 2.0 : walked > P ? walked - P / 2.0 : walked / 2) * (B > 1 ? 0.8 : 1);
+            const double load = a_cu * seen / walked, own = x.rate + (x.loaded - x.rate) * (load < 1 ? load : 1);
+            const double rate = (own > memory ? own : memory) / 1000 / n;
             const double rounds = a_cu <= 1 ? a_cu : alike ? std::ceil(a_cu) : a_cu + 0.6;
-            const double start = x.rows >= 64 ? 0.6 * x.start : x.start;  // (several of those share a CU)
+            const double start = x.rows >= 64 && x.groups == 1 ? 0.6 * x.start : x.start;  // (several of those share a CU)
             const double longest = x.start + walked * rate, work = rounds * (start + seen * rate);
             double t = longest > work ? longest : work;
             if (n > 1) t += 5 + rows * pairs * n * (d + 2) * 8 / 4e6;  // the join: a launch, partial results out and back
             if (t < least) {
                 least = t;
-                best = {x.rows, n};
+                best = {x.rows, x.groups, n};
             }
         }
     }
     return best;
 }
 
-template <int D, int NP, int ROWS, bool TREE>
+template <int D, int NP, int ROWS, bool TREE, int WK = ROWS == 64 ? 2 : 1>
 void launch_tile(const PagedAttn& a, hipStream_t s) {
     const int G = a.H_q / a.H_kv, tiles = (int)(((long long)a.P * G + ROWS - 1) / ROWS);
     const unsigned grid = (unsigned)((long long)a.B * a.H_kv * tiles * a.splits);
     using KV = std::conditional_t<NP == 1, uint16_t, float>;
     if constexpr (ROWS <= 2) paged_row_kernel<D, KV, ROWS, TREE><<<grid, 64 * kRowWaves, 0, s>>>(a, tiles);
     else if constexpr (ROWS <= 32) paged_few_kernel<D, NP, ROWS, TREE><<<grid, 64 * Few<D, NP, ROWS>::WAVES, 0, s>>>(a, tiles);
-    else paged_tile_kernel<D, NP, ROWS / 32, TREE><<<grid, 256, 0, s>>>(a, tiles);
+    else paged_tile_kernel<D, NP, ROWS / 32, WK, TREE><<<grid, 2 * ROWS * WK, 0, s>>>(a, tiles);
 }
 
 template <int D, int NP, bool TREE>
 void launch_rows(const PagedAttn& a, hipStream_t s) {
-    const int keys = a.parents ? a.max_ctx + a.P : a.max_ctx;
-    switch (plan_of(a.B, a.P, a.H_q, a.H_kv, a.d, a.kv_dtype, keys, a.window, a.splits).rows) {
-        case 1: return launch_tile<D, NP, 1, TREE>(a, s);
-        case 2:
-            if constexpr (NP == 3) return launch_tile<D, NP, 2, TREE>(a, s);
-        case 16: return launch_tile<D, NP, 16, TREE>(a, s);
-        case 32: return launch_tile<D, NP, 32, TREE>(a, s);
-        case 64: return launch_tile<D, NP, 64, TREE>(a, s);
-        default: return launch_tile<D, NP, 128, TREE>(a, s);
+    const Plan p = plan_of(a.B, a.P, a.H_q, a.H_kv, a.d, a.kv_dtype, a.parents ? a.max_ctx + a.P : a.max_ctx, a.window, a.splits);
+    if (p.rows == 1) return launch_tile<D, NP, 1, TREE>(a, s);
+    if constexpr (NP == 3) {
+        if (p.rows == 2) return launch_tile<D, NP, 2, TREE>(a, s);
+    } else {
+        if (p.groups == 2) return launch_tile<D, NP, 128, TREE, 2>(a, s);
     }
+    if (p.rows == 16) return launch_tile<D, NP, 16, TREE>(a, s);
+    if (p.rows == 32) return launch_tile<D, NP, 32, TREE>(a, s);
+    if (p.rows == 64) return launch_tile<D, NP, 64, TREE>(a, s);
+    launch_tile<D, NP, 128, TREE>(a, s);
 }
 
 template <int D, int NP>
