@@ -12,11 +12,11 @@
 // each 16, read transposed from V's rows (ds_read_b64_tr_b16).  A bf16 cache is one
 // part and takes three products, an fp32 cache six of the nine (the rest are below
 // 2^-24).  Statistics and outputs are fp32.
-#include <cmath>
 #include <type_traits>
 
 #include "device_util.h"
 #include "paged.h"
+#include "paged_plan.h"
 
 namespace ie {
 namespace {
@@ -1418,70 +1418,6 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn a) {
     reinterpret_cast<float4*>(a.O + r * D)[c] = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
-// Which kernel, and how many splits: the least estimated time.  A form has tiles of 1 or 2 rows (paged_row_kernel),
-// 16 or 32 (paged_few_kernel), 64 or 128 (paged_tile_kernel); a workgroup of it takes `start` us and `rate` us for every
-// 1000 keys, measured with 8 workgroups on the card (8 KV heads over 512 and 2560 keys), `loaded` with one or two on every
-// CU (32 and 64 sequences; the smallest forms, whose keys come from HBM then: prompts of 1000 tokens).
-struct Form {
-    int rows;
-    float start, rate, loaded;
-    int groups = 1;  // of waves with keys of their own, of 128 rows
-};
-constexpr int kForms = 5;
-constexpr Form kTiles[2][2][kForms] = {
-    {{{16, 5.7f, 10.5f, 12.0f}, {32, 5.8f, 19.9f, 22.0f}, {64, 5.2f, 36.1f, 39.5f}, {128, 5.8f, 53.0f, 53.0f}, {}},      // fp32, d 64
-     {{16, 5.7f, 29.3f, 33.0f}, {32, 8.4f, 34.3f, 40.0f}, {64, 8.2f, 62.2f, 76.0f}, {128, 7.9f, 104.0f, 112.0f}, {}}},  // d 128
-    {{{16, 5.7f, 4.4f, 5.5f}, {32, 5.9f, 9.8f, 10.2f}, {64, 5.9f, 18.3f, 18.6f}, {128, 5.7f, 27.0f, 27.0f}, {128, 7.4f, 18.4f, 27.0f, 2}},         // bf16, d 64
-     {{16, 7.5f, 6.6f, 8.8f}, {32, 8.8f, 15.5f, 18.0f}, {64, 8.1f, 25.4f, 32.3f}, {128, 7.9f, 41.0f, 42.5f}, {128, 11.0f, 28.8f, 46.4f, 2}}}};     // d 128
-// One row, and two of an fp32 cache, have no other form (us, 8 KV heads, one sequence of 2000 keys; 32 of 4000; against 16
-// rows'): fp32 d 64 one 15.8 and 26.9; 92.2 and 96.7, two 20.9 and 26.8; 94.4 and 96.7, four 30.8 and 27.0; 98.9 and
-// 96.4, d 128 two 41.7 and 65.6; 185 and 186, four 63.7 and 65.6; 192 and 186; bf16 d 64 one 11.4 and 14.3; 46.1 and
-// 47.7, two 15.3 and 14.3; 49.0 and 47.9, d 128 one 19.5 and 19.6; 93.3 and 94.0, two 25.7 and 19.8; 96.3 and 94.1.
-constexpr Form kRows[2][2][2] = {{{{1, 4.7f, 5.6f, 5.6f}, {2, 5.5f, 7.8f, 7.8f}}, {{1, 4.7f, 13.8f, 13.8f}, {2, 5.5f, 18.5f, 18.5f}}},
-                                 {{{1, 4.7f, 3.3f, 3.3f}, {}}, {{1, 4.7f, 7.3f, 7.3f}, {}}}};
-
-struct Plan {
-    int rows, groups, splits;
-};
-// asked > 0: the best form for that many splits (clamped); else the best of both.
-Plan plan_of(int B, int P, int H_q, int H_kv, int d, int kv_dtype, int max_keys, int window, int asked) {
-    const int half = kv_dtype == IE_KV_BF16, wide = d == 128;
-    const double rows = (double)P * (H_q / H_kv), pairs = (double)B * H_kv;
-    const double walked = window && (long long)window + P < max_keys ? (double)window + P : max_keys;
-    const int stages = (int)((walked + 127) / 128), most = stages < IE_PAGED_MAX_SPLITS ? stages : IE_PAGED_MAX_SPLITS;
-    const bool few = rows <= (half ? 1 : 2);
-    const Form* forms = few ? &kRows[half][wide][(int)rows - 1] : kTiles[half][wide];
-    Plan best{forms[0].rows, 1, 1};
-    double least = INFINITY;
-    for (int f = 0; f < (few ? 1 : kForms); ++f) {
-        const Form& x = forms[f];
-        if (!x.rows) continue;
-        const double tiles = (double)(((long long)rows + x.rows - 1) / x.rows), groups = tiles * pairs;
-        for (int s = asked > 0 ? asked : 1; s <= (asked > 0 ? asked : most); ++s) {
-            const int n = s < 1 ? 1 : s > most ? (most < 1 ? 1 : most) : s;
-            const double a_cu = groups * n / 256;
-            // 1000 keys of a workgroup where all CUs read their own from HBM (5.5 TB/s); tiles of a pair share theirs
-            const double memory = 1000.0 * 2 * d * (half ? 2 : 4) / (5.5e6 / 256) / tiles * (a_cu < 1 ? a_cu : 1);
-            // Workgroups of like length come in whole rounds; a causal prompt's tiles see half of its own keys on average.
-            // A batch's sequences are taken to hold four fifths of the longest's keys.
-            const bool alike = walked >= 2.0 * P;
-            const double seen = (alike ? walked - (P - 1) / 2.0 : walked > P ? walked - P / 2.0 : walked / 2) * (B > 1 ? 0.8 : 1);
-            const double load = a_cu * seen / walked, own = x.rate + (x.loaded - x.rate) * (load < 1 ? load : 1);
-            const double rate = (own > memory ? own : memory) / 1000 / n;
-            const double rounds = a_cu <= 1 ? a_cu : alike ? std::ceil(a_cu) : a_cu + 0.6;
-            const double start = x.rows >= 64 && x.groups == 1 ? 0.6 * x.start : x.start;  // (several of those share a CU)
-            const double longest = x.start + walked * rate, work = rounds * (start + seen * rate);
-            double t = longest > work ? longest : work;
-            if (n > 1) t += 5 + rows * pairs * n * (d + 2) * 8 / 4e6;  // the join: a launch, partial results out and back
-            if (t < least) {
-                least = t;
-                best = {x.rows, x.groups, n};
-            }
-        }
-    }
-    return best;
-}
-
 template <int D, int NP, int ROWS, bool TREE, int WK = ROWS == 64 ? 2 : 1>
 void launch_tile(const PagedAttn& a, hipStream_t s) {
     const int G = a.H_q / a.H_kv, tiles = (int)(((long long)a.P * G + ROWS - 1) / ROWS);
@@ -1494,7 +1430,7 @@ void launch_tile(const PagedAttn& a, hipStream_t s) {
 
 template <int D, int NP, bool TREE>
 void launch_rows(const PagedAttn& a, hipStream_t s) {
-    const Plan p = plan_of(a.B, a.P, a.H_q, a.H_kv, a.d, a.kv_dtype, a.parents ? a.max_ctx + a.P : a.max_ctx, a.window, a.splits);
+    const PagedPlan p = paged_plan(a.B, a.P, a.H_q, a.H_kv, a.d, a.kv_dtype, a.parents ? a.max_ctx + a.P : a.max_ctx, a.window, a.splits);
     if (p.rows == 1) return launch_tile<D, NP, 1, TREE>(a, s);
     if constexpr (NP == 3) {
         if (p.rows == 2) return launch_tile<D, NP, 2, TREE>(a, s);
@@ -1520,7 +1456,8 @@ void launch_d(const PagedAttn& a, hipStream_t s) {
     if (a.splits > 1) {
         const long long rows = (long long)a.B * a.P * a.H_q;
         constexpr int per = 256 / (D / 4);  // rows of a workgroup, or an eighth of them
-        if (a.splits <= 4) paged_merge_kernel<D, 1><<<(unsigned)((rows + per - 1) / per), 256, 0, s>>>(a);
+        // (with very many rows, whose grid of eighths would pass 2^32 threads, a row's splits have one group of lanes)
+        if (a.splits <= 4 || rows > 1 << 20) paged_merge_kernel<D, 1><<<(unsigned)((rows + per - 1) / per), 256, 0, s>>>(a);
         else paged_merge_kernel<D, 8><<<(unsigned)((rows * 8 + per - 1) / per), 256, 0, s>>>(a);
     }
 }
@@ -1528,7 +1465,7 @@ void launch_d(const PagedAttn& a, hipStream_t s) {
 }  // namespace
 
 int paged_attn_splits(int B, int P, int H_q, int H_kv, int d, int kv_dtype, int max_keys, int window, int asked) {
-    return plan_of(B, P, H_q, H_kv, d, kv_dtype, max_keys, window, asked).splits;
+    return paged_plan(B, P, H_q, H_kv, d, kv_dtype, max_keys, window, asked).splits;
 }
 
 void launch_paged_attn(const PagedAttn& a, hipStream_t s) {

@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cmath>
+#include <initializer_list>
 
 #include "paged.h"
 
@@ -10,6 +11,11 @@ namespace {
 using ie::fail;
 
 bool aligned(const void* p, size_t a) { return ((uintptr_t)p % a) == 0; }
+bool words(std::initializer_list<const void*> p) {
+    for (const void* x : p)
+        if (!aligned(x, 4)) return false;
+    return true;
+}
 bool overlap(const void* a, size_t na, const void* b, size_t nb) {
     const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
     return x < y + nb && y < x + na;
@@ -66,6 +72,8 @@ int check_attn(const char* fn, ie::PagedAttn& a, long long keys, int block_size,
     if (!a.Q || !a.O || !a.starts) return fail(IE_ERR_INVALID, "%s: null pointer", fn);
     if (!aligned(a.Q, 16) || !aligned(a.O, 16))
         return fail(IE_ERR_INVALID, "%s: Q and O must be 16-byte aligned", fn);
+    if (!words({a.starts, a.lens, a.first, a.end, a.parents, a.slopes}))
+        return fail(IE_ERR_INVALID, "%s: an array of ints or floats is not 4-byte aligned", fn);
     const size_t bytes = (size_t)a.B * a.P * a.H_q * a.d * sizeof(float);
     if (overlap(a.Q, bytes, a.O, bytes)) return fail(IE_ERR_INVALID, "%s: O overlaps Q", fn);
     if (keys > 0 && (st = check_cache(fn, a.k, a.v, a.pages.table)) != IE_OK) return st;
@@ -114,6 +122,8 @@ int ie_rope_kv_write(int B, int P, const float* Q_src, const float* K_src, const
         return fail(IE_ERR_INVALID, "%s: null pointer", fn);
     if (!aligned(Q_src, 16) || !aligned(K_src, 16) || !aligned(V_src, 16) || !aligned(Q_out, 16))
         return fail(IE_ERR_INVALID, "%s: Q_src, K_src, V_src and Q_out must be 16-byte aligned", fn);
+    if (!words({inv_freq, starts, lens, positions}))
+        return fail(IE_ERR_INVALID, "%s: an array of ints or floats is not 4-byte aligned", fn);
     if ((st = check_cache(fn, k_cache, v_cache, block_table)) != IE_OK) return st;
     const size_t n = (size_t)B * P, out = n * q_row * sizeof(float);
     const size_t q_bytes = ((n - 1) * q_stride + q_row) * sizeof(float), kv_bytes = ((n - 1) * kv_stride + kv_row) * sizeof(float);
@@ -195,6 +205,8 @@ int ie_kv_cache_keep(int B, int max_count, int n_layers, void* const* k_caches, 
     if (B > 65535) return fail(IE_ERR_UNSUPPORTED, "%s: more than 65535 sequences", fn);
     if (B == 0 || max_count == 0 || n_layers == 0) return IE_OK;
     if (!k_caches || !v_caches || !context_lens || !paths || !counts) return fail(IE_ERR_INVALID, "%s: null pointer", fn);
+    if (!words({context_lens, paths, counts}))
+        return fail(IE_ERR_INVALID, "%s: an array of ints is not 4-byte aligned", fn);
     for (int l = 0; l < n_layers; ++l)
         if ((st = check_cache(fn, k_caches[l], v_caches[l], block_table)) != IE_OK) return st;
     ie::KeepRows a{};

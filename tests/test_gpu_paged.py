@@ -7,6 +7,7 @@ import torch
 
 import paged_oracle as po
 from conftest import rng
+from paged_forms import FORMS
 
 pytestmark = pytest.mark.gpu
 
@@ -228,6 +229,63 @@ def test_other_branches_never_arrive(ie, dev, half):
     clean = torch.tensor([not ({2, 5, 20} & set(line)) for line in po.lines(parents[0])], device=dev)
     off = (got.double() - want[0]).abs() - want[1]
     assert bool((off[0, clean] <= 0).all()) and bool(torch.isnan(got[0, ~clean]).all())
+
+
+# ------------------------------------------------------------------ every form of the kernels
+def ragged(r, B, top):
+    """Positions before the queries: one sequence at `top`, the others anywhere, one at 0."""
+    starts = [int(x) for x in r.integers(0, top + 1, B)]
+    starts[0] = top
+    if B > 2:
+        starts[B // 2] = 0
+    return starts
+
+
+@pytest.mark.parametrize("kv,d,rows,groups,splits,call", FORMS)
+def test_every_form_ranges(ie, dev, kv, d, rows, groups, splits, call):
+    B, P, H, G, keys = call
+    r = rng(rows + d + kv + splits)
+    starts = ragged(r, B, keys - P)
+    lens = [P] + [int(x) for x in r.integers(0, P + 1, B - 1)]
+    check_ranges(ie, dev, r, B, P, H, G, d, 16, bool(kv), starts, cap=4.0, q_scale=3.0)
+    check_ranges(ie, dev, r, B, P, H, G, d, 24, bool(kv), starts, lens, slopes=True, scale=0.1)
+    check_ranges(ie, dev, r, B, P, H, G, d, 16, bool(kv), starts, lens, q_scale=400.0)  # (weights far apart)
+    first = r.integers(-5, keys, (B, P)).astype(np.int32)
+    end = (first + r.integers(-30, keys, (B, P))).astype(np.int32)
+    check_ranges(ie, dev, r, B, P, H, G, d, 32, bool(kv), starts, lens, first=first, end=end, cap=30.0, slopes=True)
+    table, caches, q, top = case(r, dev, B, P, H, G, d, 16, bool(kv), starts)
+    # one key that every other query sees is not finite
+    x = starts[0] // 2
+    first = np.zeros((B, P), np.int32)
+    first[0, ::2] = x + 1
+    want = po.ranges(q, caches, table, 16, starts, None, top, first)
+    caches[0][table[0, x // 16], x % 16] = float("nan")
+    caches[1][table[0, x // 16], x % 16] = float("inf")
+    got = ie.paged_attn(q, *caches, i32(table, dev), i32(starts, dev), top, first=i32(first, dev))
+    off = (got.double() - want[0]).abs() - want[1]
+    assert bool((off[1:] <= 0).all()) and bool((off[0, ::2] <= 0).all()) and bool(torch.isnan(got[0, 1::2]).all())
+    # and again in other splits: the same answers, the same bits again
+    if splits > 1:
+        for s in (1, 2, splits + 1):
+            again = [ie.paged_attn(q, *caches, i32(table, dev), i32(starts, dev), top, first=i32(first, dev), splits=s) for _ in range(2)]
+            off = (again[0].double() - want[0]).abs() - want[1]
+            assert bool((off[1:] <= 0).all()) and torch.equal(again[0].view(torch.int32), again[1].view(torch.int32))
+
+
+@pytest.mark.parametrize("kv,d,rows,groups,splits,call", [f for f in FORMS if f[5][1] <= 256])
+def test_every_form_tree(ie, dev, kv, d, rows, groups, splits, call):
+    B, T, H, G, keys = call
+    r = rng(rows + d + kv + splits)
+    ctx = ragged(r, B, keys - T)
+    table, caches, q, _ = case(r, dev, B, T, H, G, d, 16, bool(kv), ctx)
+    parents = [list(shapes(r, T).values())[b % 5] for b in range(B)]
+    lens = [T] + [int(x) for x in r.integers(0, T + 1, B - 1)]
+    for kw in ({}, dict(window=max(2, T // 3), cap=20.0, slopes=normal(r, dev, H * G).abs())):
+        want = po.tree(q, caches, table, 16, ctx, parents, lens, **kw)
+        got = ie.tree_attn(q, *caches, i32(table, dev), i32(ctx, dev), i32(parents, dev), max(ctx), lens=i32(lens, dev),
+                           out=torch.full_like(q, 7.0), **kw)
+        near(got, want)
+        assert bool((got[~want[2]] == 7.0).all())
 
 
 # ------------------------------------------------------------------ rotated writes

@@ -11,6 +11,7 @@ import torch
 
 import paged_oracle as po
 from conftest import ROOT, rng
+from paged_forms import FORMS
 
 P = 4096  # stands for a device pointer: no call below reaches HIP
 OUT = 1 << 40
@@ -71,14 +72,17 @@ CASES = [(rope, LAYOUT + CACHE + [(dict(n=-1), INVALID), (dict(Hq=-1), INVALID),
                                   (dict(freq=None), INVALID), (dict(starts=None), INVALID), (dict(Q=P + 4), INVALID),
                                   (dict(K=P + 8), INVALID), (dict(V=P + 4), INVALID), (dict(out=OUT + 8), INVALID),
                                   (dict(out=P), INVALID), (dict(out=P + 16), INVALID), (dict(K=OUT - 16), INVALID),
-                                  (dict(nbps=2**27), UNSUPPORTED), (dict(n=2**21 + 1), UNSUPPORTED)]),
-         (attn, LAYOUT + CACHE + SCORES + [(dict(starts=None), INVALID)]),
+                                  (dict(freq=P + 2), INVALID), (dict(starts=P + 1), INVALID), (dict(lens=P + 2), INVALID),
+                                  (dict(pos=P + 3), INVALID), (dict(nbps=2**27), UNSUPPORTED), (dict(n=2**21 + 1), UNSUPPORTED)]),
+         (attn, LAYOUT + CACHE + SCORES + [(dict(starts=None), INVALID), (dict(starts=P + 2), INVALID), (dict(first=P + 1), INVALID),
+                                           (dict(end=P + 2), INVALID), (dict(slopes=P + 2), INVALID)]),
          (tree, LAYOUT + CACHE + [(a | ({"mx": a["mx"] - 4} if a.get("mx") == 65 else {}), s) for a, s in SCORES]
-          + [(dict(ctx=None), INVALID), (dict(parents=None), INVALID), (dict(n=257, nbps=99), UNSUPPORTED),
+          + [(dict(ctx=None), INVALID), (dict(parents=None), INVALID), (dict(parents=P + 2), INVALID), (dict(lens=P + 2), INVALID), (dict(n=257, nbps=99), UNSUPPORTED),
              (dict(mx=2**31 - 1), INVALID)]),
          (keep, LAYOUT + [(dict(most=-1), INVALID), (dict(layers=-1), INVALID), (dict(k=None), INVALID), (dict(v=None), INVALID),
                           (dict(k=(P, None)), INVALID), (dict(v=(P, P + 4)), INVALID), (dict(table=None), INVALID),
                           (dict(ctx=None), INVALID), (dict(paths=None), INVALID), (dict(counts=None), INVALID),
+                          (dict(paths=P + 2), INVALID), (dict(counts=P + 1), INVALID),
                           (dict(B=65536), UNSUPPORTED), (dict(nbps=2**27), UNSUPPORTED)])]
 
 
@@ -137,9 +141,39 @@ int main() {
     printf("%lld", bad);
 }
 ''')
-    inc = [f"-I{ROOT}/include", f"-I{ROOT}/cuda-llm-inference-engine_amd/csrc", "-I/opt/rocm/include", "-D__HIP_PLATFORM_AMD__"]
-    subprocess.run(["g++", "-std=c++17", "-O1", *inc, str(src), "-o", str(tmp_path / "pages")], check=True)
+    subprocess.run(["g++", "-std=c++17", "-O1", *INCLUDES, "-I/opt/rocm/include", "-D__HIP_PLATFORM_AMD__", str(src), "-o", str(tmp_path / "pages")], check=True)
     assert subprocess.run([str(tmp_path / "pages")], capture_output=True, text=True, check=True).stdout == "0"
+
+
+INCLUDES = [f"-I{ROOT}/include", f"-I{ROOT}/cuda-llm-inference-engine_amd/csrc"]
+
+
+def test_plans(ie, tmp_path):
+    """paged_plan: the GPU tests' calls reach every form; splits stay within their limits and are those of the C ABI; an
+    asked number is kept."""
+    exe = str(tmp_path / "plan")
+    subprocess.run(["g++", "-std=c++17", "-O1", *INCLUDES, os.path.join(ROOT, "tests", "paged_plan.cpp"), "-o", exe], check=True)
+
+    def plans(calls):
+        out = subprocess.run([exe], input="\n".join(" ".join(map(str, c)) for c in calls), capture_output=True, text=True, check=True)
+        return [tuple(map(int, line.split())) for line in out.stdout.splitlines()]
+
+    calls = [(B, P, H * G, H, d, kv, keys, 0, 0) for kv, d, _, _, _, (B, P, H, G, keys) in FORMS]
+    assert plans(calls) == [(rows, groups, splits) for _, _, rows, groups, splits, _ in FORMS]
+    forms = {(kv, d, rows, groups) for kv, d, rows, groups, _, _ in FORMS}
+    assert forms == {(kv, d, rows, groups) for kv in (0, 1) for d in (64, 128)
+                     for rows, groups in ((1, 1), (2, 1), (16, 1), (32, 1), (64, 1), (128, 1), (128, 2))
+                     if not (kv and rows == 2) and not (not kv and groups == 2)}
+    calls = [(B, P, H * G, H, d, kv, keys, window, asked) for B in (1, 3, 70, 5000) for P in (1, 2, 20, 513, 9000) for H, G in ((1, 1), (8, 4))
+             for d in (64, 128) for kv in (0, 1) for keys in (1, 127, 128, 129, 70000, 2**30) for window in (0, 1, 500, 2**31 - 1)
+             for asked in (0, 1, 5, 64, 2**31 - 1)]
+    for (B, P, Hq, H, d, kv, keys, window, asked), (rows, groups, splits) in zip(calls, plans(calls), strict=True):
+        walked = min(keys, window + P) if window else keys
+        most = min(64, -(-walked // 128))
+        assert splits == min(asked, most) if asked else 1 <= splits <= most
+        assert rows in (1, 2, 16, 32, 64, 128) and (rows <= 16 or rows < 2 * P * (Hq // H)) and (groups == 1 or rows == 128)
+        if B * P * Hq * 64 < 2**21:  # (past it the C ABI may cut the splits)
+            assert ie.paged_attn_num_splits(B, P, Hq, H, d, kv, keys, window, asked) == splits
 
 
 def test_oracle_closed_forms():
