@@ -88,8 +88,8 @@ __device__ __forceinline__ RowOf row_of(const RopeWrite& a, int row) {
 // ..), or side by side where pairs are interleaved, behind the rotated ones and of V.  VEC is 4 where rot is a multiple of 8,
 // 2 of 4, else 1.  `tok` rows to a workgroup where a row has few units, else gridDim.y workgroups to a row, and N units
 // to a thread.  A row's angles are computed once a workgroup, for all of its heads, while the units' channels arrive.
-// Bound by HBM: reads 4 bytes a value, writes 4 of Q and 2 or 4 of K and V; 4 x 2000 rows of (32 + 16) x 128 into bf16
-// pages take 36 us, 4.2 TB/s (of 196 MB), with one unit a thread 43.
+// Bound by HBM: reads 4 bytes a value, writes 4 of Q and 2 or 4 of K and V; four ragged sequences of at most 2000 rows
+// of (32 + 16) x 128 into bf16 pages (150 MB) take 36 us, 4.2 TB/s, with one unit a thread 43.
 template <typename KV, int VEC, int N>
 __global__ __launch_bounds__(256) void rope_write_kernel(RopeWrite a, int units, int tok) {
     __shared__ float2 cs[512];  // (tok * rot / 2: a row has at least d / VEC units)

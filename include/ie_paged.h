@@ -43,7 +43,8 @@ extern "C" {
  * NULL: P rows each (values past P count as P).  Rows from lens[b] on are
  * left out: neither the cache nor Q_out has them; a row whose cache position is
  * negative or past its table's row has Q_out alone.  inv_freq [rot_dim / 2],
- * starts and lens [B] and positions [B, P] are device arrays. */
+ * starts and lens [B] and positions [B, P] are device arrays.  No two rows of a
+ * call go to the same row of the cache (sequences that share a page write past it). */
 int ie_rope_kv_write(int B, int P, const float* Q_src, const float* K_src, const float* V_src, int q_stride,
                      int kv_stride, int H_q, int H_kv, int d, int rot_dim, int interleaved, const float* inv_freq, const int* starts,
                      const int* lens, const int* positions, float* Q_out, void* k_cache, void* v_cache, int kv_dtype,
