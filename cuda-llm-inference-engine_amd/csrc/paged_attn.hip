@@ -17,6 +17,7 @@
 #include "device_util.h"
 #include "paged.h"
 #include "paged_plan.h"
+#include "paged_walk.h"
 
 namespace ie {
 namespace {
@@ -398,6 +399,98 @@ __device__ __forceinline__ Limits limits_of(const Row& row, int ctx) {
     return x;
 }
 
+// ---- gaps between rows' ranges (paged_walk.h)
+// Only `first` and `end` can leave one: otherwise a token's keys begin no later than where the token's before it end.
+template <bool TREE>
+__device__ __forceinline__ bool has_ranges(const PagedAttn& a) {
+    return !TREE && (a.first || a.end);
+}
+
+// Of a wave's M rows, row i in lane i: the lanes whose range begins a part and those whose range ends one; no gap: none.
+struct Gaps {
+    uint32_t begins, ends;
+};
+template <int M, bool TREE>
+__device__ __forceinline__ Gaps gaps_of(const PagedAttn& a, const Row& row) {
+    const Gaps none{0, 0};
+    if (M == 1 || !has_ranges<TREE>(a)) return none;
+    const KeyRange mine{row.live ? row.lo : 0, row.live ? row.hi : 0};
+    const bool some = mine.lo < mine.hi;
+    // (a range that begins where the shortest ends, or before, leaves none; this is all that most tiles take)
+    if (wave_imax(some ? mine.lo : 0) <= wave_imin(some ? mine.hi : 0x7fffffff)) return none;
+    const int i = threadIdx.x & (M - 1);
+    bool begin = some, end = some;
+#pragma unroll 1
+    for (int j = 0; j < M; ++j) {
+        const KeyRange other{__builtin_amdgcn_readlane(mine.lo, j), __builtin_amdgcn_readlane(mine.hi, j)};
+        begin &= !hides_begin(mine, other, j < i);
+        end &= !hides_end(mine, other, j < i);
+    }
+    constexpr uint32_t rows = (uint32_t)((1ull << M) - 1);
+    const Gaps g{(uint32_t)__ballot(begin) & rows, (uint32_t)__ballot(end) & rows};
+    return g.begins & (g.begins - 1) ? g : none;
+}
+// The key to look up at p.
+__device__ __forceinline__ int seen_at(const Gaps& g, const Row& row, int p) {
+    if (g.begins == 0) return p;
+    int begin = -1, end = -1;
+#pragma unroll 1
+    for (uint32_t left = g.begins; left; left &= left - 1) {
+        const int x = __builtin_amdgcn_readlane(row.lo, __builtin_ctz(left));
+        if (x <= p) begin = max(begin, x);
+    }
+#pragma unroll 1
+    for (uint32_t left = g.ends; left; left &= left - 1) {
+        const int x = __builtin_amdgcn_readlane(row.hi, __builtin_ctz(left));
+        if (x <= p) end = max(end, x);
+    }
+    return stand_in(p, begin, end);
+}
+
+// The same of a workgroup's N rows, by token, in LDS: where parts begin and end, in any order.
+template <int N>
+struct TileGaps {
+    KeyRange range[N];
+    int begin[N], end[N], count[2];
+};
+// Number of parts, 0 without a gap.  Called by the whole workgroup: `row` is the calling lane's, of token `token` of the
+// tile's `tokens`, and `real` where the call has such a row; most_lo and least_hi are the largest lo and the least hi of
+// rows that see a key.
+template <int N>
+__device__ __forceinline__ int find_gaps(TileGaps<N>& s, const Row& row, bool real, int token, int tokens, int most_lo, int least_hi) {
+    if (most_lo <= least_hi) return 0;
+    const int t = threadIdx.x;
+    if (real) s.range[token] = KeyRange{row.live ? row.lo : 0, row.live ? row.hi : 0};  // (a token's heads: the same)
+    if (t < 2) s.count[t] = 0;
+    __syncthreads();
+    if (t < tokens) {
+        const KeyRange mine = s.range[t];
+        bool begin = mine.lo < mine.hi, end = begin;
+#pragma unroll 1
+        for (int j = 0; j < tokens; ++j) {
+            const KeyRange other = s.range[j];
+            begin &= !hides_begin(mine, other, j < t);
+            end &= !hides_end(mine, other, j < t);
+        }
+        if (begin) s.begin[atomicAdd(&s.count[0], 1)] = mine.lo;
+        if (end) s.end[atomicAdd(&s.count[1], 1)] = mine.hi;
+    }
+    __syncthreads();
+    const int parts = __builtin_amdgcn_readfirstlane(s.count[0]);
+    return parts > 1 ? parts : 0;
+}
+template <int N>
+__device__ __forceinline__ int seen_at(const TileGaps<N>& s, int parts, int p) {
+    if (parts == 0) return p;
+    int begin = -1, end = -1;
+#pragma unroll 1
+    for (int k = 0; k < parts; ++k) {
+        if (s.begin[k] <= p) begin = max(begin, s.begin[k]);
+        if (s.end[k] <= p) end = max(end, s.end[k]);
+    }
+    return stand_in(p, begin, end);
+}
+
 // The products s of a block's keys from c0 on become their weights; st.o is scaled where their unit moves.
 template <int D, int M, bool TREE, typename Tree>
 __device__ __forceinline__ void weigh(const PagedAttn& a, const Tree& tree, const Row& row, const Limits& lim, float slope,
@@ -686,8 +779,9 @@ __global__ __launch_bounds__(64 * WR * WK, NP == 1 && WR == 4 ? 2 : 1) void page
     constexpr int NT = D / 32, KS = D / 16;
     __shared__ __attribute__((aligned(1024))) int8_t lds[T::LDS];
     __shared__ uint32_t slots[2][T::THREADS];  // a thread's each, SK of them keys of the stage
-    __shared__ int bounds[T::W][2];
+    __shared__ int bounds[T::W][4];
     __shared__ Tree tree;
+    __shared__ std::conditional_t<TREE, NoTree, TileGaps<32 * WR>> gaps;
     const int tid = threadIdx.x, lane = tid & 63, i = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), rw = wave % WR, kw = wave / WR;
     const Place at = place_of<TREE, T::SHARED>(a, tiles);
@@ -699,9 +793,17 @@ __global__ __launch_bounds__(64 * WR * WK, NP == 1 && WR == 4 ? 2 : 1) void page
     if constexpr (TREE) grow_tree(tree, a.parents + (size_t)b * a.P, a.P, a.window);
     const Row row = row_of<TREE>(a, tree, r, b, kvh, at.start, at.len);
     const Limits lim = limits_of<TREE>(row, ctx);
+    const bool some = row.live && row.lo < row.hi;
     if (lane == 0) {
         bounds[wave][0] = lim.lo;
         bounds[wave][1] = lim.hi;
+    }
+    if (has_ranges<TREE>(a)) {
+        const int lo = wave_imax(some ? row.lo : 0), hi = wave_imin(some ? row.hi : 0x7fffffff);
+        if (lane == 0) {
+            bounds[wave][2] = lo;
+            bounds[wave][3] = hi;
+        }
     }
     __syncthreads();
     int kbeg = 0x7fffffff, kend = 0;
@@ -712,6 +814,20 @@ __global__ __launch_bounds__(64 * WR * WK, NP == 1 && WR == 4 ? 2 : 1) void page
     }
     kend = __builtin_amdgcn_readfirstlane(kend);  // (scalars, and all that follows from them)
     kbeg = min(__builtin_amdgcn_readfirstlane(kbeg), kend);
+    int parts = 0;
+    if constexpr (!TREE) {
+        if (has_ranges<TREE>(a)) {
+            int lo = 0, hi = 0x7fffffff;
+#pragma unroll
+            for (int w = 0; w < T::W; ++w) {
+                lo = max(lo, bounds[w][2]);
+                hi = min(hi, bounds[w][3]);
+            }
+            const int G = a.H_q / a.H_kv, r0 = at.tile * 32 * WR, t0 = r0 / G, t1 = (min(r0 + 32 * WR, a.P * G) - 1) / G;
+            parts = find_gaps(gaps, row, r < a.P * G, row.t - t0, t1 - t0 + 1, __builtin_amdgcn_readfirstlane(lo),
+                              __builtin_amdgcn_readfirstlane(hi));
+        }
+    }
     // this split's stages
     const int all = (kend - kbeg + T::SK - 1) / T::SK, per = (all + a.splits - 1) / a.splits;
     const int s0 = min(at.split * per, all), s1 = min(s0 + per, all);
@@ -721,7 +837,11 @@ __global__ __launch_bounds__(64 * WR * WK, NP == 1 && WR == 4 ? 2 : 1) void page
     const size_t row_bytes = (size_t)a.H_kv * D * sizeof(KV);
     const int8_t* kbase = reinterpret_cast<const int8_t*>(static_cast<const KV*>(a.k) + (size_t)kvh * D);
     const int8_t* vbase = reinterpret_cast<const int8_t*>(static_cast<const KV*>(a.v) + (size_t)kvh * D);
-    auto pos_of = [&](int s) { return min(kbeg + s * T::SK + tid, k1 - 1); };  // of a stage's key tid
+    auto pos_of = [&](int s) {  // of a stage's key tid
+        const int p = min(kbeg + s * T::SK + tid, k1 - 1);
+        if constexpr (TREE) return p;
+        else return seen_at(gaps, parts, p);
+    };
     // bf16: a stage's rows straight into LDS; a wave's load fills 1 KiB, its lanes' addresses are
     // permuted so that the chunks land swizzled.
     constexpr int RPL = 1024 / T::ROW, LOADS = T::SK / RPL / T::W;
@@ -928,7 +1048,8 @@ __global__ __launch_bounds__((64 * Few<D, NP, M>::WAVES), (Few<D, NP, M>::WAVES 
     const uint32_t pages_at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_i8)(int8_t*)pages_all[wave]);
     uint32_t* const slots = slots_all[wave];
     auto first = [&](int j) { return k0 + 32 * (W * j + wave); };           // key of block j
-    auto pos_of = [&](int j) { return min(first(j) + (lane & 31), k1 - 1); };  // of this lane's key
+    const Gaps gaps = gaps_of<M, TREE>(a, row);
+    auto pos_of = [&](int j) { return seen_at(gaps, row, min(first(j) + (lane & 31), k1 - 1)); };  // of this lane's key
     auto ask_pages = [&](int j) { copy4(table + page_of(a.pages, pos_of(j)), pages_at + (j & (2 * DEEP - 1)) * 256); };
     constexpr int RPC = 1024 / T::ROW;  // rows of a copy
     const int lane_row = lane / T::CH;
@@ -1171,7 +1292,8 @@ __global__ __launch_bounds__(64 * kRowWaves, 2) void paged_row_kernel(PagedAttn 
     }
     // batch n of this wave: keys first(n) on
     auto first = [&](int n) { return k0 + T::BK * (W * n + wave); };
-    auto pos_of = [&](int n) { return min(first(n) + (lane & (T::BK - 1)), k1 - 1); };
+    const Gaps gaps = gaps_of<R, TREE>(a, mine);
+    auto pos_of = [&](int n) { return seen_at(gaps, mine, min(first(n) + (lane & (T::BK - 1)), k1 - 1)); };
     const int n1 = k1 > k0 ? ((k1 - k0 + T::BK - 1) / T::BK - wave + W - 1) / W : 0;
     int8_t* const lds = lds_all + wave * 2 * T::PART;
     const uint32_t lds_at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_i8)lds);

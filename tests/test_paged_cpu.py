@@ -202,3 +202,55 @@ def test_oracle_closed_forms():
     for pairs in (False, True):
         y, _ = po.rotated(x, torch.tensor([0, 5, 1000]), f, pairs)
         assert torch.equal(y[0], x[0].double()) and (y.norm(dim=-1) - x.double().norm(dim=-1)).abs().max() < 1e-12
+
+
+def test_walk_between_ranges(tmp_path):
+    """paged_walk.h: what a walk over rows' ranges looks up is seen by a row, a key that is seen is looked up as itself, and
+    parts are found once each; ranges that touch, repeat, nest, are empty or have gaps of one key among them."""
+    src = tmp_path / "walk.cpp"
+    src.write_text('''
+#include "paged_walk.h"
+#include <cstdio>
+#include <cstdlib>
+#include <vector>
+int main() {
+    long long wrong = 0, gaps = 0;
+    srand(1);
+    for (int round = 0; round < 20000; ++round) {
+        const int n = 1 + rand() % (round % 3 ? 6 : 128), span = 2 + rand() % (round % 2 ? 40 : 2000), wide = 1 + rand() % (1 + span / 3);
+        std::vector<ie::KeyRange> rows;
+        for (int i = 0; i < n; ++i) {
+            const int lo = rand() % span;
+            rows.push_back(rand() % 8 ? ie::KeyRange{lo, lo + rand() % wide} : ie::KeyRange{lo + 3, lo});
+            if (rand() % 4 == 0) rows.back() = rows[rand() % (i + 1)];
+        }
+        std::vector<char> seen(2 * span + 2, 0);
+        int least = 1 << 30, most = 0;
+        for (auto r : rows)
+            for (int j = r.lo; j < r.hi; ++j) seen[j] = 1, least = j < least ? j : least, most = j + 1 > most ? j + 1 : most;
+        std::vector<int> begin, end;
+        for (int i = 0; i < n; ++i) {
+            if (rows[i].lo >= rows[i].hi) continue;
+            bool b = true, e = true;
+            for (int j = 0; j < n; ++j) b &= !ie::hides_begin(rows[i], rows[j], j < i), e &= !ie::hides_end(rows[i], rows[j], j < i);
+            if (b) begin.push_back(rows[i].lo);
+            if (e) end.push_back(rows[i].hi);
+        }
+        size_t parts = 0;
+        for (int j = 0; j < most; ++j) parts += seen[j] && !(j && seen[j - 1]);
+        wrong += begin.size() != parts || end.size() != parts;
+        gaps += parts > 1;
+        for (int p = least, last = least; p < most; ++p) {
+            if (seen[p]) last = p;
+            int b = -1, e = -1;
+            for (int x : begin) b = x <= p && x > b ? x : b;
+            for (int x : end) e = x <= p && x > e ? x : e;
+            wrong += ie::stand_in(p, b, e) != last;
+        }
+    }
+    printf("%lld %d", wrong, gaps > 1000);
+}
+''')
+    exe = str(tmp_path / "walk")
+    subprocess.run(["g++", "-std=c++17", "-O1", *INCLUDES, str(src), "-o", exe], check=True)
+    assert subprocess.run([exe], capture_output=True, text=True, check=True).stdout == "0 1"
