@@ -186,6 +186,14 @@ __device__ __forceinline__ float capped(float x, const Cap& c) {
     return fabsf(x) < 1.0f ? capped_small(x, c) : big;
 }
 
+// A head's slope to base 2 (0: none).  One that passes fp32 so is its largest: infinite it would make NaN of the
+// distance 0, and any other distance takes all weight either way.
+__device__ __forceinline__ float slope_of(const PagedAttn& a, int head) {
+    if (!a.slopes) return 0.0f;
+    const float x = a.slopes[head], y = x * kLog2e;
+    return __builtin_isinf(y) && !__builtin_isinf(x) ? __builtin_copysignf(__FLT_MAX__, x) : y;
+}
+
 // What turns a product q.k into a score of base 2: the factor folded into q, and the distance's factor.
 struct Scores {
     float q, slope;
@@ -193,7 +201,7 @@ struct Scores {
 __device__ __forceinline__ Scores scores_of(const PagedAttn& a, int head) {
     Scores s;
     s.q = a.cap > 0.0f ? a.scale / a.cap : a.scale * kLog2e;
-    s.slope = a.slopes ? a.slopes[head] * kLog2e : 0.0f;
+    s.slope = slope_of(a, head);
     return s;
 }
 
@@ -323,7 +331,7 @@ __device__ __forceinline__ void exact_row(const PagedAttn& a, const Tree& tree, 
     const size_t stride = (size_t)a.H_kv * D;
     const KV *K = static_cast<const KV*>(a.k) + (size_t)kvh * D, *V = static_cast<const KV*>(a.v) + (size_t)kvh * D;
     const float* q = a.Q + (((size_t)b * a.P + r.t) * a.H_q + r.head) * D;
-    const float slope = a.slopes ? a.slopes[r.head] * kLog2e : 0.0f;
+    const float slope = slope_of(a, r.head);
     const Cap cap = cap_of(a.cap);
     m = -INFINITY;
     l = 0.0f;
@@ -1268,7 +1276,7 @@ __global__ __launch_bounds__(64 * kRowWaves, 2) void paged_row_kernel(PagedAttn 
         rows[r].lo = __builtin_amdgcn_readlane(mine.lo, r);
         rows[r].hi = __builtin_amdgcn_readlane(mine.hi, r);
         rows[r].pos = __builtin_amdgcn_readlane(mine.pos, r);
-        slope[r] = a.slopes ? a.slopes[rows[r].head] * kLog2e : 0.0f;
+        slope[r] = slope_of(a, rows[r].head);
     }
     const int kbeg = min(lim.lo, lim.hi), kend = lim.hi;
     const int all = (kend - kbeg + 127) / 128, per = (all + a.splits - 1) / a.splits;

@@ -6,9 +6,36 @@ import torch
 import paged_oracle as po
 from conftest import rng
 from paged_forms import FORMS
-from test_gpu_paged import case, i32, near
+from test_gpu_paged import case, check_ranges, i32, near, ragged
 
 pytestmark = pytest.mark.gpu
+LARGEST = float(np.finfo(np.float32).max)
+
+
+# ------------------------------------------------------------------ caps and slopes near the largest fp32
+@pytest.mark.parametrize("kv,d,rows,groups,splits,call", FORMS)
+def test_a_cap_that_no_score_feels(ie, dev, kv, d, rows, groups, splits, call):
+    """The largest fp32 as a cap, which times log2(e) is no fp32 any more, is no cap; so is any that is as far off."""
+    B, P, H, G, keys = call
+    starts = ragged(rng(d + rows), B, keys - P)
+    for cap in (LARGEST, 1e37, 1e26):
+        check_ranges(ie, dev, rng(d + rows), B, P, H, G, d, 16, bool(kv), starts, cap=cap)
+
+
+@pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("P,G", [(1, 1), (2, 1), (3, 2), (100, 4)])
+def test_slopes_of_the_largest_size(ie, dev, half, P, G):
+    """A query sees itself alone, at distance 0."""
+    r = rng(P)
+    table, caches, q, top = case(r, dev, 2, P, 2, G, 64, 16, half, [0, 70])
+    slopes = torch.full((2 * G,), LARGEST, device=dev)
+    want = po.ranges(q, caches, table, 16, [0, 70], None, top, slopes=slopes)
+    got = ie.paged_attn(q, *caches, i32(table, dev), i32([0, 70], dev), top, slopes=slopes)
+    near(got, want)
+    for b, s in enumerate((0, 70)):
+        for h in range(2 * G):
+            own = po.rows(caches[1], table[b], s + P, h // G)[s:]
+            assert bool(((got[b, :, h].double() - own).abs() <= 2.0**-22 * own.abs()).all())
 
 
 # ------------------------------------------------------------------ ranges far apart

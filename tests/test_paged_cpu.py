@@ -92,6 +92,13 @@ def test_refusals(ie, f, args, status):
     assert ie.last_error()
 
 
+@pytest.mark.parametrize("f", [attn, tree])
+@pytest.mark.parametrize("args", [dict(scale=3e38), dict(cap=3e38, scale=1e20), dict(cap=2.4e38, scale=2e38)])
+def test_refuses_scores_past_fp32(ie, f, args):
+    """A scale or a cap that passes fp32 once times log2(e)."""
+    assert f(ie, **args) == INVALID and "base 2" in ie.last_error()
+
+
 def test_nothing_to_do(ie):
     """Empty calls succeed whatever their pointers."""
     assert rope(ie, B=0, K=None, k=None) == 0 and rope(ie, n=0, K=None, k=None) == 0
