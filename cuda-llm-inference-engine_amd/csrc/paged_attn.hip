@@ -607,38 +607,12 @@ __device__ __forceinline__ bool split_query(const float* row, const RawQuery<D, 
     return bad;
 }
 
-// Results of a wave's rows: outputs, or with splits partial sums.  Rows whose result is not finite, or whose query
-// has no parts, again one by one over keys k0 .. k1 - 1.
-template <int D, int M, typename KV, bool TREE, typename Tree>
-__device__ __forceinline__ void finish(const PagedAttn& a, const Tree& tree, const Row& row, int b, int kvh, int ctx, int split,
-                                       int k0, int k1, bool q_bad, const State<D, M>& st, float l) {
-    constexpr int NT = D / M, AV = Shape<M>::AV;
-    const int lane = threadIdx.x & 63, i = lane & (M - 1), g = lane / M;
-    float bad = l * 0.0f;
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int v = 0; v < AV; ++v) bad = fmaf(st.o[t][v], 0.0f, bad);
-    const uint64_t lanes = __ballot(row.live && (q_bad || !(bad == 0.0f)));
-    uint32_t again = Shape<M>::rows_of(lanes);
-    const size_t rows = (size_t)a.B * a.P * a.H_q, mine = ((size_t)b * a.P + row.t) * a.H_q + row.head;
-    if (row.live && !(again >> i & 1)) {
-        float* out;
-        float inv = 1.0f;
-        if (a.splits == 1) {
-            inv = l > 0.0f ? 1.0f / l : 0.0f;
-            out = a.O + mine * D;
-        } else {
-            out = a.ws + (split * rows + mine) * D;
-            if (g == 0) *reinterpret_cast<float2*>(a.ws + a.splits * rows * D + 2 * (split * rows + mine)) = make_float2(st.m, l);
-        }
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int v = 0; v < AV / 4; ++v)
-                *reinterpret_cast<float4*>(out + M * t + 8 * v + 4 * g) =
-                    make_float4(st.o[t][4 * v] * inv, st.o[t][4 * v + 1] * inv, st.o[t][4 * v + 2] * inv, st.o[t][4 * v + 3] * inv);
-    }
+// The rows of `again` (bit x: lane x's) one by one over keys k0 .. k1 - 1: outputs, or with splits partial sums.
+template <int D, typename KV, bool TREE, typename Tree>
+__device__ __forceinline__ void exact_rows(const PagedAttn& a, const Tree& tree, const Row& row, uint32_t again, int b, int kvh, int ctx,
+                                           int split, int k0, int k1) {
+    const int lane = threadIdx.x & 63;
+    const size_t rows = (size_t)a.B * a.P * a.H_q;
 #pragma unroll 1
     for (; again; again &= again - 1) {
         const int x = __builtin_ctz(again);
@@ -662,6 +636,41 @@ __device__ __forceinline__ void finish(const PagedAttn& a, const Tree& tree, con
         }
         for (int e = 0; e < D / 64; ++e) out[lane * (D / 64) + e] = ro[e] * inv;
     }
+}
+
+// Results of a wave's rows: outputs, or with splits partial sums.  Rows whose result is not finite, or whose query
+// has no parts, again one by one over keys k0 .. k1 - 1.
+template <int D, int M, typename KV, bool TREE, typename Tree>
+__device__ __forceinline__ void finish(const PagedAttn& a, const Tree& tree, const Row& row, int b, int kvh, int ctx, int split,
+                                       int k0, int k1, bool q_bad, const State<D, M>& st, float l) {
+    constexpr int NT = D / M, AV = Shape<M>::AV;
+    const int lane = threadIdx.x & 63, i = lane & (M - 1), g = lane / M;
+    float bad = l * 0.0f;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int v = 0; v < AV; ++v) bad = fmaf(st.o[t][v], 0.0f, bad);
+    const uint64_t lanes = __ballot(row.live && (q_bad || !(bad == 0.0f)));
+    const uint32_t again = Shape<M>::rows_of(lanes);
+    const size_t rows = (size_t)a.B * a.P * a.H_q, mine = ((size_t)b * a.P + row.t) * a.H_q + row.head;
+    if (row.live && !(again >> i & 1)) {
+        float* out;
+        float inv = 1.0f;
+        if (a.splits == 1) {
+            inv = l > 0.0f ? 1.0f / l : 0.0f;
+            out = a.O + mine * D;
+        } else {
+            out = a.ws + (split * rows + mine) * D;
+            if (g == 0) *reinterpret_cast<float2*>(a.ws + a.splits * rows * D + 2 * (split * rows + mine)) = make_float2(st.m, l);
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int v = 0; v < AV / 4; ++v)
+                *reinterpret_cast<float4*>(out + M * t + 8 * v + 4 * g) =
+                    make_float4(st.o[t][4 * v] * inv, st.o[t][4 * v + 1] * inv, st.o[t][4 * v + 2] * inv, st.o[t][4 * v + 3] * inv);
+    }
+    exact_rows<D, KV, TREE>(a, tree, row, again, b, kvh, ctx, split, k0, k1);
 }
 
 // Key groups' states through LDS into the first group's wave; `slot` numbers the others' and mine. Groups' waves
@@ -1457,25 +1466,34 @@ __global__ __launch_bounds__(64 * kRowWaves, 2) void paged_row_kernel(PagedAttn 
         }
     }
     __syncthreads();
+    // The first wave: row r, channels c ..
+    static_assert(R * D / 4 <= 64, "a wave has all rows' channels");
+    if (wave > 0) return;
     const size_t total = (size_t)a.B * a.P * a.H_q;
-#pragma unroll 1
-    for (int x = tid; x < R * D / 4; x += 64 * W) {
-        const int r = x / (D / 4), c = 4 * (x % (D / 4));
-        const Row row = row_of<TREE>(a, tree, at.tile * R + r, b, kvh, at.start, at.len);
-        if (!row.live) continue;
-        float mx = sm_m[0][r];
+    const int r = min(lane / (D / 4), R - 1), c = 4 * (lane % (D / 4));
+    const Row row = row_of<TREE>(a, tree, at.tile * R + r, b, kvh, at.start, at.len);
+    const bool on = lane < R * D / 4 && row.live;
+    float mx = sm_m[0][r];
 #pragma unroll
-        for (int w = 1; w < W; ++w) mx = fmaxf(mx, sm_m[w][r]);
-        const float mu = mx == -INFINITY ? 0.0f : mx;
-        float sum = 0.0f;
-        float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int w = 1; w < W; ++w) mx = fmaxf(mx, sm_m[w][r]);
+    const float mu = mx == -INFINITY ? 0.0f : mx;
+    float sum = 0.0f;
+    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-        for (int w = 0; w < W; ++w) {
-            const float f = exp2_sm(sm_m[w][r] - mu);
-            const float4 z = *reinterpret_cast<const float4*>(&sm_o[w][r][c]);
-            sum = fmaf(f, sm_l[w][r], sum);
-            y.x = fmaf(f, z.x, y.x), y.y = fmaf(f, z.y, y.y), y.z = fmaf(f, z.z, y.z), y.w = fmaf(f, z.w, y.w);
-        }
+    for (int w = 0; w < W; ++w) {
+        const float f = exp2_sm(sm_m[w][r] - mu);
+        const float4 z = *reinterpret_cast<const float4*>(&sm_o[w][r][c]);
+        sum = fmaf(f, sm_l[w][r], sum);
+        y.x = fmaf(f, z.x, y.x), y.y = fmaf(f, z.y, y.y), y.z = fmaf(f, z.z, y.z), y.w = fmaf(f, z.w, y.w);
+    }
+    // A row that is not finite again by itself: weights of up to 2^8 may have taken sums of large values past fp32.
+    const float bad = fmaf(sum, 0.0f, fmaf(y.x, 0.0f, fmaf(y.y, 0.0f, fmaf(y.z, 0.0f, y.w * 0.0f))));
+    const uint64_t lanes = __ballot(on && !(bad == 0.0f));
+    uint32_t again = 0;
+#pragma unroll
+    for (int x = 0; x < R; ++x)
+        if (lanes >> (x * (D / 4)) & ((1ull << (D / 4)) - 1)) again |= 1u << x;
+    if (on && !(again >> r & 1)) {
         const size_t to = ((size_t)b * a.P + row.t) * a.H_q + row.head;
         float* out = a.O + to * D;
         float inv = 1.0f;
@@ -1487,6 +1505,7 @@ __global__ __launch_bounds__(64 * kRowWaves, 2) void paged_row_kernel(PagedAttn 
         }
         *reinterpret_cast<float4*>(out + c) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
     }
+    exact_rows<D, KV, TREE>(a, tree, mine, again, b, kvh, ctx, at.split, k0, k1);
 }
 
 // O rows from their splits' partials: D / 4 lanes a row, SG times, each of which has every SG-th split; four splits'

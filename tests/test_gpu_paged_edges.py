@@ -71,3 +71,24 @@ def test_pages_between_ranges_are_not_read(ie, dev, kv, d, rows, groups, splits,
         outs.append(ie.paged_attn(q, *caches, i32(table, dev), i32(starts, dev), top, first=i32(first, dev), end=i32(end, dev)))
         near(outs[-1], want)
     assert torch.equal(*outs)
+
+
+# ------------------------------------------------------------------ values near the largest fp32
+@pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("P,G,d", [(1, 1, 64), (1, 1, 128), (2, 1, 64), (1, 2, 128), (1, 4, 64), (30, 1, 128), (100, 2, 64)])
+@pytest.mark.parametrize("splits", [1, 3])
+def test_weights_of_large_values(ie, dev, half, P, G, d, splits):
+    """100 keys whose score is 5.3 above the 500 before them, values of 5e35: no 600 of them pass fp32's largest, four
+    times the weight that the later keys have in the earlier ones' unit, 200, do."""
+    r = rng(P + d)
+    keys = 600
+    table, caches, q, top = case(r, dev, 1, P, 1, G, d, 16, half, [keys - P])
+    k = torch.zeros(keys, d)
+    k[500:, 0] = 5.3
+    place = i32(table[0], dev).long()[torch.arange(keys, device=dev) // 16], torch.arange(keys, device=dev) % 16
+    caches[0][place] = k.to(dev)[:, None].to(caches[0].dtype)
+    caches[1][place] = torch.full((keys, 1, d), 5e35, device=dev).to(caches[1].dtype)
+    q.zero_()
+    q[..., 0] = 1.0
+    want = po.ranges(q, caches, table, 16, [keys - P], None, top, scale=1.0)
+    near(ie.paged_attn(q, *caches, i32(table, dev), i32([keys - P], dev), top, scale=1.0, splits=splits), want)
