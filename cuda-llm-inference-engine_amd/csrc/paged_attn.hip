@@ -419,15 +419,13 @@ struct Gaps {
     uint32_t begins, ends;
 };
 template <int M, bool TREE>
-__device__ __forceinline__ Gaps gaps_of(const PagedAttn& a, const Row& row) {
+__device__ __forceinline__ Gaps gaps_of(const PagedAttn& a, const Row& row, const Limits& lim) {
     const Gaps none{0, 0};
-    if (M == 1 || !has_ranges<TREE>(a)) return none;
+    // (where all begin no later than any ends there is none: this is all that most tiles take)
+    if (M == 1 || !has_ranges<TREE>(a) || lim.all_lo <= lim.all_hi) return none;
     const KeyRange mine{row.live ? row.lo : 0, row.live ? row.hi : 0};
-    const bool some = mine.lo < mine.hi;
-    // (a range that begins where the shortest ends, or before, leaves none; this is all that most tiles take)
-    if (wave_imax(some ? mine.lo : 0) <= wave_imin(some ? mine.hi : 0x7fffffff)) return none;
     const int i = threadIdx.x & (M - 1);
-    bool begin = some, end = some;
+    bool begin = mine.lo < mine.hi, end = begin;
 #pragma unroll 1
     for (int j = 0; j < M; ++j) {
         const KeyRange other{__builtin_amdgcn_readlane(mine.lo, j), __builtin_amdgcn_readlane(mine.hi, j)};
@@ -462,11 +460,9 @@ struct TileGaps {
     int begin[N], end[N], count[2];
 };
 // Number of parts, 0 without a gap.  Called by the whole workgroup: `row` is the calling lane's, of token `token` of the
-// tile's `tokens`, and `real` where the call has such a row; most_lo and least_hi are the largest lo and the least hi of
-// rows that see a key.
+// tile's `tokens`, and `real` where the call has such a row.
 template <int N>
-__device__ __forceinline__ int find_gaps(TileGaps<N>& s, const Row& row, bool real, int token, int tokens, int most_lo, int least_hi) {
-    if (most_lo <= least_hi) return 0;
+__device__ __forceinline__ int find_gaps(TileGaps<N>& s, const Row& row, bool real, int token, int tokens) {
     const int t = threadIdx.x;
     if (real) s.range[token] = KeyRange{row.live ? row.lo : 0, row.live ? row.hi : 0};  // (a token's heads: the same)
     if (t < 2) s.count[t] = 0;
@@ -810,17 +806,11 @@ __global__ __launch_bounds__(64 * WR * WK, NP == 1 && WR == 4 ? 2 : 1) void page
     if constexpr (TREE) grow_tree(tree, a.parents + (size_t)b * a.P, a.P, a.window);
     const Row row = row_of<TREE>(a, tree, r, b, kvh, at.start, at.len);
     const Limits lim = limits_of<TREE>(row, ctx);
-    const bool some = row.live && row.lo < row.hi;
     if (lane == 0) {
         bounds[wave][0] = lim.lo;
         bounds[wave][1] = lim.hi;
-    }
-    if (has_ranges<TREE>(a)) {
-        const int lo = wave_imax(some ? row.lo : 0), hi = wave_imin(some ? row.hi : 0x7fffffff);
-        if (lane == 0) {
-            bounds[wave][2] = lo;
-            bounds[wave][3] = hi;
-        }
+        bounds[wave][2] = lim.all_lo;
+        bounds[wave][3] = lim.all_hi;
     }
     __syncthreads();
     int kbeg = 0x7fffffff, kend = 0;
@@ -840,9 +830,11 @@ __global__ __launch_bounds__(64 * WR * WK, NP == 1 && WR == 4 ? 2 : 1) void page
                 lo = max(lo, bounds[w][2]);
                 hi = min(hi, bounds[w][3]);
             }
-            const int G = a.H_q / a.H_kv, r0 = at.tile * 32 * WR, t0 = r0 / G, t1 = (min(r0 + 32 * WR, a.P * G) - 1) / G;
-            parts = find_gaps(gaps, row, r < a.P * G, row.t - t0, t1 - t0 + 1, __builtin_amdgcn_readfirstlane(lo),
-                              __builtin_amdgcn_readfirstlane(hi));
+            // (as in gaps_of)
+            if (__builtin_amdgcn_readfirstlane(lo) > __builtin_amdgcn_readfirstlane(hi)) {
+                const int G = a.H_q / a.H_kv, r0 = at.tile * 32 * WR, t0 = r0 / G, t1 = (min(r0 + 32 * WR, a.P * G) - 1) / G;
+                parts = find_gaps(gaps, row, r < a.P * G, row.t - t0, t1 - t0 + 1);
+            }
         }
     }
     // this split's stages
@@ -1065,7 +1057,7 @@ __global__ __launch_bounds__((64 * Few<D, NP, M>::WAVES), (Few<D, NP, M>::WAVES 
     const uint32_t pages_at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_i8)(int8_t*)pages_all[wave]);
     uint32_t* const slots = slots_all[wave];
     auto first = [&](int j) { return k0 + 32 * (W * j + wave); };           // key of block j
-    const Gaps gaps = gaps_of<M, TREE>(a, row);
+    const Gaps gaps = gaps_of<M, TREE>(a, row, lim);
     auto pos_of = [&](int j) { return seen_at(gaps, row, min(first(j) + (lane & 31), k1 - 1)); };  // of this lane's key
     auto ask_pages = [&](int j) { copy4(table + page_of(a.pages, pos_of(j)), pages_at + (j & (2 * DEEP - 1)) * 256); };
     constexpr int RPC = 1024 / T::ROW;  // rows of a copy
@@ -1309,7 +1301,7 @@ __global__ __launch_bounds__(64 * kRowWaves, 2) void paged_row_kernel(PagedAttn 
     }
     // batch n of this wave: keys first(n) on
     auto first = [&](int n) { return k0 + T::BK * (W * n + wave); };
-    const Gaps gaps = gaps_of<R, TREE>(a, mine);
+    const Gaps gaps = gaps_of<R, TREE>(a, mine, lim);
     auto pos_of = [&](int n) { return seen_at(gaps, mine, min(first(n) + (lane & (T::BK - 1)), k1 - 1)); };
     const int n1 = k1 > k0 ? ((k1 - k0 + T::BK - 1) / T::BK - wave + W - 1) / W : 0;
     int8_t* const lds = lds_all + wave * 2 * T::PART;
