@@ -333,42 +333,52 @@ __device__ __forceinline__ void exact_row(const PagedAttn& a, const Tree& tree, 
     const float* q = a.Q + (((size_t)b * a.P + r.t) * a.H_q + r.head) * D;
     const float slope = slope_of(a, r.head);
     const Cap cap = cap_of(a.cap);
-    m = -INFINITY;
-    l = 0.0f;
-    for (int i = 0; i < N; ++i) o[i] = 0.0f;
     k0 = max(k0, TREE ? min(r.lo, ctx) : r.lo);
     k1 = min(k1, r.hi);
+    // The unit m is the largest score, and 2^32 more where that took a sum of large values past fp32 (2^30 keys at most;
+    // weights of 2^-94 are lost then).
 #pragma unroll 1
-    for (int c0 = k0; c0 < k1; c0 += 64) {
-        const int j = c0 + lane;
-        const bool seen = j < k1 && (seen_bits<TREE>(tree, r, c0 + (lane & 32), ctx) >> (lane & 31) & 1);
-        float s = -INFINITY;
-        uint32_t slot = 0;
-        if (seen) {
-            slot = cache_row(a.pages, table, j);
-            const KV* k = K + slot * stride;
-            float acc[4] = {};
+    for (float room = 0.0f;; room = 32.0f) {
+        float top = -INFINITY;
+        m = -INFINITY;
+        l = 0.0f;
+        for (int i = 0; i < N; ++i) o[i] = 0.0f;
+#pragma unroll 1
+        for (int c0 = k0; c0 < k1; c0 += 64) {
+            const int j = c0 + lane;
+            const bool seen = j < k1 && (seen_bits<TREE>(tree, r, c0 + (lane & 32), ctx) >> (lane & 31) & 1);
+            float s = -INFINITY;
+            uint32_t slot = 0;
+            if (seen) {
+                slot = cache_row(a.pages, table, j);
+                const KV* k = K + slot * stride;
+                float acc[4] = {};
 #pragma unroll 4
-            for (int e = 0; e < D; e += 4)
-                for (int i = 0; i < 4; ++i) acc[i] = fmaf(q[e + i], as_float(k[e + i]), acc[i]);
-            s = a.scale * ((acc[0] + acc[1]) + (acc[2] + acc[3]));
-            s = a.cap > 0.0f ? capped(s / a.cap, cap) : s * kLog2e;
-            int at = j;
-            if constexpr (TREE) at = j < ctx ? j : ctx + tree.depth[j - ctx];
-            if (a.slopes) s = fmaf(-slope, fabsf((float)(r.pos - at)), s);
-        }
-        const float mn = fmaxf(m, wave_max(s)), mu = mn == -INFINITY ? 0.0f : mn;
-        const float alpha = exp2_sm(m - mu), p = seen ? exp2_sm(s - mu) : 0.0f;
-        l = fmaf(l, alpha, wave_sum(p));
-        m = mn;
-        for (int i = 0; i < N; ++i) o[i] *= alpha;
+                for (int e = 0; e < D; e += 4)
+                    for (int i = 0; i < 4; ++i) acc[i] = fmaf(q[e + i], as_float(k[e + i]), acc[i]);
+                s = a.scale * ((acc[0] + acc[1]) + (acc[2] + acc[3]));
+                s = a.cap > 0.0f ? capped(s / a.cap, cap) : s * kLog2e;
+                int at = j;
+                if constexpr (TREE) at = j < ctx ? j : ctx + tree.depth[j - ctx];
+                if (a.slopes) s = fmaf(-slope, fabsf((float)(r.pos - at)), s);
+            }
+            top = fmaxf(top, wave_max(s));
+            const float mn = top + room, mu = mn == -INFINITY ? 0.0f : mn;
+            const float alpha = exp2_sm(m - mu), p = seen ? exp2_sm(s - mu) : 0.0f;
+            l = fmaf(l, alpha, wave_sum(p));
+            m = mn;
+            for (int i = 0; i < N; ++i) o[i] *= alpha;
 #pragma unroll 1
-        for (uint64_t left = __ballot(seen); left; left &= left - 1) {
-            const int k = __builtin_ctzll(left);
-            const float w = __shfl(p, k);
-            const KV* v = V + (uint32_t)__shfl((int)slot, k) * stride + lane * N;
-            for (int i = 0; i < N; ++i) o[i] = fmaf(w, as_float(v[i]), o[i]);
+            for (uint64_t left = __ballot(seen); left; left &= left - 1) {
+                const int k = __builtin_ctzll(left);
+                const float w = __shfl(p, k);
+                const KV* v = V + (uint32_t)__shfl((int)slot, k) * stride + lane * N;
+                for (int i = 0; i < N; ++i) o[i] = fmaf(w, as_float(v[i]), o[i]);
+            }
         }
+        float bad = 0.0f;
+        for (int i = 0; i < N; ++i) bad = fmaf(o[i], 0.0f, bad);
+        if (room > 0.0f || !__ballot(!(bad == 0.0f))) return;
     }
 }
 
@@ -1505,6 +1515,7 @@ __global__ __launch_bounds__(64 * kRowWaves, 2) void paged_row_kernel(PagedAttn 
 // 16000 keys, 8 x 4 x 128 in 16 splits: 31.0 us in all with a row's splits one after another, 20.3 so).
 template <int D, int SG>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn a) {
+    static_assert(IE_PAGED_MAX_SPLITS <= 128, "a row's parts and their rounding within 2^8");
     constexpr int L = D / 4, PER = 256 / (L * SG);
     const size_t rows = (size_t)a.B * a.P * a.H_q;
     const int c = threadIdx.x % L, sg = threadIdx.x / L % SG, local = threadIdx.x / (L * SG);
@@ -1513,9 +1524,10 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn a) {
     const float2* ml = reinterpret_cast<const float2*>(a.ws + a.splits * rows * D);
     float m = -INFINITY, l = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    auto add = [&](float xm, float xl, float4 y) {  // (an empty part has xm = -inf, xl = 0 and no y)
+    // Parts count times 2^-8: as many as there can be, each finite, stay so together.
+    auto add = [&](float xm, float xl, float4 y, float times) {  // (an empty part has xm = -inf, xl = 0 and no y)
         const float mn = fmaxf(m, xm), mu = mn == -INFINITY ? 0.0f : mn;
-        const float fa = exp2_sm(m - mu), fb = exp2_sm(xm - mu);
+        const float fa = exp2_sm(m - mu), fb = exp2_sm(xm - mu) * times;
         m = mn;
         l = l * fa + xl * fb;
         o.x = o.x * fa + y.x * fb;
@@ -1538,7 +1550,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn a) {
                 }
             }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) add(x[k].x, x[k].y, y[k]);
+            for (int k = 0; k < 4; ++k) add(x[k].x, x[k].y, y[k], 0x1p-8f);
         }
     }
     if constexpr (SG > 1) {
@@ -1551,7 +1563,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn a) {
 #pragma unroll
         for (int k = 1; k < SG; ++k) {
             const float2 x = sm[threadIdx.x + k * L];
-            add(x.x, x.y, so[threadIdx.x + k * L]);
+            add(x.x, x.y, so[threadIdx.x + k * L], 1.0f);
         }
     }
     if (!live) return;

@@ -92,3 +92,16 @@ def test_weights_of_large_values(ie, dev, half, P, G, d, splits):
     q[..., 0] = 1.0
     want = po.ranges(q, caches, table, 16, [keys - P], None, top, scale=1.0)
     near(ie.paged_attn(q, *caches, i32(table, dev), i32([keys - P], dev), top, scale=1.0, splits=splits), want)
+
+
+@pytest.mark.parametrize("kv,d,rows,groups,splits,call", FORMS)
+def test_sums_of_large_values(ie, dev, kv, d, rows, groups, splits, call):
+    """Values up to 3e38, whose weighted sum before its division passes fp32's largest; the answer does not."""
+    B, P, H, G, keys = call
+    r = rng(rows + d)
+    starts = ragged(r, B, keys - P)
+    table, caches, q, top = case(r, dev, B, P, H, G, d, 16, bool(kv), starts, fill=0.0)
+    caches[1].copy_(torch.rand(caches[1].shape, device=dev) * 2e38 + 1e38)
+    want = po.ranges(q, caches, table, 16, starts, None, top)
+    for s in {1, splits}:
+        near(ie.paged_attn(q, *caches, i32(table, dev), i32(starts, dev), top, splits=s), want)
