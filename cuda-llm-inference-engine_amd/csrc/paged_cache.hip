@@ -14,13 +14,15 @@ __device__ __forceinline__ uint32_t cache_row(const PageMap& m, const int* table
     return (uint32_t)table[page] * (uint32_t)m.block + (uint32_t)(p - page * m.block);
 }
 
-// cos and sin of pos * freq.  The product has 31 + 24 bits and the turns' rest is
-// taken from it in 64 bits; the rest as an fp32 number and what that leaves,
+// cos and sin of pos * freq.  The product has up to 31 + 24 bits, more than a double: its rounding, exact by
+// fma, and the rest of 1 / 2 pi go along, so the turns' rest is right to 2^-50 of a turn as far as a position
+// times a frequency has whole turns to take off (2^50).  The rest as an fp32 number and what that leaves,
 // whose first order is added: without it a rest near half a turn is off by 2^-25 of
 // a turn, 1.9e-7, three times what the functions themselves are.
 __device__ __forceinline__ float2 turn(long long pos, float freq) {
-    const double turns = (double)pos * (double)freq * 0.15915494309189535;
-    const double rest = turns - rint(turns);
+    constexpr double per = 0x1.45f306dc9c883p-3, more = -0x1.6b01ec5417056p-57;  // 1 / 2 pi
+    const double p = (double)pos * (double)freq, low = fma((double)pos, (double)freq, -p);
+    const double rest = fma(p, per, -rint(p * per)) + fma(p, more, low * per);
     const float hi = (float)rest, lo = (float)(rest - (double)hi) * 6.2831853f;
     float s, c;
     sincospif(2.0f * hi, &s, &c);

@@ -35,8 +35,8 @@ extern "C" {
  * + t) * kv_stride (the rows of a QKV projection serve as they lie; multiples of 4,
  * at least a row), and goes to cache position starts[b] + t.  Its angles
  * are a_i = pos * inv_freq[i], i < rot_dim / 2, pos = positions[b * P + t]
- * (positions NULL: starts[b] + t), the product and its rest over full turns in
- * 64 bits; channels (x, y) = (i, i + rot_dim / 2), or (2 i, 2 i + 1) where
+ * (positions NULL: starts[b] + t), less their full turns to 2^-50 of one (up to
+ * 2^50 of them); channels (x, y) = (i, i + rot_dim / 2), or (2 i, 2 i + 1) where
  * interleaved is not 0, become (x cos - y sin, y cos + x sin).  Channels from
  * rot_dim on (even, 0 .. d) pass as they are, as does V.  K and V are rounded to
  * the cache's type once; Q_out [B, P, H_q, d] is fp32 (H_q may be 0: no Q).  lens

@@ -1,4 +1,6 @@
 """include/ie_paged.h on the GPU at the edges of what it takes (paged_oracle has the tolerances)."""
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -105,3 +107,47 @@ def test_sums_of_large_values(ie, dev, kv, d, rows, groups, splits, call):
     want = po.ranges(q, caches, table, 16, starts, None, top)
     for s in {1, splits}:
         near(ie.paged_attn(q, *caches, i32(table, dev), i32(starts, dev), top, splits=s), want)
+
+
+# ------------------------------------------------------------------ far positions
+def turns(pos, freq):
+    """pos * freq / 2 pi less its whole turns, from 300 bits of pi."""
+    one = 1 << 300
+
+    def atan_inverse(x):
+        term, total, n, sign = one // x, 0, 1, 1
+        while term:
+            total += sign * (term // n)
+            term //= x * x
+            n += 2
+            sign = -sign
+        return total
+
+    two_pi = 8 * (4 * atan_inverse(5) - atan_inverse(239))
+    out = []
+    for f in freq:
+        num, den = float(f).as_integer_ratio()
+        rest = (pos * num * one // den) * one // two_pi % one
+        out.append((rest - one if rest > one // 2 else rest) / one)
+    return np.array(out)
+
+
+@pytest.mark.parametrize("pairs", [False, True])
+@pytest.mark.parametrize("pos", [0, 1, -1, 77, 10**5, 2**24 - 1, 2**30 + 12345, -2**31, 2**31 - 1])
+def test_rope_angles(ie, dev, pairs, pos):
+    """Cosines and sines of far positions and of frequencies above 1 against angles whose whole turns are taken off
+    in integers.  A unit vector's rotation is its cosine and sine, each off by 4 U at most."""
+    r = rng(5)
+    freq = np.concatenate([10000.0 ** (-np.arange(24) / 24), r.random(20) * 3, r.random(10) * 100, [1.0, 0.0, 2.0, 64.0, 1e-30, 1e4, 1e6, 3.5, 0.1, 99.0]])
+    freq = freq.astype(np.float32)
+    x = torch.zeros(1, 1, 1, 128, device=dev)
+    x[..., 0::2 if pairs else 1] = 1.0
+    if not pairs:
+        x[..., 64:] = 0.0
+    kc = torch.zeros(1, 16, 1, 128, device=dev)
+    got = ie.rope_kv_write(x, x, x, torch.from_numpy(freq).to(dev), i32([3], dev), kc, kc.clone(), i32([[0]], dev),
+                           positions=i32([[pos]], dev), interleaved=pairs)[0, 0, 0].cpu().double().numpy()
+    angle = 2 * math.pi * turns(pos, freq)
+    cos, sin = (got[0::2], got[1::2]) if pairs else (got[:64], got[64:])
+    assert np.abs(cos - np.cos(angle)).max() <= 4 * po.U and np.abs(sin - np.sin(angle)).max() <= 4 * po.U
+    assert np.array_equal(kc[0, 3, 0].cpu().double().numpy(), got)
