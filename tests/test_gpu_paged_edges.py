@@ -7,8 +7,8 @@ import torch
 
 import paged_oracle as po
 from conftest import rng
-from paged_forms import FORMS
-from test_gpu_paged import case, check_ranges, i32, near, ragged
+from paged_forms import ASKED, FORMS
+from test_gpu_paged import case, check_ranges, i32, near, normal, ragged
 
 pytestmark = pytest.mark.gpu
 LARGEST = float(np.finfo(np.float32).max)
@@ -151,3 +151,72 @@ def test_rope_angles(ie, dev, pairs, pos):
     cos, sin = (got[0::2], got[1::2]) if pairs else (got[:64], got[64:])
     assert np.abs(cos - np.cos(angle)).max() <= 4 * po.U and np.abs(sin - np.sin(angle)).max() <= 4 * po.U
     assert np.array_equal(kc[0, 3, 0].cpu().double().numpy(), got)
+
+
+# ------------------------------------------------------------------ many sequences, long paths, many rows
+@pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("B", [63, 64, 65, 100])
+@pytest.mark.parametrize("P,G", [(1, 1), (2, 3), (20, 2)])
+def test_many_sequences(ie, dev, half, B, P, G):
+    """Up to 64 sequences come by length, more as they are."""
+    r = rng(B + P)
+    starts = ragged(r, B, 300)
+    lens = [P] + [int(x) for x in r.integers(0, P + 1, B - 1)]
+    check_ranges(ie, dev, r, B, P, 1, G, 64, 16, half, starts, lens)
+    check_ranges(ie, dev, r, B, P, 1, G, 64, 16, half, starts, lens, splits=2)
+
+
+@pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("n", [63, 64, 65, 128, 200])
+def test_keep_long_paths(ie, dev, half, n):
+    """Paths of more entries than a wave looks up at once: whole, cut at 64 and 65, ending at entry 64 by themselves."""
+    r = rng(n)
+    ctx = [0, 9, 40, 100]
+    paths = [sorted(int(x) for x in r.choice(300, n, replace=False)) for _ in ctx]
+    if n > 64:
+        paths[2][64] = paths[2][63]  # ends there
+    paths[3] = list(range(n))  # stays
+    counts = [n, min(n, 64), n, n]
+    moves = [paths[0], paths[1][:64], paths[2][:64], paths[3]]
+    table, pages = po.tables(r, [c + 300 for c in ctx], 16)
+    t = torch.bfloat16 if half else torch.float32
+    k, v = (normal(r, dev, 2, pages, 16, 3, 64).to(t) for _ in range(2))
+    want = [k.clone(), v.clone()]
+    for w, c in zip(want, (k, v)):
+        for b, move in enumerate(moves):
+            for j, p in enumerate(move):
+                x, y = ctx[b] + j, ctx[b] + p
+                w[:, table[b, x // 16], x % 16] = c[:, table[b, y // 16], y % 16]
+    ie.kv_cache_keep(list(k), list(v), i32(table, dev), i32(ctx, dev), i32(paths, dev), i32(counts, dev))
+    assert torch.equal(k, want[0]) and torch.equal(v, want[1])
+
+
+def test_a_join_of_many_rows(ie, dev):
+    """More than 2^20 rows in six parts each."""
+    r = rng(1)
+    B, G, d = 70, 16384, 64
+    starts = ragged(r, B, 700)
+    table, caches, q, top = case(r, dev, B, 1, 1, 1, d, 16, True, starts)
+    q = torch.randn(B, 1, G, d, device=dev, generator=torch.Generator(dev).manual_seed(2))
+    got = ie.paged_attn(q, *caches, i32(table, dev), i32(starts, dev), top, splits=6)
+    for h in ([0, 1, 2, 3], [G // 2 + 1], [G - 2, G - 1]):
+        near(got[:, :, h], po.ranges(q[:, :, h].contiguous(), caches, table, 16, starts, None, top))
+
+
+@pytest.mark.parametrize("kv,d,rows,groups,splits,call", ASKED)
+def test_forms_in_asked_splits(ie, dev, kv, d, rows, groups, splits, call):
+    """Forms that the plan splits only when asked, with ranges and as trees."""
+    B, P, H, G, keys = call
+    r = rng(rows + d)
+    starts = ragged(r, B, keys - P)
+    lens = [P] + [int(x) for x in r.integers(0, P + 1, B - 1)]
+    check_ranges(ie, dev, r, B, P, H, G, d, 24, bool(kv), starts, lens, slopes=True, cap=20.0, splits=splits)
+    first = r.integers(-5, keys, (B, P)).astype(np.int32)
+    end = (first + r.integers(-30, keys, (B, P))).astype(np.int32)
+    check_ranges(ie, dev, r, B, P, H, G, d, 16, bool(kv), starts, lens, first=first, end=end, splits=splits)
+    table, caches, q, _ = case(r, dev, B, P, H, G, d, 16, bool(kv), starts)
+    parents = [[int(r.integers(max(-1, t - 4), t)) if t else -1 for t in range(P)] for _ in range(B)]
+    want = po.tree(q, caches, table, 16, starts, parents, lens, window=12)
+    got = ie.tree_attn(q, *caches, i32(table, dev), i32(starts, dev), i32(parents, dev), max(starts), lens=i32(lens, dev), window=12,
+                       splits=splits)
+    near(got, want)

@@ -11,7 +11,7 @@ import torch
 
 import paged_oracle as po
 from conftest import ROOT, rng
-from paged_forms import FORMS
+from paged_forms import ASKED, FORMS
 
 P = 4096  # stands for a device pointer: no call below reaches HIP
 OUT = 1 << 40
@@ -261,3 +261,13 @@ int main() {
     exe = str(tmp_path / "walk")
     subprocess.run(["g++", "-std=c++17", "-O1", *INCLUDES, str(src), "-o", exe], check=True)
     assert subprocess.run([exe], capture_output=True, text=True, check=True).stdout == "0 1"
+
+
+def test_forms_in_asked_splits(tmp_path):
+    """The calls of ASKED reach their forms, so that every form is tested in several splits."""
+    exe = str(tmp_path / "plan")
+    subprocess.run(["g++", "-std=c++17", "-O1", *INCLUDES, os.path.join(ROOT, "tests", "paged_plan.cpp"), "-o", exe], check=True)
+    calls = "\n".join(f"{B} {P} {H * G} {H} {d} {kv} {keys} 0 {splits}" for kv, d, _, _, splits, (B, P, H, G, keys) in ASKED)
+    out = subprocess.run([exe], input=calls, capture_output=True, text=True, check=True).stdout.split("\n")
+    assert out[:-1] == [f"{rows} {groups} {splits}" for _, _, rows, groups, splits, _ in ASKED]
+    assert {f[:4] for f in FORMS} == {f[:4] for f in FORMS + ASKED if f[4] > 1}
