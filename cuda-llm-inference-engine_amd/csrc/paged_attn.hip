@@ -48,8 +48,10 @@ template <int N>
 __device__ __forceinline__ void copies_left() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
-// Waits for the wave's LDS reads: what copies overwrite has been read.
-__device__ __forceinline__ void reads_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+// Waits for the wave's own reads and writes of LDS: what copies overwrite has been read, and what other waves read behind a
+// barrier has been written.  (The compiler's wait for the latter is missing where a loop ends with the write and begins with
+// the barrier.)
+__device__ __forceinline__ void lds_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
 __device__ __forceinline__ int page_of(const PageMap& m, int p) {
     return m.mul ? (int)(__umulhi((uint32_t)p, m.mul) >> m.shift) : p;
@@ -968,9 +970,10 @@ __global__ __launch_bounds__(64 * WR * WK, NP == 1 && WR == 4 ? 2 : 1) void page
 #pragma unroll 1
     for (int s = s0; s < s1; ++s) {
         int buf = 0;
+        lds_done();  // (slots of the last iteration)
         if constexpr (NP == 1) {
             buf = (s - s0) & 1;
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            copies_left<0>();
             __syncthreads();  // stage s is there, and the other buffer read
             if (s + 1 < s1) copy(s + 1, buf ^ 1);
         } else {
@@ -1082,13 +1085,13 @@ __global__ __launch_bounds__((64 * Few<D, NP, M>::WAVES), (Few<D, NP, M>::WAVES 
         const uint32_t page = (uint32_t)pages_all[wave][j & (2 * DEEP - 1)][lane & 31];
         slots[lane & 31] = page * (uint32_t)a.pages.block + (uint32_t)(p - in * a.pages.block);
         ask_pages(j + DEEP);
-        reads_done();
+        lds_done();
 #pragma unroll
         for (int c = 0; c < C; ++c)
             copy16(kbase + (slots[lane_row + c * RPC] * row_bytes + col(c, false)), lds_at + (j & (DEEP - 1)) * T::PART + c * 1024);
     };
     auto ask_v = [&](int j) {  // (after ask_k(j))
-        reads_done();
+        lds_done();
 #pragma unroll
         for (int c = 0; c < C; ++c)
             copy16(vbase + (slots[lane_row + c * RPC] * row_bytes + col(c, true)),
@@ -1323,12 +1326,12 @@ __global__ __launch_bounds__(64 * kRowWaves, 2) void paged_row_kernel(PagedAttn 
         const int p = pos_of(n);
         slots[lane] = (uint32_t)pages_all[wave][n & 1][lane] * (uint32_t)a.pages.block + (uint32_t)(p - page_of(a.pages, p) * a.pages.block);
         ask_pages(n + 1);
-        reads_done();
+        lds_done();
 #pragma unroll
         for (int u = 0; u < U; ++u) copy16(kbase + slots[u * T::KPI + grp] * row_bytes, lds_at + u * 1024);
     };
     auto ask_v = [&] {  // (after ask_k of the same batch)
-        reads_done();
+        lds_done();
 #pragma unroll
         for (int u = 0; u < U; ++u) copy16(vbase + slots[u * T::KPI + grp] * row_bytes, lds_at + T::PART + u * 1024);
     };

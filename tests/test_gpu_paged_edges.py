@@ -220,3 +220,31 @@ def test_forms_in_asked_splits(ie, dev, kv, d, rows, groups, splits, call):
     got = ie.tree_attn(q, *caches, i32(table, dev), i32(starts, dev), i32(parents, dev), max(starts), lens=i32(lens, dev), window=12,
                        splits=splits)
     near(got, want)
+
+
+# ------------------------------------------------------------------ many workgroups of many stages, again and again
+@pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("d,H,G,P,splits,kind", [(128, 8, 4, 4096, 1, "docs"), (64, 8, 4, 4096, 1, "docs"), (128, 8, 2, 2048, 1, "causal"),
+                                                 (64, 4, 1, 2500, 1, "causal"), (128, 2, 8, 1000, 3, "causal"), (128, 4, 8, 255, 1, "tree"),
+                                                 (64, 4, 8, 255, 3, "tree")])
+def test_large_calls_repeat_their_bits(ie, dev, half, d, H, G, P, splits, kind):
+    """150 calls of many workgroups at once, their waves at different speeds: each has the same bits, and they are right."""
+    r = rng(P + d)
+    B, starts = (2, [1500, 900]) if kind == "tree" else (1, [0])
+    table, caches, q, top = case(r, dev, B, P, H, G, d, 32, half, starts)
+    tb, at = i32(table, dev), i32(starts, dev)
+    if kind == "tree":
+        parents = [[int(r.integers(max(-1, t - 6), t)) if t else -1 for t in range(P)] for _ in range(B)]
+        want = po.tree(q, caches, table, 32, starts, parents)
+        pa = i32(parents, dev)
+        call = lambda: ie.tree_attn(q, *caches, tb, at, pa, max(starts), splits=splits)
+    else:
+        cuts = np.sort(r.integers(0, P, P // 500))
+        first = np.concatenate([[0], cuts])[np.searchsorted(cuts, np.arange(P), side="right")].astype(np.int32)[None] if kind == "docs" else None
+        want = po.ranges(q, caches, table, 32, starts, None, top, first)
+        fi = None if first is None else i32(first, dev)
+        call = lambda: ie.paged_attn(q, *caches, tb, at, top, first=fi, splits=splits)
+    got = call()
+    near(got, want)
+    different = sum((call() != got).any().long() for _ in range(150))
+    assert int(different) == 0
