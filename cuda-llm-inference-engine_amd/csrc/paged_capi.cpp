@@ -78,16 +78,13 @@ int check_attn(const char* fn, ie::PagedAttn& a, long long keys, int block_size,
     if (overlap(a.Q, bytes, a.O, bytes)) return fail(IE_ERR_INVALID, "%s: O overlaps Q", fn);
     if (keys > 0 && (st = check_cache(fn, a.k, a.v, a.pages.table)) != IE_OK) return st;
     if (a.scale == 0.0f) a.scale = 1.0f / sqrtf((float)a.d);
-    if (a.cap > 0 && !std::isfinite(a.scale / a.cap))
-        return fail(IE_ERR_INVALID, "%s: scale / cap = %g / %g passes fp32", fn, (double)a.scale, (double)a.cap);
-    // cap tanh(x) with x = scale q.k / cap is scale q.k to fp32 where |x| < 2^-12; with scale / cap below 2^-80
-    // that is any product under 2^68, and the cap is none: folded into the queries, so small a factor would bring
-    // their values below what three bf16 parts hold, and further down below fp32's least normal.
-    if (a.cap > 0 && a.scale / a.cap < 0x1p-80f) a.cap = 0;
-    // scores are kept times log2(e)
-    constexpr float log2e = 1.4426950408889634f;
-    if (!std::isfinite(a.cap * log2e) || (a.cap == 0 && !std::isfinite(a.scale * log2e)))
-        return fail(IE_ERR_INVALID, "%s: scale=%g or cap=%g passes fp32 to base 2", fn, (double)a.scale, (double)a.cap);
+    // cap tanh(s / cap) is s to fp32 where |s| < 2^-12 cap; from 2^80 on a cap is none (folded into the queries it would
+    // bring their values below what three bf16 parts hold, and times log2(e) the largest pass fp32).
+    if (a.cap >= 0x1p80f) a.cap = 0;
+    // The factor of a product q.k, to base 2 where there is no cap
+    const float factor = a.cap > 0 ? a.scale / a.cap : a.scale * 1.4426950408889634f;
+    if (!std::isfinite(factor) || (a.cap > 0 && factor < 0x1p-126f))
+        return fail(IE_ERR_INVALID, "%s: scale=%g and cap=%g leave fp32's normal range", fn, (double)a.scale, (double)a.cap);
     a.splits = workspace ? ie_paged_attn_num_splits(a.B, a.P, a.H_q, a.H_kv, a.d, a.kv_dtype, (int)keys, a.window, num_splits) : 1;
     if (!workspace && num_splits > 1 &&
         ie_paged_attn_num_splits(a.B, a.P, a.H_q, a.H_kv, a.d, a.kv_dtype, (int)keys, a.window, num_splits) > 1)

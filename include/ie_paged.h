@@ -72,14 +72,14 @@ size_t ie_paged_attn_workspace_bytes(int B, int P, int H_q, int d, int num_split
  * a row apart, end = max(prefix, pos + 1) lets a prefix see itself whole.  With
  * h the query head, G = H_q / H_kv, the score of key j is
  *   s = scale * (q . K[j, h / G])          (scale 0: 1 / sqrt(d))
- *   s = cap * tanh(s / cap)                (cap 0, or above 2^80 scale: none)
+ *   s = cap * tanh(s / cap)                (cap 0, or from 2^80 on: none)
  *   s = s - slopes[h] * |pos - j|          (slopes [H_q] fp32, NULL: none)
  * and O [B, P, H_q, d] = sum_j softmax(s)_j V[j, h / G].  A query that sees no
  * key gives zeros; rows from lens[b] on are left as they were.  Q, O fp32,
  * token-major; starts [B] and lens [B] are device int32.  Values at keys that a
  * query does not see never reach it, infinite and NaN ones included; one
- * that it sees makes what fp32 arithmetic makes of it.  Scores are held times
- * log2(e): a scale without a cap, or a cap, that passes fp32 so is refused.
+ * that it sees makes what fp32 arithmetic makes of it.  Refused are a scale that
+ * passes fp32 times log2(e) and a scale / cap outside its normal range.
  * A NULL workspace stands for num_splits = 1; otherwise workspace_bytes must
  * cover ie_paged_attn_workspace_bytes of ie_paged_attn_num_splits' count.  A
  * repeated call repeats its bits; those of a token may depend on the chunk and

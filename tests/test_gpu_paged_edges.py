@@ -40,6 +40,14 @@ def test_slopes_of_the_largest_size(ie, dev, half, P, G):
             assert bool(((got[b, :, h].double() - own).abs() <= 2.0**-22 * own.abs()).all())
 
 
+@pytest.mark.parametrize("kv,d,rows,groups,splits,call", FORMS)
+def test_small_scales_of_large_queries(ie, dev, kv, d, rows, groups, splits, call):
+    """A scale of 1e-28 for queries of 1e28: scores that the cap bends."""
+    B, P, H, G, keys = call
+    starts = ragged(rng(d + rows), B, keys - P)
+    check_ranges(ie, dev, rng(d + rows), B, P, H, G, d, 16, bool(kv), starts, cap=5.0, scale=1e-28, q_scale=1e28)
+
+
 # ------------------------------------------------------------------ ranges far apart
 @pytest.mark.parametrize("kv,d,rows,groups,splits,call", [f for f in FORMS if f[5][1] > 1])
 def test_pages_between_ranges_are_not_read(ie, dev, kv, d, rows, groups, splits, call):
