@@ -337,8 +337,10 @@ __device__ __forceinline__ void exact_row(const PagedAttn& a, const Tree& tree, 
     const Cap cap = cap_of(a.cap);
     k0 = max(k0, TREE ? min(r.lo, ctx) : r.lo);
     k1 = min(k1, r.hi);
-    // The unit m is the largest score, and 2^32 more where that took a sum of large values past fp32 (2^30 keys at most;
-    // weights of 2^-94 are lost then).
+    // The unit m is the largest score, and 2^32 more where that took a sum of large values past fp32 (2^30 keys at most).
+    // Weights of 2^-94 are lost then: what they make of an infinite value is the first sum's.
+    float before[N];
+    for (int i = 0; i < N; ++i) before[i] = 0.0f;
 #pragma unroll 1
     for (float room = 0.0f;; room = 32.0f) {
         float top = -INFINITY;
@@ -379,7 +381,11 @@ __device__ __forceinline__ void exact_row(const PagedAttn& a, const Tree& tree, 
             }
         }
         float bad = 0.0f;
-        for (int i = 0; i < N; ++i) bad = fmaf(o[i], 0.0f, bad);
+        for (int i = 0; i < N; ++i) {
+            if (o[i] != o[i] && __builtin_isinf(before[i])) o[i] = before[i];
+            before[i] = o[i];
+            bad = fmaf(o[i], 0.0f, bad);
+        }
         if (room > 0.0f || !__ballot(!(bad == 0.0f))) return;
     }
 }

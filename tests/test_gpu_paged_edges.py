@@ -117,6 +117,23 @@ def test_sums_of_large_values(ie, dev, kv, d, rows, groups, splits, call):
         near(ie.paged_attn(q, *caches, i32(table, dev), i32(starts, dev), top, splits=s), want)
 
 
+@pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("P,G", [(1, 1), (2, 1), (3, 2), (100, 4)])
+def test_an_infinite_value_that_is_seen(ie, dev, half, P, G):
+    """It makes its channel infinite, with a weight of 2^-50 and with one of 2^-110 (an fp32 number all the same), and no other."""
+    table, caches, q, top = case(rng(P), dev, 1, P, 1, G, 64, 16, half, [70])
+    k, v = caches
+    q.zero_()
+    q[..., 0] = 1.0
+    k[table[0, 0], :, :, 0] = 1.0
+    for gap in (50, 110):
+        k[..., 0] = 1.0
+        k[table[0, 0], 3, :, 0] = 1.0 - gap / 2
+        v[table[0, 0], 3, :, 7] = math.inf
+        got = ie.paged_attn(q, k, v, i32(table, dev), i32([70], dev), top, scale=2 * math.log(2))
+        assert bool((got[..., 7] == math.inf).all()) and bool(torch.isfinite(got[..., :7]).all()) and bool(torch.isfinite(got[..., 8:]).all())
+
+
 # ------------------------------------------------------------------ far positions
 def turns(pos, freq):
     """pos * freq / 2 pi less its whole turns, from 300 bits of pi."""
