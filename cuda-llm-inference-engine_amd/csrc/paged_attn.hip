@@ -150,9 +150,11 @@ __device__ __forceinline__ void product(const Parts<N> (&a)[NT], const Parts<3>&
 
 // ---- scores
 // cap * tanh(x), cap with the factor to base 2.  Below 1 x (cap + y P(y)), y = x^2, P the polynomial nearest to
-// cap (tanh(x) / x - 1) / y there (weighted least squares: 4.6e-9 of the value off, with fp32's
-// steps 7e-8), below 0.55 one of degree 3 (3.7e-08, with fp32's steps 1e-7): nine instructions or six, which is all that a block takes whose
-// scores lie there.  Above it 1 - 2 / (1 + e^2x), whose rounding is that of a value near 1.
+// cap (tanh(x) / x - 1) / y there (weighted least squares: 5.6e-9 of the value off, with fp32's
+// steps and the cap's own 1.5e-7), below 0.55 one of degree 3 (3.8e-8, with fp32's steps 1.5e-7): nine instructions or six, which is all
+// that a block takes whose scores lie there (2 x 2048 x 8 x 2 x 128 at scores below 0.4 of the cap 129.7 -> 126.0 us for the
+// second; the kernel of one row, which waits for memory, has the first alone).  Above it 1 - 2 / (1 + e^2x), whose
+// rounding is that of a value near 1; a block with one such score takes it for all (160 us).
 struct Cap {
     float cap, p[7], low[4];
 };
@@ -611,7 +613,7 @@ __device__ __forceinline__ bool split_query(const float* row, const RawQuery<D, 
         q[s] = split8(z);
     }
     bool bad = false;
-    if (__ballot(!(least >= 0x1p-98f && most < 0x1p64f))) {  // (seldom; zeros among them)
+    if (__ballot(!(least >= 0x1p-98f && most < 0x1p64f))) {  // (a zero anywhere among them, as of a padded head, is enough)
 #pragma unroll 1
         for (int e = 0; e < D; ++e) {
             const float x = row[e], y = fabsf(x * scale);

@@ -55,7 +55,8 @@ inline PagedPlan paged_plan(int B, int P, int H_q, int H_kv, int d, int kv_dtype
             // 1000 keys of a workgroup where all CUs read their own from HBM (5.5 TB/s); tiles of a pair share theirs
             const double memory = 1000.0 * 2 * d * (half ? 2 : 4) / (5.5e6 / 256) / tiles * (a_cu < 1 ? a_cu : 1);
             // Workgroups of like length come in whole rounds; a causal prompt's tiles see half of its own keys on average.
-            // A batch's sequences are taken to hold four fifths of the longest's keys.
+            // A batch's sequences are taken to hold four fifths of the longest's keys: no call says how many they hold (alike
+            // ones, 32 of 8192, take two splits for it: 192 us, in one 186).  0.6 of a round and of a start are as rough.
             const bool alike = walked >= 2.0 * P;
             const double seen = (alike ? walked - (P - 1) / 2.0 : walked > P ? walked - P / 2.0 : walked / 2) * (B > 1 ? 0.8 : 1);
             const double load = a_cu * seen / walked, own = x.rate + (x.loaded - x.rate) * (load < 1 ? load : 1);

@@ -75,7 +75,7 @@ size_t ie_paged_attn_workspace_bytes(int B, int P, int H_q, int d, int num_split
  *   s = cap * tanh(s / cap)                (cap 0, or from 2^80 on: none)
  *   s = s - slopes[h] * |pos - j|          (slopes [H_q] fp32, NULL: none)
  * and O [B, P, H_q, d] = sum_j softmax(s)_j V[j, h / G].  A query that sees no
- * key gives zeros; rows from lens[b] on are left as they were.  Q, O fp32,
+ * key, or none above minus infinity, gives zeros; rows from lens[b] on are left as they were.  Q, O fp32,
  * token-major; starts [B] and lens [B] are device int32.  Values at keys that a
  * query does not see never reach it, infinite and NaN ones included; one
  * that it sees makes what fp32 arithmetic makes of it.  Refused are a scale that
@@ -112,8 +112,8 @@ int ie_tree_attn(int B, int T, int H_q, int H_kv, int d, const float* Q, const v
  * moves to context_lens[b] + j, j = 0 .. counts[b] - 1 (paths int32 [B, max_count],
  * counts and context_lens int32 [B], device; counts past max_count count as it).
  * A path ascends; it ends before an entry that is not above the one before it
- * (the first: not below 0) or whose row is past the table's.  Rows behind the
- * moved ones keep their bytes and count as dropped.  No page that a path moves
+ * (the first: not below 0) or whose row is past the table's.  No cache stands
+ * twice among them.  Rows behind the moved ones keep their bytes and count as dropped.  No page that a path moves
  * rows into may be shared. */
 int ie_kv_cache_keep(int B, int max_count, int n_layers, void* const* k_caches, void* const* v_caches, int kv_dtype,
                      const int* block_table, int num_blocks_per_seq, int block_size, int n_heads, int d_head,
